@@ -408,6 +408,112 @@ int inf_binary_bcast(int op, const void* a, const void* b, void* out, int64_t n,
  * next-token choice, so only rows int32 values leave the device. */
 int inf_argmax_rows(const void* x, int64_t rows, int64_t cols, int64_t ld, int32_t* out, inf_dtype dt, void* stream);
 
+/* ---- generation from a paged key-value cache ------------------------------
+ * No counterpart in the reference, which has no generation loop.  Rows (the
+ * sequences of a batch) of different lengths share pools of pages; the row's
+ * table names its pages, so a cache grows page by page, sequences of a prompt
+ * share its pages, and beam search reorders numbers instead of keys and values.
+ *
+ * Everything that changes from token to token (lengths, tables, positions,
+ * beams) is read from device memory, and the plans depend on the shapes given
+ * here alone: a captured step can be replayed as the sequences grow.  Page
+ * numbers are checked on the device: one outside the pool is never followed. */
+
+/* The cache of one layer: key j of row n and head h lies at
+ * k + table[n * table_stride + j / page_size] * sk.b + h * sk.h +
+ * (j % page_size) * sk.t, its D elements contiguous; values likewise.
+ * Strides as in inf_strides, b the page's; rows 16-byte aligned.  D is 32, 64
+ * or 128, page_size a power of two, rows <= 65535, max_pages * page_size (a
+ * row's capacity) <= 2^30.  lens[n] is row n's length, with the
+ * new tokens of the step: inf_kv_append writes the last ones, the attention reads
+ * all.  Pages may be shared by rows as long as nothing writes to them. */
+typedef struct {
+    void* k;
+    void* v;
+    inf_strides sk, sv;
+    const int32_t* table; /* device, [rows, max_pages], rows table_stride apart */
+    const int32_t* lens;  /* device, [rows] */
+    int64_t table_stride;
+    int rows, heads, D, page_size, max_pages, n_pages;
+    inf_dtype dt; /* INF_F32 or INF_BF16 */
+} inf_paged_kv;
+
+/* Writes the keys and values k, v [rows, heads, T, D] (strided views; rows aligned as the
+ * attention's) of row n's last counts[n] positions: tokens t < counts[n] go to positions
+ * lens[n] - counts[n] + t; the others are padding and are not read.  counts (device, [rows],
+ * each 0..T) may be NULL: T tokens in every row.  A token whose position is negative or past
+ * the capacity, or whose page is not in the pool, is dropped.
+ * weights and positions (either may be NULL): dense [rows, heads, capacity]; the new tokens'
+ * weights become 0 and their positions seen[n] - counts[n] + t, where seen (device, [rows])
+ * counts the tokens that row n has ever had; NULL: lens, which is the same until
+ * inf_kv_evict takes some away. */
+int inf_kv_append(const inf_paged_kv* cache, const void* k, inf_strides sk, const void* v, inf_strides sv,
+                  const int32_t* counts, int T, float* weights, int32_t* positions, const int32_t* seen,
+                  void* stream);
+
+/* Attention of one new token per row over its whole cache: o[n, i] = sum_j p_j v_j with
+ * p = softmax_j(scale q[n, i] . k_j), j < lens[n], keys and values of head i / (q_heads / heads).
+ * q, o: [rows, q_heads, 1, D] views; q_heads a multiple of the cache's heads.  max_len
+ * (1..capacity) bounds the rows' lengths for the plan and the workspace; a row of length 0
+ * or less gives zeros, one longer than max_len or with a page outside the pool NaN.  What lies
+ * in a row's pages behind its length does not matter.
+ * weights_out (may be NULL): dense [rows, heads, capacity]; position j < lens[n] becomes
+ * weights_in's (0 where that is NULL; it may be weights_out) plus its probabilities summed over the
+ * query heads of its head; other positions are left as they are.
+ * workspace: inf_attn_decode_paged_workspace bytes for the same arguments (0 for short
+ * caches without weights: then it may be NULL), 256-byte aligned.  Calls that share one must
+ * not overlap.  Results do not depend on scheduling: the same bits on every run. */
+int inf_attn_decode_paged_workspace(const inf_paged_kv* cache, int q_heads, int max_len, int weights,
+                                    size_t* out_bytes);
+int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides sq, void* o, inf_strides so,
+                          int q_heads, int max_len, float scale, const float* weights_in, float* weights_out,
+                          void* workspace, size_t ws_bytes, void* stream);
+
+/* Cuts every (row, head) of more than `keep` positions to `keep`: those among the `recent`
+ * (<= keep) newest positions stay (position >= newest + 1 - recent), then those of the largest
+ * weights, of equal weights the lower slot's (NaN counts as below all).  The kept slots
+ * behind the first `keep` fill the holes among these, in order; a slot that stays is not
+ * moved, so the order of a row's positions changes, which attention does not see, and
+ * the slots past the cut keep what they had.  weights_out and positions_out (dense
+ * [rows, heads, capacity], may be the inputs) get the kept ones' in their first `keep` slots,
+ * shorter rows' in their first lens[n]; lens_out (may be cache->lens) is min(lens[n], keep).
+ * A row longer than max_len is left as it is.  Pages that are written must not
+ * be shared with another row.  workspace: inf_kv_evict_workspace bytes, 4-byte aligned. */
+int inf_kv_evict_workspace(const inf_paged_kv* cache, int keep, int max_len, size_t* out_bytes);
+int inf_kv_evict(const inf_paged_kv* cache, const float* weights_in, float* weights_out, const int32_t* positions_in,
+                 int32_t* positions_out, int32_t* lens_out, int keep, int recent, int max_len, void* workspace,
+                 size_t ws_bytes, void* stream);
+
+/* Beam search's step: of a group's beams x vocab candidates the best `beams` (<= 32), best first.
+ * Candidate (b, t) scores scores[b] + logits[b, t] - lse(logits[b]), in 64 bits; equal scores go to
+ * the lower b, then the lower t, and within a beam the logits decide.  logits: [groups * beams, vocab],
+ * rows ld elements apart, of any alignment; scores, finished, and the results tokens, parents (the
+ * beam b within the group), scores_out and finished_out: [groups, beams].
+ * A finished beam (finished[b] != 0; NULL: none) has one candidate, token eos at its own score.
+ * finished_out (may be NULL): whether the parent was finished or the token is eos; eos < 0: no
+ * token ends a sequence.  A beam whose score is not finite passes it on to its candidates (so
+ * beams that start at -inf are taken last); one whose logits hold a NaN or +inf, or -inf alone,
+ * has NaN for all, which ranks below -inf.  The results may be the inputs.
+ * workspace: inf_beam_select_workspace bytes, 256-byte aligned. */
+int inf_beam_select_workspace(int64_t groups, int beams, int64_t vocab, size_t* out_bytes);
+int inf_beam_select(const void* logits, int64_t ld, const float* scores, const int32_t* finished, int64_t groups,
+                    int beams, int64_t vocab, int32_t eos, int32_t* tokens, int32_t* parents, float* scores_out,
+                    int32_t* finished_out, inf_dtype dt, void* workspace, size_t ws_bytes, void* stream);
+
+/* Lets the cache follow the beams: rows g * beams + i of group g become copies of their parents,
+ * rows g * beams + parents[g * beams + i].  The rows of a group have one length (the first one's is
+ * read).  Full pages go over by number.  The last, partly filled page is each row's own: a row that
+ * is not its own parent gets the parent's copied to its page spare[row] (all layers in one launch:
+ * cache is the first layer's, the others' pools lie k_layer_stride and v_layer_stride elements on),
+ * and its former page becomes spare_out[row].  Table entries behind that page stay the row's own.
+ * So with one spare page per row, and each row's entries from the partly filled page on in no other
+ * row's table, nothing is ever written to a page that two rows read.
+ * table_out must not overlap cache->table; spare_out may be spare.  A parent outside the
+ * group gives a row of pages -1. */
+int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stride, int64_t v_layer_stride,
+                     const int32_t* parents, int beams, int32_t* table_out, int64_t table_out_stride,
+                     const int32_t* spare, int32_t* spare_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

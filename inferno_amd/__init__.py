@@ -70,6 +70,14 @@ EXPORTS = (
     "inf_attn_decode_static",
     "inf_set_deterministic",
     "inf_get_deterministic",
+    "inf_kv_append",
+    "inf_attn_decode_paged_workspace",
+    "inf_attn_decode_paged",
+    "inf_kv_evict_workspace",
+    "inf_kv_evict",
+    "inf_beam_select_workspace",
+    "inf_beam_select",
+    "inf_beam_reorder",
     "inf_last_error_detail",
 )
 
@@ -85,6 +93,15 @@ class AdamWTensor(ctypes.Structure):
 
     _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p),
                 ("n", ctypes.c_int64)]
+
+
+class PagedKVStruct(ctypes.Structure):
+    """inf_paged_kv: pools of pages, table and lengths of a paged key-value cache."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("sk", Strides), ("sv", Strides),
+                ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("rows", ctypes.c_int), ("heads", ctypes.c_int), ("D", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("n_pages", ctypes.c_int), ("dt", ctypes.c_int)]
 
 
 class InfernoError(RuntimeError):
@@ -165,6 +182,16 @@ def lib() -> ctypes.CDLL:
         L.inf_attn_decode_static.argtypes = [vp, S, vp, S, vp, S, vp, S, i32, i32, i32, i32, f32, i32, vp]
         L.inf_set_deterministic.argtypes = [i32]
         L.inf_get_deterministic.argtypes = []
+        kv = ctypes.POINTER(PagedKVStruct)
+        szp = ctypes.POINTER(sz)
+        L.inf_kv_append.argtypes = [kv, vp, S, vp, S, vp, i32, vp, vp, vp, vp]
+        L.inf_attn_decode_paged_workspace.argtypes = [kv, i32, i32, i32, szp]
+        L.inf_attn_decode_paged.argtypes = [kv, vp, S, vp, S, i32, i32, f32, vp, vp, vp, sz, vp]
+        L.inf_kv_evict_workspace.argtypes = [kv, i32, i32, szp]
+        L.inf_kv_evict.argtypes = [kv, vp, vp, vp, vp, vp, i32, i32, i32, vp, sz, vp]
+        L.inf_beam_select_workspace.argtypes = [i64, i32, i64, szp]
+        L.inf_beam_select.argtypes = [vp, i64, vp, vp, i64, i32, i64, i32, vp, vp, vp, vp, i32, vp, sz, vp]
+        L.inf_beam_reorder.argtypes = [kv, i32, i64, i64, vp, i32, vp, i64, vp, vp, vp]
         for name in EXPORTS[11:-1]:
             getattr(L, name).restype = i32
         L.inf_last_error_detail.argtypes = []
@@ -244,6 +271,17 @@ from .nn import (  # noqa: E402
     layernorm_fwd,
     binary_bcast,
 )
+from .paged import (  # noqa: E402
+    PagedKV,
+    attn_decode_paged,
+    attn_decode_paged_workspace,
+    beam_reorder,
+    beam_select,
+    beam_select_workspace,
+    kv_append,
+    kv_evict,
+    kv_evict_workspace,
+)
 
 __all__ = [
     "lib",
@@ -254,6 +292,12 @@ __all__ = [
     "softmax_bwd",
     "softmax_axis_fwd",
     "softmax_axis_bwd",
+    "PagedKV",
+    "kv_append",
+    "attn_decode_paged",
+    "kv_evict",
+    "beam_select",
+    "beam_reorder",
     "strides_of",
     "workspace_bytes",
     "set_deterministic",

@@ -1,0 +1,319 @@
+// beam.hip -- beam search's selection: of a group's beams x vocabulary candidates the best
+// `beams` by score + logit - lse.
+//
+// The logits are read once.  A workgroup holds up to 8192 columns of one beam in registers, forms
+// their maximum and sum of exponentials and finds their best `beams`; a second launch joins a
+// beam's parts to its lse and ranks what is left of a group, some hundreds of candidates, by the
+// whole score in 64 bits.  Within a beam the score's order is the logits', so the first step needs
+// no lse and is exact; between beams scores can lie close together, and there the sums of
+// exponentials are held in 64 bits as well.  Equal scores go to the lower beam, then the lower
+// token.
+//
+// The best few of many: with each lane's largest value known, the beams-th largest of a wave's 64 is
+// at most the beams-th largest of all its values, so only values from it up can matter: about as
+// many as there are beams.  They are picked into LDS, and each counts those that are better.
+#include "common.h"
+#include "kernels.h"
+
+namespace inf {
+
+namespace {
+
+constexpr int kBeamCols = 8192;  // columns of a workgroup at most: 32 per thread
+constexpr int kBeamList = 1024;  // candidates in LDS; more of them (equal ones) are picked one by one
+
+// Order of the floats as unsigned numbers, -0 as 0, NaN below -inf; 0 stands for no value.
+__device__ __forceinline__ uint32_t ordered_logit(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 1u;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float logit_of(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint64_t ordered_score(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+    if ((b & 0x7fffffffffffffffull) > 0x7ff0000000000000ull) return 1ull;
+    return b >> 63 ? ~b : b | (1ull << 63);
+}
+
+// A lower bound, to the 20 highest bits, of the n-th largest of the wave's values.
+__device__ __forceinline__ uint32_t wave_nth(uint32_t v, int n) {
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t up = t | (1u << bit);
+        if (__popcll(__ballot(v >= up)) >= n) t = up;
+    }
+    return t;
+}
+
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
+    const uint32_t lo = __shfl_xor((uint32_t)v, m, 64), hi = __shfl_xor((uint32_t)(v >> 32), m, 64);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ double shfl_xor_d(double v, int m) {
+    return __longlong_as_double((long long)shfl_xor64((uint64_t)__double_as_longlong(v), m));
+}
+
+// Whether a beam reads its logits: not if it is finished, or its score is not finite (then all
+// its candidates have that score).
+__device__ __forceinline__ bool beam_lives(const BeamSelectParams& p, int64_t row) {
+    return !(p.finished && p.finished[row]) && isfinite(p.scores[row]);
+}
+
+}  // namespace
+
+template <typename E>
+__global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
+    using T = typename E::T;
+    constexpr int GE = 16 / sizeof(T), NV = kBeamCols / 256 / GE;  // columns of a 16-byte load, loads per thread
+    __shared__ uint64_t list[kBeamList];
+    __shared__ int count;
+    __shared__ float wmax[4];
+    __shared__ double wsum[4];
+    __shared__ uint64_t wbest[4];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int64_t row = blockIdx.x / p.nsplit;
+    const int split = blockIdx.x % p.nsplit;
+    if (!beam_lives(p, row)) return;
+    // columns counted from the 16-byte boundary at or before the row's start
+    const T* x = (const T*)p.logits + row * p.ld;
+    const int mis = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % GE);
+    const int64_t end = min((int64_t)(split + 1) * p.chunk, p.vocab + mis);
+    float v[NV * GE];
+    uint32_t lane_best = 0;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+        const int64_t c = (int64_t)split * p.chunk + (int64_t)(u * 256 + tid) * GE;
+        if (c >= mis && c + GE <= end) {
+            const u32x4 raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + (c - mis)));
+#pragma unroll
+            for (int e = 0; e < GE; ++e) {
+                if constexpr (sizeof(T) == 4)
+                    v[u * GE + e] = __uint_as_float(raw[e]);
+                else
+                    v[u * GE + e] = __uint_as_float(e & 1 ? raw[e >> 1] & 0xffff0000u : raw[e >> 1] << 16);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < GE; ++e)
+                v[u * GE + e] = c + e >= mis && c + e < end ? E::ld(x + (c + e - mis)) : 0.f;
+        }
+    }
+    auto column = [&](int i) { return (int64_t)split * p.chunk + (int64_t)(i / GE * 256 + tid) * GE + i % GE; };
+    auto there = [&](int i) { return column(i) >= mis && column(i) < end; };
+    auto key = [&](int i) {
+        return (uint64_t)ordered_logit(v[i]) << 32 | (uint32_t)~(uint32_t)(column(i) - mis);
+    };
+#pragma unroll
+    for (int i = 0; i < NV * GE; ++i)
+        if (there(i)) {
+            mx = fmaxf(mx, v[i]);
+            lane_best = max(lane_best, ordered_logit(v[i]));
+        }
+    mx = wave_max(mx);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < NV * GE; ++i)
+        if (there(i)) sum += (double)fast_exp2((v[i] - ref) * kLog2e);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) sum += shfl_xor_d(sum, m);
+    if (lane == 0) {
+        wmax[wave] = mx;
+        wsum[wave] = sum;
+    }
+    if (tid == 0) count = 0;
+    const uint32_t least = wave_nth(lane_best, p.beams);
+    __syncthreads();
+    if (tid == 0) {
+        const float M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
+        double S = 0.0;
+        for (int i = 0; i < 4; ++i) S += wmax[i] == -INFINITY ? wsum[i] : wsum[i] * exp((double)wmax[i] - (double)M);
+        p.maxs[blockIdx.x] = M;
+        p.sums[blockIdx.x] = S;
+    }
+#pragma unroll
+    for (int i = 0; i < NV * GE; ++i)
+        if (there(i) && ordered_logit(v[i]) >= least) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kBeamList) list[at] = key(i);
+        }
+    __syncthreads();
+    const int n = count;
+    uint64_t* out = p.cand + (int64_t)blockIdx.x * p.beams;
+    if (n <= kBeamList) {
+        if (tid < p.beams && tid >= n) out[tid] = 0;  // fewer columns than beams
+        for (int i = tid; i < n; i += 256) {
+            const uint64_t mine = list[i];
+            int better = 0;
+            for (int j = 0; j < n; ++j) better += list[j] > mine;
+            if (better < p.beams) out[better] = mine;
+        }
+        return;
+    }
+    uint64_t before = ~0ull;
+    for (int k = 0; k < p.beams; ++k) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < NV * GE; ++i) {
+            const uint64_t x = there(i) ? key(i) : 0;
+            if (x < before && x > best) best = x;
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) best = max(best, shfl_xor64(best, m));
+        if (lane == 0) wbest[wave] = best;
+        __syncthreads();
+        before = max(max(wbest[0], wbest[1]), max(wbest[2], wbest[3]));
+        if (tid == 0) out[k] = before;
+        __syncthreads();
+    }
+}
+
+__global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
+    enum { kLives, kFinished, kFlat };  // a flat beam's candidates are the first tokens, all with its score
+    __shared__ double base[kMaxBeams];  // score - lse; the score of a beam that is finished or flat
+    __shared__ int kind[kMaxBeams];
+    __shared__ uint64_t ls[kBeamList], lt[kBeamList];
+    __shared__ int count;
+    __shared__ uint64_t ws[4], wt[4];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int64_t row0 = (int64_t)blockIdx.x * p.beams;
+    for (int b = wave; b < p.beams; b += 4) {
+        const int64_t row = row0 + b;
+        if (!beam_lives(p, row)) {
+            if (lane == 0) {
+                base[b] = (double)p.scores[row];
+                kind[b] = p.finished && p.finished[row] ? kFinished : kFlat;
+            }
+            continue;
+        }
+        float M = -INFINITY;
+        for (int i = lane; i < p.nsplit; i += 64) M = fmaxf(M, p.maxs[row * p.nsplit + i]);
+        M = wave_max(M);
+        double S = 0.0;
+        for (int i = lane; i < p.nsplit; i += 64) {
+            const float m = p.maxs[row * p.nsplit + i];
+            const double s = p.sums[row * p.nsplit + i];
+            S += m == -INFINITY ? s : s * exp((double)m - (double)M);
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) S += shfl_xor_d(S, m);
+        if (lane == 0) {
+            // a NaN or +inf among the logits, or nothing above -inf: the sum is NaN, infinite or 0
+            const double lse = (double)M + log(S);
+            const bool fine = isfinite(lse);
+            base[b] = fine ? (double)p.scores[row] - lse : __longlong_as_double(0x7ff8000000000000ll);
+            kind[b] = fine ? kLives : kFlat;
+        }
+    }
+    if (tid == 0) count = 0;
+    __syncthreads();
+    // Candidate i of the group: its score as an ordered number (0: there is none) and its place.
+    const int per = p.nsplit * p.beams, total = p.beams * per;
+    auto candidate = [&](int i, uint64_t& at) -> uint64_t {
+        const int b = i / per, j = i - b * per;
+        uint32_t token = (uint32_t)j;
+        double score = base[b];
+        if (kind[b] == kLives) {
+            const uint64_t c = p.cand[(row0 + b) * per + j];
+            if (!c) return 0;
+            token = ~(uint32_t)c;
+            score += (double)logit_of((uint32_t)(c >> 32));
+        } else if (kind[b] == kFinished) {
+            if (j) return 0;
+            token = (uint32_t)p.eos;
+        } else if (j >= p.beams || j >= p.vocab) {
+            return 0;
+        }
+        at = (uint64_t)b << 32 | token;
+        return ordered_score(score);
+    };
+    auto emit = [&](int k, uint64_t s, uint64_t at) {
+        const int b = (int)(at >> 32), token = (int)(uint32_t)at;
+        const int64_t o = row0 + k;
+        p.tokens[o] = token;
+        p.parents[o] = b;
+        p.scores_out[o] = (float)__longlong_as_double((long long)(s == 1 ? 0x7ff8000000000000ull
+                                                                  : s >> 63 ? s & ~(1ull << 63) : ~s));
+        if (p.finished_out) p.finished_out[o] = kind[b] == kFinished || token == p.eos;
+    };
+    uint32_t best = 0;
+    uint64_t at = 0;
+    for (int i = tid; i < total; i += 256) best = max(best, (uint32_t)(candidate(i, at) >> 32));
+    const uint32_t least = wave_nth(best, p.beams);
+    for (int i = tid; i < total; i += 256) {
+        const uint64_t s = candidate(i, at);
+        if (s && (uint32_t)(s >> 32) >= least) {
+            const int k = atomicAdd(&count, 1);
+            if (k < kBeamList) {
+                ls[k] = s;
+                lt[k] = at;
+            }
+        }
+    }
+    __syncthreads();
+    const int n = count;
+    if (n <= kBeamList) {
+        for (int i = tid; i < n; i += 256) {
+            const uint64_t s = ls[i], t = lt[i];
+            int better = 0;
+            for (int j = 0; j < n; ++j) better += ls[j] > s || (ls[j] == s && lt[j] < t);
+            if (better < p.beams) emit(better, s, t);
+        }
+        return;
+    }
+    uint64_t s0 = ~0ull, t0 = 0;  // the one picked last
+    for (int k = 0; k < p.beams; ++k) {
+        uint64_t s1 = 0, t1 = ~0ull;
+        for (int i = tid; i < total; i += 256) {
+            const uint64_t s = candidate(i, at);
+            if (s && (s < s0 || (s == s0 && at > t0)) && (s > s1 || (s == s1 && at < t1))) {
+                s1 = s;
+                t1 = at;
+            }
+        }
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) {
+            const uint64_t s = shfl_xor64(s1, m), t = shfl_xor64(t1, m);
+            if (s > s1 || (s == s1 && t < t1)) {
+                s1 = s;
+                t1 = t;
+            }
+        }
+        if (lane == 0) {
+            ws[wave] = s1;
+            wt[wave] = t1;
+        }
+        __syncthreads();
+        s0 = ws[0];
+        t0 = wt[0];
+        for (int w = 1; w < 4; ++w)
+            if (ws[w] > s0 || (ws[w] == s0 && wt[w] < t0)) {
+                s0 = ws[w];
+                t0 = wt[w];
+            }
+        if (tid == 0) emit(k, s0, t0);
+        __syncthreads();
+    }
+}
+
+void beam_select_plan(int64_t groups, int beams, int64_t vocab, int* nsplit, int64_t* chunk) {
+    int64_t ch = kBeamCols;
+    while (ch > 2048 && groups * beams * ((vocab + ch - 1) / ch) < 256) ch /= 2;
+    *chunk = ch;
+    *nsplit = (int)((vocab + 7 + ch - 1) / ch);  // a row starts up to 7 columns behind a 16-byte boundary
+}
+
+int launch_beam_select(const BeamSelectParams& p, int bf16, hipStream_t s) {
+    const dim3 grid((unsigned)(p.groups * p.beams * p.nsplit));
+    if (bf16)
+        hipLaunchKernelGGL(beam_part_kernel<BF16>, grid, dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL(beam_part_kernel<F32>, grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)p.groups), dim3(256), 0, s, p);
+    return (int)hipGetLastError();
+}
+
+}  // namespace inf

@@ -1,0 +1,315 @@
+// capi_paged.cpp -- the extern "C" entry points of generation from a paged
+// key-value cache (include/inferno_hip.h): argument validation on the host,
+// workspace sizing, launches.  Nothing here allocates.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+#include <utility>
+
+#include "inferno_hip.h"
+#include "kernels.h"
+
+namespace {
+
+constexpr size_t kAlign = 256;
+constexpr int64_t kMaxRowStride = int64_t(1) << 22;  // as the other attention views'
+constexpr int64_t kMaxBlocks = int64_t(1) << 30;
+
+bool dtype_ok(int dt) { return dt == INF_F32 || dt == INF_BF16; }
+int esz(inf_dtype dt) { return dt == INF_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+int hip_status(int e) { return e == 0 ? INF_OK : INF_ERR_HIP; }
+size_t round_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+inf::View4 view(const inf_strides& s) { return inf::View4{s.b, s.h, s.t}; }
+
+// Strides of a [b, h, t, D] view whose rows allow accesses of `bytes` bytes.
+int check_view(const void* p, const inf_strides& s, int es, int bytes) {
+    if (!p) return INF_ERR_NULL_POINTER;
+    if (s.d != 1 || s.b < 0 || s.h < 0 || s.t < 0 || s.t > kMaxRowStride) return INF_ERR_BAD_STRIDE;
+    const int64_t n = bytes / es;
+    if (!aligned(p, (size_t)bytes) || s.b % n || s.h % n || s.t % n) return INF_ERR_ALIGNMENT;
+    return INF_OK;
+}
+
+// Every element of a written view has an address of its own: ordered by stride, each is at
+// least the span of the dims inside it.
+int check_apart(const inf_strides& s, int64_t B, int64_t H, int64_t T, int64_t D, int64_t layers = 1,
+                int64_t layer_stride = 0) {
+    struct Dim { int64_t n, stride; } d[4] = {{layers, layer_stride}, {B, s.b}, {H, s.h}, {T, s.t}};
+    std::sort(d, d + 4, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+    int64_t span = D;
+    for (const Dim& x : d) {
+        if (x.n <= 1) continue;
+        if (x.stride < span) return INF_ERR_BAD_STRIDE;
+        span = x.stride * (x.n - 1) + span;
+    }
+    return INF_OK;
+}
+
+int check_shape(const inf_paged_kv* c) {
+    if (!c) return INF_ERR_NULL_POINTER;
+    if (!dtype_ok(c->dt)) return INF_ERR_BAD_DTYPE;
+    if (c->rows < 1 || c->heads < 1 || c->D < 1 || c->page_size < 1 || c->max_pages < 1 || c->n_pages < 1)
+        return INF_ERR_BAD_SHAPE;
+    if (c->D != 32 && c->D != 64 && c->D != 128) return INF_ERR_UNSUPPORTED;
+    if (c->page_size & (c->page_size - 1)) {
+        inf::set_error_detail("paged cache: page_size must be a power of two, got " + std::to_string(c->page_size));
+        return INF_ERR_UNSUPPORTED;
+    }
+    if (c->rows > 65535 || (int64_t)c->rows * c->heads > (1 << 24) ||
+        (int64_t)c->max_pages * c->page_size > (1 << 30))
+        return INF_ERR_BAD_SHAPE;
+    return INF_OK;
+}
+
+// The cache, for a call that reads it, or writes it too.
+int check_cache(const inf_paged_kv* c, bool written, inf::PagedView* out) {
+    int st = check_shape(c);
+    if (st != INF_OK) return st;
+    if ((st = check_view(c->k, c->sk, esz(c->dt), 16)) || (st = check_view(c->v, c->sv, esz(c->dt), 16))) return st;
+    if (!c->table || !c->lens) return INF_ERR_NULL_POINTER;
+    if (!aligned(c->table, 4) || !aligned(c->lens, 4)) return INF_ERR_ALIGNMENT;
+    if (c->table_stride < c->max_pages) return INF_ERR_BAD_STRIDE;
+    if (written && ((st = check_apart(c->sk, c->n_pages, c->heads, c->page_size, c->D)) ||
+                    (st = check_apart(c->sv, c->n_pages, c->heads, c->page_size, c->D))))
+        return st;
+    int shift = 0;
+    while ((1 << shift) < c->page_size) ++shift;
+    *out = inf::PagedView{c->k, c->v, view(c->sk), view(c->sv), c->table, c->lens, c->table_stride,
+                          c->rows, c->heads, c->n_pages, c->max_pages, shift, c->D};
+    return INF_OK;
+}
+
+int64_t capacity(const inf_paged_kv* c) { return (int64_t)c->max_pages * c->page_size; }
+
+// The part of the decode's workspace that holds the splits' results, and the scores behind it.
+struct DecodeSizes {
+    int nsplit, chunk;
+    int64_t score_ld;
+    size_t part, scores;
+};
+DecodeSizes decode_sizes(const inf_paged_kv* c, int q_heads, int max_len, bool weights) {
+    DecodeSizes s{};
+    inf::paged_decode_plan(c->rows, c->heads, q_heads / c->heads, max_len, c->D, c->dt == INF_BF16, &s.nsplit, &s.chunk);
+    s.score_ld = (int64_t)s.nsplit * s.chunk;
+    const size_t rows = (size_t)c->rows * q_heads;
+    if (s.nsplit > 1 || weights) s.part = round_up(rows * s.nsplit * (c->D + 2) * sizeof(float));
+    if (weights) s.scores = round_up(rows * s.score_ld * sizeof(float));
+    return s;
+}
+
+int check_decode(const inf_paged_kv* c, int q_heads, int max_len) {
+    const int st = check_shape(c);
+    if (st != INF_OK) return st;
+    if (q_heads < 1 || q_heads % c->heads || max_len < 1 || max_len > capacity(c)) return INF_ERR_BAD_SHAPE;
+    if ((int64_t)c->rows * q_heads > (1 << 24)) return INF_ERR_BAD_SHAPE;
+    return INF_OK;
+}
+
+int check_evict(const inf_paged_kv* c, int keep, int max_len) {
+    const int st = check_shape(c);
+    if (st != INF_OK) return st;
+    if (keep < 1 || max_len < 1 || max_len > capacity(c)) return INF_ERR_BAD_SHAPE;
+    return INF_OK;
+}
+
+int evict_moves(int keep, int max_len) { return std::max(0, std::min(keep, max_len - keep)); }
+
+int check_beams(int64_t groups, int beams, int64_t vocab) {
+    if (groups < 1 || beams < 1 || vocab < 1 || vocab > INT32_MAX) return INF_ERR_BAD_SHAPE;
+    if (beams > inf::kMaxBeams) {
+        inf::set_error_detail("beam selection: at most " + std::to_string(inf::kMaxBeams) + " beams, got " +
+                              std::to_string(beams));
+        return INF_ERR_UNSUPPORTED;
+    }
+    if (groups > (1 << 24)) return INF_ERR_BAD_SHAPE;
+    int ns = 0;
+    int64_t ch = 0;
+    inf::beam_select_plan(groups, beams, vocab, &ns, &ch);
+    return groups * beams * ns > kMaxBlocks ? INF_ERR_BAD_SHAPE : INF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int inf_kv_append(const inf_paged_kv* cache, const void* k, inf_strides sk, const void* v, inf_strides sv,
+                  const int32_t* counts, int T, float* weights, int32_t* positions, const int32_t* seen,
+                  void* stream) {
+    inf::KvAppendParams p{};
+    int st = check_cache(cache, true, &p.c);
+    if (st != INF_OK) return st;
+    if (T < 0) return INF_ERR_BAD_SHAPE;
+    if (T == 0) return INF_OK;
+    const int es = esz(cache->dt);
+    if ((st = check_view(k, sk, es, 4 * es)) || (st = check_view(v, sv, es, 4 * es))) return st;
+    if ((int64_t)T * cache->heads * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    p.k = k; p.v = v;
+    p.sk = view(sk); p.sv = view(sv);
+    p.counts = counts;
+    p.Tn = T;
+    p.wide = check_view(k, sk, es, 16) == INF_OK && check_view(v, sv, es, 16) == INF_OK;
+    p.weights = weights;
+    p.positions = positions;
+    p.seen = seen;
+    return hip_status(inf::launch_kv_append(p, cache->dt == INF_BF16, (hipStream_t)stream));
+}
+
+int inf_attn_decode_paged_workspace(const inf_paged_kv* cache, int q_heads, int max_len, int weights,
+                                    size_t* out_bytes) {
+    if (!out_bytes) return INF_ERR_NULL_POINTER;
+    *out_bytes = 0;
+    const int st = check_decode(cache, q_heads, max_len);
+    if (st != INF_OK) return st;
+    const DecodeSizes s = decode_sizes(cache, q_heads, max_len, weights != 0);
+    *out_bytes = s.part + s.scores;
+    return INF_OK;
+}
+
+int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides sq, void* o, inf_strides so,
+                          int q_heads, int max_len, float scale, const float* weights_in, float* weights_out,
+                          void* workspace, size_t ws_bytes, void* stream) {
+    inf::PagedDecodeParams p{};
+    int st = check_decode(cache, q_heads, max_len);
+    if (st != INF_OK || (st = check_cache(cache, false, &p.c))) return st;
+    if (!(scale > 0.f) || !std::isfinite(scale)) return INF_ERR_BAD_SCALE;
+    const int es = esz(cache->dt);
+    if ((st = check_view(q, sq, es, 4 * es)) || (st = check_view(o, so, es, 4 * es)) ||
+        (st = check_apart(so, cache->rows, q_heads, 1, cache->D)))
+        return st;
+    if (weights_in && !weights_out) return INF_ERR_NULL_POINTER;
+    const DecodeSizes s = decode_sizes(cache, q_heads, max_len, weights_out != nullptr);
+    const int64_t tiles = (q_heads / cache->heads + 15) / 16;
+    if ((int64_t)cache->rows * cache->heads * s.nsplit * tiles > kMaxBlocks ||
+        (int64_t)cache->rows * (q_heads + (int64_t)cache->heads * ((max_len + 1023) / 1024)) > kMaxBlocks)
+        return INF_ERR_BAD_SHAPE;
+    if (s.part + s.scores && (!workspace || ws_bytes < s.part + s.scores)) return INF_ERR_WORKSPACE;
+    if (s.part + s.scores && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
+    p.q = q; p.o = o;
+    p.sq = view(sq); p.so = view(so);
+    p.Hq = q_heads;
+    p.G = q_heads / cache->heads;
+    p.head_tiles = (int)tiles;
+    p.max_len = max_len;
+    p.nsplit = s.nsplit;
+    p.chunk = s.chunk;
+    p.cs = scale * 1.4426950408889634f;
+    p.part = static_cast<float*>(workspace);
+    if (weights_out) p.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + s.part);
+    p.score_ld = s.score_ld;
+    p.w_in = weights_in;
+    p.w_out = weights_out;
+    return hip_status(inf::launch_attn_decode_paged(p, cache->dt == INF_BF16, (hipStream_t)stream));
+}
+
+int inf_kv_evict_workspace(const inf_paged_kv* cache, int keep, int max_len, size_t* out_bytes) {
+    if (!out_bytes) return INF_ERR_NULL_POINTER;
+    *out_bytes = 0;
+    const int st = check_evict(cache, keep, max_len);
+    if (st != INF_OK) return st;
+    *out_bytes = round_up((size_t)cache->rows * cache->heads * (2 * (size_t)evict_moves(keep, max_len) + 1) * 4);
+    return INF_OK;
+}
+
+int inf_kv_evict(const inf_paged_kv* cache, const float* weights_in, float* weights_out, const int32_t* positions_in,
+                 int32_t* positions_out, int32_t* lens_out, int keep, int recent, int max_len, void* workspace,
+                 size_t ws_bytes, void* stream) {
+    inf::KvEvictParams p{};
+    int st = check_evict(cache, keep, max_len);
+    if (st != INF_OK || (st = check_cache(cache, true, &p.c))) return st;
+    if (recent < 0 || recent > keep) return INF_ERR_BAD_SHAPE;
+    if (!weights_in || !weights_out || !positions_in || !positions_out || !lens_out) return INF_ERR_NULL_POINTER;
+    size_t need = 0;
+    inf_kv_evict_workspace(cache, keep, max_len, &need);
+    if (!workspace || ws_bytes < need) return INF_ERR_WORKSPACE;
+    if (!aligned(workspace, 4)) return INF_ERR_ALIGNMENT;
+    p.w_in = weights_in; p.w_out = weights_out;
+    p.pos_in = positions_in; p.pos_out = positions_out;
+    p.lens_out = lens_out;
+    p.keep = keep; p.recent = recent; p.max_len = max_len;
+    p.moves = evict_moves(keep, max_len);
+    p.list = static_cast<int32_t*>(workspace);
+    if ((int64_t)cache->rows * cache->heads * (p.moves / 8 + 1) > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    return hip_status(inf::launch_kv_evict(p, cache->dt == INF_BF16, (hipStream_t)stream));
+}
+
+int inf_beam_select_workspace(int64_t groups, int beams, int64_t vocab, size_t* out_bytes) {
+    if (!out_bytes) return INF_ERR_NULL_POINTER;
+    *out_bytes = 0;
+    const int st = check_beams(groups, beams, vocab);
+    if (st != INF_OK) return st;
+    int ns = 0;
+    int64_t ch = 0;
+    inf::beam_select_plan(groups, beams, vocab, &ns, &ch);
+    const size_t parts = (size_t)groups * beams * ns;
+    *out_bytes = round_up(parts * 8) + round_up(parts * 8 * beams) + round_up(parts * 4);
+    return INF_OK;
+}
+
+int inf_beam_select(const void* logits, int64_t ld, const float* scores, const int32_t* finished, int64_t groups,
+                    int beams, int64_t vocab, int32_t eos, int32_t* tokens, int32_t* parents, float* scores_out,
+                    int32_t* finished_out, inf_dtype dt, void* workspace, size_t ws_bytes, void* stream) {
+    if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
+    const int st = check_beams(groups, beams, vocab);
+    if (st != INF_OK) return st;
+    if (!logits || !scores || !tokens || !parents || !scores_out) return INF_ERR_NULL_POINTER;
+    if (eos >= vocab || (finished && eos < 0)) return INF_ERR_BAD_SHAPE;
+    if (ld < vocab) return INF_ERR_BAD_STRIDE;
+    if (!aligned(logits, (size_t)esz(dt))) return INF_ERR_ALIGNMENT;
+    size_t need = 0;
+    inf_beam_select_workspace(groups, beams, vocab, &need);
+    if (!workspace || ws_bytes < need) return INF_ERR_WORKSPACE;
+    if (!aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
+    inf::BeamSelectParams p{};
+    p.logits = logits; p.scores = scores; p.finished = finished;
+    p.groups = groups; p.vocab = vocab; p.ld = ld;
+    p.beams = beams;
+    p.eos = eos < 0 ? -1 : eos;
+    inf::beam_select_plan(groups, beams, vocab, &p.nsplit, &p.chunk);
+    const size_t parts = (size_t)groups * beams * p.nsplit;
+    char* ws = static_cast<char*>(workspace);
+    p.sums = reinterpret_cast<double*>(ws);
+    p.cand = reinterpret_cast<uint64_t*>(ws + round_up(parts * 8));
+    p.maxs = reinterpret_cast<float*>(ws + round_up(parts * 8) + round_up(parts * 8 * beams));
+    p.tokens = tokens; p.parents = parents; p.scores_out = scores_out; p.finished_out = finished_out;
+    return hip_status(inf::launch_beam_select(p, dt == INF_BF16, (hipStream_t)stream));
+}
+
+int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stride, int64_t v_layer_stride,
+                     const int32_t* parents, int beams, int32_t* table_out, int64_t table_out_stride,
+                     const int32_t* spare, int32_t* spare_out, void* stream) {
+    inf::BeamReorderParams p{};
+    int st = check_cache(cache, true, &p.c);
+    if (st != INF_OK) return st;
+    if (layers < 1 || layers > 65535 || beams < 1 || cache->rows % beams) return INF_ERR_BAD_SHAPE;
+    if (!parents || !table_out || !spare || !spare_out) return INF_ERR_NULL_POINTER;
+    if (layers > 1) {
+        const int es = esz(cache->dt);
+        if (k_layer_stride < 0 || v_layer_stride < 0) return INF_ERR_BAD_STRIDE;
+        if (k_layer_stride * es % 16 || v_layer_stride * es % 16) return INF_ERR_ALIGNMENT;
+        if ((st = check_apart(cache->sk, cache->n_pages, cache->heads, cache->page_size, cache->D, layers,
+                              k_layer_stride)) ||
+            (st = check_apart(cache->sv, cache->n_pages, cache->heads, cache->page_size, cache->D, layers,
+                              v_layer_stride)))
+            return st;
+    }
+    if (table_out_stride < cache->max_pages) return INF_ERR_BAD_STRIDE;
+    // rows read the tables of other rows: the new ones lie elsewhere
+    const int32_t *t0 = cache->table, *t1 = t0 + (cache->rows - 1) * cache->table_stride + cache->max_pages;
+    const int32_t *u0 = table_out, *u1 = u0 + (cache->rows - 1) * table_out_stride + cache->max_pages;
+    if (t0 < u1 && u0 < t1) return INF_ERR_BAD_STRIDE;
+    if ((int64_t)cache->heads * cache->page_size * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    p.layers = layers;
+    p.beams = beams;
+    p.k_layer = k_layer_stride; p.v_layer = v_layer_stride;
+    p.parents = parents;
+    p.table_out = table_out;
+    p.table_out_stride = table_out_stride;
+    p.spare = spare; p.spare_out = spare_out;
+    return hip_status(inf::launch_beam_reorder(p, cache->dt == INF_BF16, (hipStream_t)stream));
+}
+
+}  // extern "C"

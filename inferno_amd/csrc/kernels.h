@@ -326,6 +326,102 @@ struct MaskedFill {       // element strides; mstride is the mask's, padded on t
 int launch_masked_fill(const void* in, const void* mask, void* out, const MaskedFill& m, int elem_bytes,
                        int mask_bytes, uint64_t fill_bits, hipStream_t s);
 
+// ---- generation from a paged key-value cache (paged.hip, beam.hip) ------------
+// Pools of pages [n_pages, heads, 1 << page_shift slots, D] through element strides
+// (View4's b is the page's), a table of page numbers per row and the rows' lengths, both in
+// device memory.  Kernels check every page number against n_pages before using it.
+struct PagedView {
+    void* k;
+    void* v;
+    View4 sk, sv;
+    const int32_t* table;  // [rows], table_stride elements apart
+    const int32_t* lens;   // [rows]
+    int64_t table_stride;
+    int rows, heads, n_pages, max_pages, page_shift, D;
+    __host__ __device__ int64_t cap() const { return (int64_t)max_pages << page_shift; }
+};
+
+struct KvAppendParams {
+    PagedView c;
+    const void* k;         // new keys [rows, heads, Tn, D]
+    const void* v;
+    View4 sk, sv;
+    const int32_t* counts;  // [rows] tokens of each row, or null: Tn
+    int Tn;
+    int wide;              // 16-byte rows on both sides (bf16; fp32 rows always are)
+    float* weights;        // [rows, heads, cap] or null
+    int32_t* positions;    // [rows, heads, cap] or null
+    const int32_t* seen;   // [rows] or null: the lengths
+};
+
+struct PagedDecodeParams {
+    PagedView c;
+    const void* q;
+    void* o;
+    View4 sq, so;
+    int Hq, G;             // query heads; of them per key-value head
+    int head_tiles;        // tiles of 16 query heads per key-value head
+    int max_len;
+    int nsplit, chunk;     // splits of a row, keys per split (a multiple of kPagedStep)
+    float cs;              // scale * log2(e)
+    float* part;           // workspace [rows * Hq, nsplit, D + 2]
+    float* scores;         // workspace [rows * Hq, score_ld] (weights asked for) or null
+    int64_t score_ld;
+    const float* w_in;     // [rows, heads, cap] or null (zeros)
+    float* w_out;          // [rows, heads, cap] or null
+};
+constexpr int kPagedStep = 128;      // keys a workgroup takes per step: 4 waves x 32
+constexpr int kPagedMaxSplit = 512;
+void paged_decode_plan(int rows, int heads, int G, int max_len, int D, int bf16, int* nsplit, int* chunk);
+
+struct KvEvictParams {
+    PagedView c;
+    const float* w_in;
+    float* w_out;
+    const int32_t* pos_in;
+    int32_t* pos_out;
+    int32_t* lens_out;
+    int keep, recent, max_len;
+    int moves;             // most moves of a (row, head): min(keep, max_len - keep)
+    int32_t* list;         // workspace [rows * heads][2 * moves + 1]: holes, sources (last first), their number
+};
+
+struct BeamSelectParams {
+    const void* logits;    // [groups * beams, vocab], row stride ld
+    const float* scores;   // [groups, beams]
+    const int32_t* finished;  // [groups, beams] or null
+    int64_t groups, vocab, ld;
+    int beams, eos;
+    int nsplit;
+    int64_t chunk;         // columns per split
+    double* sums;          // workspace [rows, nsplit]: sum of exp(x - max)
+    float* maxs;           // workspace [rows, nsplit]
+    uint64_t* cand;        // workspace [rows, nsplit, beams]: (ordered logit, ~column), best first
+    int32_t* tokens;
+    int32_t* parents;
+    float* scores_out;
+    int32_t* finished_out;  // or null
+};
+constexpr int kMaxBeams = 32;
+void beam_select_plan(int64_t groups, int beams, int64_t vocab, int* nsplit, int64_t* chunk);
+
+struct BeamReorderParams {
+    PagedView c;
+    int layers, beams;
+    int64_t k_layer, v_layer;  // elements from one layer's pool to the next one's
+    const int32_t* parents;    // [rows]: beam of the same group
+    int32_t* table_out;        // [rows], table_out_stride elements apart
+    int64_t table_out_stride;
+    const int32_t* spare;      // [rows]
+    int32_t* spare_out;        // [rows]
+};
+
+int launch_kv_append(const KvAppendParams& p, int bf16, hipStream_t s);
+int launch_attn_decode_paged(const PagedDecodeParams& p, int bf16, hipStream_t s);
+int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s);
+int launch_beam_select(const BeamSelectParams& p, int bf16, hipStream_t s);
+int launch_beam_reorder(const BeamReorderParams& p, int bf16, hipStream_t s);
+
 // Tile shapes the host needs for grids and workspace sizing.
 // Query rows per forward workgroup: 4 waves x 32 (bf16), 8 waves x 32 (fp32).
 constexpr int kFwdBM = 128;

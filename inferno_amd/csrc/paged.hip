@@ -1,0 +1,706 @@
+// paged.hip -- a key-value cache in pages: writing new tokens to it, attention of one new
+// token per row over it, eviction from it, and its reordering under beam search.
+//
+// Key j of a row lies in slot j % P of page table[row][j / P] (P a power of two), the same
+// page for every key-value head and for keys and values.  Page numbers come from device
+// memory, so each is checked against the pool's size before it is used: one out of range
+// is never followed (a store is dropped; attention makes the row NaN).
+#include <type_traits>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace inf {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+namespace {
+
+__device__ __forceinline__ f32x4 mfma16x16x32bf16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16x16x4(float a, float b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// The page that holds position j of a row, -1 where the table names none of the pool's.
+__device__ __forceinline__ int page_of(const PagedView& c, const int32_t* table, int j) {
+    const int p = table[j >> c.page_shift];
+    return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+}
+
+template <typename E>
+__device__ __forceinline__ void store1(E* dst, float v) {
+    if constexpr (sizeof(E) == 4)
+        *dst = v;
+    else
+        *dst = f32_to_bf16(v);
+}
+
+}  // namespace
+
+// ============================================================================
+// Append.  One thread per 16-byte piece (8-byte where bf16 rows are aligned to that only)
+// of a token's key and of its value, pieces of a row fastest, then heads, then tokens: the
+// source, a projection's output, is read in the order that it has, and each row of D
+// elements is one contiguous run on both sides.
+// ============================================================================
+template <int BYTES>
+__global__ __launch_bounds__(256) void kv_append_kernel(KvAppendParams p, int pieces, int esz) {
+    using V = typename std::conditional<BYTES == 16, u32x4, u32x2>::type;
+    const int row = blockIdx.y;
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const int th = i / pieces, c = i - th * pieces;
+    const int t = th / p.c.heads, h = th - t * p.c.heads;
+    const int count = p.counts ? min(p.counts[row], p.Tn) : p.Tn;
+    if (t >= count) return;
+    const int len = p.c.lens[row];
+    const int64_t slot = (int64_t)len - count + t;
+    if (slot < 0 || slot >= p.c.cap()) return;
+    const int page = page_of(p.c, p.c.table + row * p.c.table_stride, (int)slot);
+    if (page < 0) return;
+    const int in_page = (int)slot & ((1 << p.c.page_shift) - 1);
+    const char* ks = (const char*)p.k + (row * p.sk.b + h * p.sk.h + t * p.sk.t) * esz + c * BYTES;
+    const char* vs = (const char*)p.v + (row * p.sv.b + h * p.sv.h + t * p.sv.t) * esz + c * BYTES;
+    char* kd = (char*)p.c.k + (page * p.c.sk.b + h * p.c.sk.h + in_page * p.c.sk.t) * esz + c * BYTES;
+    char* vd = (char*)p.c.v + (page * p.c.sv.b + h * p.c.sv.h + in_page * p.c.sv.t) * esz + c * BYTES;
+    const V kx = *reinterpret_cast<const V*>(ks);
+    const V vx = *reinterpret_cast<const V*>(vs);
+    *reinterpret_cast<V*>(kd) = kx;
+    *reinterpret_cast<V*>(vd) = vx;
+    if (c == 0) {
+        const int64_t m = ((int64_t)row * p.c.heads + h) * p.c.cap() + slot;
+        if (p.weights) p.weights[m] = 0.f;
+        if (p.positions) p.positions[m] = p.seen ? p.seen[row] - count + t : (int)slot;
+    }
+}
+
+int launch_kv_append(const KvAppendParams& p, int bf16, hipStream_t s) {
+    const int esz = bf16 ? 2 : 4, bytes = p.wide ? 16 : 8;
+    const int pieces = p.c.D * esz / bytes;
+    const int64_t n = (int64_t)p.Tn * p.c.heads * pieces;
+    const dim3 grid((unsigned)((n + 255) / 256), (unsigned)p.c.rows);
+    if (p.wide)
+        hipLaunchKernelGGL((kv_append_kernel<16>), grid, dim3(256), 0, s, p, pieces, esz);
+    else
+        hipLaunchKernelGGL((kv_append_kernel<8>), grid, dim3(256), 0, s, p, pieces, esz);
+    return (int)hipGetLastError();
+}
+
+// ============================================================================
+// Attention of one query per row: s_j = q k_j scale, p = softmax(s), o = sum_j p_j v_j, for
+// the G query heads of a key-value head at once.
+//
+// A workgroup takes `chunk` keys of one (row, key-value head), its waves 32 keys in turn, all on
+// the matrix cores with up to 16 query heads as the columns: S^T = K Q^T (keys x heads), then
+// O^T += V^T P^T (D x heads).  A head's scores, maximum, sum and output then lie in one
+// lane column, so that the softmax needs two exchanges per 32 keys, and each lane's 8
+// probabilities are the second product's operand as they are: its sum over keys may
+// run in any order, so the value rows are loaded in the order that the first product's result
+// has.  A lane holds D / 16 neighbouring columns of 8 value rows; one column of them is one
+// operand (bf16: eight 16-bit halves picked together; fp32: a register each).  Neither operand
+// passes through LDS, and a row of K or V is read from HBM once for all heads.  bf16
+// probabilities are taken in two parts (16 bits), whose products cost no time here.
+//
+// Keys behind the end are read as the last one and their scores are -inf, their values zero, so
+// whatever their slots hold does not count.
+// ============================================================================
+template <int D, typename E, bool SMALL>
+__global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
+    constexpr int ES = sizeof(E);
+    constexpr int NK = D * ES / 64;       // 16-byte pieces of a key row per lane
+    constexpr int VD = D / 16;            // columns of a value row per lane
+    constexpr int VW = VD * ES / 4;       // ... in 32-bit words
+    constexpr int LD = D + 4;
+    extern __shared__ __attribute__((aligned(16))) float lds[];  // o [4][heads][LD], then m, l [4][16]
+
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    // the tiles of more than 16 query heads read the same keys: neighbours on one XCD
+    const int ht = p.head_tiles;
+    int unit = blockIdx.x, tile = 0;
+    if (ht > 1) {
+        const int grp = blockIdx.x >> 3;
+        tile = grp % ht;
+        unit = grp / ht * 8 + (blockIdx.x & 7);
+        if (unit >= p.c.rows * p.c.heads * p.nsplit) return;
+    }
+    const int split = unit % p.nsplit, rh = unit / p.nsplit;
+    const int row = rh / p.c.heads, h = rh % p.c.heads;
+    const int g0 = tile * 16, gn = min(16, p.G - g0);  // query heads of this tile
+    const bool direct = p.nsplit == 1 && !p.scores;
+    const int len = p.c.lens[row];
+    const int j0 = split * p.chunk;
+    const int j1 = len > p.max_len ? 0 : min(len, j0 + p.chunk);
+    if (j0 >= j1) {
+        if (direct)  // an empty row is 0, one longer than max_len NaN
+            for (int i = tid; i < gn * D; i += 256)
+                store1((E*)p.o + row * p.so.b + (h * p.G + g0 + i / D) * p.so.h + i % D,
+                       len > p.max_len ? __builtin_nanf("") : 0.f);
+        return;
+    }
+    const int32_t* table = p.c.table + row * p.c.table_stride;
+    const E* K = (const E*)p.c.k + h * p.c.sk.h;
+    const E* V = (const E*)p.c.v + h * p.c.sv.h;
+
+    // Q^T: column = head, rows 16 bytes of d as the key rows are read
+    u32x4 qf[NK];
+    {
+        const E* q = (const E*)p.q + row * p.sq.b + (int64_t)(h * p.G + g0 + min(col, gn - 1)) * p.sq.h;
+#pragma unroll
+        for (int s = 0; s < NK; ++s) {
+            const u32x2* src = reinterpret_cast<const u32x2*>((const char*)q + 64 * s + 16 * g);
+            const u32x2 a = src[0], b = src[1];
+            qf[s] = col < gn ? u32x4{a[0], a[1], b[0], b[1]} : u32x4{0, 0, 0, 0};
+        }
+    }
+
+    f32x4 acc[VD];
+#pragma unroll
+    for (int j = 0; j < VD; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    bool bad = false;
+    const int mask = (1 << p.c.page_shift) - 1;
+    float* sc = p.scores ? p.scores + ((int64_t)row * p.Hq + h * p.G + g0 + col) * p.score_ld : nullptr;
+
+    for (int base = j0 + 32 * wave; base < j1; base += kPagedStep) {
+        u32x4 kr[2][NK];
+        uint32_t vr[2][4][VW];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int b = __builtin_amdgcn_readfirstlane(min(base + 16 * t, j1 - 1));
+            // pages of 16 keys or more: one page for the 16 keys
+            int page = 0;
+            if constexpr (!SMALL) page = page_of(p.c, table, b);
+            {
+                const int key = min(base + 16 * t + col, j1 - 1);
+                int pg = page;
+                if constexpr (SMALL) pg = page_of(p.c, table, key);
+                bad |= pg < 0;
+                const char* src = (const char*)(K + max(pg, 0) * p.c.sk.b + (key & mask) * p.c.sk.t) + 16 * g;
+#pragma unroll
+                for (int s = 0; s < NK; ++s)
+                    kr[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + 64 * s));
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = min(base + 16 * t + 4 * g + r, j1 - 1);
+                int pg = page;
+                if constexpr (SMALL) pg = page_of(p.c, table, key);
+                const char* src = (const char*)(V + max(pg, 0) * p.c.sv.b + (key & mask) * p.c.sv.t + VD * col);
+                if constexpr (VW == 1) {
+                    vr[t][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(src));
+                } else if constexpr (VW == 2) {
+                    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(src));
+                    vr[t][r][0] = x[0];
+                    vr[t][r][1] = x[1];
+                } else {
+#pragma unroll
+                    for (int w = 0; w < VW; w += 4) {
+                        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + 4 * w));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) vr[t][r][w + e] = x[e];
+                    }
+                }
+            }
+        }
+        f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < NK; ++s) {
+                if constexpr (ES == 2) {
+                    st[t] = mfma16x16x32bf16(__builtin_bit_cast(bf16x8, kr[t][s]), __builtin_bit_cast(bf16x8, qf[s]),
+                                             st[t]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        st[t] = mfma16x16x4(__uint_as_float(kr[t][s][e]), __uint_as_float(qf[s][e]), st[t]);
+                }
+            }
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = st[i >> 2][i & 3] * p.cs;
+        if (base + 32 > j1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (base + 16 * (i >> 2) + 4 * g + (i & 3) >= j1) {
+                    x[i] = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) vr[i >> 2][i & 3][w] = 0;
+                }
+        }
+        if (sc && col < gn) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                *reinterpret_cast<f32x4*>(sc + base + 16 * t + 4 * g) =
+                    f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+        }
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
+        mx = fmaxf(mx, shfl_xor(mx, 16));
+        mx = max_xor32(mx);
+        const float ref = mx == -INFINITY ? 0.f : mx;  // no key above -inf yet: keep everything at 0
+        const float alpha = fast_exp2(m - ref);
+        m = mx;
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < VD; ++j) acc[j] *= alpha;
+        float pr[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            pr[i] = fast_exp2(x[i] - ref);
+            l += pr[i];
+        }
+        if constexpr (ES == 2) {
+            bf16x8 ph, pm;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                ph[i] = (__bf16)pr[i];
+                pm[i] = (__bf16)(pr[i] - (float)ph[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < VD; ++j) {
+                const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;  // high or low halves of two words
+                u32x4 a;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    a[i] = __builtin_amdgcn_perm(vr[i >> 1][2 * (i & 1) + 1][j >> 1], vr[i >> 1][2 * (i & 1)][j >> 1],
+                                                 sel);
+                acc[j] = mfma16x16x32bf16(__builtin_bit_cast(bf16x8, a), ph, acc[j]);
+                acc[j] = mfma16x16x32bf16(__builtin_bit_cast(bf16x8, a), pm, acc[j]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < VD; ++j)
+                    acc[j] = mfma16x16x4(__uint_as_float(vr[i >> 2][i & 3][j]), pr[i], acc[j]);
+        }
+    }
+
+    // Join the waves: lane (col, g) holds head col's o[VD (4 g + r) + j] in acc[j][r].
+    l += shfl_xor(l, 16);
+    l += shfl_xor(l, 32);
+    if (__any(bad)) l = __builtin_nanf("");
+    float* ms = lds + 4 * gn * LD;
+    float* ls = ms + 64;
+    if (col < gn) {
+        float* dst = lds + (wave * gn + col) * LD + 4 * VD * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < VD; ++j) dst[VD * r + j] = acc[j][r];
+    }
+    if (g == 0) {
+        ms[wave * 16 + col] = m;
+        ls[wave * 16 + col] = l;
+    }
+    __syncthreads();
+    for (int i = tid; i < gn * D; i += 256) {
+        const int head = i / D, d = i % D;
+        const float M = fmaxf(fmaxf(ms[head], ms[16 + head]), fmaxf(ms[32 + head], ms[48 + head]));
+        const float ref = M == -INFINITY ? 0.f : M;
+        float L = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float wt = fast_exp2(ms[w * 16 + head] - ref);
+            L += ls[w * 16 + head] * wt;
+            o += lds[(w * gn + head) * LD + d] * wt;
+        }
+        const int hq = h * p.G + g0 + head;
+        if (direct) {
+            store1((E*)p.o + row * p.so.b + hq * p.so.h + d, o / L);
+        } else {
+            float* out = p.part + (((int64_t)row * p.Hq + hq) * p.nsplit + split) * (D + 2);
+            out[d] = o;
+            if (d == 0) {
+                out[D] = M;
+                out[D + 1] = L;
+            }
+        }
+    }
+}
+
+// Joins the splits: the first rows * Hq workgroups write o, the others (where weights are asked
+// for) take 1024 positions of a (row, key-value head) each and add the heads' probabilities
+// exp2(score - max) / sum to the weights, in the order of the heads.
+template <int D, typename E>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, int wblocks) {
+    __shared__ float wsh[kPagedMaxSplit];
+    __shared__ float osh[256];
+    __shared__ float top[256], inv[256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int nout = p.c.rows * p.Hq;
+    if ((int)blockIdx.x < nout) {
+        const int row = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq;
+        const int len = p.c.lens[row];
+        E* out = (E*)p.o + row * p.so.b + hq * p.so.h;
+        if (len <= 0 || len > p.max_len) {
+            if (tid < D) store1(out + tid, len <= 0 ? 0.f : __builtin_nanf(""));
+            return;
+        }
+        const int ns = (len + p.chunk - 1) / p.chunk;
+        const float* part = p.part + (int64_t)blockIdx.x * p.nsplit * (D + 2);
+        float M = -INFINITY;
+        for (int i = lane; i < ns; i += 64) M = fmaxf(M, part[(int64_t)i * (D + 2) + D]);
+        M = wave_max(M);
+        const float ref = M == -INFINITY ? 0.f : M;
+        float L = 0.f;
+        for (int i = lane; i < ns; i += 64) {
+            const float w = fast_exp2(part[(int64_t)i * (D + 2) + D] - ref);
+            L += part[(int64_t)i * (D + 2) + D + 1] * w;
+            if (wave == 0) wsh[i] = w;
+        }
+        L = wave_sum(L);
+        __syncthreads();
+        constexpr int NG = 256 / D;
+        const int d = tid % D, grp = tid / D;
+        float o = 0.f;
+#pragma unroll 8
+        for (int i = grp; i < ns; i += NG) o += part[(int64_t)i * (D + 2) + d] * wsh[i];
+        osh[tid] = o;
+        __syncthreads();
+        if (tid < D) {
+            float r = osh[tid];
+#pragma unroll
+            for (int i = 1; i < NG; ++i) r += osh[tid + i * D];
+            store1(out + tid, r / L);
+        }
+        return;
+    }
+    const int b = blockIdx.x - nout;
+    const int rh = b / wblocks, j0 = (b % wblocks) * 1024;
+    const int row = rh / p.c.heads, h = rh % p.c.heads;
+    const int len = p.c.lens[row];
+    const int n = min(len, p.max_len);
+    if (j0 >= n) return;
+    const int ns = (n + p.chunk - 1) / p.chunk;
+    const int64_t hq0 = (int64_t)row * p.Hq + h * p.G;
+    const int64_t at = (int64_t)rh * p.c.cap() + j0;
+    float w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int j = tid + 256 * u;
+        w[u] = p.w_in && j0 + j < n ? p.w_in[at + j] : 0.f;
+    }
+    for (int h0 = 0; h0 < p.G; h0 += 256) {
+        const int gn = min(256, p.G - h0);
+        __syncthreads();
+        for (int i = wave; i < gn; i += 4) {  // a wave joins a head's splits
+            const float* part = p.part + (hq0 + h0 + i) * p.nsplit * (D + 2);
+            float M = -INFINITY, L = 0.f;
+            if (len <= p.max_len) {
+                for (int s = lane; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 2) + D]);
+                M = wave_max(M);
+                const float ref = M == -INFINITY ? 0.f : M;
+                for (int s = lane; s < ns; s += 64)
+                    L += part[(int64_t)s * (D + 2) + D + 1] * fast_exp2(part[(int64_t)s * (D + 2) + D] - ref);
+                L = wave_sum(L);
+            }
+            if (lane == 0) {
+                top[i] = M;
+                inv[i] = len > p.max_len || M == -INFINITY ? __builtin_nanf("") : 1.f / L;
+            }
+        }
+        __syncthreads();
+        for (int i = 0; i < gn; ++i) {
+            const float* sc = p.scores + (hq0 + h0 + i) * p.score_ld + j0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = tid + 256 * u;
+                if (j0 + j < n) w[u] += fast_exp2(sc[j] - top[i]) * inv[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int j = tid + 256 * u;
+        if (j0 + j < n) p.w_out[at + j] = w[u];
+    }
+}
+
+void paged_decode_plan(int rows, int heads, int G, int max_len, int D, int bf16, int* nsplit, int* chunk) {
+    const int64_t units = (int64_t)rows * heads * ((G + 15) / 16);
+    int64_t ch = (int64_t)(128 << 10) / (2 * D * (bf16 ? 2 : 4));
+    while (ch > kPagedStep && units * ((max_len + ch - 1) / ch) < 1024) ch /= 2;
+    if (ch < kPagedStep) ch = kPagedStep;
+    const int64_t least = ((int64_t)max_len + kPagedMaxSplit - 1) / kPagedMaxSplit;
+    if (ch < least) ch = least;
+    ch = (ch + kPagedStep - 1) / kPagedStep * kPagedStep;
+    *chunk = (int)ch;
+    *nsplit = (int)((max_len + ch - 1) / ch);
+}
+
+template <int D, typename E>
+static int launch_paged_t(const PagedDecodeParams& p, hipStream_t s) {
+    int64_t units = (int64_t)p.c.rows * p.c.heads * p.nsplit;
+    if (p.head_tiles > 1) units = (units + 7) / 8 * 8 * p.head_tiles;
+    const size_t lds = (size_t)(4 * (p.G < 16 ? p.G : 16) * (D + 4) + 128) * sizeof(float);
+    if (p.c.page_shift < 4)
+        hipLaunchKernelGGL((paged_split_kernel<D, E, true>), dim3((unsigned)units), dim3(256), lds, s, p);
+    else
+        hipLaunchKernelGGL((paged_split_kernel<D, E, false>), dim3((unsigned)units), dim3(256), lds, s, p);
+    if (p.nsplit > 1 || p.scores) {
+        const int wblocks = p.scores ? (p.max_len + 1023) / 1024 : 0;
+        const int64_t blocks = (int64_t)p.c.rows * p.Hq + (int64_t)p.c.rows * p.c.heads * wblocks;
+        hipLaunchKernelGGL((paged_join_kernel<D, E>), dim3((unsigned)blocks), dim3(256), 0, s, p, wblocks);
+    }
+    return (int)hipGetLastError();
+}
+
+int launch_attn_decode_paged(const PagedDecodeParams& p, int bf16, hipStream_t s) {
+    switch (p.c.D) {
+        case 32: return bf16 ? launch_paged_t<32, uint16_t>(p, s) : launch_paged_t<32, float>(p, s);
+        case 64: return bf16 ? launch_paged_t<64, uint16_t>(p, s) : launch_paged_t<64, float>(p, s);
+        case 128: return bf16 ? launch_paged_t<128, uint16_t>(p, s) : launch_paged_t<128, float>(p, s);
+        default: return (int)hipErrorInvalidValue;
+    }
+}
+
+// ============================================================================
+// Eviction.  A (row, head) with more than `keep` positions keeps the `recent` newest and, of
+// the others, those of the largest weights (equal ones: the lower slot).  One workgroup finds
+// the weight of the last one kept, by a radix select over the weights as ordered integers, and
+// lists the holes before the cut and the kept positions behind it; then every hole takes one
+// of those.  Attention does not mind the order of the keys, so nothing else moves: a
+// tenth of the cache evicted moves a tenth of it at most, where closing the gaps would move
+// nearly all.  No position is both read and written, so moves run in any order.
+// ============================================================================
+namespace {
+
+// Order of the floats as unsigned numbers (-0 as 0); NaN, below all, is 0.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0u;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+
+}  // namespace
+
+__global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictParams p) {
+    __shared__ uint32_t hist[2048];
+    __shared__ uint32_t wave_gt[kEvictWaves], wave_eq[kEvictWaves];
+    __shared__ uint32_t found[2];
+    __shared__ int newest[kEvictWaves];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int rh = blockIdx.x, row = rh / p.c.heads;
+    const int stored = p.c.lens[row], len = min(max(stored, 0), (int)p.c.cap());
+    const float* w = p.w_in + (int64_t)rh * p.c.cap();
+    const int32_t* pos = p.pos_in + (int64_t)rh * p.c.cap();
+    float* wo = p.w_out + (int64_t)rh * p.c.cap();
+    int32_t* po = p.pos_out + (int64_t)rh * p.c.cap();
+    int32_t* list = p.list + (int64_t)rh * (2 * p.moves + 1);
+    const int keep = p.keep;
+    if (len <= keep || stored > p.max_len) {
+        if (tid == 0) list[2 * p.moves] = 0;
+        if (wo != w)
+            for (int j = tid; j < len; j += kEvictThreads) wo[j] = w[j];
+        if (po != pos)
+            for (int j = tid; j < len; j += kEvictThreads) po[j] = pos[j];
+        return;
+    }
+    int top = INT32_MIN;
+    for (int j = tid; j < len; j += kEvictThreads) top = max(top, pos[j]);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) top = max(top, __shfl_xor(top, m, 64));
+    if (lane == 0) newest[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < kEvictWaves; ++i) top = max(top, newest[i]);
+    const int64_t safe = (int64_t)top - p.recent;  // positions past this one stay
+    auto key = [&](int j) { return (int64_t)pos[j] > safe ? 0xffffffffu : ordered(w[j]); };
+
+    // The keep-th largest key, eleven bits at a time from the top; `need` of those that share the
+    // bits found so far are kept.
+    uint32_t prefix = 0, need = (uint32_t)keep;
+    const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = shifts[pass], bins = 1 << widths[pass];
+        for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
+        __syncthreads();
+        for (int j = tid; j < len; j += kEvictThreads) {
+            const uint32_t k = key(j);
+            if (pass == 0 || (k >> (shift + widths[pass])) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {  // lane i: bins from the top, 32 each
+            const int per = bins / 64;
+            uint32_t mine = 0;
+            for (int i = 0; i < per; ++i) mine += hist[bins - 1 - (lane * per + i)];
+            uint32_t before = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t up = __shfl_up(before, d, 64);
+                if (lane >= d) before += up;
+            }
+            before -= mine;
+            if (before < need && before + mine >= need) {
+                for (int i = 0; i < per; ++i) {
+                    const uint32_t n = hist[bins - 1 - (lane * per + i)];
+                    if (before + n >= need) {
+                        found[0] = (prefix << widths[pass]) | (uint32_t)(bins - 1 - (lane * per + i));
+                        found[1] = need - before;
+                        break;
+                    }
+                    before += n;
+                }
+            }
+        }
+        __syncthreads();
+        prefix = found[0];
+        need = found[1];
+        __syncthreads();
+    }
+    const uint32_t last = prefix;  // `need` of the keys equal to it are kept, the lower slots
+
+    // Each wave walks one stretch of the slots; what the stretches before it hold comes first.
+    const int stretch = ((len + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64;
+    const int a = min(len, wave * stretch), b = min(len, a + stretch);
+    uint32_t gt = 0, eq = 0;
+    for (int j = a + lane; j < b; j += 64) {
+        const uint32_t k = key(j);
+        gt += k > last;
+        eq += k == last;
+    }
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        gt += __shfl_xor(gt, m, 64);
+        eq += __shfl_xor(eq, m, 64);
+    }
+    if (lane == 0) {
+        wave_gt[wave] = gt;
+        wave_eq[wave] = eq;
+    }
+    __syncthreads();
+    uint32_t eq_before = 0, kept_before = 0;
+    for (int i = 0; i < wave; ++i) {
+        const uint32_t e = wave_eq[i];
+        kept_before += wave_gt[i] + (eq_before < need ? min(e, need - eq_before) : 0u);
+        eq_before += e;
+    }
+    const uint64_t lower = (1ull << lane) - 1;
+    for (int j0 = a; j0 < b; j0 += 64) {
+        const int j = j0 + lane;
+        const uint32_t k = j < b ? key(j) : 0u;
+        const uint64_t same = __ballot(j < b && k == last);
+        const bool kept = j < b && (k > last || (k == last && eq_before + __popcll(same & lower) < need));
+        const uint64_t all = __ballot(kept);
+        const uint32_t before = kept_before + __popcll(all & lower);
+        if (j < b) {
+            if (j < keep) {
+                if (!kept) {
+                    list[j - before] = j;
+                } else {
+                    if (wo != w) wo[j] = w[j];
+                    if (po != pos) po[j] = pos[j];
+                }
+            } else if (kept) {
+                list[p.moves + (keep - 1 - (int)before)] = j;  // the last one kept comes first
+            }
+            // the holes before the cut: as many as kept ones behind it
+            if (j == keep) list[2 * p.moves] = keep - (int)before;
+        }
+        eq_before += __popcll(same);
+        kept_before += __popcll(all);
+    }
+}
+
+// Each move: a row of K, one of V, its weight and its position.
+__global__ __launch_bounds__(256) void kv_evict_move_kernel(KvEvictParams p, int pieces, int esz, int blocks) {
+    const int rh = blockIdx.x / blocks, row = rh / p.c.heads, h = rh % p.c.heads;
+    const int32_t* list = p.list + (int64_t)rh * (2 * p.moves + 1);
+    const int n = list[2 * p.moves];
+    const int per = 256 / pieces;  // moves per workgroup
+    const int i = (blockIdx.x % blocks) * per + threadIdx.x / pieces, c = threadIdx.x % pieces;
+    if (blockIdx.x % blocks == 0 && h == 0 && threadIdx.x == 0) {
+        const int len = p.c.lens[row];
+        p.lens_out[row] = len > p.keep && len <= p.max_len ? p.keep : len;
+    }
+    if (i >= n) return;
+    const int dst = list[i], src = list[p.moves + n - 1 - i];
+    const int32_t* table = p.c.table + row * p.c.table_stride;
+    const int pd = page_of(p.c, table, dst), ps = page_of(p.c, table, src);
+    const int mask = (1 << p.c.page_shift) - 1;
+    if (pd >= 0 && ps >= 0) {
+        const int64_t ko = h * p.c.sk.h, vo = h * p.c.sv.h;
+        const u32x4 kx = *reinterpret_cast<const u32x4*>(
+            (const char*)p.c.k + (ps * p.c.sk.b + ko + (src & mask) * p.c.sk.t) * esz + 16 * c);
+        const u32x4 vx = *reinterpret_cast<const u32x4*>(
+            (const char*)p.c.v + (ps * p.c.sv.b + vo + (src & mask) * p.c.sv.t) * esz + 16 * c);
+        *reinterpret_cast<u32x4*>((char*)p.c.k + (pd * p.c.sk.b + ko + (dst & mask) * p.c.sk.t) * esz + 16 * c) = kx;
+        *reinterpret_cast<u32x4*>((char*)p.c.v + (pd * p.c.sv.b + vo + (dst & mask) * p.c.sv.t) * esz + 16 * c) = vx;
+    }
+    if (c == 0) {
+        const int64_t at = (int64_t)rh * p.c.cap();
+        p.w_out[at + dst] = p.w_in[at + src];
+        p.pos_out[at + dst] = p.pos_in[at + src];
+    }
+}
+
+int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s) {
+    const int esz = bf16 ? 2 : 4, pieces = p.c.D * esz / 16, per = 256 / pieces;
+    const int blocks = p.moves ? (p.moves + per - 1) / per : 1;
+    const int64_t rh = (int64_t)p.c.rows * p.c.heads;
+    hipLaunchKernelGGL(kv_evict_select_kernel, dim3((unsigned)rh), dim3(kEvictThreads), 0, s, p);
+    hipLaunchKernelGGL(kv_evict_move_kernel, dim3((unsigned)(rh * blocks)), dim3(256), 0, s, p, pieces, esz, blocks);
+    return (int)hipGetLastError();
+}
+
+// ============================================================================
+// Reordering under beam search.  Full pages are only read from here on, so a beam takes its
+// parent's by number.  The last, partly filled page will be written by each beam on its own: a
+// beam that is not its own parent copies it into its spare page, and the page that it had becomes
+// its spare.  Nobody writes a page that another one reads, so one launch does it for all layers.
+// ============================================================================
+__global__ __launch_bounds__(256) void beam_reorder_kernel(BeamReorderParams p, int pieces, int esz) {
+    const int row = blockIdx.x, layer = blockIdx.y;
+    const int first = row / p.beams * p.beams;
+    const int len = min(max(p.c.lens[first], 0), (int)p.c.cap());
+    const int full = len >> p.c.page_shift, part = len & ((1 << p.c.page_shift) - 1);
+    const int pb = p.parents[row];
+    const bool ok = (unsigned)pb < (unsigned)p.beams;
+    const int parent = first + (ok ? pb : 0);
+    const int32_t* own = p.c.table + row * p.c.table_stride;
+    const int32_t* from = p.c.table + parent * p.c.table_stride;
+    const bool copy = ok && parent != row && part;
+    if (layer == 0 && blockIdx.z == 0) {
+        int32_t* out = p.table_out + row * p.table_out_stride;
+        for (int i = threadIdx.x; i < p.c.max_pages; i += 256) {
+            int v = own[i];
+            if (!ok && len) v = -1;  // no such parent: the row names no page, and reads as NaN
+            else if (i < full) v = from[i];
+            else if (i == full && copy) v = p.spare[row];
+            out[i] = v;
+        }
+        if (threadIdx.x == 0) p.spare_out[row] = copy ? own[full] : p.spare[row];
+    }
+    if (!copy) return;
+    const int src = from[full], dst = p.spare[row];
+    if ((unsigned)src >= (unsigned)p.c.n_pages || (unsigned)dst >= (unsigned)p.c.n_pages) return;
+    const int n = p.c.heads * part * pieces;
+    for (int i = blockIdx.z * 256 + threadIdx.x; i < n; i += 256 * gridDim.z) {
+        const int hs = i / pieces, c = i - hs * pieces;
+        const int h = hs / part, t = hs - h * part;
+        const int64_t ko = layer * p.k_layer + h * p.c.sk.h + t * p.c.sk.t;
+        const int64_t vo = layer * p.v_layer + h * p.c.sv.h + t * p.c.sv.t;
+        const u32x4 kx = *reinterpret_cast<const u32x4*>((const char*)p.c.k + (ko + src * p.c.sk.b) * esz + 16 * c);
+        const u32x4 vx = *reinterpret_cast<const u32x4*>((const char*)p.c.v + (vo + src * p.c.sv.b) * esz + 16 * c);
+        *reinterpret_cast<u32x4*>((char*)p.c.k + (ko + dst * p.c.sk.b) * esz + 16 * c) = kx;
+        *reinterpret_cast<u32x4*>((char*)p.c.v + (vo + dst * p.c.sv.b) * esz + 16 * c) = vx;
+    }
+}
+
+int launch_beam_reorder(const BeamReorderParams& p, int bf16, hipStream_t s) {
+    const int esz = bf16 ? 2 : 4, pieces = p.c.D * esz / 16;
+    // pieces of a whole page; a workgroup takes up to four rounds of them
+    const int64_t n = ((int64_t)p.c.heads * pieces << p.c.page_shift);
+    int64_t z = (n + 1023) / 1024;
+    if (z > 1024) z = 1024;
+    const dim3 grid((unsigned)p.c.rows, (unsigned)p.layers, (unsigned)z);
+    hipLaunchKernelGGL(beam_reorder_kernel, grid, dim3(256), 0, s, p, pieces, esz);
+    return (int)hipGetLastError();
+}
+
+}  // namespace inf
