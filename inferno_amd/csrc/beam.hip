@@ -19,7 +19,7 @@ namespace inf {
 
 namespace {
 
-constexpr int kBeamCols = 8192;  // columns of a workgroup at most: 32 per thread
+constexpr int kBeamCols = 8192;  // columns of a workgroup at most: 32 per thread, in registers
 constexpr int kBeamList = 1024;  // candidates in LDS; more of them (equal ones) are picked one by one
 
 // Order of the floats as unsigned numbers, -0 as 0, NaN below -inf; 0 stands for no value.
@@ -63,10 +63,11 @@ __device__ __forceinline__ bool beam_lives(const BeamSelectParams& p, int64_t ro
 
 }  // namespace
 
-template <typename E>
+// N: columns per thread, 256 N per workgroup.
+template <typename E, int N>
 __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
     using T = typename E::T;
-    constexpr int GE = 16 / sizeof(T), NV = kBeamCols / 256 / GE;  // columns of a 16-byte load, loads per thread
+    constexpr int GE = 16 / sizeof(T), NV = N / GE;  // columns of a 16-byte load, loads per thread
     __shared__ uint64_t list[kBeamList];
     __shared__ int count;
     __shared__ float wmax[4];
@@ -76,18 +77,19 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
     const int64_t row = blockIdx.x / p.nsplit;
     const int split = blockIdx.x % p.nsplit;
     if (!beam_lives(p, row)) return;
-    // columns counted from the 16-byte boundary at or before the row's start
+    // Columns counted from the 16-byte boundary at or before the row's start; this workgroup's, from
+    // its first one on, are those in [lo, hi).
     const T* x = (const T*)p.logits + row * p.ld;
     const int mis = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % GE);
-    const int64_t end = min((int64_t)(split + 1) * p.chunk, p.vocab + mis);
-    float v[NV * GE];
-    uint32_t lane_best = 0;
-    float mx = -INFINITY;
+    const int64_t c0 = (int64_t)split * (256 * N);
+    const int lo = split == 0 ? mis : 0, hi = (int)min((int64_t)(256 * N), p.vocab + mis - c0);
+    x += c0 - mis;
+    float v[N];  // columns outside are -inf
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-        const int64_t c = (int64_t)split * p.chunk + (int64_t)(u * 256 + tid) * GE;
-        if (c >= mis && c + GE <= end) {
-            const u32x4 raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + (c - mis)));
+        const int c = (u * 256 + tid) * GE;
+        if (c >= lo && c + GE <= hi) {
+            const u32x4 raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + c));
 #pragma unroll
             for (int e = 0; e < GE; ++e) {
                 if constexpr (sizeof(T) == 4)
@@ -97,27 +99,28 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < GE; ++e)
-                v[u * GE + e] = c + e >= mis && c + e < end ? E::ld(x + (c + e - mis)) : 0.f;
+            for (int e = 0; e < GE; ++e) v[u * GE + e] = c + e >= lo && c + e < hi ? E::ld(x + c + e) : -INFINITY;
         }
     }
-    auto column = [&](int i) { return (int64_t)split * p.chunk + (int64_t)(i / GE * 256 + tid) * GE + i % GE; };
-    auto there = [&](int i) { return column(i) >= mis && column(i) < end; };
+    auto column = [&](int i) { return (i / GE * 256 + tid) * GE + i % GE; };
     auto key = [&](int i) {
-        return (uint64_t)ordered_logit(v[i]) << 32 | (uint32_t)~(uint32_t)(column(i) - mis);
+        return (uint64_t)ordered_logit(v[i]) << 32 | (uint32_t)~(uint32_t)(c0 - mis + column(i));
     };
+    float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < NV * GE; ++i)
-        if (there(i)) {
-            mx = fmaxf(mx, v[i]);
-            lane_best = max(lane_best, ordered_logit(v[i]));
-        }
+    for (int i = 0; i < N; ++i) mx = fmaxf(mx, v[i]);
+    const uint32_t lane_best = ordered_logit(mx);
     mx = wave_max(mx);
     const float ref = mx == -INFINITY ? 0.f : mx;
+    // four terms in 32 bits, which are off by 2^-23 of them at most, all further in 64
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < NV * GE; ++i)
-        if (there(i)) sum += (double)fast_exp2((v[i] - ref) * kLog2e);
+    for (int i = 0; i < N; i += 4) {
+        float t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = fast_exp2((v[i + e] - ref) * kLog2e);
+        sum += (double)((t[0] + t[1]) + (t[2] + t[3]));
+    }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) sum += shfl_xor_d(sum, m);
     if (lane == 0) {
@@ -125,7 +128,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
         wsum[wave] = sum;
     }
     if (tid == 0) count = 0;
-    const uint32_t least = wave_nth(lane_best, p.beams);
+    const float least = logit_of(max(wave_nth(lane_best, p.beams), ordered_logit(-INFINITY)));
     __syncthreads();
     if (tid == 0) {
         const float M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
@@ -135,8 +138,8 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
         p.sums[blockIdx.x] = S;
     }
 #pragma unroll
-    for (int i = 0; i < NV * GE; ++i)
-        if (there(i) && ordered_logit(v[i]) >= least) {
+    for (int i = 0; i < N; ++i)
+        if (v[i] >= least && column(i) >= lo && column(i) < hi) {
             const int at = atomicAdd(&count, 1);
             if (at < kBeamList) list[at] = key(i);
         }
@@ -157,9 +160,9 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
     for (int k = 0; k < p.beams; ++k) {
         uint64_t best = 0;
 #pragma unroll
-        for (int i = 0; i < NV * GE; ++i) {
-            const uint64_t x = there(i) ? key(i) : 0;
-            if (x < before && x > best) best = x;
+        for (int i = 0; i < N; ++i) {
+            const uint64_t y = v[i] >= least && column(i) >= lo && column(i) < hi ? key(i) : 0;
+            if (y < before && y > best) best = y;
         }
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) best = max(best, shfl_xor64(best, m));
@@ -180,44 +183,48 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     __shared__ uint64_t ws[4], wt[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t row0 = (int64_t)blockIdx.x * p.beams;
+    const int per = p.nsplit * p.beams, total = p.beams * per;
+    // the candidates' logits and columns do not wait for the lse; usually all fit in registers
+    constexpr int U = 8;
+    const bool held = total <= 256 * U;
+    uint64_t cand[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        cand[u] = held && tid + 256 * u < total ? p.cand[row0 * per + tid + 256 * u] : 0;
     for (int b = wave; b < p.beams; b += 4) {
         const int64_t row = row0 + b;
-        if (!beam_lives(p, row)) {
-            if (lane == 0) {
-                base[b] = (double)p.scores[row];
-                kind[b] = p.finished && p.finished[row] ? kFinished : kFlat;
-            }
-            continue;
-        }
+        const float score = p.scores[row];
+        const bool finished = p.finished && p.finished[row];
         float M = -INFINITY;
-        for (int i = lane; i < p.nsplit; i += 64) M = fmaxf(M, p.maxs[row * p.nsplit + i]);
-        M = wave_max(M);
         double S = 0.0;
         for (int i = lane; i < p.nsplit; i += 64) {
             const float m = p.maxs[row * p.nsplit + i];
             const double s = p.sums[row * p.nsplit + i];
-            S += m == -INFINITY ? s : s * exp((double)m - (double)M);
+            const float top = fmaxf(M, m);
+            S = (M == -INFINITY ? S : S * exp((double)M - (double)top)) +
+                (m == -INFINITY ? s : s * exp((double)m - (double)top));
+            M = top;
         }
+        const float top = wave_max(M);
+        if (M != -INFINITY) S *= exp((double)M - (double)top);
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) S += shfl_xor_d(S, m);
         if (lane == 0) {
             // a NaN or +inf among the logits, or nothing above -inf: the sum is NaN, infinite or 0
-            const double lse = (double)M + log(S);
-            const bool fine = isfinite(lse);
-            base[b] = fine ? (double)p.scores[row] - lse : __longlong_as_double(0x7ff8000000000000ll);
-            kind[b] = fine ? kLives : kFlat;
+            const double lse = (double)top + log(S);
+            const bool lives = !finished && isfinite(score), fine = isfinite(lse);
+            base[b] = !lives ? (double)score : fine ? (double)score - lse : __longlong_as_double(0x7ff8000000000000ll);
+            kind[b] = finished ? kFinished : lives && fine ? kLives : kFlat;
         }
     }
     if (tid == 0) count = 0;
     __syncthreads();
     // Candidate i of the group: its score as an ordered number (0: there is none) and its place.
-    const int per = p.nsplit * p.beams, total = p.beams * per;
-    auto candidate = [&](int i, uint64_t& at) -> uint64_t {
+    auto candidate = [&](int i, uint64_t c, uint64_t& at) -> uint64_t {
         const int b = i / per, j = i - b * per;
         uint32_t token = (uint32_t)j;
         double score = base[b];
         if (kind[b] == kLives) {
-            const uint64_t c = p.cand[(row0 + b) * per + j];
             if (!c) return 0;
             token = ~(uint32_t)c;
             score += (double)logit_of((uint32_t)(c >> 32));
@@ -241,10 +248,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     };
     uint32_t best = 0;
     uint64_t at = 0;
-    for (int i = tid; i < total; i += 256) best = max(best, (uint32_t)(candidate(i, at) >> 32));
-    const uint32_t least = wave_nth(best, p.beams);
-    for (int i = tid; i < total; i += 256) {
-        const uint64_t s = candidate(i, at);
+    auto pick = [&](uint64_t s, uint32_t least) {
         if (s && (uint32_t)(s >> 32) >= least) {
             const int k = atomicAdd(&count, 1);
             if (k < kBeamList) {
@@ -252,6 +256,26 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
                 lt[k] = at;
             }
         }
+    };
+    if (held) {
+        uint64_t s[U], place[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = place[u] = 0;
+            if (tid + 256 * u < total) s[u] = candidate(tid + 256 * u, cand[u], place[u]);
+            best = max(best, (uint32_t)(s[u] >> 32));
+        }
+        const uint32_t least = wave_nth(best, p.beams);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            at = place[u];
+            pick(s[u], least);
+        }
+    } else {
+        for (int i = tid; i < total; i += 256)
+            best = max(best, (uint32_t)(candidate(i, p.cand[row0 * per + i], at) >> 32));
+        const uint32_t least = wave_nth(best, p.beams);
+        for (int i = tid; i < total; i += 256) pick(candidate(i, p.cand[row0 * per + i], at), least);
     }
     __syncthreads();
     const int n = count;
@@ -268,7 +292,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     for (int k = 0; k < p.beams; ++k) {
         uint64_t s1 = 0, t1 = ~0ull;
         for (int i = tid; i < total; i += 256) {
-            const uint64_t s = candidate(i, at);
+            const uint64_t s = candidate(i, p.cand[row0 * per + i], at);
             if (s && (s < s0 || (s == s0 && at > t0)) && (s > s1 || (s == s1 && at < t1))) {
                 s1 = s;
                 t1 = at;
@@ -299,6 +323,8 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     }
 }
 
+// Columns per workgroup: 8192, fewer (half the time of a workgroup, twice the parts to join) where the
+// device would not be filled.
 void beam_select_plan(int64_t groups, int beams, int64_t vocab, int* nsplit, int64_t* chunk) {
     int64_t ch = kBeamCols;
     while (ch > 2048 && groups * beams * ((vocab + ch - 1) / ch) < 256) ch /= 2;
@@ -306,14 +332,20 @@ void beam_select_plan(int64_t groups, int beams, int64_t vocab, int* nsplit, int
     *nsplit = (int)((vocab + 7 + ch - 1) / ch);  // a row starts up to 7 columns behind a 16-byte boundary
 }
 
-int launch_beam_select(const BeamSelectParams& p, int bf16, hipStream_t s) {
+template <typename E>
+static int launch_select_t(const BeamSelectParams& p, hipStream_t s) {
     const dim3 grid((unsigned)(p.groups * p.beams * p.nsplit));
-    if (bf16)
-        hipLaunchKernelGGL(beam_part_kernel<BF16>, grid, dim3(256), 0, s, p);
-    else
-        hipLaunchKernelGGL(beam_part_kernel<F32>, grid, dim3(256), 0, s, p);
+    switch (p.chunk) {
+        case 2048: hipLaunchKernelGGL((beam_part_kernel<E, 8>), grid, dim3(256), 0, s, p); break;
+        case 4096: hipLaunchKernelGGL((beam_part_kernel<E, 16>), grid, dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((beam_part_kernel<E, 32>), grid, dim3(256), 0, s, p); break;
+    }
     hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)p.groups), dim3(256), 0, s, p);
     return (int)hipGetLastError();
+}
+
+int launch_beam_select(const BeamSelectParams& p, int bf16, hipStream_t s) {
+    return bf16 ? launch_select_t<BF16>(p, s) : launch_select_t<F32>(p, s);
 }
 
 }  // namespace inf

@@ -89,14 +89,18 @@ int64_t capacity(const inf_paged_kv* c) { return (int64_t)c->max_pages * c->page
 struct DecodeSizes {
     int nsplit, chunk;
     int64_t score_ld;
-    size_t part, scores;
+    size_t part, stats, scores;
+    size_t total() const { return part + stats + scores; }
 };
 DecodeSizes decode_sizes(const inf_paged_kv* c, int q_heads, int max_len, bool weights) {
     DecodeSizes s{};
     inf::paged_decode_plan(c->rows, c->heads, q_heads / c->heads, max_len, c->D, c->dt == INF_BF16, &s.nsplit, &s.chunk);
     s.score_ld = (int64_t)s.nsplit * s.chunk;
     const size_t rows = (size_t)c->rows * q_heads;
-    if (s.nsplit > 1 || weights) s.part = round_up(rows * s.nsplit * (c->D + 2) * sizeof(float));
+    if (s.nsplit > 1 || weights) {
+        s.part = round_up(rows * s.nsplit * c->D * sizeof(float));
+        s.stats = round_up(rows * s.nsplit * 2 * sizeof(float));
+    }
     if (weights) s.scores = round_up(rows * s.score_ld * sizeof(float));
     return s;
 }
@@ -165,7 +169,7 @@ int inf_attn_decode_paged_workspace(const inf_paged_kv* cache, int q_heads, int 
     const int st = check_decode(cache, q_heads, max_len);
     if (st != INF_OK) return st;
     const DecodeSizes s = decode_sizes(cache, q_heads, max_len, weights != 0);
-    *out_bytes = s.part + s.scores;
+    *out_bytes = s.total();
     return INF_OK;
 }
 
@@ -186,8 +190,8 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
     if ((int64_t)cache->rows * cache->heads * s.nsplit * tiles > kMaxBlocks ||
         (int64_t)cache->rows * (q_heads + (int64_t)cache->heads * ((max_len + 1023) / 1024)) > kMaxBlocks)
         return INF_ERR_BAD_SHAPE;
-    if (s.part + s.scores && (!workspace || ws_bytes < s.part + s.scores)) return INF_ERR_WORKSPACE;
-    if (s.part + s.scores && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
+    if (s.total() && (!workspace || ws_bytes < s.total())) return INF_ERR_WORKSPACE;
+    if (s.total() && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
     p.q = q; p.o = o;
     p.sq = view(sq); p.so = view(so);
     p.Hq = q_heads;
@@ -197,8 +201,10 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
     p.nsplit = s.nsplit;
     p.chunk = s.chunk;
     p.cs = scale * 1.4426950408889634f;
-    p.part = static_cast<float*>(workspace);
-    if (weights_out) p.scores = reinterpret_cast<float*>(static_cast<char*>(workspace) + s.part);
+    char* ws = static_cast<char*>(workspace);
+    p.part = reinterpret_cast<float*>(ws);
+    p.stats = reinterpret_cast<float*>(ws + s.part);
+    if (weights_out) p.scores = reinterpret_cast<float*>(ws + s.part + s.stats);
     p.score_ld = s.score_ld;
     p.w_in = weights_in;
     p.w_out = weights_out;

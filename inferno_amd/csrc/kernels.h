@@ -364,7 +364,8 @@ struct PagedDecodeParams {
     int max_len;
     int nsplit, chunk;     // splits of a row, keys per split (a multiple of kPagedStep)
     float cs;              // scale * log2(e)
-    float* part;           // workspace [rows * Hq, nsplit, D + 2]
+    float* part;           // workspace [rows * Hq, nsplit, D]: unnormalised o
+    float* stats;          // workspace [rows * Hq, nsplit, 2]: maximum (log2 domain) and sum
     float* scores;         // workspace [rows * Hq, score_ld] (weights asked for) or null
     int64_t score_ld;
     const float* w_in;     // [rows, heads, cap] or null (zeros)

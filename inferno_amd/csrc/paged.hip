@@ -13,6 +13,7 @@
 namespace inf {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 namespace {
 
@@ -124,12 +125,25 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
         unit = grp / ht * 8 + (blockIdx.x & 7);
         if (unit >= p.c.rows * p.c.heads * p.nsplit) return;
     }
-    const int split = unit % p.nsplit, rh = unit / p.nsplit;
-    const int row = rh / p.c.heads, h = rh % p.c.heads;
+    const int h = unit % p.c.heads, rs = unit / p.c.heads;
+    const int split = rs % p.nsplit, row = rs / p.nsplit;
     const int g0 = tile * 16, gn = min(16, p.G - g0);  // query heads of this tile
     const bool direct = p.nsplit == 1 && !p.scores;
-    const int len = p.c.lens[row];
-    const int j0 = split * p.chunk;
+    const int32_t* table = p.c.table + row * p.c.table_stride;
+    const int j0 = split * p.chunk, base0 = j0 + 32 * wave, last_page = p.c.max_pages - 1;
+    // Pages of 16 keys or more: one page for each half of a step, the same for all lanes, read a step
+    // ahead (behind the end, where the table may hold anything, they are not used).
+    int len = p.c.lens[row];
+    int next[2] = {0, 0};
+    auto read_pages = [&](int base) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            next[t] = table[min(__builtin_amdgcn_readfirstlane(base + 16 * t) >> p.c.page_shift, last_page)];
+    };
+    if constexpr (!SMALL) {
+        read_pages(base0);
+        asm volatile("" : "+s"(len), "+s"(next[0]), "+s"(next[1]));  // both waits at once
+    }
     const int j1 = len > p.max_len ? 0 : min(len, j0 + p.chunk);
     if (j0 >= j1) {
         if (direct)  // an empty row is 0, one longer than max_len NaN
@@ -138,7 +152,6 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
                        len > p.max_len ? __builtin_nanf("") : 0.f);
         return;
     }
-    const int32_t* table = p.c.table + row * p.c.table_stride;
     const E* K = (const E*)p.c.k + h * p.c.sk.h;
     const E* V = (const E*)p.c.v + h * p.c.sv.h;
 
@@ -162,31 +175,41 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
     const int mask = (1 << p.c.page_shift) - 1;
     float* sc = p.scores ? p.scores + ((int64_t)row * p.Hq + h * p.G + g0 + col) * p.score_ld : nullptr;
 
-    for (int base = j0 + 32 * wave; base < j1; base += kPagedStep) {
-        u32x4 kr[2][NK];
-        uint32_t vr[2][4][VW];
+    u32x4 kr[2][NK];
+    uint32_t vr[2][4][VW];
+    for (int base = base0; base < j1; base += kPagedStep) {
+        // rows behind the end are read as the last key's
+        int page[2] = {next[0], next[1]};
+        if constexpr (!SMALL) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const bool in = (unsigned)page[t] < (unsigned)p.c.n_pages;
+                bad |= !in && base + 16 * t < j1;
+                page[t] = in ? page[t] : 0;
+            }
+            if (base + kPagedStep < j1) read_pages(base + kPagedStep);
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int b = __builtin_amdgcn_readfirstlane(min(base + 16 * t, j1 - 1));
-            // pages of 16 keys or more: one page for the 16 keys
-            int page = 0;
-            if constexpr (!SMALL) page = page_of(p.c, table, b);
-            {
-                const int key = min(base + 16 * t + col, j1 - 1);
-                int pg = page;
-                if constexpr (SMALL) pg = page_of(p.c, table, key);
+            const int key = min(base + 16 * t + col, j1 - 1);
+            int pg = page[t];
+            if constexpr (SMALL) {
+                pg = page_of(p.c, table, key);
                 bad |= pg < 0;
-                const char* src = (const char*)(K + max(pg, 0) * p.c.sk.b + (key & mask) * p.c.sk.t) + 16 * g;
-#pragma unroll
-                for (int s = 0; s < NK; ++s)
-                    kr[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + 64 * s));
+                pg = max(pg, 0);
             }
+            const char* src = (const char*)(K + pg * p.c.sk.b + (key & mask) * p.c.sk.t) + 16 * g;
+#pragma unroll
+            for (int s = 0; s < NK; ++s)
+                kr[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + 64 * s));
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int key = min(base + 16 * t + 4 * g + r, j1 - 1);
-                int pg = page;
-                if constexpr (SMALL) pg = page_of(p.c, table, key);
-                const char* src = (const char*)(V + max(pg, 0) * p.c.sv.b + (key & mask) * p.c.sv.t + VD * col);
+                const int pg = SMALL ? max(page_of(p.c, table, key), 0) : page[t];
+                const char* src = (const char*)(V + pg * p.c.sv.b + (key & mask) * p.c.sv.t + VD * col);
                 if constexpr (VW == 1) {
                     vr[t][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(src));
                 } else if constexpr (VW == 2) {
@@ -202,7 +225,7 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
                     }
                 }
             }
-        }
+        __builtin_amdgcn_sched_barrier(0);  // all of the step's loads before its first product
         f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -312,12 +335,9 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
         if (direct) {
             store1((E*)p.o + row * p.so.b + hq * p.so.h + d, o / L);
         } else {
-            float* out = p.part + (((int64_t)row * p.Hq + hq) * p.nsplit + split) * (D + 2);
-            out[d] = o;
-            if (d == 0) {
-                out[D] = M;
-                out[D + 1] = L;
-            }
+            const int64_t at = ((int64_t)row * p.Hq + hq) * p.nsplit + split;
+            p.part[at * D + d] = o;
+            if (d == 0) *reinterpret_cast<f32x2*>(p.stats + 2 * at) = f32x2{M, L};
         }
     }
 }
@@ -326,10 +346,10 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
 // for) take 1024 positions of a (row, key-value head) each and add the heads' probabilities
 // exp2(score - max) / sum to the weights, in the order of the heads.
 template <int D, typename E>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, int wblocks) {
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, int wblocks, int wide) {
     __shared__ float wsh[kPagedMaxSplit];
     __shared__ float osh[256];
-    __shared__ float top[256], inv[256];
+    __shared__ float top[8], inv[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nout = p.c.rows * p.Hq;
     if ((int)blockIdx.x < nout) {
@@ -341,15 +361,17 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
             return;
         }
         const int ns = (len + p.chunk - 1) / p.chunk;
-        const float* part = p.part + (int64_t)blockIdx.x * p.nsplit * (D + 2);
+        const float* part = p.part + (int64_t)blockIdx.x * p.nsplit * D;
+        const f32x2* stats = reinterpret_cast<const f32x2*>(p.stats) + (int64_t)blockIdx.x * p.nsplit;
         float M = -INFINITY;
-        for (int i = lane; i < ns; i += 64) M = fmaxf(M, part[(int64_t)i * (D + 2) + D]);
+        for (int i = lane; i < ns; i += 64) M = fmaxf(M, stats[i][0]);
         M = wave_max(M);
         const float ref = M == -INFINITY ? 0.f : M;
         float L = 0.f;
         for (int i = lane; i < ns; i += 64) {
-            const float w = fast_exp2(part[(int64_t)i * (D + 2) + D] - ref);
-            L += part[(int64_t)i * (D + 2) + D + 1] * w;
+            const f32x2 x = stats[i];
+            const float w = fast_exp2(x[0] - ref);
+            L += x[1] * w;
             if (wave == 0) wsh[i] = w;
         }
         L = wave_sum(L);
@@ -358,7 +380,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
         const int d = tid % D, grp = tid / D;
         float o = 0.f;
 #pragma unroll 8
-        for (int i = grp; i < ns; i += NG) o += part[(int64_t)i * (D + 2) + d] * wsh[i];
+        for (int i = grp; i < ns; i += NG) o += part[(int64_t)i * D + d] * wsh[i];
         osh[tid] = o;
         __syncthreads();
         if (tid < D) {
@@ -377,52 +399,57 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
     if (j0 >= n) return;
     const int ns = (n + p.chunk - 1) / p.chunk;
     const int64_t hq0 = (int64_t)row * p.Hq + h * p.G;
-    const int64_t at = (int64_t)rh * p.c.cap() + j0;
-    float w[4];
+    const int j = j0 + 4 * tid;  // this thread's 4 positions; scores are padded to whole steps
+    f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 8;         // heads whose scores are loaded together
+    for (int h0 = 0; h0 < p.G; h0 += U) {
+        const int gn = min(U, p.G - h0);
+        f32x4 sc[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int j = tid + 256 * u;
-        w[u] = p.w_in && j0 + j < n ? p.w_in[at + j] : 0.f;
-    }
-    for (int h0 = 0; h0 < p.G; h0 += 256) {
-        const int gn = min(256, p.G - h0);
+        for (int i = 0; i < U; ++i)
+            if (i < gn && j < n)
+                sc[i] = *reinterpret_cast<const f32x4*>(p.scores + (hq0 + h0 + i) * p.score_ld + j);
         __syncthreads();
         for (int i = wave; i < gn; i += 4) {  // a wave joins a head's splits
-            const float* part = p.part + (hq0 + h0 + i) * p.nsplit * (D + 2);
+            const f32x2* stats = reinterpret_cast<const f32x2*>(p.stats) + (hq0 + h0 + i) * p.nsplit;
+            f32x2 x[kPagedMaxSplit / 64];
             float M = -INFINITY, L = 0.f;
-            if (len <= p.max_len) {
-                for (int s = lane; s < ns; s += 64) M = fmaxf(M, part[(int64_t)s * (D + 2) + D]);
-                M = wave_max(M);
-                const float ref = M == -INFINITY ? 0.f : M;
-                for (int s = lane; s < ns; s += 64)
-                    L += part[(int64_t)s * (D + 2) + D + 1] * fast_exp2(part[(int64_t)s * (D + 2) + D] - ref);
-                L = wave_sum(L);
+#pragma unroll
+            for (int u = 0; u < kPagedMaxSplit / 64; ++u) {
+                x[u] = lane + 64 * u < ns ? stats[lane + 64 * u] : f32x2{-INFINITY, 0.f};
+                M = fmaxf(M, x[u][0]);
             }
+            M = wave_max(M);
+            const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int u = 0; u < kPagedMaxSplit / 64; ++u) L += x[u][1] * fast_exp2(x[u][0] - ref);
+            L = wave_sum(L);
             if (lane == 0) {
                 top[i] = M;
                 inv[i] = len > p.max_len || M == -INFINITY ? __builtin_nanf("") : 1.f / L;
             }
         }
         __syncthreads();
-        for (int i = 0; i < gn; ++i) {
-            const float* sc = p.scores + (hq0 + h0 + i) * p.score_ld + j0;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int j = tid + 256 * u;
-                if (j0 + j < n) w[u] += fast_exp2(sc[j] - top[i]) * inv[i];
-            }
-        }
+        for (int i = 0; i < U; ++i)
+            if (i < gn)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] += fast_exp2(sc[i][e] - top[i]) * inv[i];
     }
+    const int64_t at = (int64_t)rh * p.c.cap() + j;
+    if (j + 4 <= n && p.c.cap() % 4 == 0 && wide) {
+        if (p.w_in) w += *reinterpret_cast<const f32x4*>(p.w_in + at);
+        *reinterpret_cast<f32x4*>(p.w_out + at) = w;
+    } else {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int j = tid + 256 * u;
-        if (j0 + j < n) p.w_out[at + j] = w[u];
+        for (int e = 0; e < 4; ++e)
+            if (j + e < n) p.w_out[at + e] = w[e] + (p.w_in ? p.w_in[at + e] : 0.f);
     }
 }
 
 void paged_decode_plan(int rows, int heads, int G, int max_len, int D, int bf16, int* nsplit, int* chunk) {
     const int64_t units = (int64_t)rows * heads * ((G + 15) / 16);
-    int64_t ch = (int64_t)(128 << 10) / (2 * D * (bf16 ? 2 : 4));
+    int64_t ch = (int64_t)(256 << 10) / (2 * D * (bf16 ? 2 : 4));
     while (ch > kPagedStep && units * ((max_len + ch - 1) / ch) < 1024) ch /= 2;
     if (ch < kPagedStep) ch = kPagedStep;
     const int64_t least = ((int64_t)max_len + kPagedMaxSplit - 1) / kPagedMaxSplit;
@@ -443,8 +470,9 @@ static int launch_paged_t(const PagedDecodeParams& p, hipStream_t s) {
         hipLaunchKernelGGL((paged_split_kernel<D, E, false>), dim3((unsigned)units), dim3(256), lds, s, p);
     if (p.nsplit > 1 || p.scores) {
         const int wblocks = p.scores ? (p.max_len + 1023) / 1024 : 0;
+        const int wide = reinterpret_cast<uintptr_t>(p.w_in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w_out) % 16 == 0;
         const int64_t blocks = (int64_t)p.c.rows * p.Hq + (int64_t)p.c.rows * p.c.heads * wblocks;
-        hipLaunchKernelGGL((paged_join_kernel<D, E>), dim3((unsigned)blocks), dim3(256), 0, s, p, wblocks);
+        hipLaunchKernelGGL((paged_join_kernel<D, E>), dim3((unsigned)blocks), dim3(256), 0, s, p, wblocks, wide);
     }
     return (int)hipGetLastError();
 }
@@ -480,11 +508,14 @@ constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
 
 }  // namespace
 
+// N: slots per thread at most, held as keys in registers; 0: more than 65536 slots, read again in every
+// pass.  Wave w's are one stretch of the slots, 64 at a time, so that what comes before a slot is the
+// waves before, the rounds before and the lanes before.
+template <int N>
 __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictParams p) {
     __shared__ uint32_t hist[2048];
-    __shared__ uint32_t wave_gt[kEvictWaves], wave_eq[kEvictWaves];
+    __shared__ uint32_t part[kEvictWaves], part2[kEvictWaves];
     __shared__ uint32_t found[2];
-    __shared__ int newest[kEvictWaves];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int rh = blockIdx.x, row = rh / p.c.heads;
     const int stored = p.c.lens[row], len = min(max(stored, 0), (int)p.c.cap());
@@ -502,93 +533,137 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictP
             for (int j = tid; j < len; j += kEvictThreads) po[j] = pos[j];
         return;
     }
+    const int rounds = (len + kEvictThreads - 1) / kEvictThreads;
+    const int first = wave * rounds * 64 + lane;  // this lane's slots: first + 64 i < len
+    uint32_t keys[N ? N : 1];
     int top = INT32_MIN;
-    for (int j = tid; j < len; j += kEvictThreads) top = max(top, pos[j]);
+    auto each = [&](auto&& f) {  // f(round): the rounds of this wave
+        if constexpr (N > 0) {
 #pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) top = max(top, __shfl_xor(top, m, 64));
-    if (lane == 0) newest[wave] = top;
-    __syncthreads();
-    for (int i = 0; i < kEvictWaves; ++i) top = max(top, newest[i]);
-    const int64_t safe = (int64_t)top - p.recent;  // positions past this one stay
-    auto key = [&](int j) { return (int64_t)pos[j] > safe ? 0xffffffffu : ordered(w[j]); };
-
-    // The keep-th largest key, eleven bits at a time from the top; `need` of those that share the
-    // bits found so far are kept.
-    uint32_t prefix = 0, need = (uint32_t)keep;
-    const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
-    for (int pass = 0; pass < 3; ++pass) {
-        const int shift = shifts[pass], bins = 1 << widths[pass];
-        for (int i = tid; i < 2048; i += kEvictThreads) hist[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < len; j += kEvictThreads) {
-            const uint32_t k = key(j);
-            if (pass == 0 || (k >> (shift + widths[pass])) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+            for (int i = 0; i < N; ++i)
+                if (i < rounds) f(i);
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < rounds; ++i) f(i);
         }
+    };
+    each([&](int i) {
+        const int j = first + 64 * i;
+        if constexpr (N > 0) keys[i] = j < len ? ordered(w[j]) : 0u;
+        if (p.recent && j < len) top = max(top, pos[j]);
+    });
+    hist[tid] = 0;
+    hist[tid + kEvictThreads] = 0;
+    if (p.recent) {
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) top = max(top, __shfl_xor(top, m, 64));
+        if (lane == 0) part[wave] = (uint32_t)top;
         __syncthreads();
-        if (wave == 0) {  // lane i: bins from the top, 32 each
-            const int per = bins / 64;
-            uint32_t mine = 0;
-            for (int i = 0; i < per; ++i) mine += hist[bins - 1 - (lane * per + i)];
-            uint32_t before = mine;
+        for (int i = 0; i < kEvictWaves; ++i) top = max(top, (int)part[i]);
+    }
+    const int64_t safe = p.recent ? (int64_t)top - p.recent : INT64_MAX;  // positions past this one stay
+    constexpr uint32_t kSafe = 0xffffffffu;                               // above every weight's key
+    uint32_t mine = 0;  // of them, in this wave
+    if constexpr (N > 0) {
+        if (p.recent)
+            each([&](int i) {
+                const int j = first + 64 * i;
+                if (j < len && (int64_t)pos[j] > safe) keys[i] = kSafe;
+            });
+    }
+    auto key = [&](int i) -> uint32_t {
+        if constexpr (N > 0) {
+            return keys[i];
+        } else {
+            const int j = first + 64 * i;
+            return j < len ? ((int64_t)pos[j] > safe ? kSafe : ordered(w[j])) : 0u;
+        }
+    };
+    each([&](int i) { mine += __popcll(__ballot(first + 64 * i < len && key(i) == kSafe)); });
+    if (lane == 0) part2[wave] = mine;
+    __syncthreads();
+    uint32_t safes = 0;
+    for (int i = 0; i < kEvictWaves; ++i) safes += part2[i];
+
+    // The keep-th largest key, eleven bits at a time from the top (bins in falling order); `need` of those
+    // that share the bits found so far are kept.
+    uint32_t last = kSafe, need = (uint32_t)keep;
+    if (safes < need) {
+        need -= safes;
+        uint32_t prefix = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
+            const uint32_t bins = 1u << width;
+            each([&](int i) {
+                const uint32_t k = key(i);
+                const bool in = first + 64 * i < len && k != kSafe && (pass == 0 || (k >> (shift + width)) == prefix);
+                const uint32_t bin = bins - 1 - ((k >> shift) & (bins - 1));
+                // equal digits in the whole wave (weights that are all the same): one addition
+                const uint64_t who = __ballot(in);
+                if (!who) return;
+                const uint32_t one = __shfl(bin, __ffsll((unsigned long long)who) - 1, 64);
+                if (__all(!in || bin == one)) {
+                    if (lane == 0) atomicAdd(&hist[one], (uint32_t)__popcll(who));
+                } else if (in) {
+                    atomicAdd(&hist[bin], 1u);
+                }
+            });
+            __syncthreads();
+            // thread t: bins 2 t and 2 t + 1
+            const uint32_t n0 = hist[2 * tid], n1 = hist[2 * tid + 1];
+            uint32_t before = n0 + n1;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const uint32_t up = __shfl_up(before, d, 64);
                 if (lane >= d) before += up;
             }
-            before -= mine;
-            if (before < need && before + mine >= need) {
-                for (int i = 0; i < per; ++i) {
-                    const uint32_t n = hist[bins - 1 - (lane * per + i)];
-                    if (before + n >= need) {
-                        found[0] = (prefix << widths[pass]) | (uint32_t)(bins - 1 - (lane * per + i));
-                        found[1] = need - before;
-                        break;
-                    }
-                    before += n;
-                }
+            if (lane == 63) part[wave] = before;
+            before -= n0 + n1;
+            __syncthreads();
+            for (int i = 0; i < wave; ++i) before += part[i];
+            if (before < need && before + n0 + n1 >= need) {
+                const bool second = before + n0 < need;
+                found[0] = prefix << width | (bins - 1 - (2 * tid + (second ? 1u : 0u)));
+                found[1] = need - before - (second ? n0 : 0u);
             }
+            hist[2 * tid] = 0;
+            hist[2 * tid + 1] = 0;
+            __syncthreads();
+            prefix = found[0];
+            need = found[1];
         }
-        __syncthreads();
-        prefix = found[0];
-        need = found[1];
-        __syncthreads();
+        last = prefix;
     }
-    const uint32_t last = prefix;  // `need` of the keys equal to it are kept, the lower slots
 
-    // Each wave walks one stretch of the slots; what the stretches before it hold comes first.
-    const int stretch = ((len + kEvictWaves - 1) / kEvictWaves + 63) / 64 * 64;
-    const int a = min(len, wave * stretch), b = min(len, a + stretch);
+    // Kept: the keys above `last`, and the first `need` slots of those equal to it.
     uint32_t gt = 0, eq = 0;
-    for (int j = a + lane; j < b; j += 64) {
-        const uint32_t k = key(j);
-        gt += k > last;
-        eq += k == last;
-    }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        gt += __shfl_xor(gt, m, 64);
-        eq += __shfl_xor(eq, m, 64);
-    }
+    each([&](int i) {
+        const bool in = first + 64 * i < len;
+        const uint32_t k = key(i);
+        gt += __popcll(__ballot(in && k > last));
+        eq += __popcll(__ballot(in && k == last));
+    });
+    __syncthreads();
     if (lane == 0) {
-        wave_gt[wave] = gt;
-        wave_eq[wave] = eq;
+        part[wave] = gt;
+        part2[wave] = eq;
     }
     __syncthreads();
     uint32_t eq_before = 0, kept_before = 0;
     for (int i = 0; i < wave; ++i) {
-        const uint32_t e = wave_eq[i];
-        kept_before += wave_gt[i] + (eq_before < need ? min(e, need - eq_before) : 0u);
+        const uint32_t e = part2[i];
+        kept_before += part[i] + (eq_before < need ? min(e, need - eq_before) : 0u);
         eq_before += e;
     }
     const uint64_t lower = (1ull << lane) - 1;
-    for (int j0 = a; j0 < b; j0 += 64) {
-        const int j = j0 + lane;
-        const uint32_t k = j < b ? key(j) : 0u;
-        const uint64_t same = __ballot(j < b && k == last);
-        const bool kept = j < b && (k > last || (k == last && eq_before + __popcll(same & lower) < need));
+    each([&](int i) {
+        const int j = first + 64 * i;
+        const uint32_t k = key(i);
+        const uint64_t same = __ballot(j < len && k == last);
+        const bool kept = j < len && (k > last || (k == last && eq_before + __popcll(same & lower) < need));
         const uint64_t all = __ballot(kept);
-        const uint32_t before = kept_before + __popcll(all & lower);
-        if (j < b) {
+        const int before = (int)(kept_before + __popcll(all & lower));
+        if (j < len) {
             if (j < keep) {
                 if (!kept) {
                     list[j - before] = j;
@@ -597,54 +672,90 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictP
                     if (po != pos) po[j] = pos[j];
                 }
             } else if (kept) {
-                list[p.moves + (keep - 1 - (int)before)] = j;  // the last one kept comes first
+                list[p.moves + (keep - 1 - before)] = j;  // the last one kept comes first
             }
             // the holes before the cut: as many as kept ones behind it
-            if (j == keep) list[2 * p.moves] = keep - (int)before;
+            if (j == keep) list[2 * p.moves] = keep - before;
         }
         eq_before += __popcll(same);
         kept_before += __popcll(all);
-    }
+    });
 }
 
-// Each move: a row of K, one of V, its weight and its position.
+// Each move: a row of K, one of V, its weight and its position.  A thread takes its 16-byte
+// piece of U of them, the loads of all U together.
+template <int U>
 __global__ __launch_bounds__(256) void kv_evict_move_kernel(KvEvictParams p, int pieces, int esz, int blocks) {
-    const int rh = blockIdx.x / blocks, row = rh / p.c.heads, h = rh % p.c.heads;
+    const int rh = blockIdx.x / blocks, block = blockIdx.x % blocks, row = rh / p.c.heads, h = rh % p.c.heads;
     const int32_t* list = p.list + (int64_t)rh * (2 * p.moves + 1);
     const int n = list[2 * p.moves];
-    const int per = 256 / pieces;  // moves per workgroup
-    const int i = (blockIdx.x % blocks) * per + threadIdx.x / pieces, c = threadIdx.x % pieces;
-    if (blockIdx.x % blocks == 0 && h == 0 && threadIdx.x == 0) {
+    const int per = 256 / pieces;  // moves of a workgroup at a time
+    const int i0 = block * per * U + threadIdx.x / pieces, c = threadIdx.x % pieces;
+    if (block == 0 && h == 0 && threadIdx.x == 0) {
         const int len = p.c.lens[row];
         p.lens_out[row] = len > p.keep && len <= p.max_len ? p.keep : len;
     }
-    if (i >= n) return;
-    const int dst = list[i], src = list[p.moves + n - 1 - i];
+    if (i0 >= n) return;
     const int32_t* table = p.c.table + row * p.c.table_stride;
-    const int pd = page_of(p.c, table, dst), ps = page_of(p.c, table, src);
     const int mask = (1 << p.c.page_shift) - 1;
-    if (pd >= 0 && ps >= 0) {
-        const int64_t ko = h * p.c.sk.h, vo = h * p.c.sv.h;
-        const u32x4 kx = *reinterpret_cast<const u32x4*>(
-            (const char*)p.c.k + (ps * p.c.sk.b + ko + (src & mask) * p.c.sk.t) * esz + 16 * c);
-        const u32x4 vx = *reinterpret_cast<const u32x4*>(
-            (const char*)p.c.v + (ps * p.c.sv.b + vo + (src & mask) * p.c.sv.t) * esz + 16 * c);
-        *reinterpret_cast<u32x4*>((char*)p.c.k + (pd * p.c.sk.b + ko + (dst & mask) * p.c.sk.t) * esz + 16 * c) = kx;
-        *reinterpret_cast<u32x4*>((char*)p.c.v + (pd * p.c.sv.b + vo + (dst & mask) * p.c.sv.t) * esz + 16 * c) = vx;
+    const int64_t at = (int64_t)rh * p.c.cap();
+    int src[U], dst[U], ps[U], pd[U];
+    u32x4 kx[U], vx[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = min(i0 + u * per, n - 1);  // the last one again where there are no more
+        dst[u] = list[i];
+        src[u] = list[p.moves + n - 1 - i];
     }
-    if (c == 0) {
-        const int64_t at = (int64_t)rh * p.c.cap();
-        p.w_out[at + dst] = p.w_in[at + src];
-        p.pos_out[at + dst] = p.pos_in[at + src];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        pd[u] = page_of(p.c, table, dst[u]);
+        ps[u] = page_of(p.c, table, src[u]);
+    }
+    const int64_t ko = h * p.c.sk.h, vo = h * p.c.sv.h;
+    const char *K = (const char*)p.c.k + 16 * c, *V = (const char*)p.c.v + 16 * c;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int pg = max(ps[u], 0), slot = src[u] & mask;
+        kx[u] = *reinterpret_cast<const u32x4*>(K + (pg * p.c.sk.b + ko + slot * p.c.sk.t) * esz);
+        vx[u] = *reinterpret_cast<const u32x4*>(V + (pg * p.c.sv.b + vo + slot * p.c.sv.t) * esz);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (i0 + u * per >= n) break;
+        const int slot = dst[u] & mask;
+        if (pd[u] >= 0 && ps[u] >= 0) {
+            *reinterpret_cast<u32x4*>((char*)K + (pd[u] * p.c.sk.b + ko + slot * p.c.sk.t) * esz) = kx[u];
+            *reinterpret_cast<u32x4*>((char*)V + (pd[u] * p.c.sv.b + vo + slot * p.c.sv.t) * esz) = vx[u];
+        }
+        if (c == 0) {
+            p.w_out[at + dst[u]] = p.w_in[at + src[u]];
+            p.pos_out[at + dst[u]] = p.pos_in[at + src[u]];
+        }
     }
 }
 
 int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s) {
     const int esz = bf16 ? 2 : 4, pieces = p.c.D * esz / 16, per = 256 / pieces;
-    const int blocks = p.moves ? (p.moves + per - 1) / per : 1;
     const int64_t rh = (int64_t)p.c.rows * p.c.heads;
-    hipLaunchKernelGGL(kv_evict_select_kernel, dim3((unsigned)rh), dim3(kEvictThreads), 0, s, p);
-    hipLaunchKernelGGL(kv_evict_move_kernel, dim3((unsigned)(rh * blocks)), dim3(256), 0, s, p, pieces, esz, blocks);
+    const dim3 grid((unsigned)rh), block(kEvictThreads);
+    if (p.max_len <= 2 * kEvictThreads)
+        hipLaunchKernelGGL((kv_evict_select_kernel<2>), grid, block, 0, s, p);
+    else if (p.max_len <= 8 * kEvictThreads)
+        hipLaunchKernelGGL((kv_evict_select_kernel<8>), grid, block, 0, s, p);
+    else if (p.max_len <= 64 * kEvictThreads)
+        hipLaunchKernelGGL((kv_evict_select_kernel<64>), grid, block, 0, s, p);
+    else
+        hipLaunchKernelGGL((kv_evict_select_kernel<0>), grid, block, 0, s, p);
+    // four moves a thread where that leaves a thousand workgroups
+    const int64_t all = rh * ((p.moves + per - 1) / per);
+    const int u = all >= 4096 ? 4 : 1;
+    const int blocks = p.moves ? (p.moves + per * u - 1) / (per * u) : 1;
+    const dim3 g2((unsigned)(rh * blocks));
+    if (u == 4)
+        hipLaunchKernelGGL((kv_evict_move_kernel<4>), g2, dim3(256), 0, s, p, pieces, esz, blocks);
+    else
+        hipLaunchKernelGGL((kv_evict_move_kernel<1>), g2, dim3(256), 0, s, p, pieces, esz, blocks);
     return (int)hipGetLastError();
 }
 
