@@ -37,10 +37,11 @@ __device__ __forceinline__ uint64_t ordered_score(double x) {
     return b >> 63 ? ~b : b | (1ull << 63);
 }
 
-// A lower bound, to the 20 highest bits, of the n-th largest of the wave's values.
+// A lower bound, to the 16 highest bits, of the n-th largest of the wave's values.
 __device__ __forceinline__ uint32_t wave_nth(uint32_t v, int n) {
     uint32_t t = 0;
-    for (int bit = 31; bit >= 12; --bit) {
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
         const uint32_t up = t | (1u << bit);
         if (__popcll(__ballot(v >= up)) >= n) t = up;
     }
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
 #pragma unroll
     for (int i = 0; i < N; ++i) mx = fmaxf(mx, v[i]);
     const uint32_t lane_best = ordered_logit(mx);
-    mx = wave_max(mx);
+    mx = wave_all(mx, [](float a, float b) { return fmaxf(a, b); });
     const float ref = mx == -INFINITY ? 0.f : mx;
     // four terms in 32 bits, which are off by 2^-23 of them at most, all further in 64
     double sum = 0.0;
@@ -121,8 +122,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
         for (int e = 0; e < 4; ++e) t[e] = fast_exp2((v[i + e] - ref) * kLog2e);
         sum += (double)((t[0] + t[1]) + (t[2] + t[3]));
     }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) sum += shfl_xor_d(sum, m);
+    sum = wave_all(sum, [](double a, double b) { return a + b; });
     if (lane == 0) {
         wmax[wave] = mx;
         wsum[wave] = sum;
@@ -148,11 +148,16 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
     uint64_t* out = p.cand + (int64_t)blockIdx.x * p.beams;
     if (n <= kBeamList) {
         if (tid < p.beams && tid >= n) out[tid] = 0;  // fewer columns than beams
-        for (int i = tid; i < n; i += 256) {
-            const uint64_t mine = list[i];
+        // four lanes count for one value
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const int i = i0 + (tid >> 2);
+            const uint64_t mine = list[min(i, n - 1)];
             int better = 0;
-            for (int j = 0; j < n; ++j) better += list[j] > mine;
-            if (better < p.beams) out[better] = mine;
+#pragma unroll 4
+            for (int j = tid & 3; j < n; j += 4) better += list[j] > mine;
+            better += (int)dpp_u32<0xB1>((uint32_t)better);
+            better += (int)dpp_u32<0x4E>((uint32_t)better);
+            if (i < n && (tid & 3) == 0 && better < p.beams) out[better] = mine;
         }
         return;
     }
@@ -164,8 +169,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
             const uint64_t y = v[i] >= least && column(i) >= lo && column(i) < hi ? key(i) : 0;
             if (y < before && y > best) best = y;
         }
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) best = max(best, shfl_xor64(best, m));
+        best = wave_all(best, [](uint64_t a, uint64_t b) { return max(a, b); });
         if (lane == 0) wbest[wave] = best;
         __syncthreads();
         before = max(max(wbest[0], wbest[1]), max(wbest[2], wbest[3]));
@@ -191,13 +195,14 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
         cand[u] = held && tid + 256 * u < total ? p.cand[row0 * per + tid + 256 * u] : 0;
-    for (int b = wave; b < p.beams; b += 4) {
+    static_assert(kMaxBeams * 8 <= 256, "eight lanes per beam");
+    if (const int b = tid >> 3; b < p.beams) {
         const int64_t row = row0 + b;
         const float score = p.scores[row];
         const bool finished = p.finished && p.finished[row];
         float M = -INFINITY;
         double S = 0.0;
-        for (int i = lane; i < p.nsplit; i += 64) {
+        for (int i = tid & 7; i < p.nsplit; i += 8) {
             const float m = p.maxs[row * p.nsplit + i];
             const double s = p.sums[row * p.nsplit + i];
             const float top = fmaxf(M, m);
@@ -205,13 +210,18 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
                 (m == -INFINITY ? s : s * exp((double)m - (double)top));
             M = top;
         }
-        const float top = wave_max(M);
-        if (M != -INFINITY) S *= exp((double)M - (double)top);
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) S += shfl_xor_d(S, m);
-        if (lane == 0) {
+        for (int d = 1; d < 8; d <<= 1) {
+            const float m = shfl_xor(M, d);
+            const double s = shfl_xor_d(S, d);
+            const float top = fmaxf(M, m);
+            S = (M == -INFINITY ? S : S * exp((double)M - (double)top)) +
+                (m == -INFINITY ? s : s * exp((double)m - (double)top));
+            M = top;
+        }
+        if ((tid & 7) == 0) {
             // a NaN or +inf among the logits, or nothing above -inf: the sum is NaN, infinite or 0
-            const double lse = (double)top + log(S);
+            const double lse = (double)M + log(S);
             const bool lives = !finished && isfinite(score), fine = isfinite(lse);
             base[b] = !lives ? (double)score : fine ? (double)score - lse : __longlong_as_double(0x7ff8000000000000ll);
             kind[b] = finished ? kFinished : lives && fine ? kLives : kFlat;
@@ -280,11 +290,15 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     __syncthreads();
     const int n = count;
     if (n <= kBeamList) {
-        for (int i = tid; i < n; i += 256) {
-            const uint64_t s = ls[i], t = lt[i];
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const int i = i0 + (tid >> 2);
+            const uint64_t s = ls[min(i, n - 1)], t = lt[min(i, n - 1)];
             int better = 0;
-            for (int j = 0; j < n; ++j) better += ls[j] > s || (ls[j] == s && lt[j] < t);
-            if (better < p.beams) emit(better, s, t);
+#pragma unroll 4
+            for (int j = tid & 3; j < n; j += 4) better += ls[j] > s || (ls[j] == s && lt[j] < t);
+            better += (int)dpp_u32<0xB1>((uint32_t)better);
+            better += (int)dpp_u32<0x4E>((uint32_t)better);
+            if (i < n && (tid & 3) == 0 && better < p.beams) emit(better, s, t);
         }
         return;
     }

@@ -88,6 +88,48 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
+// The same reductions on the VALU alone: DPP within the rows of 16 lanes, then gfx950's
+// v_permlane16_swap and v_permlane32_swap, which give v[l] and v[l ^ 16] (v[l ^ 32]) in either order.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, true);
+}
+template <typename T, typename F>
+__device__ __forceinline__ T wave_all(T v, F op) {
+    static_assert(sizeof(T) == 4 || sizeof(T) == 8, "one or two registers");
+    constexpr int W = sizeof(T) / 4;
+    struct Words {
+        uint32_t w[W];
+    };
+    auto step = [&](auto other) {  // other(word) -> the partner's word
+        Words a = __builtin_bit_cast(Words, v), b;
+#pragma unroll
+        for (int i = 0; i < W; ++i) b.w[i] = other(a.w[i]);
+        v = op(v, __builtin_bit_cast(T, b));
+    };
+    auto swapped = [&](auto swap) {
+        Words a = __builtin_bit_cast(Words, v), b;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const auto r = swap(a.w[i]);
+            a.w[i] = r[0];
+            b.w[i] = r[1];
+        }
+        v = op(__builtin_bit_cast(T, a), __builtin_bit_cast(T, b));
+    };
+    step([](uint32_t x) { return dpp_u32<0xB1>(x); });
+    step([](uint32_t x) { return dpp_u32<0x4E>(x); });
+    step([](uint32_t x) { return dpp_u32<0x141>(x); });
+    step([](uint32_t x) { return dpp_u32<0x140>(x); });
+    swapped([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+    swapped([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+    return v;
+}
+__device__ __forceinline__ float max_xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // bf16 <-> fp32.  fp32 -> bf16 rounds to nearest even and keeps NaN a (quiet)
 // NaN; gfx950 converts in hardware (v_cvt_pk_bf16_f32, two values per
 // instruction), branch-free, where a bit-level rounding with a NaN test

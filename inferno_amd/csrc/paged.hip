@@ -261,8 +261,7 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
         float mx = m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
-        mx = fmaxf(mx, shfl_xor(mx, 16));
-        mx = max_xor32(mx);
+        mx = max_xor32(max_xor16(mx));
         const float ref = mx == -INFINITY ? 0.f : mx;  // no key above -inf yet: keep everything at 0
         const float alpha = fast_exp2(m - ref);
         m = mx;
@@ -497,25 +496,27 @@ int launch_attn_decode_paged(const PagedDecodeParams& p, int bf16, hipStream_t s
 // ============================================================================
 namespace {
 
-// Order of the floats as unsigned numbers (-0 as 0); NaN, below all, is 0.
+// Order of the floats as unsigned numbers, -0 as 0; NaN, below all, is 0.  Infinity is 0xff800000.
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
-    if ((b & 0x7fffffffu) > 0x7f800000u) return 0u;
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return x != x ? 0u : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
 
-constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+// Slots whose keys fit in LDS beside the rest (144 KB of the 160); longer rows read their weights
+// again in every pass.
+constexpr int kEvictLds = 36 << 10;
 
 }  // namespace
 
-// N: slots per thread at most, held as keys in registers; 0: more than 65536 slots, read again in every
-// pass.  Wave w's are one stretch of the slots, 64 at a time, so that what comes before a slot is the
-// waves before, the rounds before and the lanes before.
-template <int N>
-__global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictParams p) {
-    __shared__ uint32_t hist[2048];
-    __shared__ uint32_t part[kEvictWaves], part2[kEvictWaves];
+// W waves, each with one stretch of the slots, 256 at a time, four to a lane, so that what comes before a
+// slot is the waves before, the rounds before, the lanes before and the lane's own.
+template <int W, bool LDS>
+__global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p, int vec) {
+    constexpr int kThreads = 64 * W, kBins = 2048, PER = kBins / kThreads;
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t part[W], part2[W];
     __shared__ uint32_t found[2];
+    extern __shared__ __attribute__((aligned(16))) uint32_t skeys[];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int rh = blockIdx.x, row = rh / p.c.heads;
     const int stored = p.c.lens[row], len = min(max(stored, 0), (int)p.c.cap());
@@ -525,109 +526,153 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictP
     int32_t* po = p.pos_out + (int64_t)rh * p.c.cap();
     int32_t* list = p.list + (int64_t)rh * (2 * p.moves + 1);
     const int keep = p.keep;
+    const bool copy = wo != w || po != pos;
     if (len <= keep || stored > p.max_len) {
         if (tid == 0) list[2 * p.moves] = 0;
-        if (wo != w)
-            for (int j = tid; j < len; j += kEvictThreads) wo[j] = w[j];
-        if (po != pos)
-            for (int j = tid; j < len; j += kEvictThreads) po[j] = pos[j];
+        if (copy)
+            for (int j = tid; j < len; j += kThreads) {
+                wo[j] = w[j];
+                po[j] = pos[j];
+            }
         return;
     }
-    const int rounds = (len + kEvictThreads - 1) / kEvictThreads;
-    const int first = wave * rounds * 64 + lane;  // this lane's slots: first + 64 i < len
-    uint32_t keys[N ? N : 1];
-    int top = INT32_MIN;
-    auto each = [&](auto&& f) {  // f(round): the rounds of this wave
-        if constexpr (N > 0) {
+    const int rounds = (len + 4 * kThreads - 1) / (4 * kThreads);
+    const int first = 256 * wave * rounds + 4 * lane;
+    // Four slots from j on, those behind the end as 0 (in a row of any alignment, one by one).
+    auto load4 = [&](const uint32_t* src, int j) -> u32x4 {
+        if (vec && j + 4 <= len) return *reinterpret_cast<const u32x4*>(src + j);
+        u32x4 x;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i < rounds) f(i);
-        } else {
-#pragma unroll 4
-            for (int i = 0; i < rounds; ++i) f(i);
+        for (int e = 0; e < 4; ++e) x[e] = j + e < len ? src[j + e] : 0u;
+        return x;
+    };
+    struct Meta {
+        u32x4 w, pos;
+    };
+    // f(j, x) for this lane's groups of four slots in order, x = load(j); U of them are loaded together
+    auto each = [&](auto load, auto f) {
+        constexpr int U = 4;
+        for (int i = 0; i < rounds; i += U) {
+            decltype(load(0)) x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u < rounds) x[u] = load(first + 256 * (i + u));
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i + u < rounds) f(first + 256 * (i + u), x[u]);
         }
     };
-    each([&](int i) {
-        const int j = first + 64 * i;
-        if constexpr (N > 0) keys[i] = j < len ? ordered(w[j]) : 0u;
-        if (p.recent && j < len) top = max(top, pos[j]);
-    });
-    hist[tid] = 0;
-    hist[tid + kEvictThreads] = 0;
+    const uint32_t *wbits = reinterpret_cast<const uint32_t*>(w), *pbits = reinterpret_cast<const uint32_t*>(pos);
+    // Positions past `safe` stay.
+    int safe = INT32_MAX;
+    bool all_safe = false;
+    for (int i = tid; i < kBins; i += kThreads) hist[i] = 0;
     if (p.recent) {
+        int top = INT32_MIN;
+        each([&](int j) { return load4(pbits, j); }, [&](int j, u32x4 x) {
 #pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) top = max(top, __shfl_xor(top, m, 64));
+            for (int e = 0; e < 4; ++e) top = max(top, j + e < len ? (int)x[e] : INT32_MIN);
+        });
+        top = wave_all(top, [](int x, int y) { return max(x, y); });
         if (lane == 0) part[wave] = (uint32_t)top;
         __syncthreads();
-        for (int i = 0; i < kEvictWaves; ++i) top = max(top, (int)part[i]);
+        for (int i = 0; i < W; ++i) top = max(top, (int)part[i]);
+        const int64_t s = (int64_t)top - p.recent;
+        all_safe = s < INT32_MIN;
+        safe = all_safe ? INT32_MIN : (int)s;
+    } else {
+        __syncthreads();
     }
-    const int64_t safe = p.recent ? (int64_t)top - p.recent : INT64_MAX;  // positions past this one stay
-    constexpr uint32_t kSafe = 0xffffffffu;                               // above every weight's key
-    uint32_t mine = 0;  // of them, in this wave
-    if constexpr (N > 0) {
-        if (p.recent)
-            each([&](int i) {
-                const int j = first + 64 * i;
-                if (j < len && (int64_t)pos[j] > safe) keys[i] = kSafe;
-            });
-    }
-    auto key = [&](int i) -> uint32_t {
-        if constexpr (N > 0) {
-            return keys[i];
-        } else {
-            const int j = first + 64 * i;
-            return j < len ? ((int64_t)pos[j] > safe ? kSafe : ordered(w[j])) : 0u;
+    // Above every weight's key, and alone in its bin of every pass.  Slots behind the end have it too, and are
+    // taken off the counts.
+    constexpr uint32_t kSafe = 0xffffffffu;
+    auto keys_of = [&](int j, Meta x) {
+        u32x4 k;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            k[e] = (int)x.pos[e] > safe || all_safe ? kSafe : ordered(__uint_as_float(x.w[e]));
+        if (j + 4 > len) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = j + e < len ? k[e] : kSafe;
         }
+        return k;
     };
-    each([&](int i) { mine += __popcll(__ballot(first + 64 * i < len && key(i) == kSafe)); });
-    if (lane == 0) part2[wave] = mine;
+    auto meta = [&](int j) { return Meta{load4(wbits, j), p.recent ? load4(pbits, j) : u32x4{0u, 0u, 0u, 0u}}; };
+    each(meta, [&](int j, Meta x) {
+        const u32x4 k = keys_of(j, x);
+        if (LDS && j < len) *reinterpret_cast<u32x4*>(&skeys[j]) = k;
+        // often the whole wave has one bin (recent slots, equal weights)
+        const uint32_t one = __builtin_amdgcn_readfirstlane(k[0] >> 21);
+        if (__all((k[0] >> 21) == one && (k[1] >> 21) == one && (k[2] >> 21) == one && (k[3] >> 21) == one)) {
+            if (lane == 0) atomicAdd(&hist[one], 256u);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) atomicAdd(&hist[k[e] >> 21], 1u);
+        }
+    });
+    auto keys = [&](auto f) {  // f(j, four keys)
+        if constexpr (LDS)
+            each([&](int j) {
+                return j < len ? *reinterpret_cast<const u32x4*>(&skeys[j]) : u32x4{kSafe, kSafe, kSafe, kSafe};
+            }, f);
+        else
+            each(meta, [&](int j, Meta x) { f(j, keys_of(j, x)); });
+    };
     __syncthreads();
-    uint32_t safes = 0;
-    for (int i = 0; i < kEvictWaves; ++i) safes += part2[i];
 
-    // The keep-th largest key, eleven bits at a time from the top (bins in falling order); `need` of those
-    // that share the bits found so far are kept.
+    // The keep-th largest key, eleven bits at a time from the top; `need` of those that share the bits found
+    // so far are kept.
     uint32_t last = kSafe, need = (uint32_t)keep;
+    const uint32_t safes = hist[kBins - 1] - (uint32_t)(4 * kThreads * rounds - len);
     if (safes < need) {
         need -= safes;
+        __syncthreads();
+        if (tid == 0) hist[kBins - 1] = 0;
+        __syncthreads();
         uint32_t prefix = 0;
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
             const uint32_t bins = 1u << width;
-            each([&](int i) {
-                const uint32_t k = key(i);
-                const bool in = first + 64 * i < len && k != kSafe && (pass == 0 || (k >> (shift + width)) == prefix);
-                const uint32_t bin = bins - 1 - ((k >> shift) & (bins - 1));
-                // equal digits in the whole wave (weights that are all the same): one addition
-                const uint64_t who = __ballot(in);
-                if (!who) return;
-                const uint32_t one = __shfl(bin, __ffsll((unsigned long long)who) - 1, 64);
-                if (__all(!in || bin == one)) {
-                    if (lane == 0) atomicAdd(&hist[one], (uint32_t)__popcll(who));
-                } else if (in) {
-                    atomicAdd(&hist[bin], 1u);
-                }
-            });
-            __syncthreads();
-            // thread t: bins 2 t and 2 t + 1
-            const uint32_t n0 = hist[2 * tid], n1 = hist[2 * tid + 1];
-            uint32_t before = n0 + n1;
+            if (pass) {
+                keys([&](int, u32x4 k) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((k[e] >> (shift + width)) == prefix)
+                            atomicAdd(&hist[(k[e] >> shift) & (bins - 1)], 1u);
+                });
+                __syncthreads();
+            }
+            // thread t: PER bins from the top, behind those of the threads before
+            uint32_t n[PER], mine = 0;
+            uint32_t* mybins = hist + (kBins - PER * (tid + 1));
+#pragma unroll
+            for (int i = 0; i < PER; ++i) mine += n[i] = mybins[PER - 1 - i];
+            uint32_t before = mine;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const uint32_t up = __shfl_up(before, d, 64);
                 if (lane >= d) before += up;
             }
             if (lane == 63) part[wave] = before;
-            before -= n0 + n1;
+            before -= mine;
             __syncthreads();
             for (int i = 0; i < wave; ++i) before += part[i];
-            if (before < need && before + n0 + n1 >= need) {
-                const bool second = before + n0 < need;
-                found[0] = prefix << width | (bins - 1 - (2 * tid + (second ? 1u : 0u)));
-                found[1] = need - before - (second ? n0 : 0u);
+            if (before < need && before + mine >= need) {
+                uint32_t bin = 0;
+                bool done = false;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    done |= before + n[i] >= need;
+                    if (!done) {
+                        before += n[i];
+                        ++bin;
+                    }
+                }
+                found[0] = prefix << width | (kBins - 1 - (PER * tid + bin));
+                found[1] = need - before;
             }
-            hist[2 * tid] = 0;
-            hist[2 * tid + 1] = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) mybins[i] = 0;
             __syncthreads();
             prefix = found[0];
             need = found[1];
@@ -637,12 +682,17 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictP
 
     // Kept: the keys above `last`, and the first `need` slots of those equal to it.
     uint32_t gt = 0, eq = 0;
-    each([&](int i) {
-        const bool in = first + 64 * i < len;
-        const uint32_t k = key(i);
-        gt += __popcll(__ballot(in && k > last));
-        eq += __popcll(__ballot(in && k == last));
+    keys([&](int, u32x4 k) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            gt += k[e] > last;
+            eq += k[e] == last;
+        }
     });
+    gt = wave_all(gt, [](uint32_t x, uint32_t y) { return x + y; });
+    eq = wave_all(eq, [](uint32_t x, uint32_t y) { return x + y; });
+    const int behind = 256 * rounds - min(max(len - 256 * wave * rounds, 0), 256 * rounds);  // the end
+    (last == kSafe ? eq : gt) -= behind;
     __syncthreads();
     if (lane == 0) {
         part[wave] = gt;
@@ -655,31 +705,78 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(KvEvictP
         kept_before += part[i] + (eq_before < need ? min(e, need - eq_before) : 0u);
         eq_before += e;
     }
-    const uint64_t lower = (1ull << lane) - 1;
-    each([&](int i) {
-        const int j = first + 64 * i;
-        const uint32_t k = key(i);
-        const uint64_t same = __ballot(j < len && k == last);
-        const bool kept = j < len && (k > last || (k == last && eq_before + __popcll(same & lower) < need));
-        const uint64_t all = __ballot(kept);
-        const int before = (int)(kept_before + __popcll(all & lower));
-        if (j < len) {
-            if (j < keep) {
-                if (!kept) {
-                    list[j - before] = j;
-                } else {
-                    if (wo != w) wo[j] = w[j];
-                    if (po != pos) po[j] = pos[j];
-                }
-            } else if (kept) {
-                list[p.moves + (keep - 1 - before)] = j;  // the last one kept comes first
-            }
-            // the holes before the cut: as many as kept ones behind it
-            if (j == keep) list[2 * p.moves] = keep - before;
+    auto below = [](uint64_t mask, uint32_t n) {  // n and its bits under this lane
+        return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, n));
+    };
+    // Lists four slots; kept: which of them are.
+    auto place = [&](int j, u32x4 k, bool (&kept)[4]) {
+        bool same[4];
+        uint64_t m[4];
+        const int in = len - j;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            kept[e] = k[e] > last && e < in;
+            same[e] = k[e] == last && e < in;
         }
-        eq_before += __popcll(same);
-        kept_before += __popcll(all);
-    });
+        if (__any(same[0] || same[1] || same[2] || same[3])) {
+            uint32_t rank = eq_before;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                m[e] = __ballot(same[e]);
+                rank = below(m[e], rank);
+                eq_before += __popcll(m[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                kept[e] |= same[e] && rank < need;
+                rank += same[e];
+            }
+        }
+        uint32_t before = kept_before;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            m[e] = __ballot(kept[e]);
+            before = below(m[e], before);
+            kept_before += __popcll(m[e]);
+        }
+        if (j < len) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool front = j + e < keep;
+                if (front != kept[e] && e < in)  // a hole, or one to fill one (the last kept comes first)
+                    list[front ? j + e - (int)before : p.moves + keep - 1 - (int)before] = j + e;
+                if (j + e == keep) list[2 * p.moves] = keep - (int)before;  // holes before the cut
+                before += kept[e];
+            }
+        }
+    };
+    if (copy)
+        each([&](int j) { return Meta{load4(wbits, j), load4(pbits, j)}; }, [&](int j, Meta x) {
+            u32x4 k;
+            if constexpr (LDS)
+                k = *reinterpret_cast<const u32x4*>(&skeys[min(j, (len - 1) & ~3)]);
+            else
+                k = keys_of(j, p.recent ? x : Meta{x.w, u32x4{0u, 0u, 0u, 0u}});
+            bool kept[4];
+            place(j, k, kept);
+            // a hole gets its own from the moves that follow
+            if (vec && j + 4 <= keep) {
+                *reinterpret_cast<u32x4*>(wo + j) = x.w;
+                *reinterpret_cast<u32x4*>(po + j) = x.pos;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (kept[e] && j + e < keep) {
+                        wo[j + e] = __uint_as_float(x.w[e]);
+                        po[j + e] = (int)x.pos[e];
+                    }
+            }
+        });
+    else
+        keys([&](int j, u32x4 k) {
+            bool kept[4];
+            place(j, k, kept);
+        });
 }
 
 // Each move: a row of K, one of V, its weight and its position.  A thread takes its 16-byte
@@ -738,15 +835,18 @@ __global__ __launch_bounds__(256) void kv_evict_move_kernel(KvEvictParams p, int
 int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s) {
     const int esz = bf16 ? 2 : 4, pieces = p.c.D * esz / 16, per = 256 / pieces;
     const int64_t rh = (int64_t)p.c.rows * p.c.heads;
-    const dim3 grid((unsigned)rh), block(kEvictThreads);
-    if (p.max_len <= 2 * kEvictThreads)
-        hipLaunchKernelGGL((kv_evict_select_kernel<2>), grid, block, 0, s, p);
-    else if (p.max_len <= 8 * kEvictThreads)
-        hipLaunchKernelGGL((kv_evict_select_kernel<8>), grid, block, 0, s, p);
-    else if (p.max_len <= 64 * kEvictThreads)
-        hipLaunchKernelGGL((kv_evict_select_kernel<64>), grid, block, 0, s, p);
+    // a workgroup of 256 threads where a row is short: more of them at once, cheaper barriers
+    const dim3 grid((unsigned)rh);
+    const size_t lds = ((size_t)p.max_len + 3) / 4 * 16;
+    const uintptr_t any = reinterpret_cast<uintptr_t>(p.w_in) | reinterpret_cast<uintptr_t>(p.w_out) |
+                          reinterpret_cast<uintptr_t>(p.pos_in) | reinterpret_cast<uintptr_t>(p.pos_out);
+    const int vec = any % 16 == 0 && p.c.cap() % 4 == 0;
+    if (p.max_len <= 4096)
+        hipLaunchKernelGGL((kv_evict_select_kernel<4, true>), grid, dim3(256), lds, s, p, vec);
+    else if (p.max_len <= kEvictLds)
+        hipLaunchKernelGGL((kv_evict_select_kernel<16, true>), grid, dim3(1024), lds, s, p, vec);
     else
-        hipLaunchKernelGGL((kv_evict_select_kernel<0>), grid, block, 0, s, p);
+        hipLaunchKernelGGL((kv_evict_select_kernel<16, false>), grid, dim3(1024), 0, s, p, vec);
     // four moves a thread where that leaves a thousand workgroups
     const int64_t all = rh * ((p.moves + per - 1) / per);
     const int u = all >= 4096 ? 4 : 1;
