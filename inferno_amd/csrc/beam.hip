@@ -37,11 +37,12 @@ __device__ __forceinline__ uint64_t ordered_score(double x) {
     return b >> 63 ? ~b : b | (1ull << 63);
 }
 
-// A lower bound, to the 16 highest bits, of the n-th largest of the wave's values.
+// A lower bound, exact down to bit LOW, of the n-th largest of the wave's values.
+template <int LOW>
 __device__ __forceinline__ uint32_t wave_nth(uint32_t v, int n) {
     uint32_t t = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
+    for (int bit = 31; bit >= LOW; --bit) {
         const uint32_t up = t | (1u << bit);
         if (__popcll(__ballot(v >= up)) >= n) t = up;
     }
@@ -66,7 +67,7 @@ __device__ __forceinline__ bool beam_lives(const BeamSelectParams& p, int64_t ro
 
 // N: columns per thread, 256 N per workgroup.
 template <typename E, int N>
-__global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
+__global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSelectParams p) {
     using T = typename E::T;
     constexpr int GE = 16 / sizeof(T), NV = N / GE;  // columns of a 16-byte load, loads per thread
     __shared__ uint64_t list[kBeamList];
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(256) void beam_part_kernel(BeamSelectParams p) {
         wsum[wave] = sum;
     }
     if (tid == 0) count = 0;
-    const float least = logit_of(max(wave_nth(lane_best, p.beams), ordered_logit(-INFINITY)));
+    const float least = logit_of(max(wave_nth<16>(lane_best, p.beams), ordered_logit(-INFINITY)));
     __syncthreads();
     if (tid == 0) {
         const float M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
@@ -188,37 +189,47 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t row0 = (int64_t)blockIdx.x * p.beams;
     const int per = p.nsplit * p.beams, total = p.beams * per;
-    // the candidates' logits and columns do not wait for the lse; usually all fit in registers
+    // The candidates' logits and columns do not wait for the lse; up to 256 U of them stay in registers.
+    // Each part's are in order, so that a lane's step to step is no multiple of the beams: lanes that held
+    // only best ones, and lanes that held only last ones, would bound the best few badly.
     constexpr int U = 8;
-    const bool held = total <= 256 * U;
     uint64_t cand[U];
+    auto index = [&](int i0, int u) { return i0 + 256 * u + ((tid + 41 * u) & 255); };
+    auto load = [&](int i0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-        cand[u] = held && tid + 256 * u < total ? p.cand[row0 * per + tid + 256 * u] : 0;
+        for (int u = 0; u < U; ++u)
+            cand[u] = i0 + 256 * u < total && index(i0, u) < total ? p.cand[row0 * per + index(i0, u)] : 0;
+    };
+    load(0);
     static_assert(kMaxBeams * 8 <= 256, "eight lanes per beam");
     if (const int b = tid >> 3; b < p.beams) {
         const int64_t row = row0 + b;
         const float score = p.scores[row];
         const bool finished = p.finished && p.finished[row];
-        float M = -INFINITY;
-        double S = 0.0;
-        for (int i = tid & 7; i < p.nsplit; i += 8) {
-            const float m = p.maxs[row * p.nsplit + i];
-            const double s = p.sums[row * p.nsplit + i];
-            const float top = fmaxf(M, m);
-            S = (M == -INFINITY ? S : S * exp((double)M - (double)top)) +
-                (m == -INFINITY ? s : s * exp((double)m - (double)top));
+        // up to 32 parts: four a lane, loaded together
+        constexpr int P = 4;
+        float m[P], M = -INFINITY;
+        double s[P], S = 0.0;
+        for (int i0 = 0; i0 < p.nsplit; i0 += 8 * P) {
+            float top = M;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const int i = i0 + 8 * k + (tid & 7);
+                m[k] = i < p.nsplit ? p.maxs[row * p.nsplit + i] : -INFINITY;
+                s[k] = i < p.nsplit ? p.sums[row * p.nsplit + i] : 0.0;
+                top = fmaxf(top, m[k]);
+            }
+            top = fmaxf(top, __uint_as_float(dpp_u32<0xB1>(__float_as_uint(top))));
+            top = fmaxf(top, __uint_as_float(dpp_u32<0x4E>(__float_as_uint(top))));
+            top = fmaxf(top, __uint_as_float(dpp_u32<0x141>(__float_as_uint(top))));
+            if (M != -INFINITY) S *= exp((double)M - (double)top);
+#pragma unroll
+            for (int k = 0; k < P; ++k)
+                if (i0 + 8 * k < p.nsplit) S += m[k] == -INFINITY ? s[k] : s[k] * exp((double)m[k] - (double)top);
             M = top;
         }
 #pragma unroll
-        for (int d = 1; d < 8; d <<= 1) {
-            const float m = shfl_xor(M, d);
-            const double s = shfl_xor_d(S, d);
-            const float top = fmaxf(M, m);
-            S = (M == -INFINITY ? S : S * exp((double)M - (double)top)) +
-                (m == -INFINITY ? s : s * exp((double)m - (double)top));
-            M = top;
-        }
+        for (int d = 1; d < 8; d <<= 1) S += shfl_xor_d(S, d);
         if ((tid & 7) == 0) {
             // a NaN or +inf among the logits, or nothing above -inf: the sum is NaN, infinite or 0
             const double lse = (double)M + log(S);
@@ -267,25 +278,20 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
             }
         }
     };
-    if (held) {
-        uint64_t s[U], place[U];
+    for (int i0 = 0; i0 < total; i0 += 256 * U) {
+        if (i0) load(i0);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            s[u] = place[u] = 0;
-            if (tid + 256 * u < total) s[u] = candidate(tid + 256 * u, cand[u], place[u]);
-            best = max(best, (uint32_t)(s[u] >> 32));
-        }
-        const uint32_t least = wave_nth(best, p.beams);
+        for (int u = 0; u < U; ++u)
+            if (i0 + 256 * u < total && index(i0, u) < total)
+                best = max(best, (uint32_t)(candidate(index(i0, u), cand[u], at) >> 32));
+    }
+    const uint32_t least = wave_nth<4>(best, p.beams);
+    for (int i0 = 0; i0 < total; i0 += 256 * U) {
+        if (total > 256 * U) load(i0);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            at = place[u];
-            pick(s[u], least);
-        }
-    } else {
-        for (int i = tid; i < total; i += 256)
-            best = max(best, (uint32_t)(candidate(i, p.cand[row0 * per + i], at) >> 32));
-        const uint32_t least = wave_nth(best, p.beams);
-        for (int i = tid; i < total; i += 256) pick(candidate(i, p.cand[row0 * per + i], at), least);
+        for (int u = 0; u < U; ++u)
+            if (i0 + 256 * u < total && index(i0, u) < total)
+                pick(candidate(index(i0, u), cand[u], at), least);
     }
     __syncthreads();
     const int n = count;

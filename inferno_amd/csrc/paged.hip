@@ -24,6 +24,10 @@ __device__ __forceinline__ f32x4 mfma16x16x4(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ u32x4 ld16_nt(const char* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
+
 // The page that holds position j of a row, -1 where the table names none of the pool's.
 __device__ __forceinline__ int page_of(const PagedView& c, const int32_t* table, int j) {
     const int p = table[j >> c.page_shift];
@@ -201,7 +205,7 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
             const char* src = (const char*)(K + pg * p.c.sk.b + (key & mask) * p.c.sk.t) + 16 * g;
 #pragma unroll
             for (int s = 0; s < NK; ++s)
-                kr[t][s] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + 64 * s));
+                kr[t][s] = ld16_nt(src + 64 * s);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -219,7 +223,7 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
                 } else {
 #pragma unroll
                     for (int w = 0; w < VW; w += 4) {
-                        const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + 4 * w));
+                        const u32x4 x = ld16_nt(src + 4 * w);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) vr[t][r][w + e] = x[e];
                     }
@@ -814,8 +818,8 @@ __global__ __launch_bounds__(256) void kv_evict_move_kernel(KvEvictParams p, int
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int pg = max(ps[u], 0), slot = src[u] & mask;
-        kx[u] = *reinterpret_cast<const u32x4*>(K + (pg * p.c.sk.b + ko + slot * p.c.sk.t) * esz);
-        vx[u] = *reinterpret_cast<const u32x4*>(V + (pg * p.c.sv.b + vo + slot * p.c.sv.t) * esz);
+        kx[u] = ld16_nt(K + (pg * p.c.sk.b + ko + slot * p.c.sk.t) * esz);
+        vx[u] = ld16_nt(V + (pg * p.c.sv.b + vo + slot * p.c.sv.t) * esz);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -898,16 +902,18 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(BeamReorderParams p, 
         const int64_t vo = layer * p.v_layer + h * p.c.sv.h + t * p.c.sv.t;
         const u32x4 kx = *reinterpret_cast<const u32x4*>((const char*)p.c.k + (ko + src * p.c.sk.b) * esz + 16 * c);
         const u32x4 vx = *reinterpret_cast<const u32x4*>((const char*)p.c.v + (vo + src * p.c.sv.b) * esz + 16 * c);
-        *reinterpret_cast<u32x4*>((char*)p.c.k + (ko + dst * p.c.sk.b) * esz + 16 * c) = kx;
-        *reinterpret_cast<u32x4*>((char*)p.c.v + (vo + dst * p.c.sv.b) * esz + 16 * c) = vx;
+        __builtin_nontemporal_store(
+            kx, reinterpret_cast<u32x4*>((char*)p.c.k + (ko + dst * p.c.sk.b) * esz + 16 * c));
+        __builtin_nontemporal_store(
+            vx, reinterpret_cast<u32x4*>((char*)p.c.v + (vo + dst * p.c.sv.b) * esz + 16 * c));
     }
 }
 
 int launch_beam_reorder(const BeamReorderParams& p, int bf16, hipStream_t s) {
     const int esz = bf16 ? 2 : 4, pieces = p.c.D * esz / 16;
-    // pieces of a whole page; a workgroup takes up to four rounds of them
+    // pieces of a whole page; a workgroup takes up to two rounds of them
     const int64_t n = ((int64_t)p.c.heads * pieces << p.c.page_shift);
-    int64_t z = (n + 1023) / 1024;
+    int64_t z = (n + 511) / 512;
     if (z > 1024) z = 1024;
     const dim3 grid((unsigned)p.c.rows, (unsigned)p.layers, (unsigned)z);
     hipLaunchKernelGGL(beam_reorder_kernel, grid, dim3(256), 0, s, p, pieces, esz);
