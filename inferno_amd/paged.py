@@ -15,20 +15,25 @@ from . import InfernoError, PagedKVStruct, Strides, default_scale, lib
 from .ops import _check, _dt, strides_of
 
 
+# the current stream's handle on a device; the public spelling costs as much as a launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 @contextlib.contextmanager
-def _launch(device, stream):
-    """The stream handle to launch on, with the device current and, where a stream is given, new
-    tensors allocated for that stream."""
-    if device.type != "cuda":
-        raise ValueError(f"tensors on the GPU expected, got {device}")
+def _on(device, stream):
+    """The device, and the stream where one is given, made current: new tensors belong to it."""
     if stream is not None and not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=device)
-    with contextlib.ExitStack() as stack:
-        if stream is not None:
-            stack.enter_context(torch.cuda.stream(stream))
-        elif device.index is not None and device.index != torch.cuda.current_device():
-            stack.enter_context(torch.cuda.device(device))
-        yield torch.cuda.current_stream().cuda_stream
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        yield
+
+
+def _elsewhere(device, stream):
+    """Whether a call on tensors of this device has to make another device or stream current first."""
+    if device.type != "cuda":
+        raise ValueError(f"tensors on the GPU expected, got {device}")
+    return stream is not None or device.index != torch.cuda.current_device()
 
 
 def _of(t, name, dtype, device, shape=None):
@@ -53,14 +58,12 @@ def _size(call, *args) -> int:
 
 
 def _workspace(ws, nbytes, device):
-    """(tensor, pointer, bytes) of the workspace: the caller's, else a new one."""
+    """(tensor, pointer, bytes) of the workspace: the caller's, else a new one of nbytes() bytes."""
     if ws is None:
-        if callable(nbytes):
-            nbytes = nbytes()
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.empty(nbytes(), dtype=torch.uint8, device=device)
     elif ws.device != device or not ws.is_contiguous():
         raise ValueError(f"workspace: a dense tensor on {device} expected")
-    return ws, ws.data_ptr() or None, ws.numel() * ws.element_size()
+    return ws, ws.data_ptr() or None, ws.nbytes
 
 
 class PagedKV:
@@ -85,6 +88,7 @@ class PagedKV:
         self.k, self.v, self._table, self._lens = k, v, table, lens
         self.device, self.dtype = k.device, k.dtype
         self.layers = k.shape[0] if k.dim() == 5 else 1
+        self.layer_strides = (k.stride(0), v.stride(0)) if k.dim() == 5 else (0, 0)
         pages, heads, page_size, D = k.shape[-4:]
         self.rows, self.heads, self.D, self.page_size = table.shape[0], heads, D, page_size
         self.capacity = table.shape[1] * page_size
@@ -93,6 +97,9 @@ class PagedKV:
                                     self._row_stride(table), self.rows, heads, D, page_size, table.shape[1], pages,
                                     _dt(k))
         self.ref = ctypes.byref(self.struct)
+        self.meta_shape = (self.rows, heads, self.capacity)
+        self.scale = default_scale(D)
+        self.sizes = {}  # workspace bytes by call and arguments
 
     @staticmethod
     def _row_stride(table):
@@ -128,7 +135,7 @@ class PagedKV:
 
     def meta(self, dtype):
         """Zeros [rows, heads, capacity]: room for the weights (float32) or positions (int32)."""
-        return torch.zeros((self.rows, self.heads, self.capacity), dtype=dtype, device=self.device)
+        return torch.zeros(self.meta_shape, dtype=dtype, device=self.device)
 
 
 def _one_layer(cache, what):
@@ -136,34 +143,41 @@ def _one_layer(cache, what):
         raise ValueError(f"{what}: the cache of one layer expected (PagedKV.layer)")
 
 
-def _meta_shape(cache):
-    return (cache.rows, cache.heads, cache.capacity)
+def _bytes(cache, call, *args):
+    """The workspace bytes that the C-ABI's `call` gives, asked once per cache and arguments."""
+    n = cache.sizes.get((call, args))
+    if n is None:
+        n = cache.sizes[call, args] = _size(getattr(lib(), call), cache.ref, *args)
+    return n
 
 
 def kv_append(cache, k, v, counts=None, weights=None, positions=None, seen=None, stream=None):
     """Writes k, v [rows, heads, T, D] as the rows' last positions (``cache.lens`` counts them
     already); ``counts`` int32 [rows]: how many of the T tokens a row has.  ``weights`` float32
     and ``positions`` int32 [rows, heads, capacity] are set for the new tokens."""
-    _one_layer(cache, "kv_append")
-    if k.shape != v.shape or k.dim() != 4 or k.shape[:2] != (cache.rows, cache.heads) or k.shape[3] != cache.D:
-        raise ValueError("kv_append: k and v [rows, heads, T, D] of the cache's rows, heads and D expected")
     dev = cache.device
+    _one_layer(cache, "kv_append")
+    shape = k.shape
+    if v.shape != shape or len(shape) != 4 or shape[0] != cache.rows or shape[1] != cache.heads or shape[3] != cache.D:
+        raise ValueError("kv_append: k and v [rows, heads, T, D] of the cache's rows, heads and D expected")
     if k.dtype != cache.dtype or v.dtype != cache.dtype:
         raise TypeError("kv_append: k and v must have the cache's dtype")
     if k.device != dev or v.device != dev:
         raise ValueError(f"kv_append: k and v must be on {dev}")
     rows = (cache.rows,)
-    with _launch(dev, stream) as s:
-        st = lib().inf_kv_append(cache.ref, k.data_ptr(), strides_of(k), v.data_ptr(), strides_of(v),
-                                 _of(counts, "counts", torch.int32, dev, rows), k.shape[2],
-                                 _of(weights, "weights", torch.float32, dev, _meta_shape(cache)),
-                                 _of(positions, "positions", torch.int32, dev, _meta_shape(cache)),
-                                 _of(seen, "seen", torch.int32, dev, rows), s)
+    pc, ps = _of(counts, "counts", torch.int32, dev, rows), _of(seen, "seen", torch.int32, dev, rows)
+    pw = _of(weights, "weights", torch.float32, dev, cache.meta_shape)
+    pp = _of(positions, "positions", torch.int32, dev, cache.meta_shape)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return kv_append(cache, k, v, counts, weights, positions, seen)
+    st = lib().inf_kv_append(cache.ref, k.data_ptr(), strides_of(k), v.data_ptr(), strides_of(v), pc, shape[2], pw, pp,
+                             ps, _raw_stream(dev.index))
     _check(st, "inf_kv_append")
 
 
 def _decode_bytes(cache, q_heads, max_len, weights):
-    return _size(lib().inf_attn_decode_paged_workspace, cache.ref, q_heads, max_len, int(bool(weights)))
+    return _bytes(cache, "inf_attn_decode_paged_workspace", q_heads, max_len, int(bool(weights)))
 
 
 def attn_decode_paged_workspace(cache, q_heads, max_len=None, weights=False):
@@ -178,33 +192,36 @@ def attn_decode_paged(q, cache, scale=None, max_len=None, weights=None, weights_
     positions.  ``max_len`` bounds the lengths (the capacity by default).  ``weights_out`` (float32
     [rows, heads, capacity]) gets ``weights`` (zeros if None, may be the same tensor) plus every position's
     probabilities, summed over the query heads of its head."""
-    _one_layer(cache, "attn_decode_paged")
-    if q.dim() != 4 or q.shape[0] != cache.rows or q.shape[2] != 1 or q.shape[3] != cache.D:
-        raise ValueError("attn_decode_paged: q [rows, q_heads, 1, D] of the cache's rows and D expected")
     dev = cache.device
+    _one_layer(cache, "attn_decode_paged")
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != cache.rows or shape[2] != 1 or shape[3] != cache.D:
+        raise ValueError("attn_decode_paged: q [rows, q_heads, 1, D] of the cache's rows and D expected")
     if q.dtype != cache.dtype or q.device != dev:
         raise ValueError(f"attn_decode_paged: q must be {cache.dtype} on {dev}")
     if weights is not None and weights_out is None:
         raise ValueError("attn_decode_paged: weights without weights_out")
-    heads = q.shape[1]
+    heads = shape[1]
     max_len = cache.capacity if max_len is None else int(max_len)
-    scale = default_scale(cache.D) if scale is None else float(scale)
-    w_in = _of(weights, "weights", torch.float32, dev, _meta_shape(cache))
-    w_out = _of(weights_out, "weights_out", torch.float32, dev, _meta_shape(cache))
-    with _launch(dev, stream) as s:
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-            raise ValueError("attn_decode_paged: out must be like q")
-        ws, ptr, n = _workspace(workspace, lambda: _decode_bytes(cache, heads, max_len, w_out), dev)
-        st = lib().inf_attn_decode_paged(cache.ref, q.data_ptr(), strides_of(q), out.data_ptr(), strides_of(out), heads,
-                                         max_len, scale, w_in, w_out, ptr, n, s)
+    w_in = _of(weights, "weights", torch.float32, dev, cache.meta_shape)
+    w_out = _of(weights_out, "weights_out", torch.float32, dev, cache.meta_shape)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return attn_decode_paged(q, cache, scale, max_len, weights, weights_out, out, workspace)
+    if out is None:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != q.dtype or out.device != dev:
+        raise ValueError("attn_decode_paged: out must be like q")
+    ws, ptr, n = _workspace(workspace, lambda: _decode_bytes(cache, heads, max_len, w_out), dev)
+    st = lib().inf_attn_decode_paged(cache.ref, q.data_ptr(), strides_of(q), out.data_ptr(), strides_of(out), heads,
+                                     max_len, cache.scale if scale is None else float(scale), w_in, w_out, ptr, n,
+                                     _raw_stream(dev.index))
     _check(st, "inf_attn_decode_paged")
     return out
 
 
 def _evict_bytes(cache, keep, max_len):
-    return _size(lib().inf_kv_evict_workspace, cache.ref, keep, max_len)
+    return _bytes(cache, "inf_kv_evict_workspace", keep, max_len)
 
 
 def kv_evict_workspace(cache, keep, max_len=None):
@@ -218,28 +235,35 @@ def kv_evict(cache, weights, positions, keep, recent=0, weights_out=None, positi
     """Cuts every row and head to its ``keep`` positions of the largest weights, the ``recent`` newest
     among them, in place in the pools.  ``weights_out`` and ``positions_out`` are the inputs
     by default; returns the new lengths (``lens_out``, which may be ``cache.lens``)."""
+    dev = cache.device
     _one_layer(cache, "kv_evict")
-    dev, keep = cache.device, int(keep)
+    keep, meta = int(keep), cache.meta_shape
     max_len = cache.capacity if max_len is None else int(max_len)
-    meta = _meta_shape(cache)
-    weights_out = weights if weights_out is None else weights_out
-    positions_out = positions if positions_out is None else positions_out
-    with _launch(dev, stream) as s:
-        if lens_out is None:
-            lens_out = torch.empty(cache.rows, dtype=torch.int32, device=dev)
-        ws, ptr, n = _workspace(workspace, lambda: _evict_bytes(cache, keep, max_len), dev)
-        st = lib().inf_kv_evict(cache.ref, _of(weights, "weights", torch.float32, dev, meta),
-                                _of(weights_out, "weights_out", torch.float32, dev, meta),
-                                _of(positions, "positions", torch.int32, dev, meta),
-                                _of(positions_out, "positions_out", torch.int32, dev, meta),
-                                _of(lens_out, "lens_out", torch.int32, dev, (cache.rows,)), keep, int(recent), max_len,
-                                ptr, n, s)
+    pw, pp = _of(weights, "weights", torch.float32, dev, meta), _of(positions, "positions", torch.int32, dev, meta)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return kv_evict(cache, weights, positions, keep, recent, weights_out, positions_out, lens_out, max_len,
+                            workspace)
+    if lens_out is None:
+        lens_out = cache.lens.new_empty(cache.rows)
+    ws, ptr, n = _workspace(workspace, lambda: _evict_bytes(cache, keep, max_len), dev)
+    st = lib().inf_kv_evict(cache.ref, pw,
+                            pw if weights_out is None else _of(weights_out, "weights_out", torch.float32, dev, meta), pp,
+                            pp if positions_out is None else _of(positions_out, "positions_out", torch.int32, dev, meta),
+                            _of(lens_out, "lens_out", torch.int32, dev, (cache.rows,)), keep, int(recent), max_len, ptr,
+                            n, _raw_stream(dev.index))
     _check(st, "inf_kv_evict")
     return lens_out
 
 
+_select_sizes = {}
+
+
 def _select_bytes(groups, beams, vocab):
-    return _size(lib().inf_beam_select_workspace, groups, beams, vocab)
+    n = _select_sizes.get((groups, beams, vocab))
+    if n is None:
+        n = _select_sizes[groups, beams, vocab] = _size(lib().inf_beam_select_workspace, groups, beams, vocab)
+    return n
 
 
 def beam_select_workspace(groups, beams, vocab, device="cuda"):
@@ -250,30 +274,33 @@ def beam_select_workspace(groups, beams, vocab, device="cuda"):
 def beam_select(logits, scores, finished=None, eos=None, workspace=None, stream=None):
     """(tokens, parents, scores, finished) of the best continuations: logits [groups * beams, vocab],
     scores float32 and finished int32 [groups, beams].  ``finished`` is None in the result
-    where it is None and no ``eos`` is given."""
+    where no ``eos`` is given."""
+    dev = logits.device
     if scores.dim() != 2 or logits.dim() != 2 or logits.shape[0] != scores.numel():
         raise ValueError("beam_select: logits [groups * beams, vocab] and scores [groups, beams] expected")
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"beam_select: float32 or bfloat16 logits expected, got {logits.dtype}")
-    if logits.shape[1] > 1 and logits.stride(1) != 1:
-        raise ValueError("beam_select: the logits of a row must be adjacent")
-    dev, vocab = logits.device, logits.shape[1]
-    groups, beams = scores.shape
     if finished is not None and eos is None:
         raise ValueError("beam_select: finished beams need eos")
-    pf = _of(finished, "finished", torch.int32, dev, scores.shape)
-    ps = _of(scores, "scores", torch.float32, dev)
-    with _launch(dev, stream) as s:
-        tokens, parents = (torch.empty(scores.shape, dtype=torch.int32, device=dev) for _ in range(2))
-        scores_out = torch.empty(scores.shape, dtype=torch.float32, device=dev)
-        done = torch.empty(scores.shape, dtype=torch.int32, device=dev) if eos is not None else None
-        ws, ptr, n = _workspace(workspace, lambda: _select_bytes(groups, beams, vocab), dev)
-        st = lib().inf_beam_select(logits.data_ptr(), logits.stride(0) if logits.shape[0] > 1 else vocab, ps, pf, groups,
-                                   beams, vocab, -1 if eos is None else int(eos), tokens.data_ptr(),
-                                   parents.data_ptr(), scores_out.data_ptr(),
-                                   done.data_ptr() if done is not None else None, _dt(logits), ptr, n, s)
+    shape = scores.shape
+    ps, pf = _of(scores, "scores", torch.float32, dev), _of(finished, "finished", torch.int32, dev, shape)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return beam_select(logits, scores, finished, eos, workspace)
+    vocab, (ld, step) = logits.shape[1], logits.stride()
+    if vocab > 1 and step != 1:
+        raise ValueError("beam_select: the logits of a row must be adjacent")
+    groups, beams = shape
+    # tokens, parents and finished side by side
+    ints = scores.new_empty((3, groups, beams), dtype=torch.int32)
+    scores_out, first, n_ints = scores.new_empty(shape), ints.data_ptr(), 4 * groups * beams
+    ws, ptr, n = _workspace(workspace, lambda: _select_bytes(groups, beams, vocab), dev)
+    st = lib().inf_beam_select(logits.data_ptr(), ld if logits.shape[0] > 1 else max(ld, vocab), ps, pf, groups, beams,
+                               vocab, -1 if eos is None else int(eos), first, first + n_ints, scores_out.data_ptr(),
+                               None if eos is None else first + 2 * n_ints, _dt(logits), ptr, n, _raw_stream(dev.index))
     _check(st, "inf_beam_select")
-    return tokens, parents, scores_out, done
+    tokens, parents, done = ints.unbind()
+    return tokens, parents, scores_out, None if eos is None else done
 
 
 def beam_reorder(cache, parents, spare, table_out=None, spare_out=None, stream=None):
@@ -284,18 +311,18 @@ def beam_reorder(cache, parents, spare, table_out=None, spare_out=None, stream=N
     if parents.dim() != 2 or parents.numel() != cache.rows:
         raise ValueError("beam_reorder: parents [groups, beams] of the cache's rows expected")
     pp = _of(parents, "parents", torch.int32, dev)
-    ps = _of(spare, "spare", torch.int32, dev, (cache.rows,))
-    layered = cache.k.dim() == 5
-    with _launch(dev, stream) as s:
-        if table_out is None:
-            table_out = torch.empty(cache.table.shape, dtype=torch.int32, device=dev)
-        if spare_out is None:
-            spare_out = torch.empty(cache.rows, dtype=torch.int32, device=dev)
-        st = lib().inf_beam_reorder(cache.ref, cache.layers, cache.k.stride(0) if layered else 0,
-                                    cache.v.stride(0) if layered else 0, pp, parents.shape[1],
-                                    _of(table_out, "table_out", torch.int32, dev, cache.table.shape),
-                                    cache.table.shape[1], ps,
-                                    _of(spare_out, "spare_out", torch.int32, dev, (cache.rows,)), s)
+    ps = _of(spare, "spare", torch.int32, dev, cache.lens.shape)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return beam_reorder(cache, parents, spare, table_out, spare_out)
+    shape = cache.table.shape
+    if table_out is None:
+        table_out = spare.new_empty(shape)
+    if spare_out is None:
+        spare_out = spare.new_empty(spare.shape)
+    st = lib().inf_beam_reorder(cache.ref, cache.layers, *cache.layer_strides, pp, parents.shape[1],
+                                _of(table_out, "table_out", torch.int32, dev, shape), shape[1], ps,
+                                _of(spare_out, "spare_out", torch.int32, dev, spare.shape), _raw_stream(dev.index))
     _check(st, "inf_beam_reorder")
     return table_out, spare_out
 
