@@ -85,23 +85,25 @@ int check_cache(const inf_paged_kv* c, bool written, inf::PagedView* out) {
 
 int64_t capacity(const inf_paged_kv* c) { return (int64_t)c->max_pages * c->page_size; }
 
-// The part of the decode's workspace that holds the splits' results, and the scores behind it.
+// The decode's workspace: the shares' results (one per row and share that meet, so at most rows +
+// shares), the rows' first steps, the scores.
 struct DecodeSizes {
-    int nsplit, chunk;
+    int groups;
     int64_t score_ld;
-    size_t part, stats, scores;
-    size_t total() const { return part + stats + scores; }
+    size_t part, stats, first, scores;
+    size_t total() const { return part + stats + first + scores; }
 };
 DecodeSizes decode_sizes(const inf_paged_kv* c, int q_heads, int max_len, bool weights) {
     DecodeSizes s{};
-    inf::paged_decode_plan(c->rows, c->heads, q_heads / c->heads, max_len, c->D, c->dt == INF_BF16, &s.nsplit, &s.chunk);
-    s.score_ld = (int64_t)s.nsplit * s.chunk;
-    const size_t rows = (size_t)c->rows * q_heads;
-    if (s.nsplit > 1 || weights) {
-        s.part = round_up(rows * s.nsplit * c->D * sizeof(float));
-        s.stats = round_up(rows * s.nsplit * 2 * sizeof(float));
-    }
-    if (weights) s.scores = round_up(rows * s.score_ld * sizeof(float));
+    const int bf16 = c->dt == INF_BF16, step = inf::paged_step(c->D, bf16), blocks = inf::paged_blocks(c->rows);
+    s.groups = inf::paged_groups(c->rows, c->heads, q_heads / c->heads, max_len, c->D, bf16, weights);
+    if (s.groups == 0) return s;
+    const size_t parts = ((size_t)c->rows + (size_t)blocks * s.groups) * q_heads;
+    s.part = round_up(parts * c->D * sizeof(float));
+    s.stats = round_up(parts * 2 * sizeof(float));
+    s.first = round_up(((size_t)c->rows + blocks) * sizeof(int32_t));
+    s.score_ld = ((int64_t)max_len + step - 1) / step * step;
+    if (weights) s.scores = round_up((size_t)c->rows * q_heads * s.score_ld * sizeof(float));
     return s;
 }
 
@@ -110,6 +112,10 @@ int check_decode(const inf_paged_kv* c, int q_heads, int max_len) {
     if (st != INF_OK) return st;
     if (q_heads < 1 || q_heads % c->heads || max_len < 1 || max_len > capacity(c)) return INF_ERR_BAD_SHAPE;
     if ((int64_t)c->rows * q_heads > (1 << 24)) return INF_ERR_BAD_SHAPE;
+    // the steps of a block of rows are counted in 32 bits
+    if ((int64_t)std::min(c->rows, inf::kPagedBlock) * (max_len / inf::paged_step(c->D, c->dt == INF_BF16) + 1) >
+        (1 << 30))
+        return INF_ERR_BAD_SHAPE;
     return INF_OK;
 }
 
@@ -187,7 +193,8 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
     if (weights_in && !weights_out) return INF_ERR_NULL_POINTER;
     const DecodeSizes s = decode_sizes(cache, q_heads, max_len, weights_out != nullptr);
     const int64_t tiles = (q_heads / cache->heads + 15) / 16;
-    if ((int64_t)cache->rows * cache->heads * s.nsplit * tiles > kMaxBlocks ||
+    if ((int64_t)cache->rows * cache->heads * tiles > kMaxBlocks / 16 ||
+        (int64_t)cache->heads * tiles * s.groups > kMaxBlocks ||
         (int64_t)cache->rows * (q_heads + (int64_t)cache->heads * ((max_len + 1023) / 1024)) > kMaxBlocks)
         return INF_ERR_BAD_SHAPE;
     if (s.total() && (!workspace || ws_bytes < s.total())) return INF_ERR_WORKSPACE;
@@ -198,13 +205,13 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
     p.G = q_heads / cache->heads;
     p.head_tiles = (int)tiles;
     p.max_len = max_len;
-    p.nsplit = s.nsplit;
-    p.chunk = s.chunk;
+    p.groups = s.groups;
     p.cs = scale * 1.4426950408889634f;
     char* ws = static_cast<char*>(workspace);
     p.part = reinterpret_cast<float*>(ws);
     p.stats = reinterpret_cast<float*>(ws + s.part);
-    if (weights_out) p.scores = reinterpret_cast<float*>(ws + s.part + s.stats);
+    p.first = reinterpret_cast<int32_t*>(ws + s.part + s.stats);
+    if (weights_out) p.scores = reinterpret_cast<float*>(ws + s.part + s.stats + s.first);
     p.score_ld = s.score_ld;
     p.w_in = weights_in;
     p.w_out = weights_out;

@@ -362,18 +362,23 @@ struct PagedDecodeParams {
     int Hq, G;             // query heads; of them per key-value head
     int head_tiles;        // tiles of 16 query heads per key-value head
     int max_len;
-    int nsplit, chunk;     // splits of a row, keys per split (a multiple of kPagedStep)
+    int groups;            // shares of a block of rows (see paged_split_kernel), or 0: a workgroup takes whole rows
     float cs;              // scale * log2(e)
-    float* part;           // workspace [rows * Hq, nsplit, D]: unnormalised o
-    float* stats;          // workspace [rows * Hq, nsplit, 2]: maximum (log2 domain) and sum
+    float* part;           // workspace [parts, Hq, D]: unnormalised o
+    float* stats;          // workspace [parts, Hq, 2]: maximum (log2 domain) and sum
+    int32_t* first;        // workspace [rows + blocks]: a row's first step in its block; the blocks' steps
     float* scores;         // workspace [rows * Hq, score_ld] (weights asked for) or null
     int64_t score_ld;
     const float* w_in;     // [rows, heads, cap] or null (zeros)
     float* w_out;          // [rows, heads, cap] or null
 };
-constexpr int kPagedStep = 128;      // keys a workgroup takes per step: 4 waves x 32
-constexpr int kPagedMaxSplit = 512;
-void paged_decode_plan(int rows, int heads, int G, int max_len, int D, int bf16, int* nsplit, int* chunk);
+constexpr int kPagedBlock = 64;       // rows whose steps are shared out together: one to a lane
+constexpr int kPagedMaxGroups = 1024;
+// Keys that a workgroup takes per step: 4 waves, each with 16 KB of keys and values in its registers.
+constexpr int paged_step(int D, int bf16) { return (32 << 10) / (D * (bf16 ? 2 : 4)); }
+inline int paged_blocks(int rows) { return (rows + kPagedBlock - 1) / kPagedBlock; }
+// Shares per block of rows, 0 where workgroups take whole rows.
+int paged_groups(int rows, int heads, int G, int max_len, int D, int bf16, bool weights);
 
 struct KvEvictParams {
     PagedView c;

@@ -5,6 +5,7 @@
 // page for every key-value head and for keys and values.  Page numbers come from device
 // memory, so each is checked against the pool's size before it is used: one out of range
 // is never followed (a store is dropped; attention makes the row NaN).
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -96,23 +97,56 @@ int launch_kv_append(const KvAppendParams& p, int bf16, hipStream_t s) {
 // Attention of one query per row: s_j = q k_j scale, p = softmax(s), o = sum_j p_j v_j, for
 // the G query heads of a key-value head at once.
 //
-// A workgroup takes `chunk` keys of one (row, key-value head), its waves 32 keys in turn, all on
-// the matrix cores with up to 16 query heads as the columns: S^T = K Q^T (keys x heads), then
-// O^T += V^T P^T (D x heads).  A head's scores, maximum, sum and output then lie in one
-// lane column, so that the softmax needs two exchanges per 32 keys, and each lane's 8
-// probabilities are the second product's operand as they are: its sum over keys may
-// run in any order, so the value rows are loaded in the order that the first product's result
-// has.  A lane holds D / 16 neighbouring columns of 8 value rows; one column of them is one
-// operand (bf16: eight 16-bit halves picked together; fp32: a register each).  Neither operand
-// passes through LDS, and a row of K or V is read from HBM once for all heads.  bf16
-// probabilities are taken in two parts (16 bits), whose products cost no time here.
+// The work is cut in steps of 64 to 512 keys of a row, 64 KB.  All steps of up to 64 rows, one after the other, are
+// shared out evenly to `groups` of workgroups, one workgroup per key-value head in each, as many as the
+// device holds at once: rows of any lengths keep it busy to the end.  (Chunks of a fixed size left a last
+// round of workgroups that was partly empty: 64 rows of 1 to 8191 positions, bf16, 8 heads of D 128 with 4
+// query heads each, took 203 us, 173 now: 957 MB at 5.5 TB/s.)
+// The heads of a group read the same pages at the same time, which lie next to each other: with the heads'
+// workgroups apart that case took 319 us instead of 225.  Where a share ends in the middle of a row, the
+// row's parts are joined by a second launch.
 //
-// Keys behind the end are read as the last one and their scores are -inf, their values zero, so
-// whatever their slots hold does not count.
+// A workgroup's waves take 32 keys of a step each, all on the matrix cores with up to 16 query heads as the
+// columns: S^T = K Q^T (keys x heads), then O^T += V^T P^T (D x heads).  A head's scores, maximum, sum and
+// output then lie in one lane column, so that the softmax needs two exchanges per 32 keys, and each lane's 8
+// probabilities are the second product's operand as they are: its sum over keys may run in any order, so
+// the value rows are loaded in the order that the first product's result has.  A lane holds D / 16
+// neighbouring columns of 8 value rows; one column of them is one operand (bf16: eight 16-bit halves picked
+// together; fp32: a register each).  Neither operand passes through LDS, and a row of K or V is read from
+// HBM once for all heads.  bf16 probabilities are taken in two parts (16 bits), whose products cost no time
+// here.
+//
+// Keys behind the end are read as the last one and their scores are -inf, their values zero, so whatever
+// their slots hold does not count.
 // ============================================================================
+namespace {
+
+constexpr int kPagedPerCu = 3;  // workgroups of a CU: what the registers allow
+
+template <int D, typename E>
+__device__ __forceinline__ int paged_steps(int len, int max_len) {
+    constexpr int step = paged_step(D, sizeof(E) == 2);
+    return len > max_len ? 0 : (max(len, 0) + step - 1) / step;
+}
+
+// `all` steps in `groups` shares, the first ones a step longer where they do not come out even.
+struct Shares {
+    int q, r;
+    __device__ __forceinline__ Shares(int all, int groups) : q(all / groups), r(all - q * groups) {}
+    __device__ __forceinline__ int start(int g) const { return g * q + min(g, r); }
+    __device__ __forceinline__ int of(int step) const {
+        const int big = r * (q + 1);
+        return step < big ? step / (q + 1) : r + (step - big) / q;
+    }
+};
+
+}  // namespace
+
 template <int D, typename E, bool SMALL>
-__global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
+__global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDecodeParams p) {
     constexpr int ES = sizeof(E);
+    constexpr int STEP = paged_step(D, ES == 2);
+    constexpr int T = STEP / 64;          // tiles of 16 keys per wave
     constexpr int NK = D * ES / 64;       // 16-byte pieces of a key row per lane
     constexpr int VD = D / 16;            // columns of a value row per lane
     constexpr int VW = VD * ES / 4;       // ... in 32-bit words
@@ -127,37 +161,69 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
         const int grp = blockIdx.x >> 3;
         tile = grp % ht;
         unit = grp / ht * 8 + (blockIdx.x & 7);
-        if (unit >= p.c.rows * p.c.heads * p.nsplit) return;
+        if (unit >= p.c.heads * (p.groups ? p.groups : p.c.rows)) return;
     }
-    const int h = unit % p.c.heads, rs = unit / p.c.heads;
-    const int split = rs % p.nsplit, row = rs / p.nsplit;
+    const int h = unit % p.c.heads, group = unit / p.c.heads;
     const int g0 = tile * 16, gn = min(16, p.G - g0);  // query heads of this tile
-    const bool direct = p.nsplit == 1 && !p.scores;
-    const int32_t* table = p.c.table + row * p.c.table_stride;
-    const int j0 = split * p.chunk, base0 = j0 + 32 * wave, last_page = p.c.max_pages - 1;
-    // Pages of 16 keys or more: one page for each half of a step, the same for all lanes, read a step
-    // ahead (behind the end, where the table may hold anything, they are not used).
-    int len = p.c.lens[row];
-    int next[2] = {0, 0};
-    auto read_pages = [&](int base) {
+    const int row0 = p.groups ? blockIdx.y * kPagedBlock : group;
+    const int nrows = p.groups ? min(kPagedBlock, p.c.rows - row0) : 1;
+
+    // Lane i: the first step of the block's row i.  This share's are [step, stop) of them; row r, the first
+    // one, has [begin, end).
+    const int mylen = lane < nrows ? p.c.lens[row0 + lane] : 0;
+    int step = 0, r = 0, begin = 0, steps = paged_steps<D, E>(mylen, p.max_len), starts = steps;
+    if (nrows > 1) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-            next[t] = table[min(__builtin_amdgcn_readfirstlane(base + 16 * t) >> p.c.page_shift, last_page)];
-    };
-    if constexpr (!SMALL) {
-        read_pages(base0);
-        asm volatile("" : "+s"(len), "+s"(next[0]), "+s"(next[1]));  // both waits at once
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(starts, d, 64);
+            if (lane >= d) starts += up;
+        }
     }
-    const int j1 = len > p.max_len ? 0 : min(len, j0 + p.chunk);
-    if (j0 >= j1) {
-        if (direct)  // an empty row is 0, one longer than max_len NaN
-            for (int i = tid; i < gn * D; i += 256)
-                store1((E*)p.o + row * p.so.b + (h * p.G + g0 + i / D) * p.so.h + i % D,
-                       len > p.max_len ? __builtin_nanf("") : 0.f);
-        return;
+    const int all = __builtin_amdgcn_readlane(starts, nrows - 1);
+    int stop = all, end = __builtin_amdgcn_readlane(starts, 0);
+    starts -= steps;
+    if (p.groups) {
+        if (unit == 0 && tile == 0 && wave == 0) {
+            if (lane < nrows) p.first[row0 + lane] = starts;
+            if (lane == 0) p.first[p.c.rows + blockIdx.y] = all;
+        }
+        const Shares shares(all, p.groups);
+        step = shares.start(group);
+        stop = shares.start(group + 1);
+    } else if (!all) {  // an empty row is 0, one longer than max_len NaN
+        const int len = __builtin_amdgcn_readlane(mylen, 0);
+        for (int i = tid; i < gn * D; i += 256)
+            store1((E*)p.o + row0 * p.so.b + (h * p.G + g0 + i / D) * p.so.h + i % D,
+                   len > p.max_len ? __builtin_nanf("") : 0.f);
     }
+    if (step >= stop) return;
+    if (nrows > 1) {
+        // the last row that starts at or before `step`
+        r = __popcll(__ballot(lane < nrows && starts <= step)) - 1;
+        begin = __builtin_amdgcn_readlane(starts, r);
+        end = r + 1 < nrows ? __builtin_amdgcn_readlane(starts, r + 1) : all;
+    }
+    const int mask = (1 << p.c.page_shift) - 1, last_page = p.c.max_pages - 1;
     const E* K = (const E*)p.c.k + h * p.c.sk.h;
     const E* V = (const E*)p.c.v + h * p.c.sv.h;
+    u32x4 kr[T][NK];
+    uint32_t vr[T][4][VW];
+
+    for (;;) {  // the rows of the share
+    const int row = row0 + r, s0 = step - begin, s1 = min(stop, end) - begin;
+    const int32_t* table = p.c.table + row * p.c.table_stride;
+    const int base0 = s0 * STEP + 16 * T * wave;
+    // Pages of 16 keys or more: one page for each tile of 16 keys, the same for all lanes, read a step
+    // ahead (behind the end, where the table may hold anything, they are not used).
+    const int len = __builtin_amdgcn_readlane(mylen, r);
+    int next[T] = {};
+    auto read_pages = [&](int base) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+            next[t] = table[min(__builtin_amdgcn_readfirstlane(base + 16 * t) >> p.c.page_shift, last_page)];
+    };
+    if constexpr (!SMALL) read_pages(base0);
+    const int j1 = min(len, s1 * STEP);
 
     // Q^T: column = head, rows 16 bytes of d as the key rows are read
     u32x4 qf[NK];
@@ -176,25 +242,22 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
     for (int j = 0; j < VD; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     bool bad = false;
-    const int mask = (1 << p.c.page_shift) - 1;
     float* sc = p.scores ? p.scores + ((int64_t)row * p.Hq + h * p.G + g0 + col) * p.score_ld : nullptr;
 
-    u32x4 kr[2][NK];
-    uint32_t vr[2][4][VW];
-    for (int base = base0; base < j1; base += kPagedStep) {
+    for (int base = base0; base < j1; base += STEP) {
         // rows behind the end are read as the last key's
-        int page[2] = {next[0], next[1]};
+        int page[T] = {};
         if constexpr (!SMALL) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const bool in = (unsigned)page[t] < (unsigned)p.c.n_pages;
+            for (int t = 0; t < T; ++t) {
+                const bool in = (unsigned)next[t] < (unsigned)p.c.n_pages;
                 bad |= !in && base + 16 * t < j1;
-                page[t] = in ? page[t] : 0;
+                page[t] = in ? next[t] : 0;
             }
-            if (base + kPagedStep < j1) read_pages(base + kPagedStep);
+            if (base + STEP < j1) read_pages(base + STEP);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < T; ++t) {
             const int key = min(base + 16 * t + col, j1 - 1);
             int pg = page[t];
             if constexpr (SMALL) {
@@ -208,11 +271,15 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
                 kr[t][s] = ld16_nt(src + 64 * s);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t) {
+            // pages of four keys or more: one page for the lane's four
+            int pg = page[t];
+            if constexpr (SMALL) pg = max(page_of(p.c, table, min(base + 16 * t + 4 * g, j1 - 1)), 0);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int key = min(base + 16 * t + 4 * g + r, j1 - 1);
-                const int pg = SMALL ? max(page_of(p.c, table, key), 0) : page[t];
+                if constexpr (SMALL)
+                    if (r && p.c.page_shift < 2) pg = max(page_of(p.c, table, key), 0);
                 const char* src = (const char*)(V + pg * p.c.sv.b + (key & mask) * p.c.sv.t + VD * col);
                 if constexpr (VW == 1) {
                     vr[t][r][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(src));
@@ -229,10 +296,11 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
                     }
                 }
             }
+        }
         __builtin_amdgcn_sched_barrier(0);  // all of the step's loads before its first product
-        f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        f32x4 st[T] = {};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < T; ++t)
 #pragma unroll
             for (int s = 0; s < NK; ++s) {
                 if constexpr (ES == 2) {
@@ -244,12 +312,12 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
                         st[t] = mfma16x16x4(__uint_as_float(kr[t][s][e]), __uint_as_float(qf[s][e]), st[t]);
                 }
             }
-        float x[8];
+        float x[4 * T];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = st[i >> 2][i & 3] * p.cs;
-        if (base + 32 > j1) {
+        for (int i = 0; i < 4 * T; ++i) x[i] = st[i >> 2][i & 3] * p.cs;
+        if (base + 16 * T > j1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4 * T; ++i)
                 if (base + 16 * (i >> 2) + 4 * g + (i & 3) >= j1) {
                     x[i] = -INFINITY;
 #pragma unroll
@@ -258,13 +326,13 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
         }
         if (sc && col < gn) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < T; ++t)
                 *reinterpret_cast<f32x4*>(sc + base + 16 * t + 4 * g) =
                     f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
         }
         float mx = m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, x[i]);
+        for (int i = 0; i < 4 * T; ++i) mx = fmaxf(mx, x[i]);
         mx = max_xor32(max_xor16(mx));
         const float ref = mx == -INFINITY ? 0.f : mx;  // no key above -inf yet: keep everything at 0
         const float alpha = fast_exp2(m - ref);
@@ -272,36 +340,38 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
         l *= alpha;
 #pragma unroll
         for (int j = 0; j < VD; ++j) acc[j] *= alpha;
-        float pr[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            pr[i] = fast_exp2(x[i] - ref);
-            l += pr[i];
+        for (int i = 0; i < 4 * T; ++i) {
+            x[i] = fast_exp2(x[i] - ref);
+            l += x[i];
         }
         if constexpr (ES == 2) {
-            bf16x8 ph, pm;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                ph[i] = (__bf16)pr[i];
-                pm[i] = (__bf16)(pr[i] - (float)ph[i]);
-            }
+            for (int t = 0; t < T; t += 2) {  // 32 keys a product
+                bf16x8 ph, pm;
 #pragma unroll
-            for (int j = 0; j < VD; ++j) {
-                const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;  // high or low halves of two words
-                u32x4 a;
+                for (int i = 0; i < 8; ++i) {
+                    ph[i] = (__bf16)x[4 * t + i];
+                    pm[i] = (__bf16)(x[4 * t + i] - (float)ph[i]);
+                }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    a[i] = __builtin_amdgcn_perm(vr[i >> 1][2 * (i & 1) + 1][j >> 1], vr[i >> 1][2 * (i & 1)][j >> 1],
-                                                 sel);
-                acc[j] = mfma16x16x32bf16(__builtin_bit_cast(bf16x8, a), ph, acc[j]);
-                acc[j] = mfma16x16x32bf16(__builtin_bit_cast(bf16x8, a), pm, acc[j]);
+                for (int j = 0; j < VD; ++j) {
+                    const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;  // high or low halves of two words
+                    u32x4 a;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        a[i] = __builtin_amdgcn_perm(vr[t + (i >> 1)][2 * (i & 1) + 1][j >> 1],
+                                                     vr[t + (i >> 1)][2 * (i & 1)][j >> 1], sel);
+                    acc[j] = mfma16x16x32bf16(__builtin_bit_cast(bf16x8, a), ph, acc[j]);
+                    acc[j] = mfma16x16x32bf16(__builtin_bit_cast(bf16x8, a), pm, acc[j]);
+                }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4 * T; ++i)
 #pragma unroll
                 for (int j = 0; j < VD; ++j)
-                    acc[j] = mfma16x16x4(__uint_as_float(vr[i >> 2][i & 3][j]), pr[i], acc[j]);
+                    acc[j] = mfma16x16x4(__uint_as_float(vr[i >> 2][i & 3][j]), x[i], acc[j]);
         }
     }
 
@@ -335,22 +405,47 @@ __global__ __launch_bounds__(256) void paged_split_kernel(PagedDecodeParams p) {
             o += lds[(w * gn + head) * LD + d] * wt;
         }
         const int hq = h * p.G + g0 + head;
-        if (direct) {
+        if (!p.groups) {
             store1((E*)p.o + row * p.so.b + hq * p.so.h + d, o / L);
         } else {
-            const int64_t at = ((int64_t)row * p.Hq + hq) * p.nsplit + split;
+            // rows and shares meet in one order: row + share is a number of their own
+            const int64_t at = ((int64_t)row + blockIdx.y * p.groups + group) * p.Hq + hq;
             p.part[at * D + d] = o;
             if (d == 0) *reinterpret_cast<f32x2*>(p.stats + 2 * at) = f32x2{M, L};
         }
     }
+    step += s1 - s0;
+    if (step >= stop) return;
+    begin = step;
+    do {  // past empty rows
+        ++r;
+        end = r + 1 < nrows ? __builtin_amdgcn_readlane(starts, r + 1) : all;
+    } while (end <= step);
+    __syncthreads();  // the join's LDS is read
+    }
 }
 
-// Joins the splits: the first rows * Hq workgroups write o, the others (where weights are asked
+// The parts of a row: their number, and the first one's place in `part` and `stats` (in steps of Hq).
+struct RowParts {
+    int n;
+    int64_t at;
+};
+template <int D, typename E>
+__device__ __forceinline__ RowParts row_parts(const PagedDecodeParams& p, int row, int len) {
+    const int steps = paged_steps<D, E>(len, p.max_len);
+    if (!steps) return {0, 0};
+    const int block = row / kPagedBlock, start = p.first[row], all = p.first[p.c.rows + block];
+    const Shares shares(all, p.groups);
+    const int g0 = shares.of(start), g1 = shares.of(start + steps - 1);
+    return {g1 - g0 + 1, (int64_t)row + block * p.groups + g0};
+}
+
+// Joins the parts: the first rows * Hq workgroups write o, the others (where weights are asked
 // for) take 1024 positions of a (row, key-value head) each and add the heads' probabilities
 // exp2(score - max) / sum to the weights, in the order of the heads.
 template <int D, typename E>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, int wblocks, int wide) {
-    __shared__ float wsh[kPagedMaxSplit];
+    __shared__ float wsh[kPagedMaxGroups];
     __shared__ float osh[256];
     __shared__ float top[8], inv[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -359,20 +454,20 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
         const int row = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq;
         const int len = p.c.lens[row];
         E* out = (E*)p.o + row * p.so.b + hq * p.so.h;
-        if (len <= 0 || len > p.max_len) {
-            if (tid < D) store1(out + tid, len <= 0 ? 0.f : __builtin_nanf(""));
+        const RowParts parts = row_parts<D, E>(p, row, len);
+        if (!parts.n) {
+            if (tid < D) store1(out + tid, len > p.max_len ? __builtin_nanf("") : 0.f);
             return;
         }
-        const int ns = (len + p.chunk - 1) / p.chunk;
-        const float* part = p.part + (int64_t)blockIdx.x * p.nsplit * D;
-        const f32x2* stats = reinterpret_cast<const f32x2*>(p.stats) + (int64_t)blockIdx.x * p.nsplit;
+        const int64_t at = parts.at * p.Hq + hq;  // part i: Hq further on each
+        const f32x2* stats = reinterpret_cast<const f32x2*>(p.stats) + at;
         float M = -INFINITY;
-        for (int i = lane; i < ns; i += 64) M = fmaxf(M, stats[i][0]);
+        for (int i = lane; i < parts.n; i += 64) M = fmaxf(M, stats[(int64_t)i * p.Hq][0]);
         M = wave_max(M);
         const float ref = M == -INFINITY ? 0.f : M;
         float L = 0.f;
-        for (int i = lane; i < ns; i += 64) {
-            const f32x2 x = stats[i];
+        for (int i = lane; i < parts.n; i += 64) {
+            const f32x2 x = stats[(int64_t)i * p.Hq];
             const float w = fast_exp2(x[0] - ref);
             L += x[1] * w;
             if (wave == 0) wsh[i] = w;
@@ -381,9 +476,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
         __syncthreads();
         constexpr int NG = 256 / D;
         const int d = tid % D, grp = tid / D;
+        const float* part = p.part + at * D + d;
         float o = 0.f;
 #pragma unroll 8
-        for (int i = grp; i < ns; i += NG) o += part[(int64_t)i * D + d] * wsh[i];
+        for (int i = grp; i < parts.n; i += NG) o += part[(int64_t)i * p.Hq * D] * wsh[i];
         osh[tid] = o;
         __syncthreads();
         if (tid < D) {
@@ -400,7 +496,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
     const int len = p.c.lens[row];
     const int n = min(len, p.max_len);
     if (j0 >= n) return;
-    const int ns = (n + p.chunk - 1) / p.chunk;
+    const RowParts parts = row_parts<D, E>(p, row, len);
     const int64_t hq0 = (int64_t)row * p.Hq + h * p.G;
     const int j = j0 + 4 * tid;  // this thread's 4 positions; scores are padded to whole steps
     f32x4 w = {0.f, 0.f, 0.f, 0.f};
@@ -413,23 +509,21 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
             if (i < gn && j < n)
                 sc[i] = *reinterpret_cast<const f32x4*>(p.scores + (hq0 + h0 + i) * p.score_ld + j);
         __syncthreads();
-        for (int i = wave; i < gn; i += 4) {  // a wave joins a head's splits
-            const f32x2* stats = reinterpret_cast<const f32x2*>(p.stats) + (hq0 + h0 + i) * p.nsplit;
-            f32x2 x[kPagedMaxSplit / 64];
+        for (int i = wave; i < gn; i += 4) {  // a wave joins a head's parts
+            const f32x2* stats =
+                reinterpret_cast<const f32x2*>(p.stats) + parts.at * p.Hq + h * p.G + h0 + i;
             float M = -INFINITY, L = 0.f;
-#pragma unroll
-            for (int u = 0; u < kPagedMaxSplit / 64; ++u) {
-                x[u] = lane + 64 * u < ns ? stats[lane + 64 * u] : f32x2{-INFINITY, 0.f};
-                M = fmaxf(M, x[u][0]);
-            }
+            for (int s = lane; s < parts.n; s += 64) M = fmaxf(M, stats[(int64_t)s * p.Hq][0]);
             M = wave_max(M);
             const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int u = 0; u < kPagedMaxSplit / 64; ++u) L += x[u][1] * fast_exp2(x[u][0] - ref);
+            for (int s = lane; s < parts.n; s += 64) {
+                const f32x2 x = stats[(int64_t)s * p.Hq];
+                L += x[1] * fast_exp2(x[0] - ref);
+            }
             L = wave_sum(L);
             if (lane == 0) {
                 top[i] = M;
-                inv[i] = len > p.max_len || M == -INFINITY ? __builtin_nanf("") : 1.f / L;
+                inv[i] = !parts.n || M == -INFINITY ? __builtin_nanf("") : 1.f / L;
             }
         }
         __syncthreads();
@@ -450,28 +544,31 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
     }
 }
 
-void paged_decode_plan(int rows, int heads, int G, int max_len, int D, int bf16, int* nsplit, int* chunk) {
-    const int64_t units = (int64_t)rows * heads * ((G + 15) / 16);
-    int64_t ch = (int64_t)(256 << 10) / (2 * D * (bf16 ? 2 : 4));
-    while (ch > kPagedStep && units * ((max_len + ch - 1) / ch) < 1024) ch /= 2;
-    if (ch < kPagedStep) ch = kPagedStep;
-    const int64_t least = ((int64_t)max_len + kPagedMaxSplit - 1) / kPagedMaxSplit;
-    if (ch < least) ch = least;
-    ch = (ch + kPagedStep - 1) / kPagedStep * kPagedStep;
-    *chunk = (int)ch;
-    *nsplit = (int)((max_len + ch - 1) / ch);
+// Whole rows to the workgroups, with no parts to join, where there are many short ones: as many (row, head)
+// pairs for each slot of the device as the longest row has steps.  fp32, 12 heads of D 64, rows of up to n
+// positions, whole and in shares, us: 700 rows 117 and 142 (n = 300), 179 and 201 (500), 311 and 324 (900);
+// 260 rows 48 and 57 (300), 74 and 79 (500), but 126 and 123 (900); 256 rows 203 and 187 (1500); 70 rows of
+// 1500 75 and 60.
+int paged_groups(int rows, int heads, int G, int max_len, int D, int bf16, bool weights) {
+    const int step = paged_step(D, bf16);
+    const int64_t slots = 256 * kPagedPerCu, pairs = (int64_t)heads * ((G + 15) / 16);
+    const int64_t steps = ((int64_t)max_len + step - 1) / step;
+    if (!weights && (steps == 1 || rows * pairs >= slots * steps)) return 0;
+    const int64_t most = std::min(rows, kPagedBlock) * steps;
+    return (int)std::max<int64_t>(1, std::min({slots / pairs, most, (int64_t)kPagedMaxGroups}));
 }
 
 template <int D, typename E>
 static int launch_paged_t(const PagedDecodeParams& p, hipStream_t s) {
-    int64_t units = (int64_t)p.c.rows * p.c.heads * p.nsplit;
+    int64_t units = (int64_t)p.c.heads * (p.groups ? p.groups : p.c.rows);
     if (p.head_tiles > 1) units = (units + 7) / 8 * 8 * p.head_tiles;
+    const dim3 grid((unsigned)units, p.groups ? (unsigned)paged_blocks(p.c.rows) : 1u);
     const size_t lds = (size_t)(4 * (p.G < 16 ? p.G : 16) * (D + 4) + 128) * sizeof(float);
     if (p.c.page_shift < 4)
-        hipLaunchKernelGGL((paged_split_kernel<D, E, true>), dim3((unsigned)units), dim3(256), lds, s, p);
+        hipLaunchKernelGGL((paged_split_kernel<D, E, true>), grid, dim3(256), lds, s, p);
     else
-        hipLaunchKernelGGL((paged_split_kernel<D, E, false>), dim3((unsigned)units), dim3(256), lds, s, p);
-    if (p.nsplit > 1 || p.scores) {
+        hipLaunchKernelGGL((paged_split_kernel<D, E, false>), grid, dim3(256), lds, s, p);
+    if (p.groups) {
         const int wblocks = p.scores ? (p.max_len + 1023) / 1024 : 0;
         const int wide = reinterpret_cast<uintptr_t>(p.w_in) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w_out) % 16 == 0;
         const int64_t blocks = (int64_t)p.c.rows * p.Hq + (int64_t)p.c.rows * p.c.heads * wblocks;

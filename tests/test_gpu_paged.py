@@ -157,6 +157,42 @@ def test_decode(ia, heads, group, page, max_pages, lens, D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,heads,group,D,page,longest,weigh", [
+    (150, 2, 1, 64, 16, 700, False),    # three blocks of rows, in shares
+    (130, 1, 17, 32, 8, 1100, True),    # two tiles of query heads, with weights
+    (64, 3, 2, 128, 32, 400, False),    # a block that is just full
+    (65, 1, 1, 128, 16, 300, True),
+    (700, 4, 1, 32, 16, 520, False),    # many short rows: whole ones to the workgroups
+    (600, 2, 18, 64, 64, 100, False),   # ... of one step, in two tiles of query heads
+])
+def test_decode_many_rows(ia, rows, heads, group, D, page, longest, weigh, dtype):
+    """Rows of random lengths, a third of them empty, some next to each other."""
+    print(f"[case] paged decode {rows} rows {heads}x{group} D{D} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(rows)
+    lens = (torch.rand(rows, generator=gen) * longest).long() + 1
+    lens[torch.rand(rows, generator=gen) < 0.3] = 0
+    lens[-5:] = 0
+    lens[1] = longest
+    lens = lens.tolist()
+    c, ks, vs, _ = make_cache(ia, gen, lens, heads, D, page, dtype)
+    q = rnd(gen, (rows, heads * group, 1, D), dtype, 1.5)
+    w = torch.full(c.meta_shape, -5.0, device="cuda") if weigh else None
+    out = ia.attn_decode_paged(q.cuda(), c, max_len=longest, weights_out=w)
+    ps = check_decode(q, out, ks, vs, heads, ia.default_scale(D), dtype)
+    for r, n in enumerate(lens):
+        if not n:
+            assert (out[r] == 0).all()
+        elif weigh:
+            p, rel = ps[r]
+            want, bound = p.view(heads, group, n).sum(1), (rel * p).view(heads, group, n).sum(1)
+            assert ((w[r, :, :n].double().cpu() - want).abs() <= bound + (group + 1) * 2.0**-24 * want).all(), r
+        if weigh:
+            assert (w[r, :, n:] == -5.0).all()
+    c.lens = torch.zeros(rows, dtype=torch.int32, device="cuda")  # nothing in any row
+    assert (ia.attn_decode_paged(q.cuda(), c, max_len=longest, weights_out=w) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("layout", ["slots", "joint"])
 def test_decode_layouts(ia, layout, dtype):
     """Pools of other orders, queries out of a packed projection, a strided output, a wide table."""
