@@ -440,14 +440,21 @@ __device__ __forceinline__ RowParts row_parts(const PagedDecodeParams& p, int ro
     return {g1 - g0 + 1, (int64_t)row + block * p.groups + g0};
 }
 
+// (M, L), a maximum and a sum of exponentials below it, with another such pair.
+__device__ __forceinline__ void join_part(float& M, float& L, float m, float l) {
+    const float top = fmaxf(M, m), ref = top == -INFINITY ? 0.f : top;
+    L = L * fast_exp2(M - ref) + l * fast_exp2(m - ref);
+    M = top;
+}
+
 // Joins the parts: the first rows * Hq workgroups write o, the others (where weights are asked
 // for) take 1024 positions of a (row, key-value head) each and add the heads' probabilities
 // exp2(score - max) / sum to the weights, in the order of the heads.
 template <int D, typename E>
 __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, int wblocks, int wide) {
     __shared__ float wsh[kPagedMaxGroups];
-    __shared__ float osh[256];
-    __shared__ float top[8], inv[8];
+    __shared__ f32x4 osh[256];
+    __shared__ f32x2 heads[4][8], scale[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nout = p.c.rows * p.Hq;
     if ((int)blockIdx.x < nout) {
@@ -461,31 +468,29 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
         }
         const int64_t at = parts.at * p.Hq + hq;  // part i: Hq further on each
         const f32x2* stats = reinterpret_cast<const f32x2*>(p.stats) + at;
-        float M = -INFINITY;
-        for (int i = lane; i < parts.n; i += 64) M = fmaxf(M, stats[(int64_t)i * p.Hq][0]);
-        M = wave_max(M);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
+        float M = -INFINITY, L = 0.f;
         for (int i = lane; i < parts.n; i += 64) {
             const f32x2 x = stats[(int64_t)i * p.Hq];
-            const float w = fast_exp2(x[0] - ref);
-            L += x[1] * w;
-            if (wave == 0) wsh[i] = w;
+            join_part(M, L, x[0], x[1]);
+            if (wave == 0) wsh[i] = x[0];
         }
-        L = wave_sum(L);
+        const float last = M;
+        M = wave_all(M, [](float x, float y) { return fmaxf(x, y); });
+        const float ref = M == -INFINITY ? 0.f : M;
+        L = wave_all(L * fast_exp2(last - ref), [](float x, float y) { return x + y; });
         __syncthreads();
-        constexpr int NG = 256 / D;
-        const int d = tid % D, grp = tid / D;
+        constexpr int W = D / 4, NG = 256 / W;  // lanes to a part, parts at a time
+        const int d = 4 * (tid % W), grp = tid / W;
         const float* part = p.part + at * D + d;
-        float o = 0.f;
-#pragma unroll 8
-        for (int i = grp; i < parts.n; i += NG) o += part[(int64_t)i * p.Hq * D] * wsh[i];
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = grp; i < parts.n; i += NG)
+            o += *reinterpret_cast<const f32x4*>(part + (int64_t)i * p.Hq * D) * fast_exp2(wsh[i] - ref);
         osh[tid] = o;
         __syncthreads();
         if (tid < D) {
-            float r = osh[tid];
-#pragma unroll
-            for (int i = 1; i < NG; ++i) r += osh[tid + i * D];
+            float r = 0.f;
+            for (int i = 0; i < min(NG, parts.n); ++i) r += osh[i * W + tid / 4][tid % 4];
             store1(out + tid, r / L);
         }
         return;
@@ -499,7 +504,18 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
     const RowParts parts = row_parts<D, E>(p, row, len);
     const int64_t hq0 = (int64_t)row * p.Hq + h * p.G;
     const int j = j0 + 4 * tid;  // this thread's 4 positions; scores are padded to whole steps
+    const int64_t wat = (int64_t)rh * p.c.cap() + j;
+    const bool whole = j + 4 <= n && p.c.cap() % 4 == 0 && wide;
     f32x4 w = {0.f, 0.f, 0.f, 0.f};
+    if (p.w_in) {
+        if (whole) {
+            w = *reinterpret_cast<const f32x4*>(p.w_in + wat);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < n) w[e] = p.w_in[wat + e];
+        }
+    }
     constexpr int U = 8;         // heads whose scores are loaded together
     for (int h0 = 0; h0 < p.G; h0 += U) {
         const int gn = min(U, p.G - h0);
@@ -508,39 +524,42 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
         for (int i = 0; i < U; ++i)
             if (i < gn && j < n)
                 sc[i] = *reinterpret_cast<const f32x4*>(p.scores + (hq0 + h0 + i) * p.score_ld + j);
-        __syncthreads();
-        for (int i = wave; i < gn; i += 4) {  // a wave joins a head's parts
-            const f32x2* stats =
-                reinterpret_cast<const f32x2*>(p.stats) + parts.at * p.Hq + h * p.G + h0 + i;
-            float M = -INFINITY, L = 0.f;
-            for (int s = lane; s < parts.n; s += 64) M = fmaxf(M, stats[(int64_t)s * p.Hq][0]);
-            M = wave_max(M);
-            const float ref = M == -INFINITY ? 0.f : M;
-            for (int s = lane; s < parts.n; s += 64) {
+        // thread t: head t % 8, every 32nd part
+        const int mine = tid & 7;
+        float M = -INFINITY, L = 0.f;
+        if (mine < gn) {
+            const f32x2* stats = reinterpret_cast<const f32x2*>(p.stats) + parts.at * p.Hq + h * p.G + h0 + mine;
+#pragma unroll 8
+            for (int s = tid >> 3; s < parts.n; s += 32) {
                 const f32x2 x = stats[(int64_t)s * p.Hq];
-                L += x[1] * fast_exp2(x[0] - ref);
+                join_part(M, L, x[0], x[1]);
             }
-            L = wave_sum(L);
-            if (lane == 0) {
-                top[i] = M;
-                inv[i] = !parts.n || M == -INFINITY ? __builtin_nanf("") : 1.f / L;
-            }
+        }
+#pragma unroll
+        for (int d = 8; d < 64; d <<= 1) {
+            const float m = shfl_xor(M, d), l = shfl_xor(L, d);
+            join_part(M, L, m, l);
+        }
+        if (lane < 8) heads[wave][lane] = f32x2{M, L};
+        __syncthreads();
+        if (tid < 8) {
+#pragma unroll
+            for (int k = 1; k < 4; ++k) join_part(M, L, heads[k][tid][0], heads[k][tid][1]);
+            scale[tid] = f32x2{M, !parts.n || M == -INFINITY ? __builtin_nanf("") : 1.f / L};
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < U; ++i)
             if (i < gn)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] += fast_exp2(sc[i][e] - top[i]) * inv[i];
+                for (int e = 0; e < 4; ++e) w[e] += fast_exp2(sc[i][e] - scale[i][0]) * scale[i][1];
     }
-    const int64_t at = (int64_t)rh * p.c.cap() + j;
-    if (j + 4 <= n && p.c.cap() % 4 == 0 && wide) {
-        if (p.w_in) w += *reinterpret_cast<const f32x4*>(p.w_in + at);
-        *reinterpret_cast<f32x4*>(p.w_out + at) = w;
+    if (whole) {
+        *reinterpret_cast<f32x4*>(p.w_out + wat) = w;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (j + e < n) p.w_out[at + e] = w[e] + (p.w_in ? p.w_in[at + e] : 0.f);
+            if (j + e < n) p.w_out[wat + e] = w[e];
     }
 }
 
