@@ -310,10 +310,11 @@ int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stri
             return st;
     }
     if (table_out_stride < cache->max_pages) return INF_ERR_BAD_STRIDE;
-    // rows read the tables of other rows: the new ones lie elsewhere
+    // rows read the tables of other rows, and every layer its row's spare page: the new ones lie elsewhere
     const int32_t *t0 = cache->table, *t1 = t0 + (cache->rows - 1) * cache->table_stride + cache->max_pages;
     const int32_t *u0 = table_out, *u1 = u0 + (cache->rows - 1) * table_out_stride + cache->max_pages;
     if (t0 < u1 && u0 < t1) return INF_ERR_BAD_STRIDE;
+    if (spare < spare_out + cache->rows && spare_out < spare + cache->rows) return INF_ERR_BAD_STRIDE;
     if ((int64_t)cache->heads * cache->page_size * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
     p.layers = layers;
     p.beams = beams;

@@ -647,9 +647,11 @@ def test_reorder(ia, groups, beams, layers, heads, D, page, length, layout, dtyp
     if part:
         tails = table[:, full].tolist() + new_spare.tolist()
         assert len(set(tails)) == 2 * rows
-    # spare in place
-    again, s2 = ia.beam_reorder(c, parents.cuda(), spare, spare_out=spare)
-    assert s2 is spare and torch.equal(spare.cpu(), sr) and torch.equal(again.cpu(), tr)
+    # the other rows' and layers' copies read the tables and spare pages: not in place
+    with pytest.raises(ia.InfernoError):
+        ia.beam_reorder(c, parents.cuda(), spare, spare_out=spare)
+    with pytest.raises(ia.InfernoError):
+        ia.beam_reorder(c, parents.cuda(), spare, table_out=c.table)
 
 
 def test_reorder_bad_parent(ia):

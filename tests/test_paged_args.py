@@ -61,7 +61,7 @@ def evict(c, **kw):
 
 
 def reorder(c, **kw):
-    a = dict(layers=1, kl=0, vl=0, parents=FAKE, beams=2, out=FAKE + 4096, stride=4, spare=FAKE, spare_out=FAKE)
+    a = dict(layers=1, kl=0, vl=0, parents=FAKE, beams=2, out=FAKE + 4096, stride=4, spare=FAKE, spare_out=FAKE + 256)
     a.update(kw)
     return ia.lib().inf_beam_reorder(ctypes.byref(c), a["layers"], a["kl"], a["vl"], a["parents"], a["beams"], a["out"],
                                      a["stride"], a["spare"], a["spare_out"], None)
@@ -148,6 +148,7 @@ def test_evict_arguments(kw, status):
 @pytest.mark.parametrize("kw,status", [
     (dict(layers=0), 2), (dict(beams=0), 2), (dict(beams=3), 2),       # 4 rows
     (dict(parents=None), 1), (dict(out=None), 1), (dict(spare=None), 1), (dict(spare_out=None), 1),
+    (dict(spare_out=FAKE), 3), (dict(spare_out=FAKE + 12), 3), (dict(spare_out=FAKE - 12), 3),  # over the spare pages
     (dict(stride=3), 3), (dict(out=FAKE), 3), (dict(out=FAKE + 60), 3), (dict(out=FAKE - 60), 3),  # over the table
     (dict(layers=2, kl=2048 * 32, vl=-4), 3), (dict(layers=2, kl=2048 * 32 + 2, vl=2048 * 32), 7),
     (dict(layers=2, kl=2048, vl=2048 * 32), 3),                        # layers on one another
