@@ -10,6 +10,7 @@
 // flow into Wqkv, the input and (through it) the LayerNorm before it.
 #pragma once
 #include "inferno/modules/linear.h"
+#include "inferno/modules/pagedkvcache.h"
 
 namespace Inferno {
 
@@ -38,6 +39,8 @@ public:
     // cached position before it (t == 1: the single-query decode kernel; t > 1:
     // the causal kernel with Tq = t < Tk).  No graph is recorded.
     Tensor forward_cached(const Tensor& x, KVCache& cache);
+    // The same through layer `layer` of a paged cache, between its begin(t) and end().
+    Tensor forward_paged(const Tensor& x, PagedKVCache& cache, size_t layer);
     Linear& qkv_proj() { return Wqkv_layer; }
     Linear& out_proj() { return W_out; }
 

@@ -21,7 +21,13 @@
 //       greedy generation with one KV cache per layer on hip:0 (prefill of a
 //       random P-token prompt, then N tokens one at a time through the
 //       single-query decode kernel); prints one JSON line with the prefill
-//       time and the per-token decode time.
+//       time and the per-token decode time.  --beams K [--page-size S]: beam
+//       search over a paged cache instead.  --budget M [--recent R]
+//       [--capacity Q] [--page-size S]: the cache holds at most Q positions
+//       (M + M / 8 + 1, and the prompt at least) and is cut to the M most
+//       attended ones whenever it is full, the R (M / 4) newest among them.
+//   gpt beam-check / paged-check <dir> <cpu|hip> [options]
+//       beam search, or given tokens, through a paged cache, written to files.
 //   gpt decode-check <dir> <cpu|hip> [--prefill P]
 //       full causal forward of tokens.bin vs incremental decoding (prefill of P
 //       tokens, then one at a time); writes logits_full.bin and logits_inc.bin.
@@ -112,6 +118,13 @@ public:
         Tensor n = gelu(feedforward1.forward(static_cast<const Tensor&>(normed2)));
         return feedforward2.forward(static_cast<const Tensor&>(n));
     }
+    // The same through layer `layer` of a paged cache.
+    Tensor forward_paged(const Tensor& x, const Tensor& normed, PagedKVCache& cache, size_t layer, Tensor* h) {
+        Tensor a = attn.forward_paged(normed, cache, layer);
+        Tensor normed2 = add_layer_norm(x, a, layernorm2.gamma(), layernorm2.beta(), layernorm2.eps(), h);
+        Tensor n = gelu(feedforward1.forward(static_cast<const Tensor&>(normed2)));
+        return feedforward2.forward(static_cast<const Tensor&>(n));
+    }
     MultiHeadAttention attn;
     LayerNorm layernorm1, layernorm2;
     Linear feedforward1, feedforward2;
@@ -168,6 +181,27 @@ public:
             LayerNorm& next = i + 1 < blocks.size() ? blocks[i + 1]->layernorm1 : layernorm1;
             normed = add_layer_norm(h, mlp, next.gamma(), next.beta(), next.eps(), &x);  // x = h + mlp
         }
+        if (m_tied) return matmul(normed, emb1.weight().transpose(0, 1), "logits");
+        return linear1->forward(static_cast<const Tensor&>(normed));
+    }
+    // A paged cache for all blocks, `groups` sequences (of options.beams rows each) of up to `capacity` positions.
+    PagedKVCache make_paged_cache(size_t groups, size_t capacity, const Device& dev, PagedKVCache::Options options) {
+        return PagedKVCache(blocks.size(), groups, m_heads, capacity, m_embed / m_heads, dev, DType::Float32, options);
+    }
+    // Logits [rows, t, V] of the next t tokens [rows, t], appending to the cache.
+    Tensor forward_paged(Tensor& tokens, PagedKVCache& cache) {
+        NoGradGuard ng;
+        cache.begin(tokens.shape()[1]);
+        Tensor x = emb1.forward(tokens);
+        x = pos_enc.forward_at(x, cache.seen());
+        Tensor normed = (blocks.empty() ? layernorm1 : blocks[0]->layernorm1).forward(x);
+        for (size_t i = 0; i < blocks.size(); ++i) {
+            Tensor h;
+            Tensor mlp = blocks[i]->forward_paged(x, normed, cache, i, &h);
+            LayerNorm& next = i + 1 < blocks.size() ? blocks[i + 1]->layernorm1 : layernorm1;
+            normed = add_layer_norm(h, mlp, next.gamma(), next.beta(), next.eps(), &x);  // x = h + mlp
+        }
+        cache.end();
         if (m_tied) return matmul(normed, emb1.weight().transpose(0, 1), "logits");
         return linear1->forward(static_cast<const Tensor&>(normed));
     }
@@ -357,6 +391,136 @@ static int run_generate_check(const std::string& dir, const Device& dev, size_t 
     return 0;
 }
 
+// ------------------------------------------------------------- beam search
+// N tokens after each prompt [B, P] by beam search over a paged cache: every
+// step picks the best K of a group's K x V continuations and the cache follows
+// the beams.  tokens, parents and scores hold each step's [B, K]; nothing is
+// read back before the end.
+struct BeamRun {
+    std::vector<Tensor> tokens, parents, scores;
+    // Sequence i of group b, best first: the steps' picks followed from the last one back.
+    std::vector<int32_t> sequences(size_t B, size_t K) const {
+        const size_t N = tokens.size();
+        std::vector<int32_t> out(B * K * N);
+        std::vector<std::vector<double>> tok, par;
+        for (size_t s = 0; s < N; ++s) {
+            tok.push_back(tokens[s].to_host_double());
+            par.push_back(parents[s].to_host_double());
+        }
+        for (size_t b = 0; b < B; ++b)
+            for (size_t i = 0; i < K; ++i) {
+                size_t at = i;
+                for (size_t s = N; s-- > 0;) {
+                    out[(b * K + i) * N + s] = (int32_t)tok[s][b * K + at];
+                    at = (size_t)par[s][b * K + at];
+                }
+            }
+        return out;
+    }
+};
+
+static BeamRun beam_search(GPTModel& model, const std::vector<int32_t>& prompt, size_t B, size_t P, size_t N, size_t K,
+                           size_t page_size, int eos, const Device& dev) {
+    NoGradGuard ng;
+    PagedKVCache::Options options;
+    options.beams = K;
+    options.page_size = page_size;
+    PagedKVCache cache = model.make_paged_cache(B, P + N, dev, options);
+    Tensor x(DType::Int32, prompt, std::vector<size_t>{B, P}, "prompt", dev);
+    Tensor logits = model.forward_paged(x, cache);
+    logits = logits.slice(1, P - 1, P - 1);  // [B, 1, V]; the beams of a group start from one row
+    const size_t V = logits.shape()[2];
+    if (K > 1) logits = make_view(logits, {B, K, V}, {logits.strides()[0], 0, 1}, logits.offset(), "beams").contiguous();
+    logits = logits.contiguous().reshape({B * K, V});
+    std::vector<float> start(B * K, -INFINITY);
+    for (size_t b = 0; b < B; ++b) start[b * K] = 0.f;  // of which the first one counts
+    Tensor scores(DType::Float32, start, std::vector<size_t>{B, K}, "scores", dev);
+    Tensor finished;
+    BeamRun run;
+    for (size_t i = 0; i < N; ++i) {
+        BeamStep s = beam_select(logits, scores, finished, eos);
+        run.tokens.push_back(s.tokens);
+        run.parents.push_back(s.parents);
+        run.scores.push_back(s.scores);
+        scores = s.scores;
+        finished = s.finished;
+        if (i + 1 == N) break;
+        if (K > 1) cache.reorder(s.parents);
+        Tensor next = s.tokens.reshape({B * K, 1});
+        logits = model.forward_paged(next, cache);
+    }
+    return run;
+}
+
+// gpt beam-check <dir> <cpu|hip>: beam search from given parameters and prompt (tokens.bin, [B, P] int32); writes
+// every step's picks (beam_tokens.bin, beam_parents.bin: [N, B, K] int32; beam_scores.bin: fp32) and the
+// sequences (beams.bin, [B, K, N] int32).
+static int run_beam_check(const std::string& dir, const Device& dev, size_t P, size_t N, size_t K, size_t page, int eos) {
+    std::ifstream cf(dir + "/config.txt");
+    size_t L, C, H, T, V, B;
+    if (!(cf >> L >> C >> H >> T >> V >> B)) throw Error("bad config.txt");
+    if (P < 1 || P + N > T) throw Error("beam-check: need 1 <= prompt and prompt + new <= context");
+    GPTModel model(V, T, C, H, L, true, dev, DType::Float32);
+    load_params(model, dir);
+    auto tok = read_file(dir + "/tokens.bin");
+    if (tok.size() < B * P * 4) throw Error("beam-check: tokens.bin holds fewer than B * prompt tokens");
+    std::vector<int32_t> prompt(B * P);
+    std::memcpy(prompt.data(), tok.data(), prompt.size() * 4);
+    const BeamRun run = beam_search(model, prompt, B, P, N, K, page, eos, dev);
+    std::vector<int32_t> tokens, parents;
+    std::vector<float> scores;
+    for (size_t i = 0; i < N; ++i) {
+        for (double x : run.tokens[i].to_host_double()) tokens.push_back((int32_t)x);
+        for (double x : run.parents[i].to_host_double()) parents.push_back((int32_t)x);
+        for (float x : run.scores[i].to_host_float()) scores.push_back(x);
+    }
+    auto put = [&](const char* name, const std::vector<int32_t>& v) {
+        std::ofstream f(dir + "/" + name, std::ios::binary);
+        f.write(reinterpret_cast<const char*>(v.data()), (std::streamsize)(v.size() * 4));
+    };
+    put("beam_tokens.bin", tokens);
+    put("beam_parents.bin", parents);
+    put("beams.bin", run.sequences(B, K));
+    write_f32(dir + "/beam_scores.bin", scores);
+    sync(dev);
+    std::cout << "beam-check ok\n";
+    return 0;
+}
+
+// gpt paged-check <dir> <cpu|hip>: tokens.bin [B, T] int32 through a paged cache of `capacity` positions, a
+// prompt of P and then one at a time; with a budget, a full cache is cut to that.  Writes
+// paged_logits.bin ([B, T - P + 1, V] fp32, from the prompt's last position on).
+static int run_paged_check(const std::string& dir, const Device& dev, size_t P, size_t capacity,
+                           PagedKVCache::Options options) {
+    std::ifstream cf(dir + "/config.txt");
+    size_t L, C, H, T, V, B;
+    if (!(cf >> L >> C >> H >> T >> V >> B)) throw Error("bad config.txt");
+    if (P < 1 || P > T) throw Error("paged-check: need 1 <= prompt <= context");
+    GPTModel model(V, T, C, H, L, true, dev, DType::Float32);
+    load_params(model, dir);
+    auto tok = read_file(dir + "/tokens.bin");
+    if (tok.size() < B * T * 4) throw Error("paged-check: tokens.bin holds fewer than B * T tokens");
+    std::vector<int32_t> tv(B * T);
+    std::memcpy(tv.data(), tok.data(), tv.size() * 4);
+    PagedKVCache cache = model.make_paged_cache(B, capacity ? capacity : T, dev, options);
+    const size_t n = T - P + 1;
+    std::vector<float> out(B * n * V);
+    for (size_t pos = P; pos <= T; ++pos) {
+        const size_t t = pos == P ? P : 1;
+        std::vector<int32_t> part(B * t);
+        for (size_t b = 0; b < B; ++b)
+            for (size_t i = 0; i < t; ++i) part[b * t + i] = tv[b * T + pos - t + i];
+        Tensor x(DType::Int32, part, std::vector<size_t>{B, t}, "tokens", dev);
+        Tensor logits = model.forward_paged(x, cache);
+        const std::vector<float> h = logits.slice(1, t - 1, t - 1).to_host_float();
+        for (size_t b = 0; b < B; ++b) std::memcpy(&out[(b * n + pos - P) * V], &h[b * V], V * 4);
+    }
+    write_f32(dir + "/paged_logits.bin", out);
+    sync(dev);
+    std::cout << "paged-check ok\n";
+    return 0;
+}
+
 // ----------------------------------------------------------------- generate
 // Greedy generation with KV caches on hip:0: a random prompt of P tokens per
 // sequence, then N new tokens.  Each pick stays on the device as the next
@@ -370,7 +534,14 @@ static int run_generate(int argc, char** argv) {
                  H = arg(argc, argv, "--heads", 12), V = arg(argc, argv, "--vocab", 8192),
                  B = arg(argc, argv, "--batch", 8), P = arg(argc, argv, "--prompt", 512),
                  N = arg(argc, argv, "--new", 64), T = arg(argc, argv, "--ctx", 1024);
+    const size_t K = arg(argc, argv, "--beams", 0), budget = arg(argc, argv, "--budget", 0);
+    PagedKVCache::Options paged;  // of a bounded cache
+    paged.page_size = arg(argc, argv, "--page-size", 16);
+    paged.budget = budget;
+    paged.recent = arg(argc, argv, "--recent", budget / 4);
+    const size_t capacity = arg(argc, argv, "--capacity", budget + budget / 8 + 1);
     if (P + N > T) throw Error("generate: prompt + new tokens exceed the context size");
+    if (K && budget) throw Error("generate: --beams and --budget exclude each other");
     const Device dev = Device::hip(0);
     RandomGenerator::initializeWithSeed(42);
     GPTModel model(V, T, C, H, L, true, dev, DType::Float32);
@@ -384,16 +555,38 @@ static int run_generate(int argc, char** argv) {
         const size_t t = logits.shape()[1];
         return argmax(logits.slice(1, t - 1, t - 1));
     };
+    if (K) {
+        beam_search(model, prompt, B, P, N, K, paged.page_size, -1, dev);  // warm-up
+        sync(dev);
+        const auto t0 = std::chrono::steady_clock::now();
+        const BeamRun run = beam_search(model, prompt, B, P, N, K, paged.page_size, -1, dev);
+        const std::vector<float> best = run.scores.back().to_host_float();
+        const double ms = std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
+        const std::vector<int32_t> seq = run.sequences(B, K);
+        std::printf(
+            "{\"workload\": \"GPT beam search L%zu C%zu H%zu V%zu B%zu beams %zu prompt %zu new %zu, paged KV cache\", "
+            "\"ms\": %.3f, \"ms_per_token_with_prefill\": %.4f, \"best_score\": %.6f, \"first_tokens\": [%d]}\n",
+            L, C, H, V, B, K, P, N, ms, ms / (double)N, best[0], seq[0]);
+        return 0;
+    }
     auto run_once = [&](double* prefill_ms, double* decode_ms, std::vector<int32_t>* out) {
-        auto caches = model.make_caches(B, T, dev);
+        std::vector<KVCache> caches;
+        std::unique_ptr<PagedKVCache> bounded;
+        if (budget)
+            bounded = std::make_unique<PagedKVCache>(model.make_paged_cache(B, std::max(capacity, P), dev, paged));
+        else
+            caches = model.make_caches(B, T, dev);
+        auto forward = [&](Tensor& x) {
+            return budget ? model.forward_paged(x, *bounded) : model.forward_cached(x, caches);
+        };
         Tensor xp(DType::Int32, prompt, std::vector<size_t>{B, P}, "prompt", dev);
         sync(dev);
         const auto t0 = std::chrono::steady_clock::now();
         std::vector<Tensor> picks;
-        picks.push_back(pick_last(model.forward_cached(xp, caches)));
+        picks.push_back(pick_last(forward(xp)));
         sync(dev);
         const auto t1 = std::chrono::steady_clock::now();
-        for (size_t i = 1; i < N; ++i) picks.push_back(pick_last(model.forward_cached(picks.back(), caches)));
+        for (size_t i = 1; i < N; ++i) picks.push_back(pick_last(forward(picks.back())));
         out->assign(B * N, 0);  // step-major: token i of sequence b at i * B + b
         for (size_t i = 0; i < N; ++i) {
             const std::vector<double> h = picks[i].to_host_double();
@@ -409,10 +602,10 @@ static int run_generate(int argc, char** argv) {
     run_once(&pm, &dm, &gen);
     const double steps = (double)(N - 1);
     std::printf(
-        "{\"workload\": \"GPT greedy generation L%zu C%zu H%zu V%zu B%zu prompt %zu new %zu, KV cache\", "
+        "{\"workload\": \"GPT greedy generation L%zu C%zu H%zu V%zu B%zu prompt %zu new %zu, %s\", "
         "\"prefill_ms\": %.3f, \"decode_ms_per_token\": %.4f, \"decode_tokens_per_s\": %.1f, "
         "\"first_tokens\": [%d, %d, %d]}\n",
-        L, C, H, V, B, P, N, pm, dm / steps, (double)B * steps / (dm * 1e-3), gen[0], gen.size() > 1 ? gen[1] : 0,
+        L, C, H, V, B, P, N, budget ? ("paged KV cache cut to " + std::to_string(budget)).c_str() : "KV cache", pm, dm / steps, (double)B * steps / (dm * 1e-3), gen[0], gen.size() > 1 ? gen[1] : 0,
         gen.size() > 2 ? gen[2] : 0);
     return 0;
 }
@@ -688,6 +881,20 @@ int main(int argc, char** argv) {
         if (argc >= 4 && std::strcmp(argv[1], "generate-check") == 0) {
             const Device dev = std::strcmp(argv[3], "hip") == 0 ? Device::hip(0) : Device::cpu();
             return run_generate_check(argv[2], dev, arg(argc, argv, "--prompt", 4), arg(argc, argv, "--new", 8));
+        }
+        if (argc >= 4 && std::strcmp(argv[1], "beam-check") == 0) {
+            const Device dev = std::strcmp(argv[3], "hip") == 0 ? Device::hip(0) : Device::cpu();
+            return run_beam_check(argv[2], dev, arg(argc, argv, "--prompt", 4), arg(argc, argv, "--new", 8),
+                                  arg(argc, argv, "--beams", 4), arg(argc, argv, "--page-size", 16),
+                                  (int)arg(argc, argv, "--eos", (size_t)-1));
+        }
+        if (argc >= 4 && std::strcmp(argv[1], "paged-check") == 0) {
+            const Device dev = std::strcmp(argv[3], "hip") == 0 ? Device::hip(0) : Device::cpu();
+            PagedKVCache::Options options;
+            options.page_size = arg(argc, argv, "--page-size", 16);
+            options.budget = arg(argc, argv, "--budget", 0);
+            options.recent = arg(argc, argv, "--recent", 0);
+            return run_paged_check(argv[2], dev, arg(argc, argv, "--prompt", 4), arg(argc, argv, "--capacity", 0), options);
         }
         if (argc >= 4 && std::strcmp(argv[1], "step") == 0) {
             const Device dev = std::strcmp(argv[3], "hip") == 0 ? Device::hip(0) : Device::cpu();

@@ -270,6 +270,21 @@ Tensor MultiHeadAttention::forward_cached(const Tensor& x, KVCache& cache) {
     }
 }
 
+Tensor MultiHeadAttention::forward_paged(const Tensor& x, PagedKVCache& cache, size_t layer) {
+    NoGradGuard ng;
+    if (x.ndim() != 3 || x.shape()[2] != m_embed_dim) throw Error("MultiHeadAttention: expects [B, t, C]");
+    const size_t B = x.shape()[0], t = x.shape()[1], C = m_embed_dim, H = m_num_heads, D = m_head_dim;
+    Tensor qkv = Wqkv_layer.forward(x).contiguous();  // [B, t, 3C]
+    const std::vector<size_t> hs{B, H, t, D};
+    const std::vector<size_t> hst{t * 3 * C, D, 3 * C, 1};
+    Tensor q = make_view(qkv, hs, hst, qkv.offset(), "q");
+    Tensor k = make_view(qkv, hs, hst, qkv.offset() + C, "k_new");
+    Tensor v = make_view(qkv, hs, hst, qkv.offset() + 2 * C, "v_new");
+    Tensor y4 = cache.attend(layer, q, k, v);
+    Tensor y = t == 1 ? y4.reshape({B, 1, C}) : y4.transpose(1, 2).contiguous().reshape({B, t, C});
+    return W_out.forward(static_cast<const Tensor&>(y));
+}
+
 // ------------------------------------------------------------ CrossEntropyLoss
 Tensor CrossEntropyLoss::forward(Tensor& logits, Tensor& target) { return cross_entropy(logits, target); }
 
