@@ -291,6 +291,41 @@ def test_decode_far_offsets(ia):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_writes_far_offsets(ia, dtype):
+    """Append, eviction and reordering on pages past 2^31 elements (2 x 5 GB in bf16, 10 in fp32)."""
+    print(f"[case] paged writes far offsets {dtype}", flush=True)
+    heads, D, page = 2, 64, 16
+    pages = (5 << 29) // (heads * D * page)
+    k = torch.empty(pages, heads, page, D, dtype=dtype, device="cuda")
+    v = torch.empty_like(k)
+    gen = torch.Generator().manual_seed(16)
+    table = torch.tensor([[pages - 1, pages - 7, pages - 3], [pages - 2, pages - 5, pages - 4]], dtype=torch.int32)
+    c = ia.PagedKV(k, v, table.cuda(), torch.full((2,), 40, dtype=torch.int32, device="cuda"))
+    kn, vn = (rnd(gen, (2, heads, 40, D), dtype) for _ in range(2))
+    ia.kv_append(c, kn.cuda(), vn.cuda())
+
+    def row(pool, pages_of_row, n):
+        return pool[pages_of_row.long().cuda()].transpose(0, 1).reshape(heads, -1, D)[:, :n].cpu()
+
+    for r in range(2):
+        assert torch.equal(row(k, table[r], 40), kn[r]) and torch.equal(row(v, table[r], 40), vn[r])
+    spare = torch.tensor([pages - 9, pages - 8], dtype=torch.int32)
+    new, _ = ia.beam_reorder(c, torch.tensor([[1, 0]], dtype=torch.int32).cuda(), spare.cuda())
+    assert new.tolist() == [[pages - 2, pages - 5, pages - 9], [pages - 1, pages - 7, pages - 8]]
+    for r in range(2):
+        assert torch.equal(row(k, new[r].cpu(), 40), kn[1 - r]) and torch.equal(row(v, new[r].cpu(), 40), vn[1 - r])
+    w = torch.rand(2, heads, 48, generator=gen)
+    pos = torch.arange(48, dtype=torch.int32).expand(2, heads, 48).contiguous()
+    ia.kv_evict(c, w.cuda(), pos.cuda(), 25, 3, max_len=40)
+    for r in range(2):
+        for h in range(heads):
+            holes, src = ref_evict(w[r, h].numpy(), pos[r, h].numpy(), 40, 25, 3)
+            kr, vr = kn[r, h].clone(), vn[r, h].clone()
+            kr[holes], vr[holes] = kn[r, h][src], vn[r, h][src]
+            assert torch.equal(row(k, table[r], 25)[h], kr[:25]) and torch.equal(row(v, table[r], 25)[h], vr[:25])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 def test_decode_long(ia, dtype):
     """A long row on many splits beside a short one; weights over all of it."""
     print(f"[case] paged decode long {dtype}", flush=True)
@@ -407,6 +442,8 @@ EVICT = [
     ([1500, 1025, 1024], 2000, 1024, 0, 32),
     ([1500, 700, 2000], 1600, 200, 64, 1),  # 2000 > max_len: left alone
     ([5000], 5000, 4936, 512, 64),
+    ([36864, 100], 36864, 20000, 1000, 64),  # the longest whose keys are held on the chip
+    ([36865, 36000], 36865, 36000, 1000, 64),
     ([70000, 20], 70000, 30000, 100, 128),
 ]
 
