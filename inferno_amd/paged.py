@@ -209,7 +209,7 @@ def attn_decode_paged(q, cache, scale=None, max_len=None, weights=None, weights_
         with _on(dev, stream):
             return attn_decode_paged(q, cache, scale, max_len, weights, weights_out, out, workspace)
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != q.dtype or out.device != dev:
         raise ValueError("attn_decode_paged: out must be like q")
     ws, ptr, n = _workspace(workspace, lambda: _decode_bytes(cache, heads, max_len, w_out), dev)
@@ -245,7 +245,7 @@ def kv_evict(cache, weights, positions, keep, recent=0, weights_out=None, positi
             return kv_evict(cache, weights, positions, keep, recent, weights_out, positions_out, lens_out, max_len,
                             workspace)
     if lens_out is None:
-        lens_out = cache.lens.new_empty(cache.rows)
+        lens_out = torch.empty_like(cache.lens)
     ws, ptr, n = _workspace(workspace, lambda: _evict_bytes(cache, keep, max_len), dev)
     st = lib().inf_kv_evict(cache.ref, pw,
                             pw if weights_out is None else _of(weights_out, "weights_out", torch.float32, dev, meta), pp,
@@ -291,16 +291,16 @@ def beam_select(logits, scores, finished=None, eos=None, workspace=None, stream=
     if vocab > 1 and step != 1:
         raise ValueError("beam_select: the logits of a row must be adjacent")
     groups, beams = shape
-    # tokens, parents and finished side by side
-    ints = scores.new_empty((3, groups, beams), dtype=torch.int32)
-    scores_out, first, n_ints = scores.new_empty(shape), ints.data_ptr(), 4 * groups * beams
+    tokens, parents = torch.empty_like(scores, dtype=torch.int32), torch.empty_like(scores, dtype=torch.int32)
+    scores_out = torch.empty_like(scores)
+    done = torch.empty_like(scores, dtype=torch.int32) if eos is not None else None
     ws, ptr, n = _workspace(workspace, lambda: _select_bytes(groups, beams, vocab), dev)
     st = lib().inf_beam_select(logits.data_ptr(), ld if logits.shape[0] > 1 else max(ld, vocab), ps, pf, groups, beams,
-                               vocab, -1 if eos is None else int(eos), first, first + n_ints, scores_out.data_ptr(),
-                               None if eos is None else first + 2 * n_ints, _dt(logits), ptr, n, _raw_stream(dev.index))
+                               vocab, -1 if eos is None else int(eos), tokens.data_ptr(), parents.data_ptr(),
+                               scores_out.data_ptr(), done.data_ptr() if done is not None else None, _dt(logits), ptr, n,
+                               _raw_stream(dev.index))
     _check(st, "inf_beam_select")
-    tokens, parents, done = ints.unbind()
-    return tokens, parents, scores_out, None if eos is None else done
+    return tokens, parents, scores_out, done
 
 
 def beam_reorder(cache, parents, spare, table_out=None, spare_out=None, stream=None):
@@ -317,12 +317,17 @@ def beam_reorder(cache, parents, spare, table_out=None, spare_out=None, stream=N
             return beam_reorder(cache, parents, spare, table_out, spare_out)
     shape = cache.table.shape
     if table_out is None:
-        table_out = spare.new_empty(shape)
+        table_out = torch.empty_like(cache.table, memory_format=torch.contiguous_format)
+        pt = table_out.data_ptr()
+    else:
+        pt = _of(table_out, "table_out", torch.int32, dev, shape)
     if spare_out is None:
-        spare_out = spare.new_empty(spare.shape)
+        spare_out = torch.empty_like(spare)
+        po = spare_out.data_ptr()
+    else:
+        po = _of(spare_out, "spare_out", torch.int32, dev, spare.shape)
     st = lib().inf_beam_reorder(cache.ref, cache.layers, *cache.layer_strides, pp, parents.shape[1],
-                                _of(table_out, "table_out", torch.int32, dev, shape), shape[1], ps,
-                                _of(spare_out, "spare_out", torch.int32, dev, spare.shape), _raw_stream(dev.index))
+                                pt, shape[1], ps, po, _raw_stream(dev.index))
     _check(st, "inf_beam_reorder")
     return table_out, spare_out
 
