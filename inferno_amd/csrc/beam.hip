@@ -75,6 +75,7 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     __shared__ float wmax[4];
     __shared__ double wsum[4];
     __shared__ uint64_t wbest[4];
+    __shared__ uint32_t wnth[4];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     const int64_t row = blockIdx.x / p.nsplit;
     const int split = blockIdx.x % p.nsplit;
@@ -86,27 +87,38 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     const int64_t c0 = (int64_t)split * (256 * N);
     const int lo = split == 0 ? mis : 0, hi = (int)min((int64_t)(256 * N), p.vocab + mis - c0);
     x += c0 - mis;
+    // Every load stands alone, at a place inside the row: under a condition the compiler would wait for each
+    // before the next.  Threads at the row's ends then take their columns one by one.
     float v[N];  // columns outside are -inf
+    const int first = (lo + GE - 1) / GE * GE, last = hi / GE * GE - GE;  // whole 16-byte pieces
+    u32x4 raw[NV];
+    if (first <= last) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u)
+            raw[u] = __builtin_nontemporal_load(
+                reinterpret_cast<const u32x4*>(x + min(max((u * 256 + tid) * GE, first), last)));
+    }
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
+#pragma unroll
+        for (int e = 0; e < GE; ++e) {
+            if constexpr (sizeof(T) == 4)
+                v[u * GE + e] = __uint_as_float(raw[u][e]);
+            else
+                v[u * GE + e] = __uint_as_float(e & 1 ? raw[u][e >> 1] & 0xffff0000u : raw[u][e >> 1] << 16);
+        }
         const int c = (u * 256 + tid) * GE;
-        if (c >= lo && c + GE <= hi) {
-            const u32x4 raw = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(x + c));
+        if (c < first || c > last) {
 #pragma unroll
             for (int e = 0; e < GE; ++e) {
-                if constexpr (sizeof(T) == 4)
-                    v[u * GE + e] = __uint_as_float(raw[e]);
-                else
-                    v[u * GE + e] = __uint_as_float(e & 1 ? raw[e >> 1] & 0xffff0000u : raw[e >> 1] << 16);
+                const bool in = c + e >= lo && c + e < hi;
+                v[u * GE + e] = -INFINITY;
+                if (in) v[u * GE + e] = E::ld(x + c + e);
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < GE; ++e) v[u * GE + e] = c + e >= lo && c + e < hi ? E::ld(x + c + e) : -INFINITY;
         }
     }
-    auto column = [&](int i) { return (i / GE * 256 + tid) * GE + i % GE; };
-    auto key = [&](int i) {
-        return (uint64_t)ordered_logit(v[i]) << 32 | (uint32_t)~(uint32_t)(c0 - mis + column(i));
+    auto key = [&](float y, int c) {
+        return (uint64_t)ordered_logit(y) << 32 | (uint32_t)~(uint32_t)(c0 - mis + c);
     };
     float mx = -INFINITY;
 #pragma unroll
@@ -129,8 +141,12 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
         wsum[wave] = sum;
     }
     if (tid == 0) count = 0;
-    const float least = logit_of(max(wave_nth<16>(lane_best, p.beams), ordered_logit(-INFINITY)));
+    const uint32_t nth = wave_nth<16>(lane_best, p.beams);
+    if (lane == 0) wnth[wave] = nth;
     __syncthreads();
+    // Columns of -inf, those outside among them, are not picked.
+    constexpr float kLowest = -3.402823466e38f;
+    const float least = logit_of(max(max(max(wnth[0], wnth[1]), max(wnth[2], wnth[3])), ordered_logit(kLowest)));
     if (tid == 0) {
         const float M = fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3]));
         double S = 0.0;
@@ -138,17 +154,30 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
         p.maxs[blockIdx.x] = M;
         p.sums[blockIdx.x] = S;
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (v[i] >= least && column(i) >= lo && column(i) < hi) {
+    auto pick = [&](int i) {
+        if (v[i] >= least) {
             const int at = atomicAdd(&count, 1);
-            if (at < kBeamList) list[at] = key(i);
+            if (at < kBeamList) list[at] = key(v[i], (i / GE * 256 + tid) * GE + i % GE);
         }
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) pick(i);
     __syncthreads();
     const int n = count;
     uint64_t* out = p.cand + (int64_t)blockIdx.x * p.beams;
     if (n <= kBeamList) {
-        if (tid < p.beams && tid >= n) out[tid] = 0;  // fewer columns than beams
+        if (n < p.beams && wave == 0) {
+            // fewer above -inf than beams: the lowest columns of the others (where there is a NaN, nobody asks)
+            int at = n;
+            for (int c = lo; c < hi && at < p.beams; c += 64) {
+                const bool rest = c + lane < hi && !(E::ld(x + c + lane) >= kLowest);
+                const uint64_t m = __ballot(rest);
+                const int i = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+                if (rest && i < p.beams) out[i] = key(-INFINITY, c + lane);
+                at += __popcll(m);
+            }
+            if (lane < p.beams && lane >= at) out[lane] = 0;  // fewer columns than beams
+        }
         // four lanes count for one value
         for (int i0 = 0; i0 < n; i0 += 64) {
             const int i = i0 + (tid >> 2);
@@ -165,9 +194,9 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     uint64_t before = ~0ull;
     for (int k = 0; k < p.beams; ++k) {
         uint64_t best = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const uint64_t y = v[i] >= least && column(i) >= lo && column(i) < hi ? key(i) : 0;
+#pragma unroll 4
+        for (int c = lo + tid; c < hi; c += 256) {
+            const uint64_t y = key(E::ld(x + c), c);
             if (y < before && y > best) best = y;
         }
         best = wave_all(best, [](uint64_t a, uint64_t b) { return max(a, b); });
@@ -179,28 +208,48 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     }
 }
 
-__global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
+// One workgroup of 16 waves a group (4 waves: 17.1 us instead of 16.8 with 32 groups of 8 beams and 50257 bf16
+// columns, 24.0 instead of 20.7 with 16 groups of 16 beams).
+__global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
+    constexpr int W = 16, kThreads = 64 * W;
     enum { kLives, kFinished, kFlat };  // a flat beam's candidates are the first tokens, all with its score
     __shared__ double base[kMaxBeams];  // score - lse; the score of a beam that is finished or flat
     __shared__ int kind[kMaxBeams];
     __shared__ uint64_t ls[kBeamList], lt[kBeamList];
     __shared__ int count;
-    __shared__ uint64_t ws[4], wt[4];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    __shared__ uint64_t ws[W], wt[W];
+    __shared__ uint32_t wall[W];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int64_t row0 = (int64_t)blockIdx.x * p.beams;
-    const int per = p.nsplit * p.beams, total = p.beams * per;
-    // The candidates' logits and columns do not wait for the lse; up to 256 U of them stay in registers.
-    // Each part's are in order, so that a lane's step to step is no multiple of the beams: lanes that held
-    // only best ones, and lanes that held only last ones, would bound the best few badly.
-    constexpr int U = 8;
-    uint64_t cand[U];
-    auto index = [&](int i0, int u) { return i0 + 256 * u + ((tid + 41 * u) & 255); };
-    auto load = [&](int i0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            cand[u] = i0 + 256 * u < total && index(i0, u) < total ? p.cand[row0 * per + index(i0, u)] : 0;
+    const int per = p.nsplit * p.beams;  // candidates of a beam
+    // A wave takes whole beams, wave, wave + W, ..., 64 of a beam's candidates at a time, so that a beam's state is the
+    // same for all lanes.  Up to U such rounds stay in registers, loaded before the lse is known.  Each part's
+    // candidates are in order, so the lanes are turned from round to round: lanes that held only best ones, and
+    // lanes that held only last ones, would bound the best few badly.
+    constexpr int U = 2;  // more only cost time: 17.2 us with 4, 17.5 with 8, of 16.8
+    const int rounds = (per + 63) / 64, all = (p.beams - wave + W - 1) / W * rounds;  // 0 or less: no beam
+    struct At {
+        int b, i, turn;
     };
-    load(0);
+    auto start = [&] { return At{wave, 0, 0}; };
+    auto next = [&](At& a) {
+        a.turn += 41;
+        if (++a.i == rounds) {
+            a.i = 0;
+            a.b += W;
+        }
+    };
+    auto place = [&](const At& a) { return 64 * a.i + ((lane + a.turn) & 63); };
+    uint64_t cand[U];
+    auto load = [&](At& a) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {  // one load after the other, under no condition
+            cand[u] = p.cand[(row0 + min(a.b, p.beams - 1)) * per + min(place(a), per - 1)];
+            next(a);
+        }
+    };
+    At loaded = start();
+    load(loaded);
     static_assert(kMaxBeams * 8 <= 256, "eight lanes per beam");
     if (const int b = tid >> 3; b < p.beams) {
         const int64_t row = row0 + b;
@@ -214,9 +263,16 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
             float top = M;
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                const int i = i0 + 8 * k + (tid & 7);
-                m[k] = i < p.nsplit ? p.maxs[row * p.nsplit + i] : -INFINITY;
-                s[k] = i < p.nsplit ? p.sums[row * p.nsplit + i] : 0.0;
+                const int64_t i = row * p.nsplit + min(i0 + 8 * k + (tid & 7), p.nsplit - 1);
+                m[k] = p.maxs[i];
+                s[k] = p.sums[i];
+            }
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                if (i0 + 8 * k + (tid & 7) >= p.nsplit) {
+                    m[k] = -INFINITY;
+                    s[k] = 0.0;
+                }
                 top = fmaxf(top, m[k]);
             }
             top = fmaxf(top, __uint_as_float(dpp_u32<0xB1>(__float_as_uint(top))));
@@ -240,9 +296,8 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     }
     if (tid == 0) count = 0;
     __syncthreads();
-    // Candidate i of the group: its score as an ordered number (0: there is none) and its place.
-    auto candidate = [&](int i, uint64_t c, uint64_t& at) -> uint64_t {
-        const int b = i / per, j = i - b * per;
+    // Beam b's candidate c, the j-th: its score as an ordered number (0: there is none) and its place.
+    auto candidate = [&](int b, int j, uint64_t c, uint64_t& at) -> uint64_t {
         uint32_t token = (uint32_t)j;
         double score = base[b];
         if (kind[b] == kLives) {
@@ -258,6 +313,23 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
         at = (uint64_t)b << 32 | token;
         return ordered_score(score);
     };
+    auto scan = [&](auto f) {  // f(score, place) for this lane's candidates
+        At a = start();
+        if (all > U) loaded = a;
+        for (int r = 0; r < all; r += U) {
+            if (all > U) load(loaded);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r + u < all) {
+                    const int j = place(a);
+                    uint64_t at;
+                    if (j < per)
+                        if (const uint64_t s = candidate(a.b, j, cand[u], at)) f(s, at);
+                }
+                next(a);
+            }
+        }
+    };
     auto emit = [&](int k, uint64_t s, uint64_t at) {
         const int b = (int)(at >> 32), token = (int)(uint32_t)at;
         const int64_t o = row0 + k;
@@ -268,35 +340,26 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
         if (p.finished_out) p.finished_out[o] = kind[b] == kFinished || token == p.eos;
     };
     uint32_t best = 0;
-    uint64_t at = 0;
-    auto pick = [&](uint64_t s, uint32_t least) {
-        if (s && (uint32_t)(s >> 32) >= least) {
+    scan([&](uint64_t s, uint64_t) { best = max(best, (uint32_t)(s >> 32)); });
+    // The group's `beams`-th is no less than any wave's.
+    const uint32_t nth = wave_nth<4>(best, p.beams);
+    if (lane == 0) wall[wave] = nth;
+    __syncthreads();
+    uint32_t least = 0;
+    for (int w = 0; w < W; ++w) least = max(least, wall[w]);
+    scan([&](uint64_t s, uint64_t at) {
+        if ((uint32_t)(s >> 32) >= least) {
             const int k = atomicAdd(&count, 1);
             if (k < kBeamList) {
                 ls[k] = s;
                 lt[k] = at;
             }
         }
-    };
-    for (int i0 = 0; i0 < total; i0 += 256 * U) {
-        if (i0) load(i0);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + 256 * u < total && index(i0, u) < total)
-                best = max(best, (uint32_t)(candidate(index(i0, u), cand[u], at) >> 32));
-    }
-    const uint32_t least = wave_nth<4>(best, p.beams);
-    for (int i0 = 0; i0 < total; i0 += 256 * U) {
-        if (total > 256 * U) load(i0);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + 256 * u < total && index(i0, u) < total)
-                pick(candidate(index(i0, u), cand[u], at), least);
-    }
+    });
     __syncthreads();
     const int n = count;
     if (n <= kBeamList) {
-        for (int i0 = 0; i0 < n; i0 += 64) {
+        for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
             const int i = i0 + (tid >> 2);
             const uint64_t s = ls[min(i, n - 1)], t = lt[min(i, n - 1)];
             int better = 0;
@@ -311,13 +374,12 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
     uint64_t s0 = ~0ull, t0 = 0;  // the one picked last
     for (int k = 0; k < p.beams; ++k) {
         uint64_t s1 = 0, t1 = ~0ull;
-        for (int i = tid; i < total; i += 256) {
-            const uint64_t s = candidate(i, p.cand[row0 * per + i], at);
-            if (s && (s < s0 || (s == s0 && at > t0)) && (s > s1 || (s == s1 && at < t1))) {
+        scan([&](uint64_t s, uint64_t at) {
+            if ((s < s0 || (s == s0 && at > t0)) && (s > s1 || (s == s1 && at < t1))) {
                 s1 = s;
                 t1 = at;
             }
-        }
+        });
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) {
             const uint64_t s = shfl_xor64(s1, m), t = shfl_xor64(t1, m);
@@ -333,7 +395,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(BeamSelectParams p) {
         __syncthreads();
         s0 = ws[0];
         t0 = wt[0];
-        for (int w = 1; w < 4; ++w)
+        for (int w = 1; w < W; ++w)
             if (ws[w] > s0 || (ws[w] == s0 && wt[w] < t0)) {
                 s0 = ws[w];
                 t0 = wt[w];
@@ -360,7 +422,7 @@ static int launch_select_t(const BeamSelectParams& p, hipStream_t s) {
         case 4096: hipLaunchKernelGGL((beam_part_kernel<E, 16>), grid, dim3(256), 0, s, p); break;
         default: hipLaunchKernelGGL((beam_part_kernel<E, 32>), grid, dim3(256), 0, s, p); break;
     }
-    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)p.groups), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)p.groups), dim3(1024), 0, s, p);
     return (int)hipGetLastError();
 }
 

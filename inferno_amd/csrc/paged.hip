@@ -630,8 +630,8 @@ constexpr int kEvictLds = 36 << 10;
 
 // W waves, each with one stretch of the slots, 256 at a time, four to a lane, so that what comes before a
 // slot is the waves before, the rounds before, the lanes before and the lane's own.
-template <int W, bool LDS>
-__global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p, int vec) {
+template <int W, bool LDS, bool VEC>
+__global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p) {
     constexpr int kThreads = 64 * W, kBins = 2048, PER = kBins / kThreads;
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t part[W], part2[W];
@@ -658,12 +658,13 @@ __global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p
     }
     const int rounds = (len + 4 * kThreads - 1) / (4 * kThreads);
     const int first = 256 * wave * rounds + 4 * lane;
-    // Four slots from j on, those behind the end as 0 (in a row of any alignment, one by one).
+    // Four slots from j on, one by one where rows are not aligned; behind the end, anything.  Loads never stand
+    // under a condition: the compiler would wait for each before the next.
     auto load4 = [&](const uint32_t* src, int j) -> u32x4 {
-        if (vec && j + 4 <= len) return *reinterpret_cast<const u32x4*>(src + j);
+        if constexpr (VEC) return *reinterpret_cast<const u32x4*>(src + min(j, (len - 1) & ~3));
         u32x4 x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = j + e < len ? src[j + e] : 0u;
+        for (int e = 0; e < 4; ++e) x[e] = src[min(j + e, len - 1)];
         return x;
     };
     struct Meta {
@@ -676,7 +677,7 @@ __global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p
             decltype(load(0)) x[U];
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i + u < rounds) x[u] = load(first + 256 * (i + u));
+                x[u] = load(first + 256 * (i + u));
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (i + u < rounds) f(first + 256 * (i + u), x[u]);
@@ -732,9 +733,8 @@ __global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p
     });
     auto keys = [&](auto f) {  // f(j, four keys)
         if constexpr (LDS)
-            each([&](int j) {
-                return j < len ? *reinterpret_cast<const u32x4*>(&skeys[j]) : u32x4{kSafe, kSafe, kSafe, kSafe};
-            }, f);
+            each([&](int j) { return *reinterpret_cast<const u32x4*>(&skeys[min(j, (len - 1) & ~3)]); },
+                 [&](int j, u32x4 k) { f(j, j < len ? k : u32x4{kSafe, kSafe, kSafe, kSafe}); });
         else
             each(meta, [&](int j, Meta x) { f(j, keys_of(j, x)); });
     };
@@ -880,7 +880,7 @@ __global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p
             bool kept[4];
             place(j, k, kept);
             // a hole gets its own from the moves that follow
-            if (vec && j + 4 <= keep) {
+            if (VEC && j + 4 <= keep) {
                 *reinterpret_cast<u32x4*>(wo + j) = x.w;
                 *reinterpret_cast<u32x4*>(po + j) = x.pos;
             } else {
@@ -960,13 +960,19 @@ int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s) {
     const size_t lds = ((size_t)p.max_len + 3) / 4 * 16;
     const uintptr_t any = reinterpret_cast<uintptr_t>(p.w_in) | reinterpret_cast<uintptr_t>(p.w_out) |
                           reinterpret_cast<uintptr_t>(p.pos_in) | reinterpret_cast<uintptr_t>(p.pos_out);
-    const int vec = any % 16 == 0 && p.c.cap() % 4 == 0;
-    if (p.max_len <= 4096)
-        hipLaunchKernelGGL((kv_evict_select_kernel<4, true>), grid, dim3(256), lds, s, p, vec);
-    else if (p.max_len <= kEvictLds)
-        hipLaunchKernelGGL((kv_evict_select_kernel<16, true>), grid, dim3(1024), lds, s, p, vec);
+    auto select = [&](auto v) {
+        constexpr bool kVec = decltype(v)::value;
+        if (p.max_len <= 4096)
+            hipLaunchKernelGGL((kv_evict_select_kernel<4, true, kVec>), grid, dim3(256), lds, s, p);
+        else if (p.max_len <= kEvictLds)
+            hipLaunchKernelGGL((kv_evict_select_kernel<16, true, kVec>), grid, dim3(1024), lds, s, p);
+        else
+            hipLaunchKernelGGL((kv_evict_select_kernel<16, false, kVec>), grid, dim3(1024), 0, s, p);
+    };
+    if (any % 16 == 0 && p.c.cap() % 4 == 0)
+        select(std::true_type{});
     else
-        hipLaunchKernelGGL((kv_evict_select_kernel<16, false>), grid, dim3(1024), 0, s, p, vec);
+        select(std::false_type{});
     // four moves a thread where that leaves a thousand workgroups
     const int64_t all = rh * ((p.moves + per - 1) / per);
     const int u = all >= 4096 ? 4 : 1;
