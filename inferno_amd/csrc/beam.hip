@@ -87,10 +87,14 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     const int64_t c0 = (int64_t)split * (256 * N);
     const int lo = split == 0 ? mis : 0, hi = (int)min((int64_t)(256 * N), p.vocab + mis - c0);
     x += c0 - mis;
-    // Every load stands alone, at a place inside the row: under a condition the compiler would wait for each
-    // before the next.  Threads at the row's ends then take their columns one by one.
-    float v[N];  // columns outside are -inf
-    const int first = (lo + GE - 1) / GE * GE, last = hi / GE * GE - GE;  // whole 16-byte pieces
+    // The row's whole 16-byte pieces are this thread's N columns, and the few columns before and behind them one
+    // more.  Every load stands alone, at a place inside the row: under a condition the compiler would wait for
+    // each before the next.
+    const int first = (lo + GE - 1) / GE * GE, last = hi / GE * GE - GE;
+    const int head = first <= last ? first - lo : hi - lo, tail = first <= last ? hi - last - GE : 0;
+    const int edge = tid < head ? lo + tid : last + GE + tid - head;
+    float v[N + 1];  // columns outside are -inf
+    v[N] = -INFINITY;
     u32x4 raw[NV];
     if (first <= last) {
 #pragma unroll
@@ -98,36 +102,33 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
             raw[u] = __builtin_nontemporal_load(
                 reinterpret_cast<const u32x4*>(x + min(max((u * 256 + tid) * GE, first), last)));
     }
+    if (tid < head + tail) v[N] = E::ld(x + edge);
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
-#pragma unroll
-        for (int e = 0; e < GE; ++e) {
-            if constexpr (sizeof(T) == 4)
-                v[u * GE + e] = __uint_as_float(raw[u][e]);
-            else
-                v[u * GE + e] = __uint_as_float(e & 1 ? raw[u][e >> 1] & 0xffff0000u : raw[u][e >> 1] << 16);
-        }
         const int c = (u * 256 + tid) * GE;
-        if (c < first || c > last) {
+        const bool in = c >= first && c <= last;
 #pragma unroll
-            for (int e = 0; e < GE; ++e) {
-                const bool in = c + e >= lo && c + e < hi;
-                v[u * GE + e] = -INFINITY;
-                if (in) v[u * GE + e] = E::ld(x + c + e);
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t two = in ? raw[u][e] : sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+            if constexpr (sizeof(T) == 4) {
+                v[u * GE + e] = __uint_as_float(two);
+            } else {
+                v[u * GE + 2 * e] = __uint_as_float(two << 16);
+                v[u * GE + 2 * e + 1] = __uint_as_float(two & 0xffff0000u);
             }
         }
     }
     auto key = [&](float y, int c) {
         return (uint64_t)ordered_logit(y) << 32 | (uint32_t)~(uint32_t)(c0 - mis + c);
     };
-    float mx = -INFINITY;
+    float mx = v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) mx = fmaxf(mx, v[i]);
     const uint32_t lane_best = ordered_logit(mx);
     mx = wave_all(mx, [](float a, float b) { return fmaxf(a, b); });
     const float ref = mx == -INFINITY ? 0.f : mx;
     // four terms in 32 bits, which are off by 2^-23 of them at most, all further in 64
-    double sum = 0.0;
+    double sum = fast_exp2((v[N] - ref) * kLog2e);
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
         float t[4];
@@ -154,14 +155,19 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
         p.maxs[blockIdx.x] = M;
         p.sums[blockIdx.x] = S;
     }
-    auto pick = [&](int i) {
-        if (v[i] >= least) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kBeamList) list[at] = key(v[i], (i / GE * 256 + tid) * GE + i % GE);
-        }
+    auto pick = [&](float y, int c) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kBeamList) list[at] = key(y, c);
     };
+    if (v[N] >= least) pick(v[N], edge);
+    uint32_t hits = 0;  // few, and read again: a copy of the code for each column would take longer to fetch
 #pragma unroll
-    for (int i = 0; i < N; ++i) pick(i);
+    for (int i = 0; i < N; ++i) hits |= (v[i] >= least) << i;
+#pragma unroll 1
+    for (; hits; hits &= hits - 1) {
+        const int i = __builtin_ctz(hits), c = (i / GE * 256 + tid) * GE + i % GE;
+        pick(E::ld(x + c), c);
+    }
     __syncthreads();
     const int n = count;
     uint64_t* out = p.cand + (int64_t)blockIdx.x * p.beams;

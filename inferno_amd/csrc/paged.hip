@@ -670,9 +670,12 @@ __global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p
     struct Meta {
         u32x4 w, pos;
     };
-    // f(j, x) for this lane's groups of four slots in order, x = load(j); U of them are loaded together
+    // f(j, x) for this lane's groups of four slots in order, x = load(j); U of them are loaded together.  Every loop
+    // runs a few rounds only, so the time is that of fetching its code: little of it (two rows of 32832 slots, 8
+    // heads: 36 us with U = 4 for keys in LDS as well, 32 so).
     auto each = [&](auto load, auto f) {
-        constexpr int U = 4;
+        constexpr int U = 2;
+#pragma unroll 1
         for (int i = 0; i < rounds; i += U) {
             decltype(load(0)) x[U];
 #pragma unroll
@@ -732,10 +735,14 @@ __global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p
         }
     });
     auto keys = [&](auto f) {  // f(j, four keys)
-        if constexpr (LDS)
-            each([&](int j) { return *reinterpret_cast<const u32x4*>(&skeys[min(j, (len - 1) & ~3)]); },
-                 [&](int j, u32x4 k) { f(j, j < len ? k : u32x4{kSafe, kSafe, kSafe, kSafe}); });
-        else
+        if constexpr (LDS) {
+#pragma unroll 1
+            for (int i = 0; i < rounds; ++i) {
+                const int j = first + 256 * i;
+                const u32x4 k = *reinterpret_cast<const u32x4*>(&skeys[min(j, (len - 1) & ~3)]);
+                f(j, j < len ? k : u32x4{kSafe, kSafe, kSafe, kSafe});
+            }
+        } else
             each(meta, [&](int j, Meta x) { f(j, keys_of(j, x)); });
     };
     __syncthreads();
@@ -750,6 +757,7 @@ __global__ __launch_bounds__(64 * W) void kv_evict_select_kernel(KvEvictParams p
         if (tid == 0) hist[kBins - 1] = 0;
         __syncthreads();
         uint32_t prefix = 0;
+#pragma unroll 1
         for (int pass = 0; pass < 3; ++pass) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 10 : 11;
             const uint32_t bins = 1u << width;
