@@ -629,6 +629,23 @@ def test_select_ties_and_odd_values(ia, dtype):
     check_select(ia, rnd(gen, (2 * beams, vocab), dtype), scores)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("beams,vocab,allowed", [
+    (32, 9001, (8999,)), (32, 9001, range(0, 40)), (32, 9001, (0, 64, 65, 200, 8191, 8192, 9000)), (5, 300, range(3, 300, 7)),
+    (8, 20000, range(8192, 8200)), (16, 4099, (1, 2, 3, 4096, 4098)), (32, 40000, range(100, 131)),
+])
+def test_select_allowed_tokens(ia, beams, vocab, allowed, dtype):
+    """All tokens but a few at -inf, wherever they lie: with fewer candidates than beams the lowest tokens follow."""
+    print(f"[case] select allowed {beams} V{vocab} {len(allowed)} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(vocab)
+    logits = torch.full((2 * beams, vocab), -math.inf, dtype=dtype)
+    logits[:, list(allowed)] = rnd(gen, (2 * beams, len(allowed)), dtype, 2.0)
+    check_select(ia, logits, rnd(gen, (2, beams)))
+    first = torch.full((2, beams), -math.inf)
+    first[:, 0] = 0.0
+    check_select(ia, logits, first)
+
+
 def test_select_in_place(ia):
     """The results may be the inputs, and a workspace may hold anything."""
     print("[case] select in place", flush=True)
