@@ -456,7 +456,8 @@ int inf_kv_append(const inf_paged_kv* cache, const void* k, inf_strides sk, cons
  * q, o: [rows, q_heads, 1, D] views; q_heads a multiple of the cache's heads.  max_len
  * (1..capacity) bounds the rows' lengths for the plan and the workspace; a row of length 0
  * or less gives zeros, one longer than max_len or with a page outside the pool NaN.  What lies
- * in a row's pages behind its length does not matter.
+ * in a row's pages behind its length does not matter.  An infinity or a NaN among the values before it
+ * gives an infinity or a NaN in its column; scores that are NaN, +inf or all -inf make the head's row NaN.
  * weights_out (may be NULL): dense [rows, heads, capacity]; position j < lens[n] becomes
  * weights_in's (0 where that is NULL; it may be weights_out) plus its probabilities summed over the
  * query heads of its head; other positions are left as they are.
