@@ -13,7 +13,8 @@ namespace Inferno {
 //     cache.begin(t);  for every layer: y = cache.attend(layer, q, k, v);  cache.end();
 // The first step is the prompt of each group, a row per group ([groups, H, t, D]); end() then gives
 // every beam the prompt's cache (the full pages are shared).  All later steps have t = 1 and
-// rows() rows.  A step that throws in between leaves the cache as it was before begin().
+// rows() rows.  A step that throws in between leaves the positions as begin() found them, or cut them, and the
+// attention counted so far.
 class PagedKVCache {
 public:
     struct Options {

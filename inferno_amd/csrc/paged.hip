@@ -1024,21 +1024,21 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(BeamReorderParams p, 
     const int parent = first + (ok ? pb : 0);
     const int32_t* own = p.c.table + row * p.c.table_stride;
     const int32_t* from = p.c.table + parent * p.c.table_stride;
-    const bool copy = ok && parent != row && part;
+    const bool other = ok && parent != row && part;
+    const int src = other ? from[full] : -1, dst = p.spare[row];
+    const bool copy = (unsigned)src < (unsigned)p.c.n_pages;
     if (layer == 0 && blockIdx.z == 0) {
         int32_t* out = p.table_out + row * p.table_out_stride;
         for (int i = threadIdx.x; i < p.c.max_pages; i += 256) {
             int v = own[i];
             if (!ok && len) v = -1;  // no such parent: the row names no page, and reads as NaN
             else if (i < full) v = from[i];
-            else if (i == full && copy) v = p.spare[row];
+            else if (i == full && other) v = copy ? dst : src;  // no page to copy: its number, which reads as NaN
             out[i] = v;
         }
-        if (threadIdx.x == 0) p.spare_out[row] = copy ? own[full] : p.spare[row];
+        if (threadIdx.x == 0) p.spare_out[row] = copy ? own[full] : dst;
     }
-    if (!copy) return;
-    const int src = from[full], dst = p.spare[row];
-    if ((unsigned)src >= (unsigned)p.c.n_pages || (unsigned)dst >= (unsigned)p.c.n_pages) return;
+    if (!copy || (unsigned)dst >= (unsigned)p.c.n_pages) return;
     const int n = p.c.heads * part * pieces;
     for (int i = blockIdx.z * 256 + threadIdx.x; i < n; i += 256 * gridDim.z) {
         const int hs = i / pieces, c = i - hs * pieces;

@@ -729,6 +729,27 @@ def test_reorder_bad_parent(ia):
     assert out[0].isnan().all() and out[1].isnan().all() and out[2].isfinite().all() and out[3].isnan().all()
 
 
+def test_reorder_from_a_bad_page(ia):
+    """A parent whose last page is not in the pool passes its number on: the row reads as NaN too, not as
+    what its spare page held."""
+    print("[case] reorder from a bad page", flush=True)
+    gen = torch.Generator().manual_seed(9)
+    c, _, _, spare = make_cache(ia, gen, [21] * 4, 1, 32, 16, F32, spare=4)
+    t = c.table.clone()
+    t[1, 1], t[3, 1] = -1, 10**6
+    c.table = t
+    c.k.nan_to_num_(0.5)
+    c.v.nan_to_num_(0.5)
+    sp = spare[:4].cuda()
+    table, spare_out = ia.beam_reorder(c, torch.tensor([[1, 0], [0, 0]], dtype=torch.int32, device="cuda"), sp)
+    assert table[0].tolist() == [int(t[1, 0]), -1] and int(spare_out[0]) == int(sp[0])
+    assert table[1].tolist() == [int(t[0, 0]), int(sp[1])]
+    assert table[3].tolist() == [int(t[2, 0]), int(sp[3])]
+    c.table = table
+    out = ia.attn_decode_paged(torch.ones(4, 1, 1, 32, device="cuda"), c)
+    assert out[0].isnan().all() and out[1:].isfinite().all()
+
+
 # ---- together -----------------------------------------------------------------------------------------
 
 
