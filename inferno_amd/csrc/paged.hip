@@ -129,7 +129,8 @@ int launch_kv_append(const KvAppendParams& p, int bf16, hipStream_t s) {
 // ============================================================================
 namespace {
 
-constexpr int kPagedPerCu = 3;  // workgroups of a CU: what the registers allow
+constexpr int kPagedPerCu = 3;           // workgroups of a CU: what the registers allow
+constexpr int kPagedHold = 12 << 10;     // bytes of LDS in which a wave holds scores: 144 KB a CU
 
 template <int D, typename E>
 __device__ __forceinline__ int paged_steps(int len, int max_len) {
@@ -159,7 +160,8 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
     constexpr int VD = D / 16;            // columns of a value row per lane
     constexpr int VW = VD * ES / 4;       // ... in 32-bit words
     constexpr int LD = D + 4;
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // o [4][heads][LD], then m, l [4][16]
+    // o [4][heads][LD], then m, l [4][16]; before that, the scores held
+    extern __shared__ __attribute__((aligned(16))) float lds[];
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
     // the tiles of more than 16 query heads read the same keys: neighbours on one XCD
@@ -250,9 +252,25 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
         for (int j = 0; j < VD; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
         bool bad = false;
-        float* sc = p.scores ? p.scores + ((int64_t)row * p.Hq + h * p.G + g0 + col) * p.score_ld : nullptr;
-
-        for (int base = base0; base < j1; base += STEP) {
+        // Scores are held in LDS and written many steps at a time: a few writes among the reads take HBM from the
+        // 6.3 TB/s of reads alone to the 4.9 of a copy (two rows of 131071, 2 heads of D 128, 8 query heads each,
+        // bf16: 67.4 us with a write per step, 63.4 so; the rows of 1 to 8191 above 232 and 213).
+        float* sc = p.scores ? p.scores + ((int64_t)row * p.Hq + h * p.G + g0) * p.score_ld : nullptr;
+        float* hold = lds + wave * (kPagedHold / 4);
+        const int most = kPagedHold / (64 * T * gn);
+        int held = 0;
+        auto flush = [&](int base) {  // the steps before `base`; the wave's other lanes wrote some of them
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (int i = lane; i < held * gn * 4 * T; i += 64) {
+                const int key = 4 * (i % (4 * T)), sh = i / (4 * T), s = sh / gn, head = sh - s * gn;
+                *reinterpret_cast<f32x4*>(sc + head * p.score_ld + base - (held - s) * STEP + key) =
+                    *reinterpret_cast<const f32x4*>(hold + 4 * i);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            held = 0;
+        };
+        int base = base0;
+        for (; base < j1; base += STEP) {
             // rows behind the end are read as the last key's
             int page[T] = {};
             if constexpr (!SMALL) {
@@ -332,11 +350,15 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
                         for (int w = 0; w < VW; ++w) vr[i >> 2][i & 3][w] = 0;
                     }
             }
-            if (sc && col < gn) {
+            if (sc) {
+                if (held == most) flush(base);
+                if (col < gn) {
 #pragma unroll
-                for (int t = 0; t < T; ++t)
-                    *reinterpret_cast<f32x4*>(sc + base + 16 * t + 4 * g) =
-                        f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+                    for (int t = 0; t < T; ++t)
+                        *reinterpret_cast<f32x4*>(hold + (held * gn + col) * 16 * T + 16 * t + 4 * g) =
+                            f32x4{x[4 * t], x[4 * t + 1], x[4 * t + 2], x[4 * t + 3]};
+                }
+                ++held;
             }
             float mx = m;
 #pragma unroll
@@ -381,6 +403,11 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
                     for (int j = 0; j < VD; ++j)
                         acc[j] = mfma16x16x4(__uint_as_float(vr[i >> 2][i & 3][j]), x[i], acc[j]);
             }
+        }
+
+        if (sc) {
+            flush(base);
+            __syncthreads();
         }
 
         // Join the waves: lane (col, g) holds head col's o[VD (4 g + r) + j] in acc[j][r].
@@ -524,14 +551,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedDecodeParams p, in
                 if (j + e < n) w[e] = p.w_in[wat + e];
         }
     }
-    constexpr int U = 8;         // heads whose scores are loaded together
+    constexpr int U = 8;  // heads whose scores are loaded together, under no condition, which each load would wait for
+    const float* scores = p.scores + hq0 * p.score_ld + min(j, (n - 1) & ~3);
     for (int h0 = 0; h0 < p.G; h0 += U) {
         const int gn = min(U, p.G - h0);
         f32x4 sc[U];
 #pragma unroll
         for (int i = 0; i < U; ++i)
-            if (i < gn && j < n)
-                sc[i] = *reinterpret_cast<const f32x4*>(p.scores + (hq0 + h0 + i) * p.score_ld + j);
+            sc[i] = *reinterpret_cast<const f32x4*>(scores + (int64_t)min(h0 + i, p.G - 1) * p.score_ld);
         // thread t: head t % 8, every 32nd part
         const int mine = tid & 7;
         float M = -INFINITY, L = 0.f;
@@ -590,7 +617,8 @@ static int launch_paged_t(const PagedDecodeParams& p, hipStream_t s) {
     int64_t units = (int64_t)p.c.heads * (p.groups ? p.groups : p.c.rows);
     if (p.head_tiles > 1) units = (units + 7) / 8 * 8 * p.head_tiles;
     const dim3 grid((unsigned)units, p.groups ? (unsigned)paged_blocks(p.c.rows) : 1u);
-    const size_t lds = (size_t)(4 * (p.G < 16 ? p.G : 16) * (D + 4) + 128) * sizeof(float);
+    size_t lds = (size_t)(4 * (p.G < 16 ? p.G : 16) * (D + 4) + 128) * sizeof(float);
+    if (p.scores) lds = std::max<size_t>(lds, 4 * kPagedHold);  // the same LDS first holds scores
     if (p.c.page_shift < 4)
         hipLaunchKernelGGL((paged_split_kernel<D, E, true>), grid, dim3(256), lds, s, p);
     else
