@@ -151,7 +151,9 @@ struct Shares {
 
 }  // namespace
 
-template <int D, typename E, bool SMALL>
+// SMALL: pages of fewer than 16 keys.  WEIGH: scores are written for the weights (in all variants: 8% slower where
+// the registers are few, D 128 in fp32).
+template <int D, typename E, bool SMALL, bool WEIGH>
 __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDecodeParams p) {
     constexpr int ES = sizeof(E);
     constexpr int STEP = paged_step(D, ES == 2);
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
         // Scores are held in LDS and written many steps at a time: a few writes among the reads take HBM from the
         // 6.3 TB/s of reads alone to the 4.9 of a copy (two rows of 131071, 2 heads of D 128, 8 query heads each,
         // bf16: 67.4 us with a write per step, 63.4 so; the rows of 1 to 8191 above 232 and 213).
-        float* sc = p.scores ? p.scores + ((int64_t)row * p.Hq + h * p.G + g0) * p.score_ld : nullptr;
+        float* sc = WEIGH ? p.scores + ((int64_t)row * p.Hq + h * p.G + g0) * p.score_ld : nullptr;
         float* hold = lds + wave * (kPagedHold / 4);
         const int most = kPagedHold / (64 * T * gn);
         int held = 0;
@@ -350,7 +352,7 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
                         for (int w = 0; w < VW; ++w) vr[i >> 2][i & 3][w] = 0;
                     }
             }
-            if (sc) {
+            if constexpr (WEIGH) {
                 if (held == most) flush(base);
                 if (col < gn) {
 #pragma unroll
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
             }
         }
 
-        if (sc) {
+        if constexpr (WEIGH) {
             flush(base);
             __syncthreads();
         }
@@ -619,10 +621,17 @@ static int launch_paged_t(const PagedDecodeParams& p, hipStream_t s) {
     const dim3 grid((unsigned)units, p.groups ? (unsigned)paged_blocks(p.c.rows) : 1u);
     size_t lds = (size_t)(4 * (p.G < 16 ? p.G : 16) * (D + 4) + 128) * sizeof(float);
     if (p.scores) lds = std::max<size_t>(lds, 4 * kPagedHold);  // the same LDS first holds scores
+    auto split = [&](auto small) {
+        constexpr bool kSmall = decltype(small)::value;
+        if (p.scores)
+            hipLaunchKernelGGL((paged_split_kernel<D, E, kSmall, true>), grid, dim3(256), lds, s, p);
+        else
+            hipLaunchKernelGGL((paged_split_kernel<D, E, kSmall, false>), grid, dim3(256), lds, s, p);
+    };
     if (p.c.page_shift < 4)
-        hipLaunchKernelGGL((paged_split_kernel<D, E, true>), grid, dim3(256), lds, s, p);
+        split(std::true_type{});
     else
-        hipLaunchKernelGGL((paged_split_kernel<D, E, false>), grid, dim3(256), lds, s, p);
+        split(std::false_type{});
     if (p.groups) {
         const int wblocks = p.scores ? (p.max_len + 1023) / 1024 : 0;
         const int wide = (reinterpret_cast<uintptr_t>(p.w_in) | reinterpret_cast<uintptr_t>(p.w_out)) % 16 == 0;
