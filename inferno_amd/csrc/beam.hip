@@ -420,7 +420,8 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
 }
 
 // Columns per workgroup: 8192, fewer (half the time of a workgroup, twice the parts to join) where the
-// device would not be filled.
+// device would not be filled (beams of 50257 bf16 columns, us, 8192 and 4096: 64 beams 11.6 and 12.5, 256 16.0
+// and 18.1; 32 beams, 4096 and 2048: 11.3 and 13.4).
 void beam_select_plan(int64_t groups, int beams, int64_t vocab, int* nsplit, int64_t* chunk) {
     int64_t ch = kBeamCols;
     while (ch > 2048 && groups * beams * ((vocab + ch - 1) / ch) < 256) ch /= 2;
