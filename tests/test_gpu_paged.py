@@ -193,6 +193,37 @@ def test_decode_many_rows(ia, rows, heads, group, D, page, longest, weigh, dtype
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("heads,group,D,lens", [
+    (96, 16, 32, (2500, 1, 1800)), (96, 4, 64, (4000, 3000)), (128, 12, 128, (900, 0, 1500)),
+])
+def test_decode_weights_of_long_shares(ia, heads, group, D, lens, dtype):
+    """Workgroups with many steps of several rows: the weights as from a cache of one head, whose workgroups have
+    one step each.  Scores and maxima are the same bits; sums of up to n probabilities, in any order and joined
+    from parts, are n 2^-24 off at most on either side, and so is each probability relative to itself."""
+    print(f"[case] paged decode long shares {heads}x{group} D{D} {lens} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(heads + D)
+    rows = len(lens)
+    c, _, _, _ = make_cache(ia, gen, list(lens), heads, D, 16, dtype)
+    q = rnd(gen, (rows, heads * group, 1, D), dtype, 1.5).cuda()
+    w = torch.full(c.meta_shape, -5.0, device="cuda")
+    out = ia.attn_decode_paged(q, c, weights_out=w)
+    assert out.isfinite().all()
+    rel = 2 * max(lens) * 2.0**-24
+    for h in (0, 1, heads // 2, heads - 1):
+        one = ia.PagedKV(c.k[:, h:h + 1], c.v[:, h:h + 1], c.table, c.lens)
+        w1 = torch.full(one.meta_shape, -5.0, device="cuda")
+        o1 = ia.attn_decode_paged(q[:, h * group:(h + 1) * group], one, weights_out=w1)
+        assert ((w[:, h] - w1[:, 0]).abs() <= (rel + group * 2.0**-23) * w1[:, 0].abs()).all()
+        o = out[:, h * group:(h + 1) * group].float()
+        # the outputs: the same, of sums of |p v|, and bf16's own rounding on both sides
+        top = c.v[:, h].float().nan_to_num(0.0).abs().max()
+        err = 2 * rel * top + (2.0**-7 * o1.float().abs() if dtype == BF16 else 0.0)
+        assert ((o - o1.float()).abs() <= err).all()
+    for r, n in enumerate(lens):
+        assert (w[r, :, n:] == -5.0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("layout", ["slots", "joint"])
 def test_decode_layouts(ia, layout, dtype):
     """Pools of other orders, queries out of a packed projection, a strided output, a wide table."""
