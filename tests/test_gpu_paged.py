@@ -1011,6 +1011,55 @@ def test_graph_replays_follow_the_lengths(ia):
             s["spare"].copy_(s["s2"])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_graph_replays_of_a_bounded_cache(ia, dtype):
+    """A captured step that counts, appends, attends and cuts in place, replayed while rows reach the limit at
+    different times; every replay against the eager calls, bit for bit."""
+    print(f"[case] paged graph of a bounded cache {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(21)
+    rows, heads, group, D, page, max_pages, keep, recent = 3, 2, 3, 64, 8, 5, 33, 4
+    pages = rows * max_pages + 2
+    table = torch.randperm(pages, generator=gen)[:rows * max_pages].to(torch.int32).view(rows, max_pages)
+    k, v = rnd(gen, (pages, heads, page, D), dtype), rnd(gen, (pages, heads, page, D), dtype)
+
+    def state():
+        s = dict(c=ia.PagedKV(k.cuda(), v.cuda(), table.cuda(), torch.tensor([0, 20, 33], dtype=torch.int32).cuda()),
+                 kn=torch.zeros(rows, heads, 1, D, dtype=dtype, device="cuda"),
+                 q=torch.zeros(rows, heads * group, 1, D, dtype=dtype, device="cuda"),
+                 out=torch.zeros(rows, heads * group, 1, D, dtype=dtype, device="cuda"))
+        s["w"], s["pos"], s["seen"] = s["c"].meta(F32), s["c"].meta(torch.int32), s["c"].lens.clone()
+        s["pos"].copy_(torch.arange(s["c"].capacity, device="cuda"))
+        s["ws"] = ia.attn_decode_paged_workspace(s["c"], heads * group, weights=True)
+        s["ws2"] = ia.kv_evict_workspace(s["c"], keep)
+        return s
+
+    def step(s):
+        s["c"].lens.add_(1)
+        s["seen"].add_(1)
+        ia.kv_append(s["c"], s["kn"], s["kn"], weights=s["w"], positions=s["pos"], seen=s["seen"])
+        ia.attn_decode_paged(s["q"], s["c"], weights=s["w"], weights_out=s["w"], out=s["out"], workspace=s["ws"])
+        ia.kv_evict(s["c"], s["w"], s["pos"], keep, recent, lens_out=s["c"].lens, workspace=s["ws2"])
+
+    gs, es = state(), state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(gs)
+    for rep in range(18):
+        kn, q = rnd(gen, gs["kn"].shape, dtype).cuda(), rnd(gen, gs["q"].shape, dtype, 1.5).cuda()
+        for s in (gs, es):
+            s["kn"].copy_(kn)
+            s["q"].copy_(q)
+        step(es)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in ("w", "pos", "out", "seen"):
+            assert torch.equal(gs[name], es[name]), (rep, name)
+        for name in ("k", "v", "lens"):
+            assert torch.equal(getattr(gs["c"], name), getattr(es["c"], name)), (rep, name)
+        assert gs["c"].lens.tolist() == [rep + 1, min(21 + rep, keep), keep]
+
+
 def test_other_stream(ia):
     """Calls with a stream of their own, as an object and as a handle."""
     print("[case] paged other stream", flush=True)
