@@ -83,6 +83,13 @@ int check_cache(const inf_paged_kv* c, bool written, inf::PagedView* out) {
     return INF_OK;
 }
 
+// Whether [rows, heads, capacity] arrays of 4-byte elements overlap without being the same.
+bool overlap_partly(const inf_paged_kv* c, const void* a, const void* b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t bytes = (uintptr_t)c->rows * c->heads * c->max_pages * c->page_size * 4;
+    return a && b && x != y && x < y + bytes && y < x + bytes;
+}
+
 int64_t capacity(const inf_paged_kv* c) { return (int64_t)c->max_pages * c->page_size; }
 
 // The decode's workspace: the shares' results (one per row and share that meet, so at most rows +
@@ -191,6 +198,7 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
         (st = check_apart(so, cache->rows, q_heads, 1, cache->D)))
         return st;
     if (weights_in && !weights_out) return INF_ERR_NULL_POINTER;
+    if (overlap_partly(cache, weights_in, weights_out)) return INF_ERR_BAD_STRIDE;
     const DecodeSizes s = decode_sizes(cache, q_heads, max_len, weights_out != nullptr);
     const int64_t tiles = (q_heads / cache->heads + 15) / 16;
     if ((int64_t)cache->rows * cache->heads * tiles > kMaxBlocks / 16 ||
@@ -235,6 +243,8 @@ int inf_kv_evict(const inf_paged_kv* cache, const float* weights_in, float* weig
     if (st != INF_OK || (st = check_cache(cache, true, &p.c))) return st;
     if (recent < 0 || recent > keep) return INF_ERR_BAD_SHAPE;
     if (!weights_in || !weights_out || !positions_in || !positions_out || !lens_out) return INF_ERR_NULL_POINTER;
+    if (overlap_partly(cache, weights_in, weights_out) || overlap_partly(cache, positions_in, positions_out))
+        return INF_ERR_BAD_STRIDE;
     size_t need = 0;
     inf_kv_evict_workspace(cache, keep, max_len, &need);
     if (!workspace || ws_bytes < need) return INF_ERR_WORKSPACE;

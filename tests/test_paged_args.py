@@ -115,6 +115,15 @@ def test_decode_arguments(kw, status):
     assert decode(cache(), **kw) == status
 
 
+def test_outputs_that_overlap_the_inputs_in_part():
+    c = cache()
+    whole = 4 * 2 * 64 * 4  # rows, heads, capacity, bytes
+    for off in (4, 64, whole - 4, -whole + 4):
+        assert evict(c, wo=FAKE + off) == 3 and evict(c, po=FAKE + off) == 3
+        assert decode(c, w_in=FAKE, w_out=FAKE + off, ws=FAKE, n=1 << 30) == 3
+    assert evict(c, wo=FAKE + whole, n=0) == 6  # behind them: the next check's
+
+
 def test_decode_workspace():
     L, n = ia.lib(), ctypes.c_size_t(0)
 
