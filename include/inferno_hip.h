@@ -459,8 +459,8 @@ int inf_kv_append(const inf_paged_kv* cache, const void* k, inf_strides sk, cons
  * in a row's pages behind its length does not matter.  An infinity or a NaN among the values before it
  * gives an infinity or a NaN in its column; scores that are NaN, +inf or all -inf make the head's row NaN.
  * weights_out (may be NULL): dense [rows, heads, capacity]; position j < lens[n] becomes
- * weights_in's (0 where that is NULL; it may be weights_out, but not overlap it in part) plus its probabilities summed over the
- * query heads of its head; other positions are left as they are.
+ * weights_in's (0 where that is NULL; it may be weights_out, but not overlap it in part) plus its
+ * probabilities summed over the query heads of its head; other positions are left as they are.
  * workspace: inf_attn_decode_paged_workspace bytes for the same arguments (0 for short
  * caches without weights: then it may be NULL), 256-byte aligned.  Calls that share one must
  * not overlap.  Results do not depend on scheduling: the same bits on every run. */
@@ -476,8 +476,8 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
  * behind the first `keep` fill the holes among these, in order; a slot that stays is not
  * moved, so the order of a row's positions changes, which attention does not see, and
  * the slots past the cut keep what they had.  weights_out and positions_out (dense
- * [rows, heads, capacity], may be the inputs, but not overlap them in part) get the kept ones' in their first `keep` slots,
- * shorter rows' in their first lens[n]; lens_out (may be cache->lens) is min(lens[n], keep).
+ * [rows, heads, capacity], may be the inputs, but not overlap them in part) get the kept ones' in their
+ * first `keep` slots, shorter rows' in their first lens[n]; lens_out (may be cache->lens) is min(lens[n], keep).
  * A row longer than max_len is left as it is.  Pages that are written must not
  * be shared with another row.  workspace: inf_kv_evict_workspace bytes, 4-byte aligned. */
 int inf_kv_evict_workspace(const inf_paged_kv* cache, int keep, int max_len, size_t* out_bytes);
