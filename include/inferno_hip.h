@@ -486,7 +486,9 @@ int inf_kv_evict(const inf_paged_kv* cache, const float* weights_in, float* weig
                  size_t ws_bytes, void* stream);
 
 /* Beam search's step: of a group's beams x vocab candidates the best `beams` (<= 32), best first.
- * Candidate (b, t) scores scores[b] + logits[b, t] - lse(logits[b]), in 64 bits; equal scores go to
+ * Candidate (b, t) scores scores[b] + logits[b, t] - lse(logits[b]), in 64 bits but for the exponentials
+ * under lse, which are 32-bit (it is off by 2^-18 at most, by some 2^-24 on ordinary logits; beams of equal
+ * logits have the same bits, wherever their rows start); equal scores go to
  * the lower b, then the lower t, and within a beam the logits decide.  logits: [groups * beams, vocab],
  * rows ld elements apart, of any alignment; scores, finished, and the results tokens, parents (the
  * beam b within the group), scores_out and finished_out: [groups, beams].

@@ -6,8 +6,8 @@
 // beam's parts to its lse and ranks what is left of a group, some hundreds of candidates, by the
 // whole score in 64 bits.  Within a beam the score's order is the logits', so the first step needs
 // no lse and is exact; between beams scores can lie close together, and there the sums of
-// exponentials are held in 64 bits as well.  Equal scores go to the lower beam, then the lower
-// token.
+// exponentials are held in 64 bits as well (the exponentials themselves are 32-bit).  Equal scores go to
+// the lower beam, then the lower token.
 //
 // The best few of many: with each lane's largest value known, the beams-th largest of a wave's 64 is
 // at most the beams-th largest of all its values, so only values from the best wave's up can matter:
@@ -28,6 +28,16 @@ namespace {
 
 constexpr int kBeamCols = 8192;  // columns of a workgroup at most: 32 per thread, in registers
 constexpr int kBeamList = 1024;  // candidates in LDS; more of them (equal ones) are picked one by one
+
+// 16 bytes from any address of an element.
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+__device__ __forceinline__ u32x4 ld16_any(const float* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_a4*>(p));
+}
+__device__ __forceinline__ u32x4 ld16_any(const uint16_t* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_a2*>(p));
+}
 
 // Order of the floats as unsigned numbers, -0 as 0, NaN below -inf; 0 stands for no value.
 __device__ __forceinline__ uint32_t ordered_logit(float x) {
@@ -87,33 +97,28 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     const int64_t row = blockIdx.x / p.nsplit;
     const int split = blockIdx.x % p.nsplit;
     if (!beam_lives(p, row)) return;
-    // Columns counted from the 16-byte boundary at or before the row's start; this workgroup's, from
-    // its first one on, are those in [lo, hi).
-    const T* x = (const T*)p.logits + row * p.ld;
-    const int mis = (int)(reinterpret_cast<uintptr_t>(x) / sizeof(T) % GE);
+    // This workgroup's columns are [0, hi) from its first one on.  They are counted from the row's start, so that equal
+    // rows are summed alike wherever they lie: 16 bytes are loaded from any address that a column has.
     const int64_t c0 = (int64_t)split * (256 * N);
-    const int lo = split == 0 ? mis : 0, hi = (int)min((int64_t)(256 * N), p.vocab + mis - c0);
-    x += c0 - mis;
-    // The row's whole 16-byte pieces are this thread's N columns, and the few columns before and behind them one
-    // more.  Every load stands alone, at a place inside the row: under a condition the compiler would wait for
-    // each before the next.
-    const int first = (lo + GE - 1) / GE * GE, last = hi / GE * GE - GE;
-    const int head = first <= last ? first - lo : hi - lo, tail = first <= last ? hi - last - GE : 0;
-    const int edge = tid < head ? lo + tid : last + GE + tid - head;
+    const T* x = (const T*)p.logits + row * p.ld + c0;
+    const int hi = (int)min((int64_t)(256 * N), p.vocab - c0);
+    // The whole 16-byte pieces are this thread's N columns, and the few columns behind them one more.  Every load stands
+    // alone, at a place inside the row: under a condition the compiler would wait for each before the next.
+    const int last = hi / GE * GE - GE, edge = last + GE + tid;
+    const bool tail = edge < hi;
     float v[N + 1];  // columns outside are -inf
     v[N] = -INFINITY;
     u32x4 raw[NV];
-    if (first <= last) {
+    if (last >= 0) {
 #pragma unroll
         for (int u = 0; u < NV; ++u)
-            raw[u] = __builtin_nontemporal_load(
-                reinterpret_cast<const u32x4*>(x + min(max((u * 256 + tid) * GE, first), last)));
+            raw[u] = ld16_any(x + min((u * 256 + tid) * GE, last));
     }
-    if (tid < head + tail) v[N] = E::ld(x + edge);
+    if (tail) v[N] = E::ld(x + edge);
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
         const int c = (u * 256 + tid) * GE;
-        const bool in = c >= first && c <= last;
+        const bool in = c <= last;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t two = in ? raw[u][e] : sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
@@ -126,7 +131,7 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
         }
     }
     auto key = [&](float y, int c) {
-        return (uint64_t)ordered_logit(y) << 32 | (uint32_t)~(uint32_t)(c0 - mis + c);
+        return (uint64_t)ordered_logit(y) << 32 | (uint32_t)~(uint32_t)(c0 + c);
     };
     float mx = v[N];
 #pragma unroll
@@ -134,7 +139,9 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     const uint32_t lane_best = ordered_logit(mx);
     mx = wave_all(mx, [](float a, float b) { return fmaxf(a, b); });
     const float ref = mx == -INFINITY ? 0.f : mx;
-    // four terms in 32 bits, which are off by 2^-23 of them at most, all further in 64
+    // Terms in 32 bits: one at d below the maximum is off by (2.25 |d| + 2) 2^-24 of itself (difference, product, log2 e and
+    // v_exp_f32), and sums of four by 2^-23 more.  All further sums in 64.  |d| has a mean of at most 18 under the
+    // terms' shares (2^31 columns), so the lse is off by 2^-18 at most.
     double sum = fast_exp2((v[N] - ref) * kLog2e);
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
@@ -182,7 +189,7 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
         if (n < p.beams && wave == 0) {
             // fewer above -inf than beams: the lowest columns of the others (where there is a NaN, nobody asks)
             int at = n;
-            for (int c = lo; c < hi && at < p.beams; c += 64) {
+            for (int c = 0; c < hi && at < p.beams; c += 64) {
                 const bool rest = c + lane < hi && !(E::ld(x + c + lane) >= kLowest);
                 const uint64_t m = __ballot(rest);
                 const int i =
@@ -209,7 +216,7 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     for (int k = 0; k < p.beams; ++k) {
         uint64_t best = 0;
 #pragma unroll 4
-        for (int c = lo + tid; c < hi; c += 256) {
+        for (int c = tid; c < hi; c += 256) {
             const uint64_t y = key(E::ld(x + c), c);
             if (y < before && y > best) best = y;
         }
@@ -426,7 +433,7 @@ void beam_select_plan(int64_t groups, int beams, int64_t vocab, int* nsplit, int
     int64_t ch = kBeamCols;
     while (ch > 2048 && groups * beams * ((vocab + ch - 1) / ch) < 256) ch /= 2;
     *chunk = ch;
-    *nsplit = (int)((vocab + 7 + ch - 1) / ch);  // a row starts up to 7 columns behind a 16-byte boundary
+    *nsplit = (int)((vocab + ch - 1) / ch);
 }
 
 template <typename E>
