@@ -74,6 +74,16 @@ __device__ __forceinline__ double shfl_xor_d(double v, int m) {
     return __longlong_as_double((long long)shfl_xor64((uint64_t)__double_as_longlong(v), m));
 }
 
+// A group's candidate, its score an ordered number; `at` is the beam and, inverted, the logit: logits may differ
+// by less than the last bit of their scores.
+struct Ranked {
+    uint64_t score, at;
+    uint32_t token;
+    __device__ __forceinline__ bool before(const Ranked& o) const {
+        return score > o.score || (score == o.score && (at < o.at || (at == o.at && token < o.token)));
+    }
+};
+
 // Whether a beam reads its logits: not if it is finished, or its score is not finite (then all
 // its candidates have that score).
 __device__ __forceinline__ bool beam_lives(const BeamSelectParams& p, int64_t row) {
@@ -237,8 +247,9 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
     __shared__ double base[kMaxBeams];  // score - lse; the score of a beam that is finished or flat
     __shared__ int kind[kMaxBeams];
     __shared__ uint64_t ls[kBeamList], lt[kBeamList];
+    __shared__ uint32_t lk[kBeamList];
     __shared__ int count;
-    __shared__ uint64_t ws[W], wt[W];
+    __shared__ Ranked wr[W];
     __shared__ uint32_t wall[W];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int64_t row0 = (int64_t)blockIdx.x * p.beams;
@@ -317,24 +328,25 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
     }
     if (tid == 0) count = 0;
     __syncthreads();
-    // Beam b's candidate c, the j-th: its score as an ordered number (0: there is none) and its place.
-    auto candidate = [&](int b, int j, uint64_t c, uint64_t& at) -> uint64_t {
-        uint32_t token = (uint32_t)j;
+    // Beam b's candidate c, the j-th (a score of 0: there is none).
+    auto candidate = [&](int b, int j, uint64_t c) -> Ranked {
+        Ranked r{0, (uint64_t)b << 32, (uint32_t)j};
         double score = base[b];
         if (kind[b] == kLives) {
-            if (!c) return 0;
-            token = ~(uint32_t)c;
+            if (!c) return r;
+            r.token = ~(uint32_t)c;
+            r.at |= ~(uint32_t)(c >> 32);
             score += (double)logit_of((uint32_t)(c >> 32));
         } else if (kind[b] == kFinished) {
-            if (j) return 0;
-            token = (uint32_t)p.eos;
+            if (j) return r;
+            r.token = (uint32_t)p.eos;
         } else if (j >= p.beams || j >= p.vocab) {
-            return 0;
+            return r;
         }
-        at = (uint64_t)b << 32 | token;
-        return ordered_score(score);
+        r.score = ordered_score(score);
+        return r;
     };
-    auto scan = [&](auto f) {  // f(score, place) for this lane's candidates
+    auto scan = [&](auto f) {  // f(candidate) for this lane's candidates
         At a = start();
         if (all > U) loaded = a;
         for (int r = 0; r < all; r += U) {
@@ -343,16 +355,16 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
             for (int u = 0; u < U; ++u) {
                 if (r + u < all) {
                     const int j = place(a);
-                    uint64_t at;
                     if (j < per)
-                        if (const uint64_t s = candidate(a.b, j, cand[u], at)) f(s, at);
+                        if (const Ranked r = candidate(a.b, j, cand[u]); r.score) f(r);
                 }
                 next(a);
             }
         }
     };
-    auto emit = [&](int k, uint64_t s, uint64_t at) {
-        const int b = (int)(at >> 32), token = (int)(uint32_t)at;
+    auto emit = [&](int k, const Ranked& r) {
+        const int b = (int)(r.at >> 32), token = (int)r.token;
+        const uint64_t s = r.score;
         const int64_t o = row0 + k;
         p.tokens[o] = token;
         p.parents[o] = b;
@@ -361,19 +373,20 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
         if (p.finished_out) p.finished_out[o] = kind[b] == kFinished || token == p.eos;
     };
     uint32_t best = 0;
-    scan([&](uint64_t s, uint64_t) { best = max(best, (uint32_t)(s >> 32)); });
+    scan([&](const Ranked& r) { best = max(best, (uint32_t)(r.score >> 32)); });
     // The group's `beams`-th is no less than any wave's.
     const uint32_t nth = wave_nth<4>(best, p.beams);
     if (lane == 0) wall[wave] = nth;
     __syncthreads();
     uint32_t least = 0;
     for (int w = 0; w < W; ++w) least = max(least, wall[w]);
-    scan([&](uint64_t s, uint64_t at) {
-        if ((uint32_t)(s >> 32) >= least) {
+    scan([&](const Ranked& r) {
+        if ((uint32_t)(r.score >> 32) >= least) {
             const int k = atomicAdd(&count, 1);
             if (k < kBeamList) {
-                ls[k] = s;
-                lt[k] = at;
+                ls[k] = r.score;
+                lt[k] = r.at;
+                lk[k] = r.token;
             }
         }
     });
@@ -382,46 +395,34 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
     if (n <= kBeamList) {
         for (int i0 = 0; i0 < n; i0 += kThreads / 4) {
             const int i = i0 + (tid >> 2);
-            const uint64_t s = ls[min(i, n - 1)], t = lt[min(i, n - 1)];
+            const int own = min(i, n - 1);
+            const Ranked r{ls[own], lt[own], lk[own]};
             int better = 0;
 #pragma unroll 4
-            for (int j = tid & 3; j < n; j += 4) better += ls[j] > s || (ls[j] == s && lt[j] < t);
+            for (int j = tid & 3; j < n; j += 4) better += Ranked{ls[j], lt[j], lk[j]}.before(r);
             better += (int)dpp_u32<0xB1>((uint32_t)better);
             better += (int)dpp_u32<0x4E>((uint32_t)better);
-            if (i < n && (tid & 3) == 0 && better < p.beams) emit(better, s, t);
+            if (i < n && (tid & 3) == 0 && better < p.beams) emit(better, r);
         }
         return;
     }
-    uint64_t s0 = ~0ull, t0 = 0;  // the one picked last
+    Ranked last{~0ull, 0, 0};  // the one picked last
     for (int k = 0; k < p.beams; ++k) {
-        uint64_t s1 = 0, t1 = ~0ull;
-        scan([&](uint64_t s, uint64_t at) {
-            if ((s < s0 || (s == s0 && at > t0)) && (s > s1 || (s == s1 && at < t1))) {
-                s1 = s;
-                t1 = at;
-            }
+        Ranked top{0, ~0ull, ~0u};
+        scan([&](const Ranked& r) {
+            if (last.before(r) && r.before(top)) top = r;
         });
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) {
-            const uint64_t s = shfl_xor64(s1, m), t = shfl_xor64(t1, m);
-            if (s > s1 || (s == s1 && t < t1)) {
-                s1 = s;
-                t1 = t;
-            }
+            const Ranked r{shfl_xor64(top.score, m), shfl_xor64(top.at, m), (uint32_t)__shfl_xor(top.token, m, 64)};
+            if (r.before(top)) top = r;
         }
-        if (lane == 0) {
-            ws[wave] = s1;
-            wt[wave] = t1;
-        }
+        if (lane == 0) wr[wave] = top;
         __syncthreads();
-        s0 = ws[0];
-        t0 = wt[0];
+        last = wr[0];
         for (int w = 1; w < W; ++w)
-            if (ws[w] > s0 || (ws[w] == s0 && wt[w] < t0)) {
-                s0 = ws[w];
-                t0 = wt[w];
-            }
-        if (tid == 0) emit(k, s0, t0);
+            if (wr[w].before(last)) last = wr[w];
+        if (tid == 0) emit(k, last);
         __syncthreads();
     }
 }

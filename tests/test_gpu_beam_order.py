@@ -102,3 +102,24 @@ def test_lse_of_flat_rows(ia, vocab, peak, dtype):
     mean = (p * (x.amax(1, keepdim=True) - x)).sum(1)[:, None]
     assert (tokens == vocab // 3).all()
     assert ((scores.double().cpu() - want).abs() <= (2.25 * mean + 4) * 2.0**-24 + 2.0**-24 * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("groups,beams,vocab,rest", [(1, 3, 200, -1.0), (2, 8, 9001, -2.0), (3, 4, 50257, -8.0),
+                                                     (2, 32, 9001, None)])
+def test_logits_decide_within_a_beam(ia, groups, beams, vocab, rest, dtype):
+    """Logits that differ by less than their score's last bit in 64 bits: within a beam the larger one is first all
+    the same.  rest None: all logits are such, more candidates of one score than are ranked at a time."""
+    print(f"[case] tiny logits {groups}x{beams} V{vocab} rest {rest} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(vocab)
+    n = vocab if rest is None else 2 * beams
+    tiny = (torch.arange(1, 65) * 2.0**-90).to(dtype)  # few enough for bf16 to tell them apart
+    one = torch.full((vocab,), 0.0 if rest is None else rest, dtype=dtype)
+    where = torch.randperm(vocab, generator=gen)[:n]
+    one[where] = tiny[torch.arange(n) % 64] if rest is None else tiny[:n]
+    logits = one.expand(groups * beams, vocab).contiguous()
+    tokens, parents, scores, _ = ia.beam_select(rows_at(logits, 1, 0), torch.full((groups, beams), -3.5).cuda())
+    want = torch.sort(one.float(), descending=True, stable=True).indices[:beams]
+    for g in range(groups):  # all scores are equal, so beam 0's best are taken
+        assert parents[g].tolist() == [0] * beams and tokens[g].tolist() == want.tolist()
+        assert (scores[g] == scores[g, 0]).all()
