@@ -475,7 +475,8 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
  * weights, of equal weights the lower slot's (NaN counts as below all).  The kept slots
  * behind the first `keep` fill the holes among these, in order; a slot that stays is not
  * moved, so the order of a row's positions changes, which attention does not see, and
- * the slots past the cut keep what they had.  weights_out and positions_out (dense
+ * the slots past the cut keep what they had.  A position that is moved out of a page outside the pool becomes NaN.
+ * weights_out and positions_out (dense
  * [rows, heads, capacity], may be the inputs, but not overlap them in part) get the kept ones' in their
  * first `keep` slots, shorter rows' in their first lens[n]; lens_out (may be cache->lens) is min(lens[n], keep).
  * A row longer than max_len is left as it is.  Pages that are written must not

@@ -999,7 +999,11 @@ __global__ __launch_bounds__(256) void kv_evict_move_kernel(KvEvictParams p, int
     for (int u = 0; u < U; ++u) {
         if (i0 + u * per >= n) break;
         const int slot = dst[u] & mask;
-        if (pd[u] >= 0 && ps[u] >= 0) {
+        if (ps[u] < 0) {  // no page to copy from: NaN, so that attention sees it here as it did there
+            const uint32_t nan = esz == 2 ? 0x7fc07fc0u : 0x7fc00000u;
+            kx[u] = vx[u] = u32x4{nan, nan, nan, nan};
+        }
+        if (pd[u] >= 0) {
             *reinterpret_cast<u32x4*>((char*)K + (pd[u] * p.c.sk.b + ko + slot * p.c.sk.t) * esz) = kx[u];
             *reinterpret_cast<u32x4*>((char*)V + (pd[u] * p.c.sv.b + vo + slot * p.c.sv.t) * esz) = vx[u];
         }
