@@ -478,7 +478,8 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
  * the slots past the cut keep what they had.  A position that is moved out of a page outside the pool becomes NaN.
  * weights_out and positions_out (dense
  * [rows, heads, capacity], may be the inputs, but not overlap them in part) get the kept ones' in their
- * first `keep` slots, shorter rows' in their first lens[n]; lens_out (may be cache->lens) is min(lens[n], keep).
+ * first `keep` slots, shorter rows' in their first lens[n]; lens_out (may be cache->lens, but not
+ * overlap it in part) is min(lens[n], keep).
  * A row longer than max_len is left as it is.  Pages that are written must not
  * be shared with another row.  workspace: inf_kv_evict_workspace bytes, 4-byte aligned. */
 int inf_kv_evict_workspace(const inf_paged_kv* cache, int keep, int max_len, size_t* out_bytes);
@@ -497,7 +498,8 @@ int inf_kv_evict(const inf_paged_kv* cache, const float* weights_in, float* weig
  * finished_out (may be NULL): whether the parent was finished or the token is eos; eos < 0: no
  * token ends a sequence.  A beam whose score is not finite passes it on to its candidates (so
  * beams that start at -inf are taken last); one whose logits hold a NaN or +inf, or -inf alone,
- * has NaN for all, which ranks below -inf.  The results may be the inputs.
+ * has NaN for all, which ranks below -inf.  The results may be the inputs, but
+ * not overlap them in part.
  * workspace: inf_beam_select_workspace bytes, 256-byte aligned. */
 int inf_beam_select_workspace(int64_t groups, int beams, int64_t vocab, size_t* out_bytes);
 int inf_beam_select(const void* logits, int64_t ld, const float* scores, const int32_t* finished, int64_t groups,
@@ -512,8 +514,8 @@ int inf_beam_select(const void* logits, int64_t ld, const float* scores, const i
  * and its former page becomes spare_out[row].  Table entries behind that page stay the row's own.
  * So with one spare page per row, and each row's entries from the partly filled page on in no other
  * row's table, nothing is ever written to a page that two rows read.
- * table_out must not overlap cache->table, nor spare_out spare: other rows and layers read
- * them meanwhile.  A parent outside the group gives a row of pages -1; a parent's last page outside the
+ * table_out and spare_out must overlap neither each other nor cache->table, cache->lens, parents or spare:
+ * other rows and layers read these meanwhile.  A parent outside the group gives a row of pages -1; a parent's last page outside the
  * pool goes over by number, and the row keeps its spare one. */
 int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stride, int64_t v_layer_stride,
                      const int32_t* parents, int beams, int32_t* table_out, int64_t table_out_stride,

@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
 #include <utility>
 
@@ -83,11 +84,16 @@ int check_cache(const inf_paged_kv* c, bool written, inf::PagedView* out) {
     return INF_OK;
 }
 
-// Whether [rows, heads, capacity] arrays of 4-byte elements overlap without being the same.
-bool overlap_partly(const inf_paged_kv* c, const void* a, const void* b) {
+// Whether arrays of 4-byte elements overlap (either may be null: then not).
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    const uintptr_t bytes = (uintptr_t)c->rows * c->heads * c->max_pages * c->page_size * 4;
-    return a && b && x != y && x < y + bytes && y < x + bytes;
+    return a && b && x < y + 4 * (uintptr_t)nb && y < x + 4 * (uintptr_t)na;
+}
+// The same of arrays of one size, without being the same.
+bool overlap_partly(const void* a, const void* b, int64_t n) { return a != b && overlap(a, n, b, n); }
+// ... of [rows, heads, capacity] arrays.
+bool overlap_partly(const inf_paged_kv* c, const void* a, const void* b) {
+    return overlap_partly(a, b, (int64_t)c->rows * c->heads * c->max_pages * c->page_size);
 }
 
 int64_t capacity(const inf_paged_kv* c) { return (int64_t)c->max_pages * c->page_size; }
@@ -243,7 +249,8 @@ int inf_kv_evict(const inf_paged_kv* cache, const float* weights_in, float* weig
     if (st != INF_OK || (st = check_cache(cache, true, &p.c))) return st;
     if (recent < 0 || recent > keep) return INF_ERR_BAD_SHAPE;
     if (!weights_in || !weights_out || !positions_in || !positions_out || !lens_out) return INF_ERR_NULL_POINTER;
-    if (overlap_partly(cache, weights_in, weights_out) || overlap_partly(cache, positions_in, positions_out))
+    if (overlap_partly(cache, weights_in, weights_out) || overlap_partly(cache, positions_in, positions_out) ||
+        overlap_partly(cache->lens, lens_out, cache->rows))
         return INF_ERR_BAD_STRIDE;
     size_t need = 0;
     inf_kv_evict_workspace(cache, keep, max_len, &need);
@@ -281,6 +288,10 @@ int inf_beam_select(const void* logits, int64_t ld, const float* scores, const i
     if (!logits || !scores || !tokens || !parents || !scores_out) return INF_ERR_NULL_POINTER;
     if (eos >= vocab || (finished && eos < 0)) return INF_ERR_BAD_SHAPE;
     if (ld < vocab) return INF_ERR_BAD_STRIDE;
+    // a group's results must not lie over what another group still reads
+    for (const void* out : {(const void*)tokens, (const void*)parents, (const void*)scores_out, (const void*)finished_out})
+        if (overlap_partly(out, scores, groups * beams) || overlap_partly(out, finished, groups * beams))
+            return INF_ERR_BAD_STRIDE;
     if (!aligned(logits, (size_t)esz(dt))) return INF_ERR_ALIGNMENT;
     size_t need = 0;
     inf_beam_select_workspace(groups, beams, vocab, &need);
@@ -320,11 +331,14 @@ int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stri
             return st;
     }
     if (table_out_stride < cache->max_pages) return INF_ERR_BAD_STRIDE;
-    // rows read the tables of other rows, and every layer its row's spare page: the new ones lie elsewhere
-    const int32_t *t0 = cache->table, *t1 = t0 + (cache->rows - 1) * cache->table_stride + cache->max_pages;
-    const int32_t *u0 = table_out, *u1 = u0 + (cache->rows - 1) * table_out_stride + cache->max_pages;
-    if (t0 < u1 && u0 < t1) return INF_ERR_BAD_STRIDE;
-    if (spare < spare_out + cache->rows && spare_out < spare + cache->rows) return INF_ERR_BAD_STRIDE;
+    // rows read the tables of other rows, and every layer its row's parent and spare page: the new ones lie elsewhere
+    const int64_t rows = cache->rows, nt = (rows - 1) * cache->table_stride + cache->max_pages,
+                  nu = (rows - 1) * table_out_stride + cache->max_pages;
+    auto read = [&](const int32_t* out, int64_t n) {
+        return overlap(out, n, cache->table, nt) || overlap(out, n, cache->lens, rows) || overlap(out, n, parents, rows) ||
+               overlap(out, n, spare, rows);
+    };
+    if (read(table_out, nu) || read(spare_out, rows) || overlap(table_out, nu, spare_out, rows)) return INF_ERR_BAD_STRIDE;
     if ((int64_t)cache->heads * cache->page_size * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
     p.layers = layers;
     p.beams = beams;
