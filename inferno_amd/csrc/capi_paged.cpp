@@ -18,6 +18,7 @@ namespace {
 constexpr size_t kAlign = 256;
 constexpr int64_t kMaxRowStride = int64_t(1) << 22;  // as the other attention views'
 constexpr int64_t kMaxBlocks = int64_t(1) << 30;
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;  // of a launch, along one axis of its grid
 
 bool dtype_ok(int dt) { return dt == INF_F32 || dt == INF_BF16; }
 int esz(inf_dtype dt) { return dt == INF_F32 ? 4 : 2; }
@@ -152,7 +153,7 @@ int check_beams(int64_t groups, int beams, int64_t vocab) {
     int ns = 0;
     int64_t ch = 0;
     inf::beam_select_plan(groups, beams, vocab, &ns, &ch);
-    return groups * beams * ns > kMaxBlocks ? INF_ERR_BAD_SHAPE : INF_OK;
+    return groups * beams * ns * 256 > kMaxThreads || groups * 1024 > kMaxThreads ? INF_ERR_BAD_SHAPE : INF_OK;
 }
 
 }  // namespace
@@ -207,9 +208,9 @@ int inf_attn_decode_paged(const inf_paged_kv* cache, const void* q, inf_strides 
     if (overlap_partly(cache, weights_in, weights_out)) return INF_ERR_BAD_STRIDE;
     const DecodeSizes s = decode_sizes(cache, q_heads, max_len, weights_out != nullptr);
     const int64_t tiles = (q_heads / cache->heads + 15) / 16;
-    if ((int64_t)cache->rows * cache->heads * tiles > kMaxBlocks / 16 ||
-        (int64_t)cache->heads * tiles * s.groups > kMaxBlocks ||
-        (int64_t)cache->rows * (q_heads + (int64_t)cache->heads * ((max_len + 1023) / 1024)) > kMaxBlocks)
+    const int64_t join = q_heads + (weights_out ? (int64_t)cache->heads * ((max_len + 1023) / 1024) : 0);
+    if (inf::paged_units(cache->rows, cache->heads, (int)tiles, s.groups) * 256 > kMaxThreads ||
+        (s.groups && cache->rows * join * 256 > kMaxThreads))
         return INF_ERR_BAD_SHAPE;
     if (s.total() && (!workspace || ws_bytes < s.total())) return INF_ERR_WORKSPACE;
     if (s.total() && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
@@ -262,7 +263,11 @@ int inf_kv_evict(const inf_paged_kv* cache, const float* weights_in, float* weig
     p.keep = keep; p.recent = recent; p.max_len = max_len;
     p.moves = evict_moves(keep, max_len);
     p.list = static_cast<int32_t*>(workspace);
-    if ((int64_t)cache->rows * cache->heads * (p.moves / 8 + 1) > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    const int64_t rh = (int64_t)cache->rows * cache->heads;
+    p.move_unroll = inf::evict_unroll(rh, p.moves, cache->D, cache->dt == INF_BF16);
+    const int64_t blocks = inf::evict_blocks(p.moves, p.move_unroll, cache->D, cache->dt == INF_BF16);
+    if (rh * inf::evict_threads(max_len) > kMaxThreads || rh * blocks * 256 > kMaxThreads) return INF_ERR_BAD_SHAPE;
+    p.move_blocks = (int)blocks;
     return hip_status(inf::launch_kv_evict(p, cache->dt == INF_BF16, (hipStream_t)stream));
 }
 

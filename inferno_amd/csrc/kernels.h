@@ -377,6 +377,11 @@ constexpr int kPagedMaxGroups = 1024;
 // Keys that a workgroup takes per step: 4 waves, each with 16 KB of keys and values in its registers.
 constexpr int paged_step(int D, int bf16) { return (32 << 10) / (D * (bf16 ? 2 : 4)); }
 inline int paged_blocks(int rows) { return (rows + kPagedBlock - 1) / kPagedBlock; }
+// Workgroups along x: a head's `groups` shares, or rows where there are none, the tiles of query heads on one XCD.
+inline int64_t paged_units(int rows, int heads, int head_tiles, int groups) {
+    const int64_t units = (int64_t)heads * (groups ? groups : rows);
+    return head_tiles > 1 ? (units + 7) / 8 * 8 * head_tiles : units;
+}
 // Shares per block of rows, 0 where workgroups take whole rows.
 int paged_groups(int rows, int heads, int G, int max_len, int D, int bf16, bool weights);
 
@@ -389,8 +394,22 @@ struct KvEvictParams {
     int32_t* lens_out;
     int keep, recent, max_len;
     int moves;             // most moves of a (row, head): min(keep, max_len - keep)
+    int move_unroll, move_blocks;  // moves a thread takes; workgroups of a (row, head)
     int32_t* list;         // workspace [rows * heads][2 * moves + 1]: holes, sources (last first), their number
 };
+
+// Threads of the selection's workgroups: 256 where a row is short, more of them at once, cheaper barriers.
+inline int evict_threads(int max_len) { return max_len <= 4096 ? 256 : 1024; }
+// Moves of 256 threads at a time, each thread with 16 bytes of a key and of its value.
+inline int evict_per(int D, int bf16) { return 256 * 16 / (D * (bf16 ? 2 : 4)); }
+inline int64_t evict_blocks(int moves, int unroll, int D, int bf16) {
+    const int64_t per = (int64_t)evict_per(D, bf16) * unroll;
+    return moves ? (moves + per - 1) / per : 1;
+}
+// Four moves a thread where that leaves a thousand workgroups.
+inline int evict_unroll(int64_t rh, int moves, int D, int bf16) {
+    return moves && rh * evict_blocks(moves, 1, D, bf16) >= 4096 ? 4 : 1;
+}
 
 struct BeamSelectParams {
     const void* logits;    // [groups * beams, vocab], row stride ld

@@ -616,9 +616,8 @@ int paged_groups(int rows, int heads, int G, int max_len, int D, int bf16, bool 
 
 template <int D, typename E>
 static int launch_paged_t(const PagedDecodeParams& p, hipStream_t s) {
-    int64_t units = (int64_t)p.c.heads * (p.groups ? p.groups : p.c.rows);
-    if (p.head_tiles > 1) units = (units + 7) / 8 * 8 * p.head_tiles;
-    const dim3 grid((unsigned)units, p.groups ? (unsigned)paged_blocks(p.c.rows) : 1u);
+    const dim3 grid((unsigned)paged_units(p.c.rows, p.c.heads, p.head_tiles, p.groups),
+                    p.groups ? (unsigned)paged_blocks(p.c.rows) : 1u);
     size_t lds = (size_t)(4 * (p.G < 16 ? p.G : 16) * (D + 4) + 128) * sizeof(float);
     if (p.scores) lds = std::max<size_t>(lds, 4 * kPagedHold);  // the same LDS first holds scores
     auto split = [&](auto small) {
@@ -1015,16 +1014,15 @@ __global__ __launch_bounds__(256) void kv_evict_move_kernel(KvEvictParams p, int
 }
 
 int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s) {
-    const int esz = bf16 ? 2 : 4, pieces = p.c.D * esz / 16, per = 256 / pieces;
+    const int esz = bf16 ? 2 : 4, pieces = p.c.D * esz / 16, blocks = p.move_blocks;
     const int64_t rh = (int64_t)p.c.rows * p.c.heads;
-    // a workgroup of 256 threads where a row is short: more of them at once, cheaper barriers
     const dim3 grid((unsigned)rh);
     const size_t lds = ((size_t)p.max_len + 3) / 4 * 16;
     const uintptr_t any = reinterpret_cast<uintptr_t>(p.w_in) | reinterpret_cast<uintptr_t>(p.w_out) |
                           reinterpret_cast<uintptr_t>(p.pos_in) | reinterpret_cast<uintptr_t>(p.pos_out);
     auto select = [&](auto v) {
         constexpr bool kVec = decltype(v)::value;
-        if (p.max_len <= 4096)
+        if (evict_threads(p.max_len) == 256)
             hipLaunchKernelGGL((kv_evict_select_kernel<4, true, kVec>), grid, dim3(256), lds, s, p);
         else if (p.max_len <= kEvictLds)
             hipLaunchKernelGGL((kv_evict_select_kernel<16, true, kVec>), grid, dim3(1024), lds, s, p);
@@ -1035,12 +1033,8 @@ int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s) {
         select(std::true_type{});
     else
         select(std::false_type{});
-    // four moves a thread where that leaves a thousand workgroups
-    const int64_t all = rh * ((p.moves + per - 1) / per);
-    const int u = all >= 4096 ? 4 : 1;
-    const int blocks = p.moves ? (p.moves + per * u - 1) / (per * u) : 1;
     const dim3 g2((unsigned)(rh * blocks));
-    if (u == 4)
+    if (p.move_unroll == 4)
         hipLaunchKernelGGL((kv_evict_move_kernel<4>), g2, dim3(256), 0, s, p, pieces, esz, blocks);
     else
         hipLaunchKernelGGL((kv_evict_move_kernel<1>), g2, dim3(256), 0, s, p, pieces, esz, blocks);
