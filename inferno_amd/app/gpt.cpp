@@ -459,7 +459,8 @@ static int run_beam_check(const std::string& dir, const Device& dev, size_t P, s
     std::ifstream cf(dir + "/config.txt");
     size_t L, C, H, T, V, B;
     if (!(cf >> L >> C >> H >> T >> V >> B)) throw Error("bad config.txt");
-    if (P < 1 || P + N > T) throw Error("beam-check: need 1 <= prompt and prompt + new <= context");
+    if (P < 1 || N < 1 || P > T || N > T - P)
+        throw Error("beam-check: need 1 <= prompt, 1 <= new and prompt + new <= context");
     GPTModel model(V, T, C, H, L, true, dev, DType::Float32);
     load_params(model, dir);
     auto tok = read_file(dir + "/tokens.bin");
@@ -540,7 +541,8 @@ static int run_generate(int argc, char** argv) {
     paged.budget = budget;
     paged.recent = arg(argc, argv, "--recent", budget / 4);
     const size_t capacity = arg(argc, argv, "--capacity", budget + budget / 8 + 1);
-    if (P + N > T) throw Error("generate: prompt + new tokens exceed the context size");
+    if (!B || !P || !N || !V) throw Error("generate: batch, prompt, new and vocab must be at least 1");
+    if (P > T || N > T - P) throw Error("generate: prompt + new tokens exceed the context size");
     if (K && budget) throw Error("generate: --beams and --budget exclude each other");
     const Device dev = Device::hip(0);
     RandomGenerator::initializeWithSeed(42);
