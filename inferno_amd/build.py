@@ -55,10 +55,9 @@ CXX = os.environ.get("CXX", "g++")
 # product and sum roundings.
 HOST_FLAGS = ["-std=c++20", "-O2", "-fPIC", "-ffp-contract=off", "-Wall", "-Wno-unused-function",
               "-D__HIP_PLATFORM_AMD__", f"-I{ROOT / 'include'}", f"-I{ROCM / 'include'}"]
-DRIVER_SRC = ROOT / "tests" / "cpp" / "api_driver.cpp"
+DRIVER_SRCS = [ROOT / "tests" / "cpp" / f"{name}.cpp" for name in ("api_driver", "paged_driver")]
 APP_SRC = PKG / "app" / "gpt.cpp"
 APP = PKG / "gpt"
-DRIVER = ROOT / "tests" / "cpp" / "api_driver"
 
 
 def _run(cmd, what):
@@ -68,7 +67,7 @@ def _run(cmd, what):
 
 
 def build_host(verbose: bool = True) -> Path:
-    """libinferno.so (Tensor, autograd, ops) linked against libinferno_hip.so, plus the test driver."""
+    """libinferno.so (Tensor, autograd, ops) linked against libinferno_hip.so, plus the test drivers."""
     BUILD.mkdir(exist_ok=True)
     objs = []
     with cf.ThreadPoolExecutor(max_workers=min(8, len(CPP_SOURCES))) as ex:
@@ -83,10 +82,11 @@ def build_host(verbose: bool = True) -> Path:
     _run([CXX, "-shared", "-o", str(tmp), *map(str, objs), f"-L{PKG}", "-linferno_hip", f"-L{ROCM / 'lib'}",
           "-lamdhip64", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{ROCM / 'lib'}"], "link libinferno.so")
     os.replace(tmp, HOST_LIB)
-    if DRIVER_SRC.exists():
-        _run([CXX, *HOST_FLAGS, str(DRIVER_SRC), "-o", str(DRIVER), f"-L{PKG}", "-linferno", "-linferno_hip",
-              f"-L{ROCM / 'lib'}", "-lamdhip64", f"-Wl,-rpath,{PKG}", f"-Wl,-rpath,{ROCM / 'lib'}",
-              "-Wl,-rpath,$ORIGIN/../../inferno_amd"], "build api_driver")
+    for src in DRIVER_SRCS:
+        if src.exists():
+            _run([CXX, *HOST_FLAGS, str(src), "-o", str(src.with_suffix("")), f"-L{PKG}", "-linferno", "-linferno_hip",
+                  f"-L{ROCM / 'lib'}", "-lamdhip64", f"-Wl,-rpath,{PKG}", f"-Wl,-rpath,{ROCM / 'lib'}",
+                  "-Wl,-rpath,$ORIGIN/../../inferno_amd"], f"build {src.stem}")
     _run([CXX, *HOST_FLAGS, str(APP_SRC), "-o", str(APP), f"-L{PKG}", "-linferno", "-linferno_hip",
           f"-L{ROCM / 'lib'}", "-lamdhip64", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{ROCM / 'lib'}"], "build gpt app")
     if verbose:
