@@ -244,7 +244,10 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
 __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
     constexpr int W = 16, kThreads = 64 * W;
     enum { kLives, kFinished, kFlat };  // a flat beam's candidates are the first tokens, all with its score
-    __shared__ double base[kMaxBeams];  // score - lse; the score of a beam that is finished or flat
+    __shared__ double base[kMaxBeams];  // score - log(sum); the score of a beam that is finished or flat
+    // The logits' maximum.  It is taken from the logits first: where they are far from 0 (all at the type's lowest value,
+    // a row without tokens), a sum with the lse would lose the score.
+    __shared__ float maximum[kMaxBeams];
     __shared__ int kind[kMaxBeams];
     __shared__ uint64_t ls[kBeamList], lt[kBeamList];
     __shared__ uint32_t lk[kBeamList];
@@ -320,9 +323,10 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
         for (int d = 1; d < 8; d <<= 1) S += shfl_xor_d(S, d);
         if ((tid & 7) == 0) {
             // a NaN or +inf among the logits, or nothing above -inf: the sum is NaN, infinite or 0
-            const double lse = (double)M + log(S);
-            const bool lives = !finished && isfinite(score), fine = isfinite(lse);
-            base[b] = !lives ? (double)score : fine ? (double)score - lse : __longlong_as_double(0x7ff8000000000000ll);
+            const double ls = log(S);
+            const bool lives = !finished && isfinite(score), fine = isfinite(M) && isfinite(ls);
+            base[b] = !lives ? (double)score : fine ? (double)score - ls : __longlong_as_double(0x7ff8000000000000ll);
+            maximum[b] = M;
             kind[b] = finished ? kFinished : lives && fine ? kLives : kFlat;
         }
     }
@@ -336,7 +340,7 @@ __global__ __launch_bounds__(1024) void beam_join_kernel(BeamSelectParams p) {
             if (!c) return r;
             r.token = ~(uint32_t)c;
             r.at |= ~(uint32_t)(c >> 32);
-            score += (double)logit_of((uint32_t)(c >> 32));
+            score += (double)logit_of((uint32_t)(c >> 32)) - (double)maximum[b];
         } else if (kind[b] == kFinished) {
             if (j) return r;
             r.token = (uint32_t)p.eos;

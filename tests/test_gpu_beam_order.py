@@ -67,6 +67,7 @@ def test_equal_beams_lower_first(ia, groups, beams, vocab, pad, shift, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("groups,beams,vocab,pad", [
     (1, 8, 50257, 0), (4, 16, 50257, 0), (5, 16, 30011, 3), (64, 4, 16385, 0), (3, 32, 8193, 1), (2, 4, 4099, 0),
+    (1, 4, 100003, 0), (2, 8, 300007, 1),  # more parts than lanes join at a time
 ])
 def test_ordinary_logits(ia, groups, beams, vocab, pad, dtype):
     """Ordinary logits of odd vocabularies in every width: the candidates of all beams in 64 bits, and each score."""
@@ -123,3 +124,32 @@ def test_logits_decide_within_a_beam(ia, groups, beams, vocab, rest, dtype):
     for g in range(groups):  # all scores are equal, so beam 0's best are taken
         assert parents[g].tolist() == [0] * beams and tokens[g].tolist() == want.tolist()
         assert (scores[g] == scores[g, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("value", ["lowest", "largest", 2.0**40, -(2.0**100), 2.0**20])
+@pytest.mark.parametrize("vocab", [40, 9001])
+def test_logits_far_from_zero(ia, vocab, value, dtype):
+    """A beam whose logits are all at the type's lowest value (all tokens masked), or far from 0: its score counts as much
+    as any other's, by (score + (logit - maximum)) - log(sum)."""
+    print(f"[case] logits at {value} V{vocab} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(vocab)
+    groups, beams = 2, 4
+    far = {"lowest": torch.finfo(dtype).min, "largest": torch.finfo(dtype).max}.get(value, value)
+    logits = (torch.randn(groups, beams, vocab, generator=gen) * 2).to(dtype)
+    logits[0, 1:3] = far
+    logits[1] = far
+    logits[1, :, vocab // 2:] = torch.tensor(far * (0.5 if far > 0 else 1.0), dtype=dtype)  # half of them, or all, at the top
+    logits = logits.view(groups * beams, vocab)
+    scores = torch.randn(groups, beams, generator=gen) - torch.tensor([[9.0, 2.0, 1.0, 9.0], [5.0, 5.0, 5.0, 5.0]])
+    scores[1, 2] = scores[1, 1]
+    tokens, parents, out, _ = (x if x is None else x.cpu() for x in ia.beam_select(rows_at(logits, 1, 0), scores.cuda()))
+    x = logits.double().view(groups, beams, vocab)
+    d = x - x.amax(2, keepdim=True)
+    p = torch.exp(d)
+    every = scores.double()[:, :, None] + (d - p.sum(2, keepdim=True).log())
+    best = torch.sort(every.view(groups, -1), dim=1, descending=True, stable=True)
+    assert (parents.long() * vocab + tokens).tolist() == best.indices[:, :beams].tolist()
+    mean = (p / p.sum(2, keepdim=True) * -d).sum(2).amax(1)
+    bound = (2.25 * mean[:, None] + 4) * 2.0**-24 + 2.0**-24 * best.values[:, :beams].abs()
+    assert ((out.double() - best.values[:, :beams]).abs() <= bound).all()
