@@ -453,7 +453,7 @@ int inf_kv_append(const inf_paged_kv* cache, const void* k, inf_strides sk, cons
 
 /* Attention of one new token per row over its whole cache: o[n, i] = sum_j p_j v_j with
  * p = softmax_j(scale q[n, i] . k_j), j < lens[n], keys and values of head i / (q_heads / heads).
- * q, o: [rows, q_heads, 1, D] views; q_heads a multiple of the cache's heads.  max_len
+ * q, o: [rows, q_heads, 1, D] views (o may be q itself); q_heads a multiple of the cache's heads.  max_len
  * (1..capacity) bounds the rows' lengths for the plan and the workspace; a row of length 0
  * or less gives zeros, one longer than max_len or with a page outside the pool NaN.  What lies
  * in a row's pages behind its length does not matter.  An infinity or a NaN among the values before it

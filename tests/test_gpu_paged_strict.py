@@ -82,6 +82,24 @@ def test_decode_long(ia, strict, dtype):  # noqa: F811
     base.test_decode_long(ia, dtype)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,heads,group,longest", [(1, 2, 1, 1000), (70, 2, 18, 300), (600, 4, 1, 200)])
+def test_output_over_the_queries(ia, rows, heads, group, longest, dtype):  # noqa: F811
+    """o may be q itself: whole rows to a workgroup, and shares with a join."""
+    print(f"[case] paged decode in place {rows} rows {heads}x{group} {dtype}", flush=True)
+    gen = torch.Generator().manual_seed(rows)
+    lens = torch.randint(0, longest + 1, (rows,), generator=gen).tolist()
+    lens[0] = longest
+    c, ks, vs, _ = base.make_cache(ia, gen, lens, heads, 64, 16, dtype)
+    q = base.rnd(gen, (rows, heads * group, 1, 64), dtype, 1.5)
+    for weigh in (False, True):
+        w = torch.zeros(c.meta_shape, device="cuda") if weigh else None
+        x = q.cuda()
+        assert ia.attn_decode_paged(x, c, max_len=longest, weights_out=w, out=x) is x
+        check_decode(q, x, ks, vs, heads, ia.default_scale(64), dtype)
+
+
 for _name in ("test_decode", "test_decode_many_rows", "test_decode_layouts", "test_decode_bad_rows_are_nan",
               "test_decode_infinite_scores", "test_decode_long"):  # the parameters of the same tests there
     _test = globals()[_name]
