@@ -21,7 +21,8 @@ public:
         size_t page_size = 16;  // a power of two
         size_t beams = 1;       // rows of a group
         // With a budget (1 .. capacity - 1), a full cache is cut to that many positions per head, the `recent`
-        // newest and those that got the most attention in the single-position steps so far.
+        // newest and those that got the most attention in the single-position steps so far (a prompt of more than one
+        // position adds none: a cache that is cut right after it keeps the first slots and the newest).
         // Without one a full cache throws.  Not together with beams, whose rows share pages.
         size_t budget = 0, recent = 0;
     };

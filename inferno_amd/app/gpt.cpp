@@ -24,8 +24,9 @@
 //       time and the per-token decode time.  --beams K [--page-size S]: beam
 //       search over a paged cache instead.  --budget M [--recent R]
 //       [--capacity Q] [--page-size S]: the cache holds at most Q positions
-//       (M + M / 8 + 1, and the prompt at least) and is cut to the M most
-//       attended ones whenever it is full, the R (M / 4) newest among them.
+//       (M + M / 8 + 1, and the prompt at least) and is cut to M whenever it
+//       is full: the R (M / 4) newest ones, and those that got the most
+//       attention from the new tokens (the prompt's own is not counted).
 //   gpt beam-check / paged-check <dir> <cpu|hip> [options]
 //       beam search, or given tokens, through a paged cache, written to files.
 //   gpt decode-check <dir> <cpu|hip> [--prefill P]

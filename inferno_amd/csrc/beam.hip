@@ -14,9 +14,9 @@
 // two or three times as many as there are beams.  They are picked into LDS, and each counts those
 // that are better.
 //
-// 32 groups of 8 beams, 50257 bf16 columns, 26 MB: 16.0 us, 10.7 the first launch (4.3 would be the
+// 32 groups of 8 beams, 50257 bf16 columns, 26 MB: 16.1 us, 10.8 the first launch (4.3 would be the
 // reads alone at HBM's rate, 2 a launch; all its workgroups run at once, so that what follows the reads
-// is not hidden by others' reads) and 5.1 the second.  One group of 4 beams, 8192 fp32 columns: 9.2 us,
+// is not hidden by others' reads) and 5.3 the second.  One group of 4 beams, 8192 fp32 columns: 8.9 us,
 // two launches of 4 us each that are latency throughout.  Much of that is the fetching of code that
 // runs once: loops stay rolled where values are few.
 #include "common.h"

@@ -659,7 +659,7 @@ int launch_attn_decode_paged(const PagedDecodeParams& p, int bf16, hipStream_t s
 // nearly all.  No position is both read and written, so moves run in any order.
 //
 // Half of 2048 positions, 32 rows of 12 heads of D 64, fp32: 62 us, 11 of them the selection;
-// the moves are single rows of 256 bytes, 230 MB read and written at 4.6 TB/s.  64 of 32832
+// the moves are single rows of 256 bytes, 230 MB read and written at 4.5 TB/s.  64 of 32832
 // positions, 2 rows of 8 heads: 32 us, of which 28 are the selection on 16 CUs, five walks over
 // a row's keys.  (Other CUs copying the weights meanwhile: 1 us less, not worth their code.)
 // ============================================================================
