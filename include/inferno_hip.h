@@ -515,8 +515,8 @@ int inf_beam_select(const void* logits, int64_t ld, const float* scores, const i
  * So with one spare page per row, and each row's entries from the partly filled page on in no other
  * row's table, nothing is ever written to a page that two rows read.
  * table_out and spare_out must overlap neither each other nor cache->table, cache->lens, parents or spare:
- * other rows and layers read these meanwhile.  A parent outside the group gives a row of pages -1; a parent's last page outside the
- * pool goes over by number, and the row keeps its spare one. */
+ * other rows and layers read these meanwhile.  A parent outside the group gives a row of pages -1; a
+ * parent's last page outside the pool goes over by number, and the row keeps its spare one. */
 int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stride, int64_t v_layer_stride,
                      const int32_t* parents, int beams, int32_t* table_out, int64_t table_out_stride,
                      const int32_t* spare, int32_t* spare_out, void* stream);

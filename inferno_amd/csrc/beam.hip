@@ -149,8 +149,8 @@ __global__ __launch_bounds__(256, N == 32 ? 7 : 1) void beam_part_kernel(BeamSel
     const uint32_t lane_best = ordered_logit(mx);
     mx = wave_all(mx, [](float a, float b) { return fmaxf(a, b); });
     const float ref = mx == -INFINITY ? 0.f : mx;
-    // Terms in 32 bits: one at d below the maximum is off by (2.25 |d| + 2) 2^-24 of itself (difference, product, log2 e and
-    // v_exp_f32), and sums of four by 2^-23 more.  All further sums in 64.  |d| has a mean of at most 18 under the
+    // Terms in 32 bits: one at d below the maximum is off by (2.25 |d| + 2) 2^-24 of itself (difference, product,
+    // log2 e and v_exp_f32), and sums of four by 2^-23 more.  All further sums in 64.  |d| has a mean of at most 18 under the
     // terms' shares (2^31 columns), so the lse is off by 2^-18 at most.
     double sum = fast_exp2((v[N] - ref) * kLog2e);
 #pragma unroll

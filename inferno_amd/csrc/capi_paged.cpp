@@ -294,7 +294,7 @@ int inf_beam_select(const void* logits, int64_t ld, const float* scores, const i
     if (eos >= vocab || (finished && eos < 0)) return INF_ERR_BAD_SHAPE;
     if (ld < vocab) return INF_ERR_BAD_STRIDE;
     // a group's results must not lie over what another group still reads
-    for (const void* out : {(const void*)tokens, (const void*)parents, (const void*)scores_out, (const void*)finished_out})
+    for (const void* out : std::initializer_list<const void*>{tokens, parents, scores_out, finished_out})
         if (overlap_partly(out, scores, groups * beams) || overlap_partly(out, finished, groups * beams))
             return INF_ERR_BAD_STRIDE;
     if (!aligned(logits, (size_t)esz(dt))) return INF_ERR_ALIGNMENT;
@@ -340,10 +340,11 @@ int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stri
     const int64_t rows = cache->rows, nt = (rows - 1) * cache->table_stride + cache->max_pages,
                   nu = (rows - 1) * table_out_stride + cache->max_pages;
     auto read = [&](const int32_t* out, int64_t n) {
-        return overlap(out, n, cache->table, nt) || overlap(out, n, cache->lens, rows) || overlap(out, n, parents, rows) ||
-               overlap(out, n, spare, rows);
+        return overlap(out, n, cache->table, nt) || overlap(out, n, cache->lens, rows) ||
+               overlap(out, n, parents, rows) || overlap(out, n, spare, rows);
     };
-    if (read(table_out, nu) || read(spare_out, rows) || overlap(table_out, nu, spare_out, rows)) return INF_ERR_BAD_STRIDE;
+    if (read(table_out, nu) || read(spare_out, rows) || overlap(table_out, nu, spare_out, rows))
+        return INF_ERR_BAD_STRIDE;
     if ((int64_t)cache->heads * cache->page_size * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
     p.layers = layers;
     p.beams = beams;
