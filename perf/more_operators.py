@@ -11,7 +11,7 @@ cannot do without.
 8 bits: a row's scale is its largest magnitude times 1/127, its values are whole multiples of it.
 4 bits: blocks of 32 channels share a power of two, 2^(byte - 127); a value is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6
 times it, with a sign (bit 3).  Byte i of a row holds channel 2 i in its low half, 2 i + 1 in its high one.
-A cache is pools of pages [pages, key-value heads, slots, D / 2] of such bytes and [pages, heads, slots, D / 32]
+A cache is pools of pages [pages, key-value heads, slots, D / 2] of such bytes and [pages, heads, D / 32, slots]
 of scales for the keys and for the values, a table [rows, pages of a row] that names each row's pages, and the
 rows' lengths.
 """
@@ -78,7 +78,7 @@ def draw(rng):
         # the largest product and the most bytes are the largest listed case's
         most = min(16384, (1 << 40) // (K * N), (800 << 20) // (4 * (K + N)))
         return dict(kind=kind, M=_log(rng, 1, max(1, most)), K=K, N=N, bias=rng.random() < 0.5, dtype=dtype)
-    D, page = rng.choice([32, 64, 128]), rng.choice([8, 16, 32, 64, 128])
+    D, page = rng.choice([32, 64, 128]), rng.choice([16, 32, 64, 128])
     rows, heads = _log(rng, 1, 64), rng.randint(1, 16)
     if kind == "kv4":
         new = _log(rng, 1, max(1, min(2048, (16 << 20) // (rows * heads * D))))
@@ -154,10 +154,11 @@ def prepare(case, seed):
     s["table"] = order.reshape(rows, per_row).contiguous()
     for name in ("k", "v"):
         codes = torch.empty((rows * per_row, heads, page, D // 2), dtype=torch.uint8, device="cuda")
-        scales = torch.empty((rows * per_row, heads, page, D // 32), dtype=torch.uint8, device="cuda")
+        scales = torch.empty((rows * per_row, heads, D // 32, page), dtype=torch.uint8, device="cuda")
         for i in range(0, rows * per_row, 1 + (64 << 20) // (heads * page * D)):
             part = slice(i, i + 1 + (64 << 20) // (heads * page * D))
-            codes[part], scales[part] = _encode(_normal(gen, (*codes[part].shape[:3], D)))
+            codes[part], scale = _encode(_normal(gen, (*codes[part].shape[:3], D)))
+            scales[part] = scale.transpose(2, 3)
         s[name], s[name + "_scale"] = codes, scales
     if own:
         import inferno_amd as ia
@@ -236,11 +237,12 @@ def _decode(codes, scales):
     return x.reshape(*scales.shape[:-1], -1)
 
 
-def _rows_of(pool, table, n):
-    """The first n positions of every row, [rows, heads, n, bytes]."""
-    pages = table[:, :-(-n // pool.shape[2])].long()
-    x = pool[pages]  # [rows, pages, heads, slots, bytes]
-    return x.permute(0, 2, 1, 3, 4).reshape(x.shape[0], x.shape[2], -1, x.shape[4])[:, :, :n]
+def _rows_of(s, name, n):
+    """The first n positions of every row, [rows, heads, n, D]."""
+    pages = s["table"][:, :-(-n // s["case"]["page"])].long()
+    codes = s[name][pages].permute(0, 2, 1, 3, 4)  # [rows, heads, pages, slots, bytes]
+    scales = s[name + "_scale"][pages].permute(0, 2, 1, 4, 3)
+    return _decode(*(x.reshape(*x.shape[:2], -1, x.shape[4])[:, :, :n] for x in (codes, scales)))
 
 
 def _plain_kv4(s):
@@ -254,7 +256,7 @@ def _plain_kv4(s):
     for name in ("k", "v"):
         codes, scales = _encode(s[name + "_new"][row, :, col])
         s[name][where, :, at % page] = codes
-        s[name + "_scale"][where, :, at % page] = scales
+        s[name + "_scale"][where, :, :, at % page] = scales
     j = torch.arange(_positions(case), device="cuda")
     j = j if case["whole"] else j + s["first"].long()[:, None]
     there = (j < lens).expand(case["rows"], -1)
@@ -262,7 +264,7 @@ def _plain_kv4(s):
     out = {}
     for name in ("k", "v"):
         pages = s["table"].long().gather(1, j // page)
-        x = _decode(s[name][pages, :, j % page], s[name + "_scale"][pages, :, j % page])  # [rows, T, heads, D]
+        x = _decode(s[name][pages, :, j % page], s[name + "_scale"][pages, :, :, j % page])  # [rows, T, heads, D]
         x = x.masked_fill(~there[:, :, None, None], 0.0)  # nothing behind a row's end
         out[name] = x.transpose(1, 2).to(s[name + "_new"].dtype).contiguous()
     return out
@@ -275,7 +277,7 @@ def _scale(D):
 
 def _plain_decode(s):
     n, heads, D = s["case"]["length"], s["case"]["heads"], s["case"]["D"]
-    k, v = (_decode(_rows_of(s[x], s["table"], n), _rows_of(s[x + "_scale"], s["table"], n)) for x in ("k", "v"))
+    k, v = (_rows_of(s, x, n) for x in ("k", "v"))
     q = s["q"].float().reshape(-1, heads, s["case"]["group"], D)
     hidden = (torch.arange(n, device="cuda") >= s["lens"][:, None])[:, None, None, :]
     x = torch.matmul(q, k.transpose(2, 3).contiguous()) * _scale(D)
@@ -371,7 +373,7 @@ def _exact_kv4(case, s):
         pages = s["table"][row].long()
         for name in ("k", "v"):
             if n - count > first:  # what was there before
-                x = _values(s[name][pages], s[name + "_scale"][pages])
+                x = _values(s[name][pages], s[name + "_scale"][pages].transpose(2, 3))
                 x = x.permute(1, 0, 2, 3).reshape(case["heads"], -1, case["D"])
                 out[name][row, :, :n - count - first] = x[:, first:n - count]
             new = s[name + "_new"][row, :, :count]
@@ -387,7 +389,8 @@ def _exact_decode(case, s):
         pages = s["table"][row, :-(-n // case["page"])].long()
         for h in range(case["heads"]):
             k, v = (_values(s[x][pages, h].reshape(-1, case["D"] // 2)[:n],
-                            s[x + "_scale"][pages, h].reshape(-1, case["D"] // 32)[:n]) for x in ("k", "v"))
+                            s[x + "_scale"][pages, h].transpose(1, 2).reshape(-1, case["D"] // 32)[:n])
+                    for x in ("k", "v"))
             mine = slice(h * case["group"], (h + 1) * case["group"])
             p = torch.softmax((s["q"][row, mine].double() * k).sum(-1) * _scale(case["D"]), dim=-1)
             o[row, mine, 0] = (p[:, :, None] * v).sum(1)
