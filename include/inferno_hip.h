@@ -521,6 +521,76 @@ int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stri
                      const int32_t* parents, int beams, int32_t* table_out, int64_t table_out_stride,
                      const int32_t* spare, int32_t* spare_out, void* stream);
 
+/* ---- generation with a cache in 4 bits and weights in 8 ---------------------
+ * No counterpart in the reference, which has neither.  One token reads every
+ * weight and the whole cache: fewer bits are less time. */
+
+/* The cache of one layer in 4 bits, in pages as inf_paged_kv.  Blocks of 32 neighbouring channels of a key or value
+ * share a power of two, 2^(byte - 127); a channel is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (codes 0 to 7), or its
+ * negative (8 to 15): the FP4 of the MX formats.  Channels 2 i and 2 i + 1 of key j of row n and head h are the low and high
+ * half of byte i from k + page * sk.b + h * sk.h + (j % page_size) * sk.t on, with page = table[n * table_stride +
+ * j / page_size]; the byte of its channels 32 b .. 32 b + 31 lies at k_scale + page * sks.b + h * sks.h + b * sks.t +
+ * j % page_size.  Values likewise.  All strides in bytes; sk, sv and the pools on 16 bytes, sks, svs and the scales
+ * on 4.  D is 32, 64 or 128, page_size a power of two, at least 16; the other limits are inf_paged_kv's.
+ * Bytes are 2 to 252, or 255 for a block that reads as NaN: what inf_kv4_append writes. */
+typedef struct {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* k_scale;
+    uint8_t* v_scale;
+    inf_strides sk, sv, sks, svs; /* sks, svs: t from block to block, d (1) from slot to slot */
+    const int32_t* table; /* device, [rows, max_pages], rows table_stride apart */
+    const int32_t* lens;  /* device, [rows] */
+    int64_t table_stride;
+    int rows, heads, D, page_size, max_pages, n_pages;
+} inf_paged_kv4;
+
+/* Writes the keys and values k, v [rows, heads, T, D] (fp32 or bf16 by dt) of row n's last counts[n] positions as
+ * inf_kv_append does.  A block's power of two is that of its largest magnitude, two lower and at least 2^-125: this one comes to
+ * lie in [4, 8) times it.  Every channel goes to the nearest value of the grid, ties to the even code, past 6 to 6.
+ * A block with an infinity or a NaN reads as NaN. */
+int inf_kv4_append(const inf_paged_kv4* cache, const void* k, inf_strides sk, const void* v, inf_strides sv,
+                   const int32_t* counts, int T, inf_dtype dt, void* stream);
+
+/* Reads positions first[n] .. first[n] + T - 1 of every row (first: device, [rows]; NULL: from 0) into k, v
+ * [rows, heads, T, D] (fp32 or bf16 by dt, both exact), as the dense attention takes them: what follows a long prompt
+ * attends to.  Positions outside the row (negative, or at or past lens[n]) are zeros, in a page outside the pool NaN. */
+int inf_kv4_read(const inf_paged_kv4* cache, const int32_t* first, int T, void* k, inf_strides sk, void* v,
+                 inf_strides sv, inf_dtype dt, void* stream);
+
+/* Attention of one new token per row over its whole cache, as inf_attn_decode_paged (without weights); q and o are fp32 or
+ * bf16 by dt. */
+int inf_attn_decode_kv4_workspace(const inf_paged_kv4* cache, int q_heads, int max_len, size_t* out_bytes);
+int inf_attn_decode_kv4(const inf_paged_kv4* cache, const void* q, inf_strides sq, void* o, inf_strides so,
+                        int q_heads, int max_len, float scale, inf_dtype dt, void* workspace, size_t ws_bytes,
+                        void* stream);
+
+/* Rows of x [rows, cols] (row stride ldx elements, fp32 or bf16) in 8 bits: scale[r] = max_c |x[r, c]| * (1 / 127, as
+ * a float), q[r, c] = x[r, c] / scale[r] to the nearest whole number, ties to even, within +-127.  A row with an infinity
+ * or a NaN has scale NaN and zeros; one whose scale would be below 2^-126 scale 0 and zeros.
+ * transpose: the columns of x instead, q [cols, rows] and scale [cols] -- weights [in, out] with one scale per output.
+ * q's rows lie ldq bytes apart, on 16 bytes, and are written up to whole 16 bytes, with zeros; neither they nor the
+ * scales may overlap x. */
+int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpose, int8_t* q, int64_t ldq,
+                    float* scale, inf_dtype dt, void* stream);
+
+/* y[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n] + bias[n]: x [M, K] and w [N, K] in 8 bits, the sum exact
+ * (K < 2^17), y and bias (may be NULL) fp32 or bf16 by dt, rounded once.  Rows of x and w lie on 16 bytes and are read
+ * in pieces of 16 (up to K in whole 16 bytes; what lies behind K does not matter).  y must not overlap what is read.
+ * workspace: inf_gemm_i8_workspace bytes (may be 0: then NULL), 256-byte aligned.  Calls that share one must not
+ * overlap.  The same bits on every run. */
+int inf_gemm_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes);
+int inf_gemm_i8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                int64_t ldw, const float* w_scale, const void* bias, void* y, int64_t ldy, inf_dtype dt,
+                void* workspace, size_t ws_bytes, void* stream);
+
+/* A linear layer with weights in 8 bits: inf_quantize_i8 of the rows of x [M, K] (fp32 or bf16 by dt, as y), then
+ * inf_gemm_i8.  y may be x.  workspace: inf_linear_i8_workspace bytes, 256-byte aligned. */
+int inf_linear_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes);
+int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
+                  const float* w_scale, const void* bias, void* y, int64_t ldy, inf_dtype dt, void* workspace,
+                  size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

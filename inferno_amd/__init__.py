@@ -78,6 +78,15 @@ EXPORTS = (
     "inf_beam_select_workspace",
     "inf_beam_select",
     "inf_beam_reorder",
+    "inf_kv4_append",
+    "inf_kv4_read",
+    "inf_attn_decode_kv4_workspace",
+    "inf_attn_decode_kv4",
+    "inf_quantize_i8",
+    "inf_gemm_i8_workspace",
+    "inf_gemm_i8",
+    "inf_linear_i8_workspace",
+    "inf_linear_i8",
     "inf_last_error_detail",
 )
 
@@ -102,6 +111,16 @@ class PagedKVStruct(ctypes.Structure):
                 ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
                 ("rows", ctypes.c_int), ("heads", ctypes.c_int), ("D", ctypes.c_int), ("page_size", ctypes.c_int),
                 ("max_pages", ctypes.c_int), ("n_pages", ctypes.c_int), ("dt", ctypes.c_int)]
+
+
+class PagedKV4Struct(ctypes.Structure):
+    """inf_paged_kv4: pools of pages, scales, table and lengths of a paged key-value cache in 4 bits."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("sk", Strides), ("sv", Strides), ("sks", Strides), ("svs", Strides),
+                ("table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("rows", ctypes.c_int), ("heads", ctypes.c_int), ("D", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("max_pages", ctypes.c_int), ("n_pages", ctypes.c_int)]
 
 
 class InfernoError(RuntimeError):
@@ -192,6 +211,15 @@ def lib() -> ctypes.CDLL:
         L.inf_beam_select_workspace.argtypes = [i64, i32, i64, szp]
         L.inf_beam_select.argtypes = [vp, i64, vp, vp, i64, i32, i64, i32, vp, vp, vp, vp, i32, vp, sz, vp]
         L.inf_beam_reorder.argtypes = [kv, i32, i64, i64, vp, i32, vp, i64, vp, vp, vp]
+        kv4 = ctypes.POINTER(PagedKV4Struct)
+        L.inf_kv4_append.argtypes = [kv4, vp, S, vp, S, vp, i32, i32, vp]
+        L.inf_kv4_read.argtypes = [kv4, vp, i32, vp, S, vp, S, i32, vp]
+        L.inf_attn_decode_kv4_workspace.argtypes = [kv4, i32, i32, szp]
+        L.inf_attn_decode_kv4.argtypes = [kv4, vp, S, vp, S, i32, i32, f32, i32, vp, sz, vp]
+        L.inf_quantize_i8.argtypes = [vp, i64, i64, i64, i32, vp, i64, vp, i32, vp]
+        L.inf_gemm_i8_workspace.argtypes = L.inf_linear_i8_workspace.argtypes = [i64, i64, i64, szp]
+        L.inf_gemm_i8.argtypes = [i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, vp, i64, i32, vp, sz, vp]
+        L.inf_linear_i8.argtypes = [i64, i64, i64, vp, i64, vp, i64, vp, vp, vp, i64, i32, vp, sz, vp]
         for name in EXPORTS[11:-1]:
             getattr(L, name).restype = i32
         L.inf_last_error_detail.argtypes = []
@@ -282,6 +310,18 @@ from .paged import (  # noqa: E402
     kv_evict,
     kv_evict_workspace,
 )
+from .quant import (  # noqa: E402
+    PagedKV4,
+    attn_decode_kv4,
+    attn_decode_kv4_workspace,
+    gemm_i8,
+    gemm_i8_workspace,
+    kv4_append,
+    kv4_read,
+    linear_i8,
+    linear_i8_workspace,
+    quantize_i8,
+)
 
 __all__ = [
     "lib",
@@ -298,6 +338,13 @@ __all__ = [
     "kv_evict",
     "beam_select",
     "beam_reorder",
+    "PagedKV4",
+    "kv4_append",
+    "kv4_read",
+    "attn_decode_kv4",
+    "quantize_i8",
+    "gemm_i8",
+    "linear_i8",
     "strides_of",
     "workspace_bytes",
     "set_deterministic",

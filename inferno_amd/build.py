@@ -34,7 +34,8 @@ COMMON = [
 ]
 
 SOURCES = ["capi.cpp", "attn_fwd.hip", "attn_fwd_bf16.hip", "attn_bwd.hip", "attn_bwd_bf16.hip", "decode.hip", "softmax.hip", "elementwise.hip", "nn.hip",
-           "capi_nn.cpp", "gemm.cpp", "gemm_split.hip", "paged.hip", "beam.hip", "capi_paged.cpp"]
+           "capi_nn.cpp", "gemm.cpp", "gemm_split.hip", "paged.hip", "beam.hip", "capi_paged.cpp",
+           "quant.hip", "gemm_i8.hip", "paged4.hip", "capi_quant.cpp"]
 
 
 def _compile(src: Path, obj: Path) -> None:

@@ -51,20 +51,27 @@ int check_apart(const inf_strides& s, int64_t B, int64_t H, int64_t T, int64_t D
     return INF_OK;
 }
 
+// Sizes that both kinds of cache share.
+int check_sizes(int rows, int heads, int D, int page_size, int max_pages, int n_pages) {
+    if (rows < 1 || heads < 1 || D < 1 || page_size < 1 || max_pages < 1 || n_pages < 1) return INF_ERR_BAD_SHAPE;
+    if (D != 32 && D != 64 && D != 128) return INF_ERR_UNSUPPORTED;
+    if (page_size & (page_size - 1)) {
+        inf::set_error_detail("paged cache: page_size must be a power of two, got " + std::to_string(page_size));
+        return INF_ERR_UNSUPPORTED;
+    }
+    if (rows > 65535 || (int64_t)rows * heads > (1 << 24) || (int64_t)max_pages * page_size > (1 << 30))
+        return INF_ERR_BAD_SHAPE;
+    return INF_OK;
+}
 int check_shape(const inf_paged_kv* c) {
     if (!c) return INF_ERR_NULL_POINTER;
     if (!dtype_ok(c->dt)) return INF_ERR_BAD_DTYPE;
-    if (c->rows < 1 || c->heads < 1 || c->D < 1 || c->page_size < 1 || c->max_pages < 1 || c->n_pages < 1)
-        return INF_ERR_BAD_SHAPE;
-    if (c->D != 32 && c->D != 64 && c->D != 128) return INF_ERR_UNSUPPORTED;
-    if (c->page_size & (c->page_size - 1)) {
-        inf::set_error_detail("paged cache: page_size must be a power of two, got " + std::to_string(c->page_size));
-        return INF_ERR_UNSUPPORTED;
-    }
-    if (c->rows > 65535 || (int64_t)c->rows * c->heads > (1 << 24) ||
-        (int64_t)c->max_pages * c->page_size > (1 << 30))
-        return INF_ERR_BAD_SHAPE;
-    return INF_OK;
+    return check_sizes(c->rows, c->heads, c->D, c->page_size, c->max_pages, c->n_pages);
+}
+int page_shift(int page_size) {
+    int shift = 0;
+    while ((1 << shift) < page_size) ++shift;
+    return shift;
 }
 
 // The cache, for a call that reads it, or writes it too.
@@ -78,10 +85,8 @@ int check_cache(const inf_paged_kv* c, bool written, inf::PagedView* out) {
     if (written && ((st = check_apart(c->sk, c->n_pages, c->heads, c->page_size, c->D)) ||
                     (st = check_apart(c->sv, c->n_pages, c->heads, c->page_size, c->D))))
         return st;
-    int shift = 0;
-    while ((1 << shift) < c->page_size) ++shift;
     *out = inf::PagedView{c->k, c->v, view(c->sk), view(c->sv), c->table, c->lens, c->table_stride,
-                          c->rows, c->heads, c->n_pages, c->max_pages, shift, c->D};
+                          c->rows, c->heads, c->n_pages, c->max_pages, page_shift(c->page_size), c->D};
     return INF_OK;
 }
 
@@ -129,6 +134,68 @@ int check_decode(const inf_paged_kv* c, int q_heads, int max_len) {
     // the steps of a block of rows are counted in 32 bits
     if ((int64_t)std::min(c->rows, inf::kPagedBlock) * (max_len / inf::paged_step(c->D, c->dt == INF_BF16) + 1) >
         (1 << 30))
+        return INF_ERR_BAD_SHAPE;
+    return INF_OK;
+}
+
+// ---- the cache in 4 bits
+int check_shape4(const inf_paged_kv4* c) {
+    if (!c) return INF_ERR_NULL_POINTER;
+    const int st = check_sizes(c->rows, c->heads, c->D, c->page_size, c->max_pages, c->n_pages);
+    if (st != INF_OK) return st;
+    if (c->page_size < 16) {
+        inf::set_error_detail("cache in 4 bits: pages of at least 16 positions, got " + std::to_string(c->page_size));
+        return INF_ERR_UNSUPPORTED;
+    }
+    return INF_OK;
+}
+
+int check_cache4(const inf_paged_kv4* c, bool written, inf::Paged4View* out) {
+    int st = check_shape4(c);
+    if (st != INF_OK) return st;
+    if ((st = check_view(c->k, c->sk, 1, 16)) || (st = check_view(c->v, c->sv, 1, 16)) ||
+        (st = check_view(c->k_scale, c->sks, 1, 4)) || (st = check_view(c->v_scale, c->svs, 1, 4)))
+        return st;
+    if (!c->table || !c->lens) return INF_ERR_NULL_POINTER;
+    if (!aligned(c->table, 4) || !aligned(c->lens, 4)) return INF_ERR_ALIGNMENT;
+    if (c->table_stride < c->max_pages) return INF_ERR_BAD_STRIDE;
+    if (written && ((st = check_apart(c->sk, c->n_pages, c->heads, c->page_size, c->D / 2)) ||
+                    (st = check_apart(c->sv, c->n_pages, c->heads, c->page_size, c->D / 2)) ||
+                    (st = check_apart(c->sks, c->n_pages, c->heads, c->D / 32, c->page_size)) ||
+                    (st = check_apart(c->svs, c->n_pages, c->heads, c->D / 32, c->page_size))))
+        return st;
+    *out = inf::Paged4View{c->k, c->v, c->k_scale, c->v_scale, view(c->sk), view(c->sv), view(c->sks), view(c->svs),
+                           c->table, c->lens, c->table_stride, c->rows, c->heads, c->n_pages, c->max_pages,
+                           page_shift(c->page_size), c->D};
+    return INF_OK;
+}
+
+// The decode's workspace: as DecodeSizes, without scores.
+struct Decode4Sizes {
+    int groups;
+    size_t part, stats, first;
+    size_t total() const { return part + stats + first; }
+};
+Decode4Sizes decode4_sizes(const inf_paged_kv4* c, int q_heads, int max_len) {
+    Decode4Sizes s{};
+    const int blocks = inf::paged_blocks(c->rows);
+    s.groups = inf::kv4_groups(c->rows, c->heads, q_heads / c->heads, max_len, c->D);
+    if (s.groups == 0) return s;
+    const size_t parts = ((size_t)c->rows + (size_t)blocks * s.groups) * q_heads;
+    s.part = round_up(parts * c->D * sizeof(float));
+    s.stats = round_up(parts * 2 * sizeof(float));
+    s.first = round_up(((size_t)c->rows + blocks) * sizeof(int32_t));
+    return s;
+}
+
+int check_decode4(const inf_paged_kv4* c, int q_heads, int max_len) {
+    const int st = check_shape4(c);
+    if (st != INF_OK) return st;
+    if (q_heads < 1 || q_heads % c->heads || max_len < 1 || max_len > (int64_t)c->max_pages * c->page_size)
+        return INF_ERR_BAD_SHAPE;
+    if ((int64_t)c->rows * q_heads > (1 << 24)) return INF_ERR_BAD_SHAPE;
+    // the steps of a block of rows are counted in 32 bits
+    if ((int64_t)std::min(c->rows, inf::kPagedBlock) * (max_len / inf::kv4_step(c->D) + 1) > (1 << 30))
         return INF_ERR_BAD_SHAPE;
     return INF_OK;
 }
@@ -354,6 +421,88 @@ int inf_beam_reorder(const inf_paged_kv* cache, int layers, int64_t k_layer_stri
     p.table_out_stride = table_out_stride;
     p.spare = spare; p.spare_out = spare_out;
     return hip_status(inf::launch_beam_reorder(p, cache->dt == INF_BF16, (hipStream_t)stream));
+}
+
+int inf_kv4_append(const inf_paged_kv4* cache, const void* k, inf_strides sk, const void* v, inf_strides sv,
+                   const int32_t* counts, int T, inf_dtype dt, void* stream) {
+    inf::Kv4AppendParams p{};
+    if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
+    int st = check_cache4(cache, true, &p.c);
+    if (st != INF_OK) return st;
+    if (T < 0) return INF_ERR_BAD_SHAPE;
+    if (T == 0) return INF_OK;
+    const int es = esz(dt);
+    if ((st = check_view(k, sk, es, 4 * es)) || (st = check_view(v, sv, es, 4 * es))) return st;
+    if ((int64_t)T * cache->heads * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    p.k = k; p.v = v;
+    p.sk = view(sk); p.sv = view(sv);
+    p.counts = counts;
+    p.Tn = T;
+    return hip_status(inf::launch_kv4_append(p, dt == INF_BF16, (hipStream_t)stream));
+}
+
+int inf_kv4_read(const inf_paged_kv4* cache, const int32_t* first, int T, void* k, inf_strides sk, void* v,
+                 inf_strides sv, inf_dtype dt, void* stream) {
+    inf::Kv4ReadParams p{};
+    if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
+    int st = check_cache4(cache, false, &p.c);
+    if (st != INF_OK) return st;
+    if (T < 0) return INF_ERR_BAD_SHAPE;
+    if (T == 0) return INF_OK;
+    const int es = esz(dt);
+    if ((st = check_view(k, sk, es, 4 * es)) || (st = check_view(v, sv, es, 4 * es)) ||
+        (st = check_apart(sk, cache->rows, cache->heads, T, cache->D)) ||
+        (st = check_apart(sv, cache->rows, cache->heads, T, cache->D)))
+        return st;
+    if ((int64_t)T * cache->heads * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    p.k = k; p.v = v;
+    p.sk = view(sk); p.sv = view(sv);
+    p.first = first;
+    p.Tn = T;
+    return hip_status(inf::launch_kv4_read(p, dt == INF_BF16, (hipStream_t)stream));
+}
+
+int inf_attn_decode_kv4_workspace(const inf_paged_kv4* cache, int q_heads, int max_len, size_t* out_bytes) {
+    if (!out_bytes) return INF_ERR_NULL_POINTER;
+    *out_bytes = 0;
+    const int st = check_decode4(cache, q_heads, max_len);
+    if (st != INF_OK) return st;
+    *out_bytes = decode4_sizes(cache, q_heads, max_len).total();
+    return INF_OK;
+}
+
+int inf_attn_decode_kv4(const inf_paged_kv4* cache, const void* q, inf_strides sq, void* o, inf_strides so,
+                        int q_heads, int max_len, float scale, inf_dtype dt, void* workspace, size_t ws_bytes,
+                        void* stream) {
+    inf::Kv4DecodeParams p{};
+    if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
+    int st = check_decode4(cache, q_heads, max_len);
+    if (st != INF_OK || (st = check_cache4(cache, false, &p.c))) return st;
+    if (!(scale > 0.f) || !std::isfinite(scale)) return INF_ERR_BAD_SCALE;
+    const int es = esz(dt);
+    if ((st = check_view(q, sq, es, 4 * es)) || (st = check_view(o, so, es, 4 * es)) ||
+        (st = check_apart(so, cache->rows, q_heads, 1, cache->D)))
+        return st;
+    const Decode4Sizes s = decode4_sizes(cache, q_heads, max_len);
+    const int64_t tiles = (q_heads / cache->heads + 15) / 16;
+    if (inf::paged_units(cache->rows, cache->heads, (int)tiles, s.groups) * 256 > kMaxThreads ||
+        (s.groups && (int64_t)cache->rows * q_heads * 256 > kMaxThreads))
+        return INF_ERR_BAD_SHAPE;
+    if (s.total() && (!workspace || ws_bytes < s.total())) return INF_ERR_WORKSPACE;
+    if (s.total() && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
+    p.q = q; p.o = o;
+    p.sq = view(sq); p.so = view(so);
+    p.Hq = q_heads;
+    p.G = q_heads / cache->heads;
+    p.head_tiles = (int)tiles;
+    p.max_len = max_len;
+    p.groups = s.groups;
+    p.cs = scale * 1.4426950408889634f;
+    char* ws = static_cast<char*>(workspace);
+    p.part = reinterpret_cast<float*>(ws);
+    p.stats = reinterpret_cast<float*>(ws + s.part);
+    p.first = reinterpret_cast<int32_t*>(ws + s.part + s.stats);
+    return hip_status(inf::launch_attn_decode_kv4(p, dt == INF_BF16, (hipStream_t)stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,190 @@
+// capi_quant.cpp -- the extern "C" entry points of matrices in 8 bits (include/inferno_hip.h): argument
+// validation on the host, workspace sizing, launches.  Nothing here allocates.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <string>
+
+#include "inferno_hip.h"
+#include "kernels.h"
+
+namespace {
+
+constexpr size_t kAlign = 256;
+constexpr int64_t kMaxLd = int64_t(1) << 22;   // rows of a tile are addressed with 32-bit offsets
+constexpr int64_t kMaxK = (int64_t(1) << 17) - 1;  // 2^7 2^7 K stays inside 32 bits
+constexpr int64_t kMaxMN = int64_t(1) << 30;
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;  // of a launch
+
+bool dtype_ok(int dt) { return dt == INF_F32 || dt == INF_BF16; }
+int esz(inf_dtype dt) { return dt == INF_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+int hip_status(int e) { return e == 0 ? INF_OK : INF_ERR_HIP; }
+size_t round_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
+int64_t whole16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// A matrix in 8 bits: rows on 16 bytes.
+int check_i8(const void* q, int64_t ld, int64_t cols) {
+    if (!q) return INF_ERR_NULL_POINTER;
+    if (ld < whole16(cols) || ld > kMaxLd) return INF_ERR_BAD_STRIDE;
+    return aligned(q, 16) && ld % 16 == 0 ? INF_OK : INF_ERR_ALIGNMENT;
+}
+
+int check_product(int64_t M, int64_t N, int64_t K) {
+    if (M < 1 || N < 1 || K < 1 || M > kMaxMN || N > kMaxMN) return INF_ERR_BAD_SHAPE;
+    if (K > kMaxK) {
+        inf::set_error_detail("product in 8 bits: K of at most " + std::to_string(kMaxK) + ", got " + std::to_string(K));
+        return INF_ERR_UNSUPPORTED;
+    }
+    // tiles, and the join's threads, in one grid
+    return ((M + 127) / 128 + 1) * ((N + 127) / 128 + 1) * 8 * 512 > kMaxThreads || M * ((N + 3) / 4) > kMaxThreads - 256
+               ? INF_ERR_BAD_SHAPE
+               : INF_OK;
+}
+
+// What a product needs behind its operands, and a linear layer for its rows in 8 bits.
+size_t part_bytes(int64_t M, int64_t N, int64_t K) {
+    const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K);
+    return plan.ksplit > 1 ? round_up((size_t)plan.ksplit * M * ((N + 3) / 4 * 4) * 4) : 0;
+}
+size_t q_bytes(int64_t M, int64_t K) { return round_up((size_t)M * whole16(K)); }
+size_t scale_bytes(int64_t M) { return round_up((size_t)M * 4); }
+
+// Whether y [M, N] lies over the n bytes from a on (which may be null: then not).
+struct Result {
+    uintptr_t first, end;
+    bool over(const void* a, int64_t n) const {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a);
+        return a && x < end && first < x + (uintptr_t)n;
+    }
+};
+
+Result result(const void* y, int64_t ldy, int64_t M, int64_t N, inf_dtype dt) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(y);
+    return {x, x + (uintptr_t)(((M - 1) * ldy + N) * esz(dt))};
+}
+
+// The arguments that both forms of the product share.
+int check_rest(const int8_t* w, int64_t ldw, const float* sw, const void* bias, const void* y, int64_t ldy, int64_t M,
+               int64_t N, int64_t K, inf_dtype dt, const void* workspace, size_t ws_bytes, size_t need) {
+    if (!sw || !y) return INF_ERR_NULL_POINTER;
+    if (ldy < N) return INF_ERR_BAD_STRIDE;
+    const size_t es = (size_t)esz(dt);
+    if (!aligned(sw, 4) || !aligned(y, es) || !aligned(bias, es)) return INF_ERR_ALIGNMENT;
+    // other workgroups read these while one writes its results
+    const Result r = result(y, ldy, M, N, dt);
+    if (r.over(w, (N - 1) * ldw + K) || r.over(sw, 4 * N) || r.over(bias, (int64_t)es * N) ||
+        r.over(workspace, (int64_t)need))
+        return INF_ERR_BAD_STRIDE;
+    if (need && (!workspace || ws_bytes < need)) return INF_ERR_WORKSPACE;
+    if (need && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
+    return INF_OK;
+}
+
+int product(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
+            const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, inf_dtype dt, void* part,
+            hipStream_t stream) {
+    const size_t es = (size_t)esz(dt);
+    inf::GemmI8Params p{};
+    p.x = x; p.w = w;
+    p.sx = sx; p.sw = sw;
+    p.bias = bias;
+    p.y = y;
+    p.ldx = ldx; p.ldw = ldw; p.ldy = ldy;
+    p.M = (int)M; p.N = (int)N; p.K = (int)K;
+    p.wide = ldy % 4 == 0 && aligned(y, 4 * es) && aligned(bias, 4 * es) && aligned(sw, 16);
+    p.part = static_cast<int32_t*>(part);
+    p.ldp = (int)((N + 3) / 4 * 4);
+    return hip_status(inf::launch_gemm_i8(p, inf::gemm_i8_plan(M, N, K), dt == INF_BF16, stream));
+}
+
+int quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpose, int8_t* q, int64_t ldq,
+             float* scale, inf_dtype dt, hipStream_t stream) {
+    inf::QuantizeParams p{};
+    p.x = x;
+    p.q = q;
+    p.scale = scale;
+    p.rows = rows; p.cols = cols;
+    p.ldx = ldx; p.ldq = ldq;
+    // rows of bf16 as 8-byte pieces, of fp32 as 16-byte ones
+    p.wide = ldx % 4 == 0 && aligned(x, 4 * (size_t)esz(dt));
+    return hip_status(inf::launch_quantize(p, transpose, dt == INF_BF16, stream));
+}
+
+int check_x(const void* x, int64_t ldx, int64_t cols, inf_dtype dt) {
+    if (!x) return INF_ERR_NULL_POINTER;
+    if (ldx < cols) return INF_ERR_BAD_STRIDE;
+    return aligned(x, (size_t)esz(dt)) ? INF_OK : INF_ERR_ALIGNMENT;
+}
+
+}  // namespace
+
+extern "C" {
+
+int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpose, int8_t* q, int64_t ldq,
+                    float* scale, inf_dtype dt, void* stream) {
+    if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
+    if (rows < 0 || cols < 1 || rows > kMaxMN || cols > kMaxMN) return INF_ERR_BAD_SHAPE;
+    if (transpose ? rows < 1 : rows * 64 > kMaxThreads - 256) return INF_ERR_BAD_SHAPE;
+    if (rows == 0) return INF_OK;
+    int st = check_x(x, ldx, cols, dt);
+    if (st != INF_OK) return st;
+    if (!scale) return INF_ERR_NULL_POINTER;
+    if (!aligned(scale, 4)) return INF_ERR_ALIGNMENT;
+    if ((st = check_i8(q, ldq, transpose ? rows : cols))) return st;
+    // other workgroups still read x
+    const int64_t n = transpose ? cols : rows, k = whole16(transpose ? rows : cols);
+    const Result rx = result(x, ldx, rows, cols, dt);
+    if (rx.over(q, (n - 1) * ldq + k) || rx.over(scale, 4 * n)) return INF_ERR_BAD_STRIDE;
+    return quantize(x, ldx, rows, cols, transpose, q, ldq, scale, dt, (hipStream_t)stream);
+}
+
+int inf_gemm_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes) {
+    if (!out_bytes) return INF_ERR_NULL_POINTER;
+    *out_bytes = 0;
+    const int st = check_product(M, N, K);
+    if (st == INF_OK) *out_bytes = part_bytes(M, N, K);
+    return st;
+}
+
+int inf_gemm_i8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
+                int64_t ldw, const float* w_scale, const void* bias, void* y, int64_t ldy, inf_dtype dt,
+                void* workspace, size_t ws_bytes, void* stream) {
+    if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
+    int st = check_product(M, N, K);
+    if (st != INF_OK || (st = check_i8(x, ldx, K)) || (st = check_i8(w, ldw, K))) return st;
+    if (!x_scale) return INF_ERR_NULL_POINTER;
+    if (!aligned(x_scale, 4)) return INF_ERR_ALIGNMENT;
+    if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, part_bytes(M, N, K))))
+        return st;
+    const Result r = result(y, ldy, M, N, dt);
+    if (r.over(x, (M - 1) * ldx + K) || r.over(x_scale, 4 * M)) return INF_ERR_BAD_STRIDE;
+    return product(x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, (hipStream_t)stream);
+}
+
+int inf_linear_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes) {
+    if (!out_bytes) return INF_ERR_NULL_POINTER;
+    *out_bytes = 0;
+    const int st = check_product(M, N, K);
+    if (st == INF_OK) *out_bytes = q_bytes(M, K) + scale_bytes(M) + part_bytes(M, N, K);
+    return st;
+}
+
+int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
+                  const float* w_scale, const void* bias, void* y, int64_t ldy, inf_dtype dt, void* workspace,
+                  size_t ws_bytes, void* stream) {
+    if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
+    int st = check_product(M, N, K);
+    if (st != INF_OK || (st = check_x(x, ldx, K, dt)) || (st = check_i8(w, ldw, K))) return st;
+    size_t need = 0;
+    inf_linear_i8_workspace(M, N, K, &need);
+    if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, need))) return st;
+    char* ws = static_cast<char*>(workspace);
+    int8_t* q = reinterpret_cast<int8_t*>(ws);
+    float* scale = reinterpret_cast<float*>(ws + q_bytes(M, K));
+    if ((st = quantize(x, ldx, M, K, 0, q, whole16(K), scale, dt, (hipStream_t)stream))) return st;
+    return product(q, whole16(K), scale, w, ldw, w_scale, bias, y, ldy, M, N, K, dt,
+                   ws + q_bytes(M, K) + scale_bytes(M), (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -447,6 +447,96 @@ int launch_kv_evict(const KvEvictParams& p, int bf16, hipStream_t s);
 int launch_beam_select(const BeamSelectParams& p, int bf16, hipStream_t s);
 int launch_beam_reorder(const BeamReorderParams& p, int bf16, hipStream_t s);
 
+// ---- matrices in 8 bits (quant.hip, gemm_i8.hip) --------------------------------
+struct QuantizeParams {
+    const void* x;         // [rows, cols], row stride ldx
+    int8_t* q;             // rows (transposed: columns) of x, ldq bytes apart, 16-byte aligned
+    float* scale;          // [rows] (transposed: [cols])
+    int64_t rows, cols, ldx, ldq;
+    int wide;              // rows of x allow 16-byte loads
+};
+int launch_quantize(const QuantizeParams& p, int transpose, int bf16, hipStream_t s);
+
+struct GemmI8Params {
+    const int8_t* x;       // [M, K], rows ldx bytes apart, 16-byte aligned, readable up to whole 16 bytes
+    const int8_t* w;       // [N, K] likewise
+    const float* sx;       // [M]
+    const float* sw;       // [N]
+    const void* bias;      // [N] in y's type, or null
+    void* y;               // [M, N], row stride ldy
+    int64_t ldx, ldw, ldy;
+    int M, N, K;
+    int wide;              // 4 elements of y, bias and sw at once
+    int32_t* part;         // workspace [ksplit, M, ldp]: the K ranges' sums
+    int ldp;               // N in whole fours
+    // set by the launcher
+    int tiles_m, tiles_n, items;
+    int ksplit, kchunk;
+    int last_piece;        // k of a row's last 16-byte piece
+};
+struct GemmI8Plan {
+    enum Kind { kRows, kMedium, kLarge } kind = kRows;
+    int ksplit = 1, kchunk = 0;
+};
+constexpr int kI8FewRows = 64;
+// K ranges per tile; more than one needs ksplit * M * ldp sums of workspace.
+GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K);
+int launch_gemm_i8(const GemmI8Params& p, const GemmI8Plan& plan, int bf16, hipStream_t s);
+
+// ---- a paged key-value cache in 4 bits (paged4.hip) -----------------------------
+// Pools of bytes, two channels each, [n_pages, heads, slots, D / 2] and of scales [n_pages, heads, slots, D / 32],
+// through strides in bytes; table, lens and page numbers as in PagedView.
+struct Paged4View {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* ks;
+    uint8_t* vs;
+    View4 sk, sv, sks, svs;
+    const int32_t* table;
+    const int32_t* lens;
+    int64_t table_stride;
+    int rows, heads, n_pages, max_pages, page_shift, D;
+    __host__ __device__ int64_t cap() const { return (int64_t)max_pages << page_shift; }
+};
+
+struct Kv4AppendParams {
+    Paged4View c;
+    const void* k;         // new keys [rows, heads, Tn, D]
+    const void* v;
+    View4 sk, sv;
+    const int32_t* counts;  // [rows] tokens of each row, or null: Tn
+    int Tn;
+};
+
+struct Kv4ReadParams {
+    Paged4View c;
+    void* k;               // [rows, heads, Tn, D]
+    void* v;
+    View4 sk, sv;
+    const int32_t* first;  // [rows] first position, or null: 0
+    int Tn;
+};
+
+struct Kv4DecodeParams {
+    Paged4View c;
+    const void* q;
+    void* o;
+    View4 sq, so;
+    int Hq, G, head_tiles, max_len;
+    int groups;            // shares of a block of rows, or 0: a workgroup takes whole rows
+    float cs;              // scale * log2(e)
+    float* part;           // workspace [parts, Hq, D]: unnormalised o
+    float* stats;          // workspace [parts, Hq, 2]: maximum (log2 domain) and sum
+    int32_t* first;        // workspace [rows + blocks]: a row's first step in its block; the blocks' steps
+};
+// Keys that a workgroup takes per step.
+constexpr int kv4_step(int D) { return D == 128 ? 256 : 512; }
+int kv4_groups(int rows, int heads, int G, int max_len, int D);
+
+int launch_kv4_append(const Kv4AppendParams& p, int bf16, hipStream_t s);
+int launch_kv4_read(const Kv4ReadParams& p, int bf16, hipStream_t s);
+int launch_attn_decode_kv4(const Kv4DecodeParams& p, int bf16, hipStream_t s);
+
 // Tile shapes the host needs for grids and workspace sizing.
 // Query rows per forward workgroup: 4 waves x 32 (bf16), 8 waves x 32 (fp32).
 constexpr int kFwdBM = 128;

@@ -10,6 +10,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "paged_shares.h"
 
 namespace inf {
 
@@ -137,17 +138,6 @@ __device__ __forceinline__ int paged_steps(int len, int max_len) {
     constexpr int step = paged_step(D, sizeof(E) == 2);
     return len > max_len ? 0 : (max(len, 0) + step - 1) / step;
 }
-
-// `all` steps in `groups` shares, the first ones a step longer where they do not come out even.
-struct Shares {
-    int q, r;
-    __device__ __forceinline__ Shares(int all, int groups) : q(all / groups), r(all - q * groups) {}
-    __device__ __forceinline__ int start(int g) const { return g * q + min(g, r); }
-    __device__ __forceinline__ int of(int step) const {
-        const int big = r * (q + 1);
-        return step < big ? step / (q + 1) : r + (step - big) / q;
-    }
-};
 
 }  // namespace
 
@@ -462,11 +452,6 @@ __global__ __launch_bounds__(256, kPagedPerCu) void paged_split_kernel(PagedDeco
     }
 }
 
-// The parts of a row: their number, and the first one's place in `part` and `stats` (in steps of Hq).
-struct RowParts {
-    int n;
-    int64_t at;
-};
 template <int D, typename E>
 __device__ __forceinline__ RowParts row_parts(const PagedDecodeParams& p, int row, int len) {
     const int steps = paged_steps<D, E>(len, p.max_len);
@@ -475,13 +460,6 @@ __device__ __forceinline__ RowParts row_parts(const PagedDecodeParams& p, int ro
     const Shares shares(all, p.groups);
     const int g0 = shares.of(start), g1 = shares.of(start + steps - 1);
     return {g1 - g0 + 1, (int64_t)row + block * p.groups + g0};
-}
-
-// (M, L), a maximum and a sum of exponentials below it, with another such pair.
-__device__ __forceinline__ void join_part(float& M, float& L, float m, float l) {
-    const float top = fmaxf(M, m), ref = top == -INFINITY ? 0.f : top;
-    L = L * fast_exp2(M - ref) + l * fast_exp2(m - ref);
-    M = top;
 }
 
 // Joins the parts: the first rows * Hq workgroups write o, the others (where weights are asked

@@ -1,0 +1,195 @@
+// quant.hip -- rows (or columns) of a matrix in 8 bits: for each its scale, the largest magnitude times
+// 1/127, and its values as whole multiples of it, q = rint(x / scale).
+//
+// The quotient is rounded as if it were exact, ties to even: x times the scale's reciprocal may
+// come out on the wrong side of the middle between two whole numbers, so the remainder x - q scale, which one
+// fused multiply-add gives exactly (it is a multiple of the last places of x and scale, and
+// below scale), is compared with half the scale.  The same x then has the same q on any machine.
+//
+// A row with an infinity or a NaN has scale NaN and zeros; one whose scale would be subnormal has scale 0 and
+// zeros.  Magnitudes are compared as whole numbers, where NaN is above infinity and both above the others.
+#include <type_traits>
+
+#include "common.h"
+#include "kernels.h"
+
+namespace inf {
+
+namespace {
+
+constexpr float kInv127 = 1.0f / 127.0f;
+
+// The scale of a row whose largest magnitude has these bits, and its reciprocal (0 where all are zeros).
+struct RowScale {
+    float scale, inv;
+    __device__ __forceinline__ explicit RowScale(uint32_t top) {
+        const float s = __uint_as_float(top) * kInv127;
+        const bool bad = top >= 0x7f800000u, tiny = s < 1.17549435e-38f;
+        scale = bad ? __builtin_nanf("") : tiny ? 0.f : s;
+        inv = bad || tiny ? 0.f : 1.f / s;
+    }
+};
+
+// rint(x / scale) for N values.
+template <int N>
+__device__ __forceinline__ void round_all(const float (&x)[N], const RowScale& s, int (&q)[N]) {
+    const float half = 0.5f * s.scale;
+    float r[N], e[N], worst = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        r[i] = s.inv == 0.f ? 0.f : rintf(x[i] * s.inv);
+        e[i] = s.inv == 0.f ? 0.f : fmaf(-r[i], s.scale, x[i]);
+        worst = fmaxf(worst, fabsf(e[i]));
+    }
+    if (__any(worst >= half)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool odd = (int)r[i] & 1;
+            if (e[i] > half || (e[i] == half && odd)) r[i] += 1.f;
+            if (e[i] < -half || (e[i] == -half && odd)) r[i] -= 1.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i] = (int)fminf(fmaxf(r[i], -127.f), 127.f);
+}
+
+template <int N>
+__device__ __forceinline__ uint32_t pack4(const int (&q)[N], int at) {
+    return (uint32_t)(q[at] & 255) | (uint32_t)(q[at + 1] & 255) << 8 | (uint32_t)(q[at + 2] & 255) << 16 |
+           (uint32_t)(q[at + 3] & 255) << 24;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Eight columns from c on, zeros behind the last.
+template <typename E, bool VEC>
+__device__ __forceinline__ void load8(const typename E::T* row, int c, int cols, float (&x)[8]) {
+    if (VEC && c + 8 <= cols) {
+        const f32x4 a = ld4(row + c), b = ld4(row + c + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = a[i];
+            x[4 + i] = b[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = c + i < cols ? E::ld(row + c + i) : 0.f;
+    }
+}
+
+}  // namespace
+
+// W waves a row, eight neighbouring columns a thread at a time, U of them held between the two passes over
+// the row; a longer row is read twice.  q's rows are written up to whole 16 bytes, with zeros.
+template <typename E, int W, int U, bool VEC>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeParams p) {
+    constexpr int T = 64 * W;
+    __shared__ uint32_t tops[4];
+    const int tid = threadIdx.x % T, wave = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * (4 / W) + threadIdx.x / T;
+    const bool there = row < p.rows;
+    const typename E::T* x = (const typename E::T*)p.x + (there ? row : 0) * p.ldx;
+    const int cols = (int)p.cols;
+    float v[U][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        load8<E, VEC>(x, 8 * (tid + T * u), cols, v[u]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[u][i]));
+    }
+    for (int c = 8 * (tid + T * U); c < cols; c += 8 * T) {
+        float y[8];
+        load8<E, VEC>(x, c, cols, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, magnitude(y[i]));
+    }
+    top = wave_all(top, [](uint32_t a, uint32_t b) { return max(a, b); });
+    if constexpr (W > 1) {
+        if ((threadIdx.x & 63) == 0) tops[wave] = top;
+        __syncthreads();
+        top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    }
+    if (!there) return;
+    const RowScale s(top);
+    int8_t* q = p.q + row * p.ldq;
+    const int end = (cols + 15) & ~15;
+    auto write = [&](int c, const float (&y)[8]) {
+        int r[8];
+        round_all(y, s, r);
+        if (c < end) *reinterpret_cast<uint2*>(q + c) = make_uint2(pack4(r, 0), pack4(r, 4));
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) write(8 * (tid + T * u), v[u]);
+    for (int c = 8 * (tid + T * U); c < end; c += 8 * T) {
+        float y[8];
+        load8<E, VEC>(x, c, cols, y);
+        write(c, y);
+    }
+    if (tid == 0) p.scale[row] = s.scale;
+}
+
+// Columns of x as rows of q (weights [in, out], one scale for each output): a workgroup takes 32 columns, reads
+// them for their largest magnitudes and again, 16 rows a thread, for their values, which it so writes
+// transposed without passing through LDS.
+template <typename E>
+__global__ __launch_bounds__(1024) void quantize_columns_kernel(QuantizeParams p) {
+    __shared__ uint32_t tops[32][33];
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + c;
+    const bool there = col < p.cols;
+    const typename E::T* x = (const typename E::T*)p.x + (there ? col : 0);
+    uint32_t top = 0;
+#pragma unroll 8
+    for (int64_t r = g; r < p.rows; r += 32) top = max(top, magnitude(E::ld(x + r * p.ldx)));
+    tops[g][c] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, tops[i][c]);
+    const RowScale s(top);
+    const int64_t end = (p.rows + 15) & ~(int64_t)15;
+    for (int64_t r0 = 16 * g; r0 < end; r0 += 512) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = r0 + i < p.rows ? E::ld(x + (r0 + i) * p.ldx) : 0.f;
+        int q[16];
+        round_all(v, s, q);
+        if (there)
+            *reinterpret_cast<uint4*>(p.q + col * p.ldq + r0) =
+                make_uint4(pack4(q, 0), pack4(q, 4), pack4(q, 8), pack4(q, 12));
+    }
+    if (there && g == 0) p.scale[col] = s.scale;
+}
+
+template <typename E, bool VEC>
+static void launch_rows(const QuantizeParams& p, hipStream_t s) {
+    auto go = [&](auto w, auto u) {
+        constexpr int W = decltype(w)::value, U = decltype(u)::value;
+        hipLaunchKernelGGL((quantize_rows_kernel<E, W, U, VEC>), dim3((unsigned)((p.rows + 4 / W - 1) / (4 / W))),
+                           dim3(256), 0, s, p);
+    };
+    using std::integral_constant;
+    // one wave a row up to 1024 columns, else four
+    if (p.cols <= 512) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    else if (p.cols <= 1024) go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+    else if (p.cols <= 2048) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    else if (p.cols <= 4096) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+}
+
+int launch_quantize(const QuantizeParams& p, int transpose, int bf16, hipStream_t s) {
+    if (transpose) {
+        const dim3 grid((unsigned)((p.cols + 31) / 32));
+        if (bf16)
+            hipLaunchKernelGGL((quantize_columns_kernel<BF16>), grid, dim3(1024), 0, s, p);
+        else
+            hipLaunchKernelGGL((quantize_columns_kernel<F32>), grid, dim3(1024), 0, s, p);
+    } else if (bf16) {
+        p.wide ? launch_rows<BF16, true>(p, s) : launch_rows<BF16, false>(p, s);
+    } else {
+        p.wide ? launch_rows<F32, true>(p, s) : launch_rows<F32, false>(p, s);
+    }
+    return (int)hipGetLastError();
+}
+
+}  // namespace inf

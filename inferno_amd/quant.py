@@ -1,0 +1,293 @@
+"""Torch-facing helpers over the C-ABI of weights in 8 bits and of a paged key-value cache in 4 bits.
+
+As in ``paged``: the C-ABI validates shapes, strides and sizes on the host and a non-zero status
+raises InfernoError; launches go to torch's current stream on the tensors' device, or to
+``stream``.  What the C-ABI cannot see (dtypes, devices, layouts) is checked here.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import INF_BF16, INF_F32, PagedKV4Struct, Strides, default_scale, lib
+from .ops import _check, strides_of
+from .paged import PagedKV, _bytes, _elsewhere, _of, _on, _raw_stream, _size, _workspace
+
+_DT = {torch.float32: INF_F32, torch.bfloat16: INF_BF16}
+
+
+def _float(t, name):
+    """The C-ABI's type of a float32 or bfloat16 tensor."""
+    dt = _DT.get(t.dtype)
+    if dt is None:
+        raise TypeError(f"{name}: float32 or bfloat16 expected, got {t.dtype}")
+    return dt
+
+
+def _matrix(t, name, device):
+    """(pointer, row stride) of a matrix with adjacent elements in a row."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: a matrix with adjacent elements in a row expected")
+    if t.device != device:
+        raise ValueError(f"{name}: on {t.device}, the others on {device}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _matrix_i8(t, name, device):
+    if t.dtype != torch.int8:
+        raise TypeError(f"{name}: int8 expected, got {t.dtype}")
+    return _matrix(t, name, device)
+
+
+def _rows16(n, cols, device):
+    """int8 [n, cols] whose rows lie on 16 bytes."""
+    return torch.empty((n, -(-cols // 16) * 16), dtype=torch.int8, device=device)[:, :cols]
+
+
+def quantize_i8(x, transpose=False, stream=None):
+    """(q, scale): the rows of x [rows, cols] in 8 bits, q int8 [rows, cols] (rows on 16 bytes) and scale float32
+    [rows]; with ``transpose`` its columns, q [cols, rows] and scale [cols] (weights [in, out])."""
+    dev = x.device
+    dt = _float(x, "quantize_i8: x")
+    ptr, ld = _matrix(x, "quantize_i8: x", dev)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return quantize_i8(x, transpose)
+    rows, cols = x.shape
+    n, k = (cols, rows) if transpose else (rows, cols)
+    q = _rows16(n, k, dev)
+    scale = torch.empty(n, dtype=torch.float32, device=dev)
+    st = lib().inf_quantize_i8(ptr, ld, rows, cols, int(bool(transpose)), q.data_ptr(), -(-k // 16) * 16,
+                               scale.data_ptr(), dt, _raw_stream(dev.index))
+    _check(st, "inf_quantize_i8")
+    return q, scale
+
+
+_sizes = {}
+
+
+def _product_bytes(call, M, N, K):
+    n = _sizes.get((call, M, N, K))
+    if n is None:
+        n = _sizes[call, M, N, K] = _size(getattr(lib(), call), M, N, K)
+    return n
+
+
+def gemm_i8_workspace(M, N, K, device="cuda"):
+    """A workspace for gemm_i8 of these sizes."""
+    return torch.empty(_product_bytes("inf_gemm_i8_workspace", M, N, K), dtype=torch.uint8, device=device)
+
+
+def linear_i8_workspace(M, N, K, device="cuda"):
+    """A workspace for linear_i8 of these sizes."""
+    return torch.empty(_product_bytes("inf_linear_i8_workspace", M, N, K), dtype=torch.uint8, device=device)
+
+
+def _product_args(what, x, w, w_scale, bias, dtype, out, dev):
+    """(w, ldw, w_scale, bias, out's shape) of a product, checked; pointers."""
+    if x.shape[1] != w.shape[1]:
+        raise ValueError(f"{what}: x [M, K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
+    pw, ldw = _matrix_i8(w, f"{what}: w", dev)
+    ps = _of(w_scale, f"{what}: w_scale", torch.float32, dev, w.shape[:1])
+    pb = _of(bias, f"{what}: bias", dtype, dev, w.shape[:1])
+    if out is not None and (out.shape != (x.shape[0], w.shape[0]) or out.dtype != dtype):
+        raise ValueError(f"{what}: out [{x.shape[0]}, {w.shape[0]}] of {dtype} expected")
+    return pw, ldw, ps, pb
+
+
+def gemm_i8(x, x_scale, w, w_scale, bias=None, dtype=torch.float32, out=None, workspace=None, stream=None):
+    """y [M, N] = x w^T times the scales of x's rows and w's rows, plus bias: x [M, K] and w [N, K] int8 with rows on
+    16 bytes (quantize_i8's); y and bias of ``dtype``, float32 or bfloat16."""
+    dev = x.device
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError("gemm_i8: x [M, K] and w [N, K] expected")
+    px, ldx = _matrix_i8(x, "gemm_i8: x", dev)
+    psx = _of(x_scale, "gemm_i8: x_scale", torch.float32, dev, x.shape[:1])
+    dtype = out.dtype if out is not None else dtype
+    if dtype not in _DT:
+        raise TypeError(f"gemm_i8: float32 or bfloat16 expected, got {dtype}")
+    pw, ldw, psw, pb = _product_args("gemm_i8", x, w, w_scale, bias, dtype, out, dev)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return gemm_i8(x, x_scale, w, w_scale, bias, dtype, out, workspace)
+    M, K = x.shape
+    N = w.shape[0]
+    y = torch.empty((M, N), dtype=dtype, device=dev) if out is None else out
+    py, ldy = _matrix(y, "gemm_i8: out", dev)
+    if M == 0:
+        return y
+    ws, ptr, n = _workspace(workspace, lambda: _product_bytes("inf_gemm_i8_workspace", M, N, K), dev)
+    st = lib().inf_gemm_i8(M, N, K, px, ldx, psx, pw, ldw, psw, pb, py, ldy, _DT[dtype], ptr, n,
+                           _raw_stream(dev.index))
+    _check(st, "inf_gemm_i8")
+    return y
+
+
+def linear_i8(x, w, w_scale, bias=None, out=None, workspace=None, stream=None):
+    """y [M, N] = x w^T + bias with the weights in 8 bits (w int8 [N, K], w_scale [N]: quantize_i8's, with
+    ``transpose`` where they are held [in, out]); x [M, K] is taken in 8 bits row by row, y and bias have its type."""
+    dev = x.device
+    dt = _float(x, "linear_i8: x")
+    if w.dim() != 2:
+        raise ValueError("linear_i8: w [N, K] expected")
+    px, ldx = _matrix(x, "linear_i8: x", dev)
+    pw, ldw, psw, pb = _product_args("linear_i8", x, w, w_scale, bias, x.dtype, out, dev)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return linear_i8(x, w, w_scale, bias, out, workspace)
+    M, K = x.shape
+    N = w.shape[0]
+    y = torch.empty((M, N), dtype=x.dtype, device=dev) if out is None else out
+    py, ldy = _matrix(y, "linear_i8: out", dev)
+    if M == 0:
+        return y
+    ws, ptr, n = _workspace(workspace, lambda: _product_bytes("inf_linear_i8_workspace", M, N, K), dev)
+    st = lib().inf_linear_i8(M, N, K, px, ldx, pw, ldw, psw, pb, py, ldy, dt, ptr, n, _raw_stream(dev.index))
+    _check(st, "inf_linear_i8")
+    return y
+
+
+class PagedKV4:
+    """A paged key-value cache in 4 bits: pools k, v uint8 [pages, heads, page size, D / 2] (any strides with dense
+    rows) and k_scale, v_scale uint8 [pages, heads, D / 32, page size] (neighbouring slots adjacent), ``table`` int32
+    [rows, pages per row] and ``lens`` int32 [rows], all on one device.  The handle keeps the tensors; their
+    contents may change at any time, and ``table`` and ``lens`` may be set to other tensors of the same shape."""
+
+    def __init__(self, k, v, k_scale, v_scale, table, lens):
+        if k.dim() != 4 or k.shape != v.shape:
+            raise ValueError("PagedKV4: k and v of one shape [pages, heads, page size, D / 2] expected")
+        pages, heads, page_size, half = k.shape
+        if k_scale.shape != v_scale.shape or k_scale.shape != (pages, heads, half // 16, page_size) or half % 16:
+            raise ValueError("PagedKV4: k_scale and v_scale [pages, heads, D / 32, page size] expected")
+        if any(t.dtype != torch.uint8 for t in (k, v, k_scale, v_scale)):
+            raise TypeError("PagedKV4: uint8 pools and scales expected")
+        if table.dim() != 2 or lens.dim() != 1 or table.shape[0] != lens.shape[0]:
+            raise ValueError("PagedKV4: table [rows, pages] and lens [rows] expected")
+        if table.shape[1] > 1 and table.stride(1) != 1:
+            raise ValueError("PagedKV4: the entries of a row's table must be adjacent")
+        if table.dtype != torch.int32 or lens.dtype != torch.int32:
+            raise TypeError("PagedKV4: table and lens must be int32")
+        if not lens.is_contiguous():
+            raise ValueError("PagedKV4: lens: a dense tensor expected")
+        if any(t.device != k.device for t in (v, k_scale, v_scale, table, lens)):
+            raise ValueError("PagedKV4: all tensors must be on one device")
+        self.k, self.v, self.k_scale, self.v_scale, self._table, self._lens = k, v, k_scale, v_scale, table, lens
+        self.device = k.device
+        self.rows, self.heads, self.D, self.page_size = table.shape[0], heads, 2 * half, page_size
+        self.capacity = table.shape[1] * page_size
+        self.struct = PagedKV4Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                     *(Strides(*t.stride()) for t in (k, v, k_scale, v_scale)), table.data_ptr(),
+                                     lens.data_ptr(), PagedKV._row_stride(table), self.rows, heads, self.D, page_size,
+                                     table.shape[1], pages)
+        self.ref = ctypes.byref(self.struct)
+        self.scale = default_scale(self.D)
+        self.sizes = {}  # workspace bytes by call and arguments
+
+    @staticmethod
+    def empty(pages, heads, page_size, D, table, lens):
+        """A cache of new pools on the table's device."""
+        if D % 32:
+            raise ValueError("PagedKV4: D must be a multiple of 32")
+        k, v = (torch.empty((pages, heads, page_size, D // 2), dtype=torch.uint8, device=table.device) for _ in range(2))
+        ks, vs = (torch.empty((pages, heads, D // 32, page_size), dtype=torch.uint8, device=table.device)
+                  for _ in range(2))
+        return PagedKV4(k, v, ks, vs, table, lens)
+
+    table = PagedKV.table
+    lens = PagedKV.lens
+    _row_stride = staticmethod(PagedKV._row_stride)
+
+
+def _dense4(t, name, cache, T):
+    if t.dim() != 4 or t.shape != (cache.rows, cache.heads, T, cache.D):
+        raise ValueError(f"{name}: [rows, heads, T, D] of the cache's rows, heads and D expected")
+    if t.device != cache.device:
+        raise ValueError(f"{name}: on {t.device}, the cache on {cache.device}")
+
+
+def kv4_append(cache, k, v, counts=None, stream=None):
+    """Writes k, v [rows, heads, T, D] (float32 or bfloat16) as the rows' last positions (``cache.lens`` counts them
+    already); ``counts`` int32 [rows]: how many of the T tokens a row has."""
+    dev = cache.device
+    dt = _float(k, "kv4_append: k")
+    if k.dim() != 4 or v.dtype != k.dtype:
+        raise ValueError("kv4_append: k and v [rows, heads, T, D] of one type expected")
+    T = k.shape[2]
+    _dense4(k, "kv4_append: k", cache, T)
+    _dense4(v, "kv4_append: v", cache, T)
+    pc = _of(counts, "counts", torch.int32, dev, (cache.rows,))
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return kv4_append(cache, k, v, counts)
+    st = lib().inf_kv4_append(cache.ref, k.data_ptr(), strides_of(k), v.data_ptr(), strides_of(v), pc, T, dt,
+                              _raw_stream(dev.index))
+    _check(st, "inf_kv4_append")
+
+
+def kv4_read(cache, T, first=None, dtype=torch.float32, k_out=None, v_out=None, stream=None):
+    """(k, v) [rows, heads, T, D]: positions first[row] + t of every row (``first`` int32 [rows], 0 by default),
+    zeros outside a row's positions."""
+    dev = cache.device
+    T = int(T)
+    if (k_out is None) != (v_out is None):
+        raise ValueError("kv4_read: k_out and v_out go together")
+    if k_out is not None:
+        dtype = k_out.dtype
+        if v_out.dtype != dtype:
+            raise TypeError("kv4_read: k_out and v_out of one type expected")
+        _dense4(k_out, "kv4_read: k_out", cache, T)
+        _dense4(v_out, "kv4_read: v_out", cache, T)
+    if dtype not in _DT:
+        raise TypeError(f"kv4_read: float32 or bfloat16 expected, got {dtype}")
+    pf = _of(first, "first", torch.int32, dev, (cache.rows,))
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return kv4_read(cache, T, first, dtype, k_out, v_out)
+    if k_out is None:
+        k_out, v_out = torch.empty((2, cache.rows, cache.heads, max(T, 0), cache.D), dtype=dtype, device=dev)
+    st = lib().inf_kv4_read(cache.ref, pf, T, k_out.data_ptr(), strides_of(k_out), v_out.data_ptr(),
+                            strides_of(v_out), _DT[dtype], _raw_stream(dev.index))
+    _check(st, "inf_kv4_read")
+    return k_out, v_out
+
+
+def _decode_bytes(cache, q_heads, max_len):
+    return _bytes(cache, "inf_attn_decode_kv4_workspace", q_heads, max_len)
+
+
+def attn_decode_kv4_workspace(cache, q_heads, max_len=None):
+    """A workspace for attn_decode_kv4 with these arguments."""
+    n = _decode_bytes(cache, q_heads, cache.capacity if max_len is None else max_len)
+    return torch.empty(n, dtype=torch.uint8, device=cache.device)
+
+
+def attn_decode_kv4(q, cache, scale=None, max_len=None, out=None, workspace=None, stream=None):
+    """Attention of one new token per row, q [rows, q_heads, 1, D] (float32 or bfloat16), over the row's
+    ``cache.lens`` positions.  ``max_len`` bounds the lengths (the capacity by default)."""
+    dev = cache.device
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != cache.rows or shape[2] != 1 or shape[3] != cache.D:
+        raise ValueError("attn_decode_kv4: q [rows, q_heads, 1, D] of the cache's rows and D expected")
+    dt = _float(q, "attn_decode_kv4: q")
+    if q.device != dev:
+        raise ValueError(f"attn_decode_kv4: q must be on {dev}")
+    heads = shape[1]
+    max_len = cache.capacity if max_len is None else int(max_len)
+    if _elsewhere(dev, stream):
+        with _on(dev, stream):
+            return attn_decode_kv4(q, cache, scale, max_len, out, workspace)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != shape or out.dtype != q.dtype or out.device != dev:
+        raise ValueError("attn_decode_kv4: out must be like q")
+    ws, ptr, n = _workspace(workspace, lambda: _decode_bytes(cache, heads, max_len), dev)
+    st = lib().inf_attn_decode_kv4(cache.ref, q.data_ptr(), strides_of(q), out.data_ptr(), strides_of(out), heads,
+                                   max_len, cache.scale if scale is None else float(scale), dt, ptr, n,
+                                   _raw_stream(dev.index))
+    _check(st, "inf_attn_decode_kv4")
+    return out
+
+
+__all__ = ["PagedKV4", "kv4_append", "kv4_read", "attn_decode_kv4", "attn_decode_kv4_workspace", "quantize_i8",
+           "gemm_i8", "gemm_i8_workspace", "linear_i8", "linear_i8_workspace"]
