@@ -585,7 +585,7 @@ int inf_gemm_i8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, c
                 void* workspace, size_t ws_bytes, void* stream);
 
 /* A linear layer with weights in 8 bits: inf_quantize_i8 of the rows of x [M, K] (fp32 or bf16 by dt, as y), then
- * inf_gemm_i8.  y may be x.  workspace: inf_linear_i8_workspace bytes, 256-byte aligned. */
+ * inf_gemm_i8, to the same bits.  workspace: inf_linear_i8_workspace bytes (may be 0: then NULL), 256-byte aligned. */
 int inf_linear_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes);
 int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
                   const float* w_scale, const void* bias, void* y, int64_t ldy, inf_dtype dt, void* workspace,

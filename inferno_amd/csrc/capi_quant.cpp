@@ -43,12 +43,14 @@ int check_product(int64_t M, int64_t N, int64_t K) {
 }
 
 // What a product needs behind its operands, and a linear layer for its rows in 8 bits.
-size_t part_bytes(int64_t M, int64_t N, int64_t K) {
-    const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K);
+size_t part_bytes(const inf::GemmI8Plan& plan, int64_t M, int64_t N) {
     return plan.ksplit > 1 ? round_up((size_t)plan.ksplit * M * ((N + 3) / 4 * 4) * 4) : 0;
 }
 size_t q_bytes(int64_t M, int64_t K) { return round_up((size_t)M * whole16(K)); }
 size_t scale_bytes(int64_t M) { return round_up((size_t)M * 4); }
+size_t linear_bytes(const inf::GemmI8Plan& plan, int64_t M, int64_t N, int64_t K) {
+    return plan.fused ? 0 : q_bytes(M, K) + scale_bytes(M) + part_bytes(plan, M, N);
+}
 
 // Whether y [M, N] lies over the n bytes from a on (which may be null: then not).
 struct Result {
@@ -81,21 +83,22 @@ int check_rest(const int8_t* w, int64_t ldw, const float* sw, const void* bias, 
     return INF_OK;
 }
 
-int product(const int8_t* x, int64_t ldx, const float* sx, const int8_t* w, int64_t ldw, const float* sw,
-            const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, inf_dtype dt, void* part,
-            hipStream_t stream) {
-    const size_t es = (size_t)esz(dt);
+// Rows of elements that can be read four at a time.
+bool by_four(const void* x, int64_t ldx, inf_dtype dt) { return ldx % 4 == 0 && aligned(x, 4 * (size_t)esz(dt)); }
+
+// What both forms of the product have in common.
+inf::GemmI8Params product(const int8_t* w, int64_t ldw, const float* sw, const void* bias, void* y, int64_t ldy,
+                          int64_t M, int64_t N, int64_t K, inf_dtype dt) {
     inf::GemmI8Params p{};
-    p.x = x; p.w = w;
-    p.sx = sx; p.sw = sw;
+    p.w = w;
+    p.sw = sw;
     p.bias = bias;
     p.y = y;
-    p.ldx = ldx; p.ldw = ldw; p.ldy = ldy;
+    p.ldw = ldw; p.ldy = ldy;
     p.M = (int)M; p.N = (int)N; p.K = (int)K;
-    p.wide = ldy % 4 == 0 && aligned(y, 4 * es) && aligned(bias, 4 * es) && aligned(sw, 16);
-    p.part = static_cast<int32_t*>(part);
+    p.wide = by_four(y, ldy, dt) && aligned(bias, 4 * (size_t)esz(dt)) && aligned(sw, 16);
     p.ldp = (int)((N + 3) / 4 * 4);
-    return hip_status(inf::launch_gemm_i8(p, inf::gemm_i8_plan(M, N, K), dt == INF_BF16, stream));
+    return p;
 }
 
 int quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpose, int8_t* q, int64_t ldq,
@@ -106,8 +109,7 @@ int quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpo
     p.scale = scale;
     p.rows = rows; p.cols = cols;
     p.ldx = ldx; p.ldq = ldq;
-    // rows of bf16 as 8-byte pieces, of fp32 as 16-byte ones
-    p.wide = ldx % 4 == 0 && aligned(x, 4 * (size_t)esz(dt));
+    p.wide = by_four(x, ldx, dt);
     return hip_status(inf::launch_quantize(p, transpose, dt == INF_BF16, stream));
 }
 
@@ -143,7 +145,7 @@ int inf_gemm_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes) {
     if (!out_bytes) return INF_ERR_NULL_POINTER;
     *out_bytes = 0;
     const int st = check_product(M, N, K);
-    if (st == INF_OK) *out_bytes = part_bytes(M, N, K);
+    if (st == INF_OK) *out_bytes = part_bytes(inf::gemm_i8_plan(M, N, K, true), M, N);
     return st;
 }
 
@@ -155,18 +157,24 @@ int inf_gemm_i8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, c
     if (st != INF_OK || (st = check_i8(x, ldx, K)) || (st = check_i8(w, ldw, K))) return st;
     if (!x_scale) return INF_ERR_NULL_POINTER;
     if (!aligned(x_scale, 4)) return INF_ERR_ALIGNMENT;
-    if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, part_bytes(M, N, K))))
+    const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K, true);
+    if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, part_bytes(plan, M, N))))
         return st;
     const Result r = result(y, ldy, M, N, dt);
     if (r.over(x, (M - 1) * ldx + K) || r.over(x_scale, 4 * M)) return INF_ERR_BAD_STRIDE;
-    return product(x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, (hipStream_t)stream);
+    inf::GemmI8Params p = product(w, ldw, w_scale, bias, y, ldy, M, N, K, dt);
+    p.x = x;
+    p.ldx = ldx;
+    p.sx = x_scale;
+    p.part = static_cast<int32_t*>(workspace);
+    return hip_status(inf::launch_gemm_i8(p, plan, dt == INF_BF16, (hipStream_t)stream));
 }
 
 int inf_linear_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes) {
     if (!out_bytes) return INF_ERR_NULL_POINTER;
     *out_bytes = 0;
     const int st = check_product(M, N, K);
-    if (st == INF_OK) *out_bytes = q_bytes(M, K) + scale_bytes(M) + part_bytes(M, N, K);
+    if (st == INF_OK) *out_bytes = linear_bytes(inf::gemm_i8_plan(M, N, K, false), M, N, K);
     return st;
 }
 
@@ -176,15 +184,26 @@ int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, c
     if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
     int st = check_product(M, N, K);
     if (st != INF_OK || (st = check_x(x, ldx, K, dt)) || (st = check_i8(w, ldw, K))) return st;
-    size_t need = 0;
-    inf_linear_i8_workspace(M, N, K, &need);
-    if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, need))) return st;
-    char* ws = static_cast<char*>(workspace);
-    int8_t* q = reinterpret_cast<int8_t*>(ws);
-    float* scale = reinterpret_cast<float*>(ws + q_bytes(M, K));
-    if ((st = quantize(x, ldx, M, K, 0, q, whole16(K), scale, dt, (hipStream_t)stream))) return st;
-    return product(q, whole16(K), scale, w, ldw, w_scale, bias, y, ldy, M, N, K, dt,
-                   ws + q_bytes(M, K) + scale_bytes(M), (hipStream_t)stream);
+    const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K, false);
+    if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, linear_bytes(plan, M, N, K))))
+        return st;
+    if (result(y, ldy, M, N, dt).over(x, ((M - 1) * ldx + K) * esz(dt))) return INF_ERR_BAD_STRIDE;
+    inf::GemmI8Params p = product(w, ldw, w_scale, bias, y, ldy, M, N, K, dt);
+    if (plan.fused) {
+        p.xf = x;
+        p.ldxf = ldx;
+        p.wide_x = by_four(x, ldx, dt);
+    } else {
+        char* ws = static_cast<char*>(workspace);
+        int8_t* q = reinterpret_cast<int8_t*>(ws);
+        float* scale = reinterpret_cast<float*>(ws + q_bytes(M, K));
+        p.x = q;
+        p.ldx = whole16(K);
+        p.sx = scale;
+        p.part = reinterpret_cast<int32_t*>(ws + q_bytes(M, K) + scale_bytes(M));
+        if ((st = quantize(x, ldx, M, K, 0, q, p.ldx, scale, dt, (hipStream_t)stream))) return st;
+    }
+    return hip_status(inf::launch_gemm_i8(p, plan, dt == INF_BF16, (hipStream_t)stream));
 }
 
 }  // extern "C"

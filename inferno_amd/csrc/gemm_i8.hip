@@ -4,14 +4,14 @@
 //
 // The weights are the MFMA's A operand and the rows of x its B, so that a lane holds one row of x and runs of four
 // neighbouring n: scales of n come as 16-byte loads and results leave as 8 or 16 bytes.
-// MFMA layouts, lane l: A[l % 32][16 g .. 16 g + 15], g = l / 32 (32x32x32), A[l % 16][16 g ..], g = l / 16
-// (16x16x64); B likewise; D as the other 32x32 and 16x16 shapes'.  The reduction runs in any order that
-// both operands share.
+// MFMA layout (32x32x32), lane l: A[l % 32][16 g .. 16 g + 15], g = l / 32; B likewise; D as the other 32x32
+// shapes'.  The reduction runs in any order that both operands share.
 #include <algorithm>
 #include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
+#include "quant_rows.h"
 
 namespace inf {
 
@@ -20,16 +20,11 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 namespace {
 
-constexpr int kBK = 128;             // k of a tile: 128 bytes of a row
 constexpr uint32_t kNowhere = 0x80000000u;  // past the end of every buffer resource
 
 __device__ __forceinline__ i32x16 mfma32x32x32i8(i32x4 a, i32x4 b, i32x16 c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ i32x4 mfma16x16x64i8(i32x4 a, i32x4 b, i32x4 c) {
-    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
-}
-
 // The first n of 16 bytes, zeros behind them.
 __device__ __forceinline__ i32x4 first_bytes(i32x4 v, int n) {
 #pragma unroll
@@ -40,8 +35,8 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 v, int n) {
     return v;
 }
 
-// Four neighbouring results of row m from column n on.
-template <typename E>
+// Four neighbouring results of row m from column n on.  NT: past the caches, where whole lines are written.
+template <typename E, bool NT = false>
 __device__ __forceinline__ void finish4(const GemmI8Params& p, int m, int n, i32x4 sum, float sx) {
     typename E::T* y = (typename E::T*)p.y + (int64_t)m * p.ldy + n;
     const typename E::T* bias = (const typename E::T*)p.bias;
@@ -49,7 +44,14 @@ __device__ __forceinline__ void finish4(const GemmI8Params& p, int m, int n, i32
     auto one = [&](int i, float sw, float b) { return fmaf((float)sum[i] * sx, sw, b); };
     if (p.wide && n + 4 <= p.N) {
         const f32x4 sw = ld4(p.sw + n), b = bias ? ld4(bias + n) : f32x4{0.f, 0.f, 0.f, 0.f};
-        st4(y, f32x4{one(0, sw[0], b[0]), one(1, sw[1], b[1]), one(2, sw[2], b[2]), one(3, sw[3], b[3])});
+        const f32x4 v = {one(0, sw[0], b[0]), one(1, sw[1], b[1]), one(2, sw[2], b[2]), one(3, sw[3], b[3])};
+        if constexpr (!NT)
+            st4(y, v);
+        else if constexpr (sizeof(typename E::T) == 4)
+            __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(y));
+        else
+            __builtin_nontemporal_store(u16x4{f32_to_bf16(v[0]), f32_to_bf16(v[1]), f32_to_bf16(v[2]), f32_to_bf16(v[3])},
+                                        reinterpret_cast<u16x4*>(y));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -61,18 +63,29 @@ __device__ __forceinline__ void finish4(const GemmI8Params& p, int m, int n, i32
 
 // ============================================================================
 // Tiles.  A workgroup of WN x WM waves forms BN x BM results, each wave 32 x 32 blocks of them in its registers, with
-// k in steps of 128 bytes through double-buffered LDS, filled by direct-to-LDS loads one step ahead.
-// LDS rows are 128 bytes, their eight 16-byte pieces at places c ^ (row % 8): any eight rows' pieces of one
-// c lie in different banks.  A direct-to-LDS load fills 16 bytes a lane in the lanes' order, so the lanes
-// fetch the pieces in that order: eight lanes still take one whole line of a row.
+// k in steps of BK bytes through a ring of S buffers in LDS, filled by direct-to-LDS loads S - 1 steps ahead.
+// A step's 16-byte pieces of a row lie in an order that varies with the row, so that any eight rows' pieces of
+// one k lie in different banks.  A direct-to-LDS load fills 16 bytes a lane in the lanes' order, so the
+// lanes fetch the pieces in that order: four (BK = 64) or eight lanes still take one run of a row.
+//
+// One barrier a step, before its last 32 k: by then every wave has read all of the step's operands (the last 32 k's are
+// in registers), so its buffer takes the loads of S steps on, while the products of these 32 k hide the first reads of
+// the next step's.
 // ============================================================================
-template <typename E, int BN, int BM, int WN, int WM, bool SPLIT>
-__global__ __launch_bounds__(64 * WN * WM, 2) void gemm_i8_kernel(GemmI8Params p) {
+template <typename E, int BN, int BM, int WN, int WM, int BK, int S, bool SPLIT>
+__global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * BK * S > 81920 ? 1 : 2) / 4) void gemm_i8_kernel(
+    GemmI8Params p) {
     constexpr int NW = WN * WM;
     constexpr int FN = BN / WN / 32, FM = BM / WM / 32;
-    constexpr int IN = BN / 8 / NW, IM = BM / 8 / NW;  // load instructions a wave and step
-    static_assert(BN % (8 * NW) == 0 && BM % (8 * NW) == 0, "whole instructions");
-    __shared__ __attribute__((aligned(16))) char ws0[BN * kBK], ws1[BN * kBK], xs0[BM * kBK], xs1[BM * kBK];
+    constexpr int P = BK / 16, RI = 64 / P;                     // pieces a row; rows a load instruction
+    constexpr int IN = BN / RI / NW, IM = BM / RI / NW;         // instructions a wave and step
+    constexpr int KS = BK / 32;
+    static_assert(BN % (RI * NW) == 0 && BM % (RI * NW) == 0, "whole instructions");
+    static_assert(S == 2 || S == 4, "steps named at compile time");
+    // arrays of their own, so that the compiler can tell the loads into one from the reads of the others
+    __shared__ __attribute__((aligned(16))) char w0[BN * BK], x0[BM * BK], w1[BN * BK], x1[BM * BK];
+    __shared__ __attribute__((aligned(16))) char w2[S > 2 ? BN * BK : 16], x2[S > 2 ? BM * BK : 16],
+        w3[S > 2 ? BN * BK : 16], x3[S > 2 ? BM * BK : 16];
 
     const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -97,19 +110,20 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void gemm_i8_kernel(GemmI8Params p
     const int8_t* W = p.w + (int64_t)n0 * p.ldw;
     const int8_t* X = p.x + (int64_t)m0 * p.ldx;
     const int rows_n = min(p.N - n0, BN), rows_m = min(p.M - m0, BM);
-    const int piece = 16 * ((lane & 7) ^ (lane >> 3));  // this lane's of a step's row
+    auto order = [](int row) { return P == 8 ? row & 7 : (row >> 1) & 3; };
+    const int piece = 16 * ((lane % P) ^ order(lane / P));  // this lane's of a step's row
     uint32_t vw[IN], vx[IM];
 #pragma unroll
     for (int i = 0; i < IN; ++i) {
-        const int r = 8 * (wave + NW * i) + (lane >> 3);
+        const int r = RI * (wave + NW * i) + lane / P;
         vw[i] = r < rows_n ? (uint32_t)((int64_t)r * p.ldw + piece) : kNowhere;
     }
 #pragma unroll
     for (int i = 0; i < IM; ++i) {
-        const int r = 8 * (wave + NW * i) + (lane >> 3);
+        const int r = RI * (wave + NW * i) + lane / P;
         vx[i] = r < rows_m ? (uint32_t)((int64_t)r * p.ldx + piece) : kNowhere;
     }
-    auto load = [&](char* wd, char* xd, int k0) {
+    auto load = [&](char* wd, char* xd, int k0) {  // a step behind the end reads nothing: zeros
         const bool in = piece < k16 - k0;
         const auto rw = buffer_rsrc(W + k0, k0 < k16 ? (uint32_t)((int64_t)(rows_n - 1) * p.ldw + k16 - k0) : 0u);
         const auto rx = buffer_rsrc(X + k0, k0 < k16 ? (uint32_t)((int64_t)(rows_m - 1) * p.ldx + k16 - k0) : 0u);
@@ -118,6 +132,16 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void gemm_i8_kernel(GemmI8Params p
 #pragma unroll
         for (int i = 0; i < IM; ++i) buffer_ld16_lds(rx, xd + 1024 * (wave + NW * i), in ? vx[i] : kNowhere);
     };
+    // All waves' LDS reads are done, and their loads but those of the newest `steps` steps.  (__syncthreads() would
+    // wait for all loads into LDS.)
+    auto meet = [](auto steps) {
+        constexpr int n = decltype(steps)::value * (IN + IM);
+        static_assert(n < 64, "the counter's range");
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4);  // vmcnt(n) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
 
     i32x16 acc[FN][FM];
 #pragma unroll
@@ -125,58 +149,118 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void gemm_i8_kernel(GemmI8Params p
 #pragma unroll
         for (int b = 0; b < FM; ++b) acc[a][b] = i32x16{};
 
-    load(ws0, xs0, k_first);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
     const int row_n = wn * (BN / WN) + l32, row_m = wm * (BM / WM) + l32;
-    auto step = [&](int k0, const char* wc, const char* xc, char* wd, char* xd) {
-        load(wd, xd, k0 + kBK);
-        const bool ragged = k0 + kBK > k_end && k_end % 16;
-#pragma unroll
-        for (int s = 0; s < kBK / 32; ++s) {
-            const int at = 16 * ((2 * s + g) ^ (l32 & 7));
-            i32x4 a[FN], b[FM];
-#pragma unroll
-            for (int f = 0; f < FN; ++f)
-                a[f] = *reinterpret_cast<const i32x4*>(wc + (row_n + 32 * f) * kBK + at);
-#pragma unroll
-            for (int f = 0; f < FM; ++f)
-                b[f] = *reinterpret_cast<const i32x4*>(xc + (row_m + 32 * f) * kBK + at);
-            if (ragged) {
-#pragma unroll
-                for (int f = 0; f < FM; ++f) b[f] = first_bytes(b[f], k_end - (k0 + 32 * s + 16 * g));
-            }
-#pragma unroll
-            for (int f = 0; f < FN; ++f)
-#pragma unroll
-                for (int h = 0; h < FM; ++h) acc[f][h] = mfma32x32x32i8(a[f], b[h], acc[f][h]);
-        }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
+    struct Frags {
+        i32x4 a[FN], b[FM];
     };
-    for (int k0 = k_first; k0 < k_end; k0 += 2 * kBK) {
-        step(k0, ws0, xs0, ws1, xs1);
-        if (k0 + kBK < k_end) step(k0 + kBK, ws1, xs1, ws0, xs0);
+    auto read = [&](Frags& f, const char* wc, const char* xc, int s) {
+        const int at = 16 * ((2 * s + g) ^ order(l32));
+#pragma unroll
+        for (int i = 0; i < FN; ++i) f.a[i] = *reinterpret_cast<const i32x4*>(wc + (row_n + 32 * i) * BK + at);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) f.b[i] = *reinterpret_cast<const i32x4*>(xc + (row_m + 32 * i) * BK + at);
+    };
+    auto multiply = [&](const Frags& f) {
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) acc[i][j] = mfma32x32x32i8(f.a[i], f.b[j], acc[i][j]);
+    };
+    // the reads of the next 32 k between the products of these
+    auto interleave = [] {
+        constexpr int R = FN + FM, M = FN * FM;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // a read
+            __builtin_amdgcn_sched_group_barrier(0x008, M >= 2 * R ? 2 : 1, 0);  // products
+        }
+        if constexpr (M < 2 * R && M > R) __builtin_amdgcn_sched_group_barrier(0x008, M - R, 0);
+    };
+    using std::integral_constant;
+    Frags f[2];
+    // the step of k0 in its buffer; the next one's buffer.  LAST: k may end in this step.
+    auto step = [&](auto last, int k0, char* wc, char* xc, const char* wnext, const char* xnext) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (s + 1 < KS) {
+                read(f[(s + 1) & 1], wc, xc, s + 1);
+            } else {
+                meet(integral_constant<int, S - 2>{});
+                load(wc, xc, k0 + S * BK);
+                read(f[(s + 1) & 1], wnext, xnext, 0);
+            }
+            if constexpr (decltype(last)::value) {
+                if (k_end % 16) {  // the last piece's bytes behind the end
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+                        f[s & 1].b[i] = first_bytes(f[s & 1].b[i], k_end - (k0 + 32 * s + 16 * g));
+                }
+            }
+            multiply(f[s & 1]);
+            interleave();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    load(w0, x0, k_first);
+    load(w1, x1, k_first + BK);
+    if constexpr (S > 2) {
+        load(w2, x2, k_first + 2 * BK);
+        load(w3, x3, k_first + 3 * BK);
+    }
+    meet(integral_constant<int, S - 1>{});
+    read(f[0], w0, x0, 0);
+    int k0 = k_first;
+    const std::false_type whole;
+    const std::true_type last;
+    if constexpr (S > 2) {
+        for (; k0 + 4 * BK <= k_end; k0 += 4 * BK) {
+            step(whole, k0, w0, x0, w1, x1);
+            step(whole, k0 + BK, w1, x1, w2, x2);
+            step(whole, k0 + 2 * BK, w2, x2, w3, x3);
+            step(whole, k0 + 3 * BK, w3, x3, w0, x0);
+        }
+        if (k0 < k_end) step(last, k0, w0, x0, w1, x1);
+        if (k0 + BK < k_end) step(last, k0 + BK, w1, x1, w2, x2);
+        if (k0 + 2 * BK < k_end) step(last, k0 + 2 * BK, w2, x2, w3, x3);
+        if (k0 + 3 * BK < k_end) step(last, k0 + 3 * BK, w3, x3, w0, x0);
+    } else {
+        for (; k0 + 2 * BK <= k_end; k0 += 2 * BK) {
+            step(whole, k0, w0, x0, w1, x1);
+            step(whole, k0 + BK, w1, x1, w0, x0);
+        }
+        if (k0 < k_end) step(last, k0, w0, x0, w1, x1);
+        if (k0 + BK < k_end) step(last, k0 + BK, w1, x1, w0, x0);
     }
 
+    // Results leave in whole lines: each wave turns 32 rows of its block at a time in LDS (a lane holds runs of four
+    // columns of one row), pieces of 16 bytes at places that vary with the row, as above.
+    __syncthreads();
+    constexpr int U = BN / WN / 4;                       // pieces of four results in a wave's row
+    constexpr int HOLD = (BN < BM ? BN : BM) * BK / (32 * U * 16);  // waves' blocks in an array of the ring
+    static_assert(HOLD * 4 >= NW, "a block in LDS for every wave");
+    const int which = wave / HOLD;
+    i32x4* turn = reinterpret_cast<i32x4*>(which == 0 ? w0 : which == 1 ? x0 : which == 2 ? w1 : x1) + wave % HOLD * 32 * U;
 #pragma unroll
     for (int h = 0; h < FM; ++h) {
-        const int m = m0 + row_m + 32 * h;
-        if (m >= p.M) continue;
-        const float sx = SPLIT ? 0.f : p.sx[m];
 #pragma unroll
         for (int f = 0; f < FN; ++f)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + wn * (BN / WN) + 32 * f + 8 * j + 4 * g;
-                const i32x4 v = {acc[f][h][4 * j], acc[f][h][4 * j + 1], acc[f][h][4 * j + 2], acc[f][h][4 * j + 3]};
-                if constexpr (SPLIT) {
-                    if (n < p.N)
-                        *reinterpret_cast<i32x4*>(p.part + ((int64_t)split * p.M + m) * p.ldp + n) = v;
-                } else if (n < p.N) {
-                    finish4<E>(p, m, n, v, sx);
-                }
-            }
+            for (int j = 0; j < 4; ++j)
+                turn[l32 * U + ((8 * f + 2 * j + g) ^ (l32 & 7))] =
+                    i32x4{acc[f][h][4 * j], acc[f][h][4 * j + 1], acc[f][h][4 * j + 2], acc[f][h][4 * j + 3]};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < U / 2; ++i) {
+            const int r = (64 * i + lane) / U, c = (64 * i + lane) % U;
+            const int m = m0 + wm * (BM / WM) + 32 * h + r, n = n0 + wn * (BN / WN) + 4 * c;
+            const i32x4 v = turn[r * U + (c ^ (r & 7))];
+            if (m >= p.M || n >= p.N) continue;
+            if constexpr (SPLIT)
+                *reinterpret_cast<i32x4*>(p.part + ((int64_t)split * p.M + m) * p.ldp + n) = v;
+            else
+                finish4<E, true>(p, m, n, v, p.sx[m]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
@@ -195,95 +279,226 @@ __global__ __launch_bounds__(256) void gemm_i8_join_kernel(GemmI8Params p) {
 }
 
 // ============================================================================
-// Few rows: the weights go from memory straight into registers, each byte once.  A workgroup takes R x 16 outputs, its
-// NW waves a K range each, all of a step's loads ahead of its products; x comes out of the caches.
+// Few rows: a workgroup takes 32 outputs and all rows of x, and its four waves every fourth step of 128 k each, in a
+// ring of S buffers of its own: no barriers, and the whole device's loads are under way at once.  Weights pass
+// through LDS in whole lines (loaded straight into registers, 16 rows x 64 bytes at a time, with x out of the caches for
+// every 16 outputs, 32 x 16384 x 4096 took 16 us, 13 so).  The waves' sums meet in LDS.
+//
+// FUSED: x comes as it is, and the workgroup quantises all of it while its first weights are on their way.
+// Every workgroup does, so that pays where x is small.
 // ============================================================================
-template <typename E, int MT, int R, int NW>
-__global__ __launch_bounds__(64 * NW) void gemm_i8_rows_kernel(GemmI8Params p) {
-    constexpr int U = MT * R >= 4 ? 2 : 4;  // steps of 64 k whose loads are under way together
-    __shared__ i32x4 sums[NW][R * MT][64];
-    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * (16 * R);
-    const int8_t* w[R];
-    const int8_t* x[MT];
+constexpr int kRowsWaves = 4;
+
+template <typename E, int FM, int S, bool FUSED>
+__global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Params p) {
+    constexpr int BK = 128, BN = 32, NW = kRowsWaves;
+    constexpr int XB = FUSED ? 0 : 32 * FM;                  // rows of x in the ring
+    constexpr int L = (BN + XB) / 8;                         // load instructions a step
+    constexpr int STEP = (BN + XB) * BK;
+    static_assert(S == 3 || S == 4, "steps named at compile time");
+    __shared__ __attribute__((aligned(16))) char r0[NW * STEP], r1[NW * STEP], r2[NW * STEP],
+        r3[S > 3 ? NW * STEP : 16];
+    extern __shared__ __attribute__((aligned(16))) char xq[];  // FUSED: [M][x_stride]
+    __shared__ float scales[32];
+    __shared__ uint32_t tops[NW];
+
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * BN, k16 = (p.K + 15) & ~15;
+    const int8_t* W = p.w + (int64_t)n0 * p.ldw;
+    const int rows_n = min(p.N - n0, BN);
+    const int piece = 16 * ((lane & 7) ^ (lane >> 3));
+    uint32_t vw[BN / 8], vx[XB ? XB / 8 : 1];
 #pragma unroll
-    for (int r = 0; r < R; ++r) w[r] = p.w + (int64_t)min(n0 + 16 * r + l16, p.N - 1) * p.ldw + 16 * g;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) x[t] = p.x + (int64_t)min(16 * t + l16, p.M - 1) * p.ldx + 16 * g;
-    i32x4 acc[R][MT];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) acc[r][t] = i32x4{};
-    const int steps = (p.K + 63) / 64, per = (steps + NW - 1) / NW;
-    const int s1 = min(steps, per * (wave + 1));
-    const i32x4 zero = {};
-    for (int s = per * wave; s < s1; s += U) {
-        i32x4 a[U][R], b[U][MT];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            // a piece behind the end is read where the row's last one is, and counts as zeros
-            const int k = min(64 * (s + u), p.last_piece - 16 * g);
-#pragma unroll
-            for (int r = 0; r < R; ++r) a[u][r] = *reinterpret_cast<const i32x4*>(w[r] + k);
-#pragma unroll
-            for (int t = 0; t < MT; ++t) b[u][t] = *reinterpret_cast<const i32x4*>(x[t] + k);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (s + u >= s1) break;
-            const int left = p.K - (64 * (s + u) + 16 * g);
-            if (64 * (s + u) + 64 > p.K) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t) b[u][t] = left >= 16 ? b[u][t] : left <= 0 ? zero : first_bytes(b[u][t], left);
-            }
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int t = 0; t < MT; ++t) acc[r][t] = mfma16x16x64i8(a[u][r], b[u][t], acc[r][t]);
-        }
+    for (int i = 0; i < BN / 8; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        vw[i] = r < rows_n ? (uint32_t)((int64_t)r * p.ldw + piece) : kNowhere;
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int i = 0; i < XB / 8; ++i) {
+        const int r = 8 * i + (lane >> 3);
+        vx[i] = r < p.M ? (uint32_t)((int64_t)r * p.ldx + piece) : kNowhere;
+    }
+    auto load = [&](char* ring, int k0) {  // a step behind the end reads nothing: zeros
+        char* to = ring + wave * STEP;
+        const bool in = piece < k16 - k0;
+        const auto rw = buffer_rsrc(W + k0, k0 < k16 ? (uint32_t)((int64_t)(rows_n - 1) * p.ldw + k16 - k0) : 0u);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) sums[wave][r * MT + t][lane] = acc[r][t];
+        for (int i = 0; i < BN / 8; ++i) buffer_ld16_lds(rw, to + 1024 * i, in ? vw[i] : kNowhere);
+        if constexpr (XB > 0) {
+            const auto rx = buffer_rsrc(p.x + k0, k0 < k16 ? (uint32_t)((int64_t)(p.M - 1) * p.ldx + k16 - k0) : 0u);
+#pragma unroll
+            for (int i = 0; i < XB / 8; ++i) buffer_ld16_lds(rx, to + BN * BK + 1024 * i, in ? vx[i] : kNowhere);
+        }
+    };
+    // This wave's step i.  Workgroups start at different places of the whole rounds of the waves: rows are often powers
+    // of two apart, and steps of one k then lie in few of the memory's channels (8 x 8192 x 8192: 20.2 us, 13.5 so).
+    constexpr int NEXT = BK * NW;
+    const int rounds = p.K / NEXT, turn = rounds ? blockIdx.x % rounds : 0;
+    auto k_of = [&](int i) {
+        const int j = i < rounds ? (i + turn < rounds ? i + turn : i + turn - rounds) : i;
+        return j * NEXT + BK * wave;
+    };
+    load(r0, k_of(0));
+    load(r1, k_of(1));
+    load(r2, k_of(2));
+    if constexpr (S > 3) load(r3, k_of(3));
+
+    const int x_stride = ((p.K + BK - 1) & ~(BK - 1)) + 16;
+    if constexpr (FUSED) {
+        // one row to all waves, or rows to waves
+        const bool one = p.M == 1;
+        const int T = one ? 64 * NW : 64, t = one ? tid : lane;
+        for (int m = one ? 0 : wave; m < p.M; m += NW) {
+            const typename E::T* x = (const typename E::T*)p.xf + (int64_t)m * p.ldxf;
+            uint32_t top = 0;
+            auto most = [&](auto vec) {
+#pragma unroll 2
+                for (int c = 8 * t; c < p.K; c += 8 * T) {
+                    float v[8];
+                    load8<E, decltype(vec)::value>(x, c, p.K, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
+                }
+            };
+            if (p.wide_x) most(std::true_type{});
+            else most(std::false_type{});
+            top = wave_all(top, [](uint32_t a, uint32_t b) { return max(a, b); });
+            if (one) {
+                if (lane == 0) tops[wave] = top;
+                __syncthreads();
+                top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+            }
+            const RowScale s(top);
+            auto write = [&](auto vec) {
+#pragma unroll 2
+                for (int c = 8 * t; c < x_stride - 16; c += 8 * T) {
+                    float v[8];
+                    int q[8];
+                    load8<E, decltype(vec)::value>(x, c, p.K, v);
+                    round_all(v, s, q);
+                    *reinterpret_cast<uint2*>(xq + m * x_stride + c) = make_uint2(pack4(q, 0), pack4(q, 4));
+                }
+            };
+            if (p.wide_x) write(std::true_type{});
+            else write(std::false_type{});
+            if (t == 0) scales[m] = s.scale;
+        }
+        __syncthreads();
+    }
+
+    i32x16 acc[FM];
+#pragma unroll
+    for (int h = 0; h < FM; ++h) acc[h] = i32x16{};
+    const char* xrow = xq + min(l32, p.M - 1) * x_stride;  // a column past the rows is not written
+    auto step = [&](auto last, char* ring, int i) {  // last: k may end in this step
+        const int k0 = k_of(i);
+        const char* from = ring + wave * STEP;
+        asm volatile("" ::: "memory");
+        constexpr int n = (S - 1) * L;
+        static_assert(n < 64, "the counter's range");
+        __builtin_amdgcn_s_waitcnt((n & 15) | (n >> 4) << 14 | 7 << 4 | 15 << 8);  // this step's loads have landed
+        asm volatile("" ::: "memory");
+        i32x4 a[4], b[4][FM];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int at = 16 * ((2 * s + g) ^ (l32 & 7));
+            a[s] = *reinterpret_cast<const i32x4*>(from + l32 * BK + at);
+#pragma unroll
+            for (int h = 0; h < FM; ++h)
+                b[s][h] = FUSED ? *reinterpret_cast<const i32x4*>(xrow + min(k0, x_stride - 16 - BK) + 32 * s + 16 * g)
+                                : *reinterpret_cast<const i32x4*>(from + (BN + 32 * h + l32) * BK + at);
+        }
+        if (!FUSED && decltype(last)::value && k0 + BK > p.K) {  // the last piece's bytes behind the end
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int h = 0; h < FM; ++h) b[s][h] = first_bytes(b[s][h], p.K - (k0 + 32 * s + 16 * g));
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // read: the buffer is free
+        asm volatile("" ::: "memory");
+        load(ring, k_of(i + S));
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int h = 0; h < FM; ++h) acc[h] = mfma32x32x32i8(a[s], b[s][h], acc[h]);
+    };
+    const std::false_type whole;
+    const std::true_type last;
+    const int steps = (p.K - BK * wave + NEXT - 1) / NEXT;  // 0 or less: none
+    int i = 0;
+    for (; i + S <= rounds; i += S) {
+        step(whole, r0, i);
+        step(whole, r1, i + 1);
+        step(whole, r2, i + 2);
+        if constexpr (S > 3) step(whole, r3, i + 3);
+    }
+    if (i < steps) step(last, r0, i);
+    if (i + 1 < steps) step(last, r1, i + 1);
+    if (i + 2 < steps) step(last, r2, i + 2);
+    if constexpr (S > 3)
+        if (i + 3 < steps) step(last, r3, i + 3);
+
     __syncthreads();
-    for (int i = threadIdx.x; i < R * MT * 64; i += 64 * NW) {
-        const int rt = i >> 6, r = rt / MT, t = rt % MT, m = 16 * t + (i & 15), n = n0 + 16 * r + 4 * ((i >> 4) & 3);
-        i32x4 v = sums[0][rt][i & 63];
+    int* sums = reinterpret_cast<int*>(r0);  // [NW][16 FM][64]
+    static_assert(STEP >= 16 * FM * 64 * 4, "the sums fit in a buffer");
 #pragma unroll
-        for (int k = 1; k < NW; ++k) v += sums[k][rt][i & 63];
-        if (m < p.M && n < p.N) finish4<E>(p, m, n, v, p.sx[m]);
+    for (int h = 0; h < FM; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[((wave * FM + h) * 16 + r) * 64 + lane] = acc[h][r];
+    __syncthreads();
+    for (int i = wave; i < 4 * FM; i += NW) {
+        const int h = i >> 2, j = i & 3;
+        i32x4 v = {};
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] += sums[((w * FM + h) * 16 + 4 * j + r) * 64 + lane];
+        const int m = 32 * h + l32, n = n0 + 8 * j + 4 * g;
+        if (m < p.M && n < p.N) finish4<E>(p, m, n, v, FUSED ? scales[m] : p.sx[m]);
     }
 }
 
-GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K) {
+// K ranges are whole steps of any kernel.
+constexpr int kI8Step = 128;
+
+GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
     GemmI8Plan plan;
-    if (M <= kI8FewRows) {
+    plan.kchunk = (int)((K + kI8Step - 1) / kI8Step * kI8Step);
+    auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+    const int64_t steps = (K + kI8Step - 1) / kI8Step;
+    // Few rows: where their kernel is at most one workgroup a CU and no row too long for one (us, its and tiles of 64):
+    // 32 x 4096 x 4096 6.9 and 9.6, 8 x 8192 x 8192 13.5 and 14.0; but 32 x 16384 x 4096 19 and 12.9,
+    // 32 x 4096 x 16384 21 and 15.2.
+    if (M <= 64 && (N + 31) / 32 <= 256 && steps <= 64) {
         plan.kind = GemmI8Plan::kRows;
+        plan.fused = !quantised && M * K <= 16384 && M <= 32;
         return plan;
     }
-    plan.kind = M * N >= (int64_t)256 * 256 * 192 ? GemmI8Plan::kLarge : GemmI8Plan::kMedium;
-    const int64_t tile = plan.kind == GemmI8Plan::kLarge ? 256 : 128;
-    const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
-    const int64_t steps = (K + kBK - 1) / kBK;
-    if (plan.kind == GemmI8Plan::kMedium) {
-        const int64_t want = std::min<int64_t>(512 / std::max<int64_t>(tiles, 1), steps / 4);
-        plan.ksplit = (int)std::max<int64_t>(1, std::min<int64_t>(want, 8));
+    const int64_t t256 = tiles(256), rounds = (t256 + 255) / 256;
+    if (steps >= 16 && t256 * 10 >= rounds * 256 * 7) {
+        plan.kind = GemmI8Plan::k256;
+    } else if (tiles(128) >= 256) {
+        plan.kind = GemmI8Plan::k128;
+    } else {
+        plan.kind = GemmI8Plan::k64;
+        plan.deep = tiles(64) <= 512 && steps >= 16;
+        const int64_t ks = std::min<int64_t>(384 / tiles(64), steps / 8);
+        if (ks > 1 && steps * (ks - 1) > 24 * ks) {
+            plan.kchunk = (int)((steps + ks - 1) / ks * kI8Step);
+            plan.ksplit = (int)((K + plan.kchunk - 1) / plan.kchunk);
+        }
     }
-    plan.kchunk = (int)((steps + plan.ksplit - 1) / plan.ksplit * kBK);
-    plan.ksplit = (int)((K + plan.kchunk - 1) / plan.kchunk);
     return plan;
 }
 
-template <typename E, int BN, int BM, int WN, int WM, bool SPLIT>
+template <typename E, int BN, int BM, int WN, int WM, int BK, int S, bool SPLIT>
 static void launch_tiles(GemmI8Params& p, hipStream_t s) {
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
     p.items = p.tiles_m * p.tiles_n * p.ksplit;
-    hipLaunchKernelGGL((gemm_i8_kernel<E, BN, BM, WN, WM, SPLIT>), dim3((unsigned)((p.items + 7) / 8 * 8)),
+    hipLaunchKernelGGL((gemm_i8_kernel<E, BN, BM, WN, WM, BK, S, SPLIT>), dim3((unsigned)((p.items + 7) / 8 * 8)),
                        dim3(64 * WN * WM), 0, s, p);
 }
 
@@ -291,23 +506,28 @@ template <typename E>
 static int launch_t(GemmI8Params p, const GemmI8Plan& plan, hipStream_t s) {
     p.ksplit = plan.ksplit;
     p.kchunk = plan.kchunk;
-    p.last_piece = (p.K - 1) / 16 * 16;
     if (plan.kind == GemmI8Plan::kRows) {
-        const dim3 grid((unsigned)((p.N + 15) / 16));
-        auto go = [&](auto mt) {
-            hipLaunchKernelGGL((gemm_i8_rows_kernel<E, decltype(mt)::value, 1, 4>), grid, dim3(256), 0, s, p);
-        };
-        if (p.M <= 16) go(std::integral_constant<int, 1>{});
-        else if (p.M <= 32) go(std::integral_constant<int, 2>{});
-        else go(std::integral_constant<int, 4>{});
-    } else if (plan.kind == GemmI8Plan::kLarge) {
-        launch_tiles<E, 256, 256, 2, 4, false>(p, s);
+        const dim3 grid((unsigned)((p.N + 31) / 32)), block(64 * kRowsWaves);
+        if (plan.fused) {
+            const size_t lds = (size_t)p.M * (((p.K + 127) & ~127) + 16);
+            hipLaunchKernelGGL((gemm_i8_rows_kernel<E, 1, 4, true>), grid, block, lds, s, p);
+        } else if (p.M <= 32) {
+            hipLaunchKernelGGL((gemm_i8_rows_kernel<E, 1, 4, false>), grid, block, 0, s, p);
+        } else {
+            hipLaunchKernelGGL((gemm_i8_rows_kernel<E, 2, 3, false>), grid, block, 0, s, p);
+        }
+    } else if (plan.kind == GemmI8Plan::k256) {
+        launch_tiles<E, 256, 256, 2, 4, 128, 2, false>(p, s);
+    } else if (plan.kind == GemmI8Plan::k128) {
+        launch_tiles<E, 128, 128, 2, 2, 128, 2, false>(p, s);
     } else if (p.ksplit > 1) {
-        launch_tiles<E, 128, 128, 2, 2, true>(p, s);
+        launch_tiles<E, 64, 64, 2, 2, 128, 4, true>(p, s);
         hipLaunchKernelGGL((gemm_i8_join_kernel<E>), dim3((unsigned)(((int64_t)p.M * (p.ldp / 4) + 255) / 256)),
                            dim3(256), 0, s, p);
+    } else if (plan.deep) {
+        launch_tiles<E, 64, 64, 2, 2, 128, 4, false>(p, s);
     } else {
-        launch_tiles<E, 128, 128, 2, 2, false>(p, s);
+        launch_tiles<E, 64, 64, 2, 2, 128, 2, false>(p, s);
     }
     return (int)hipGetLastError();
 }

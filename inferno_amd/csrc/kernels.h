@@ -472,15 +472,19 @@ struct GemmI8Params {
     // set by the launcher
     int tiles_m, tiles_n, items;
     int ksplit, kchunk;
-    int last_piece;        // k of a row's last 16-byte piece
+    // a plan that is fused takes x as it is instead of x and sx
+    const void* xf;        // [M, K] in y's type, row stride ldxf
+    int64_t ldxf;
+    int wide_x;            // rows of xf allow loads of four elements
 };
 struct GemmI8Plan {
-    enum Kind { kRows, kMedium, kLarge } kind = kRows;
-    int ksplit = 1, kchunk = 0;
+    enum Kind { kRows, k64, k128, k256 } kind = kRows;  // few rows, or tiles of so many rows and columns
+    int ksplit = 1, kchunk = 0;  // K ranges; more than one need ksplit * M * ldp sums of workspace
+    bool fused = false;          // x is quantised by the product's kernel
+    bool deep = false;           // tiles of 64: loads three steps ahead
 };
-constexpr int kI8FewRows = 64;
-// K ranges per tile; more than one needs ksplit * M * ldp sums of workspace.
-GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K);
+// quantised: x is in 8 bits already.
+GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised);
 int launch_gemm_i8(const GemmI8Params& p, const GemmI8Plan& plan, int bf16, hipStream_t s);
 
 // ---- a paged key-value cache in 4 bits (paged4.hip) -----------------------------

@@ -175,7 +175,8 @@ def test_results_over_what_is_read():
     far = 0x10000000
     for kw in (dict(w=far), dict(w=far - 31 * 64 - 48), dict(sw=far + 900), dict(b=far - 64)):
         assert gemm(y=far, **kw) == 3 and linear(y=far, **kw) == 3
-    assert gemm(y=far, x=far + 1008) == 3 and gemm(y=far, sx=far - 28) == 3 and linear(y=far, ws=far + 512) == 3
+    assert gemm(y=far, x=far + 1008) == 3 and gemm(y=far, sx=far - 28) == 3
+    assert linear(y=far, x=far + 992) == 3 and linear(M=100, y=far, ws=far + 512) == 3
     assert quantize(q=FAKE + 2032) == 3 and quantize(s=FAKE - 28) == 3 and quantize(s=FAKE + 2044, t=1) == 3
 
 
@@ -187,7 +188,9 @@ def test_product_arguments_of_one_form():
     for M, N, K in ((1, 2304, 768), (300, 500, 4096), (5000, 5000, 100)):
         args = dict(M=M, N=N, K=K, ldx=K + 12, ldw=-(-K // 16) * 16, ldy=N)
         assert ia.lib().inf_linear_i8_workspace(M, N, K, ctypes.byref(n)) == 0 and n.value % 256 == 0
-        assert n.value >= M * K + 4 * M
+        assert n.value >= M * K + 4 * M or (M == 1 and n.value == 0)  # one row needs none
+        if not n.value:
+            continue
         assert linear(**args, ws=None, n=n.value) == 6
         assert linear(**args, ws=FAKE, n=n.value - 1) == 6
         assert linear(**args, ws=FAKE + 16, n=n.value) == 7
