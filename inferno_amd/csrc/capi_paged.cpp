@@ -454,11 +454,14 @@ int inf_kv4_read(const inf_paged_kv4* cache, const int32_t* first, int T, void* 
         (st = check_apart(sk, cache->rows, cache->heads, T, cache->D)) ||
         (st = check_apart(sv, cache->rows, cache->heads, T, cache->D)))
         return st;
-    if ((int64_t)T * cache->heads * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    // a workgroup takes at least 32 positions of a head
+    if ((int64_t)T * cache->heads * cache->D > kMaxBlocks || (T / 32 + 1) * (int64_t)cache->heads * 256 > kMaxThreads)
+        return INF_ERR_BAD_SHAPE;
     p.k = k; p.v = v;
     p.sk = view(sk); p.sv = view(sv);
     p.first = first;
     p.Tn = T;
+    p.wide = check_view(k, sk, es, 16) == INF_OK && check_view(v, sv, es, 16) == INF_OK;
     return hip_status(inf::launch_kv4_read(p, dt == INF_BF16, (hipStream_t)stream));
 }
 

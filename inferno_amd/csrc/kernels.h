@@ -519,6 +519,7 @@ struct Kv4ReadParams {
     View4 sk, sv;
     const int32_t* first;  // [rows] first position, or null: 0
     int Tn;
+    int wide;              // 16-byte rows (bf16)
 };
 
 struct Kv4DecodeParams {
@@ -532,6 +533,7 @@ struct Kv4DecodeParams {
     float* part;           // workspace [parts, Hq, D]: unnormalised o
     float* stats;          // workspace [parts, Hq, 2]: maximum (log2 domain) and sum
     int32_t* first;        // workspace [rows + blocks]: a row's first step in its block; the blocks' steps
+    int q_at;              // place of q's parts in LDS (set by the launcher)
 };
 // Keys that a workgroup takes per step.
 constexpr int kv4_step(int D) { return D == 128 ? 256 : 512; }

@@ -37,9 +37,28 @@ __device__ __forceinline__ int page_of(const Paged4View& c, const int32_t* table
     return (unsigned)p < (unsigned)c.n_pages ? p : -1;
 }
 
-// 2^(byte - 127), NaN for 255.
-__device__ __forceinline__ float block_scale(uint32_t byte) {
-    return __uint_as_float(byte == 255 ? 0x7fc00000u : byte << 23);
+// Byte i of a word as the conversions' scale, 2^(byte - 127), NaN for 255: they read its exponent alone, so that the
+// word's other bits may stay.
+template <int I = 0>
+__device__ __forceinline__ float block_scale(uint32_t word) {
+    return __uint_as_float(I < 3 ? word << (23 - 8 * I) : word >> 1);
+}
+
+// Loads of a tile's rows: scalar bases and the lanes' 32-bit offsets, past the caches.  (Through pointers, the compiler
+// takes every address as a sum of vectors.)
+constexpr int kNt = 2;
+template <int BYTES>
+__device__ __forceinline__ auto load_nt(__amdgpu_buffer_rsrc_t r, uint32_t at) {
+    if constexpr (BYTES == 16)
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, kNt));
+    else if constexpr (BYTES == 8)
+        return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)at, 0, kNt));
+    else if constexpr (BYTES == 4)
+        return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, kNt);
+    else if constexpr (BYTES == 2)
+        return (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, kNt);
+    else
+        return (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)at, 0, kNt);
 }
 
 // Eight channels of a block: four bytes.
@@ -62,17 +81,23 @@ __device__ __forceinline__ void store1(E* dst, float v) {
 }  // namespace
 
 // ============================================================================
-// Append and read: a thread takes eight channels of a token's key and of its value, four neighbouring threads a
-// block; channels fastest, then heads, then tokens, as a projection's output lies.  Bound by HBM.
+// Append: a thread takes eight channels of a token's key and of its value, four neighbouring threads a block; channels
+// fastest, then heads, then tokens, as a projection's output lies.  The values are loaded while the token's page is looked up.
 // ============================================================================
 namespace {
 
+struct Raw8 {
+    f32x4 a, b;
+};
+template <typename E>
+__device__ __forceinline__ Raw8 raw8(const E* src) {
+    return {ld4(src), ld4(src + 4)};
+}
 struct Encoded {
     uint32_t codes, byte;
 };
-template <typename E>
-__device__ __forceinline__ Encoded encode8(const E* src) {
-    const f32x4 a = ld4(src), b = ld4(src + 4);
+__device__ __forceinline__ Encoded encode8(const Raw8& x) {
+    const f32x4 a = x.a, b = x.b;
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -90,22 +115,6 @@ __device__ __forceinline__ Encoded encode8(const E* src) {
     return {q, byte};
 }
 
-template <typename E>
-__device__ __forceinline__ void store8(E* dst, uint32_t codes, float scale) {
-    f32x4 v[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bf16x2 x = i == 0 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)
-                       : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)
-                       : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)
-                                : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
-        v[i >> 1][2 * (i & 1)] = (float)x[0];
-        v[i >> 1][2 * (i & 1) + 1] = (float)x[1];
-    }
-    st4(dst, v[0]);
-    st4(dst + 4, v[1]);
-}
-
 }  // namespace
 
 template <int D, typename E>
@@ -117,13 +126,14 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendParams p) {
     const int t = th / p.c.heads, h = th - t * p.c.heads;
     const int count = p.counts ? min(p.counts[row], p.Tn) : p.Tn;
     if (t >= count) return;  // a block's threads stay together
+    const Raw8 kx = raw8((const E*)p.k + row * p.sk.b + h * p.sk.h + t * p.sk.t + 8 * c);
+    const Raw8 vx = raw8((const E*)p.v + row * p.sv.b + h * p.sv.h + t * p.sv.t + 8 * c);
     const int64_t slot = (int64_t)p.c.lens[row] - count + t;
     if (slot < 0 || slot >= p.c.cap()) return;
     const int page = page_of(p.c, p.c.table + row * p.c.table_stride, (int)slot);
     if (page < 0) return;
     const int at = (int)slot & ((1 << p.c.page_shift) - 1);
-    const Encoded k = encode8((const E*)p.k + row * p.sk.b + h * p.sk.h + t * p.sk.t + 8 * c);
-    const Encoded v = encode8((const E*)p.v + row * p.sv.b + h * p.sv.h + t * p.sv.t + 8 * c);
+    const Encoded k = encode8(kx), v = encode8(vx);
     *reinterpret_cast<uint32_t*>(p.c.k + page * p.c.sk.b + h * p.c.sk.h + at * p.c.sk.t + 4 * c) = k.codes;
     *reinterpret_cast<uint32_t*>(p.c.v + page * p.c.sv.b + h * p.c.sv.h + at * p.c.sv.t + 4 * c) = v.codes;
     if (c % 4 == 0) {
@@ -132,32 +142,76 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendParams p) {
     }
 }
 
-// Positions first[row] + t as dense rows; zeros outside the row, NaN where its table names no page of the pool's.
-template <int D, typename E>
-__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadParams p) {
-    constexpr int P = D / 8;
-    const int row = blockIdx.y;
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    const int ht = i / P, c = i % P;
-    const int h = ht / p.Tn, t = ht - h * p.Tn;
-    if (h >= p.c.heads) return;
-    const int64_t slot = (p.first ? (int64_t)p.first[row] : 0) + t;
-    uint32_t k = 0, v = 0;
-    float ks = 1.f, vs = 1.f;
-    if (slot >= 0 && slot < p.c.lens[row] && slot < p.c.cap()) {
-        const int page = page_of(p.c, p.c.table + row * p.c.table_stride, (int)slot);
-        if (page < 0) {
-            ks = vs = __builtin_nanf("");
-        } else {
-            const int at = (int)slot & ((1 << p.c.page_shift) - 1);
-            k = *reinterpret_cast<const uint32_t*>(p.c.k + page * p.c.sk.b + h * p.c.sk.h + at * p.c.sk.t + 4 * c);
-            v = *reinterpret_cast<const uint32_t*>(p.c.v + page * p.c.sv.b + h * p.c.sv.h + at * p.c.sv.t + 4 * c);
-            ks = block_scale(p.c.ks[page * p.c.sks.b + h * p.c.sks.h + c / 4 * p.c.sks.t + at]);
-            vs = block_scale(p.c.vs[page * p.c.svs.b + h * p.c.svs.h + c / 4 * p.c.svs.t + at]);
+// ============================================================================
+// Read: positions first[row] + t as dense rows; zeros outside the row, NaN where its table names no page of the pool's.  A
+// thread takes CH channels of a key and of its value, one store of 16 bytes each (8 where bf16 rows are aligned to that
+// only), past the caches and in the results' order.
+// ============================================================================
+namespace {
+
+template <int CH>
+__device__ __forceinline__ uint32_t codes_of(const uint8_t* row, int c) {
+    if constexpr (CH == 8)
+        return *reinterpret_cast<const uint32_t*>(row + 4 * c);
+    else
+        return *reinterpret_cast<const uint16_t*>(row + 2 * c);
+}
+
+template <int CH, typename E>
+__device__ __forceinline__ void store_ch(E* dst, uint32_t codes, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0),
+                 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
+    if constexpr (sizeof(E) == 4) {
+        __builtin_nontemporal_store(f32x4{(float)a[0], (float)a[1], (float)b[0], (float)b[1]},
+                                    reinterpret_cast<f32x4*>(dst));
+    } else if constexpr (CH == 8) {
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, to_bf16(codes, scale)), reinterpret_cast<u32x4*>(dst));
+    } else {
+        __builtin_nontemporal_store(u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)},
+                                    reinterpret_cast<u32x2*>(dst));
+    }
+}
+
+}  // namespace
+
+constexpr int kReadPer = 4;  // positions of a thread, all of whose loads are under way together
+
+template <int D, typename E, int CH>
+__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadParams p, int blocks) {
+    constexpr int P = D / CH, N = 256 / P;
+    const int row = blockIdx.y, h = blockIdx.x / blocks;
+    const int c = threadIdx.x % P, block = c * CH / 32;
+    const int t0 = (blockIdx.x - h * blocks) * (N * kReadPer) + threadIdx.x / P;
+    const int64_t first = p.first ? (int64_t)p.first[row] : 0, len = min((int64_t)p.c.lens[row], p.c.cap());
+    const int32_t* table = p.c.table + row * p.c.table_stride;
+    int page[kReadPer];
+#pragma unroll
+    for (int u = 0; u < kReadPer; ++u) {
+        const int64_t slot = first + t0 + N * u;
+        const bool in = t0 + N * u < p.Tn && slot >= 0 && slot < len;
+        page[u] = in ? page_of(p.c, table, (int)slot) : -2;  // -1: no page of the pool's, -2: outside the row
+    }
+    uint32_t k[kReadPer], v[kReadPer];
+    float ks[kReadPer], vs[kReadPer];
+#pragma unroll
+    for (int u = 0; u < kReadPer; ++u) {
+        const int at = (int)(first + t0 + N * u) & ((1 << p.c.page_shift) - 1);
+        k[u] = v[u] = 0;
+        ks[u] = vs[u] = page[u] == -1 ? __builtin_nanf("") : 1.f;
+        if (page[u] >= 0) {
+            k[u] = codes_of<CH>(p.c.k + page[u] * p.c.sk.b + h * p.c.sk.h + at * p.c.sk.t, c);
+            v[u] = codes_of<CH>(p.c.v + page[u] * p.c.sv.b + h * p.c.sv.h + at * p.c.sv.t, c);
+            ks[u] = block_scale(p.c.ks[page[u] * p.c.sks.b + h * p.c.sks.h + block * p.c.sks.t + at]);
+            vs[u] = block_scale(p.c.vs[page[u] * p.c.svs.b + h * p.c.svs.h + block * p.c.svs.t + at]);
         }
     }
-    store8((E*)p.k + row * p.sk.b + h * p.sk.h + t * p.sk.t + 8 * c, k, ks);
-    store8((E*)p.v + row * p.sv.b + h * p.sv.h + t * p.sv.t + 8 * c, v, vs);
+#pragma unroll
+    for (int u = 0; u < kReadPer; ++u) {
+        const int t = t0 + N * u;
+        if (t >= p.Tn) return;
+        store_ch<CH>((E*)p.k + row * p.sk.b + h * p.sk.h + t * p.sk.t + CH * c, k[u], ks[u]);
+        store_ch<CH>((E*)p.v + row * p.sv.b + h * p.sv.h + t * p.sv.t + CH * c, v[u], vs[u]);
+    }
 }
 
 namespace {
@@ -186,10 +240,16 @@ int launch_kv4_append(const Kv4AppendParams& p, int bf16, hipStream_t s) {
 }
 
 int launch_kv4_read(const Kv4ReadParams& p, int bf16, hipStream_t s) {
-    const int64_t n = (int64_t)p.Tn * p.c.heads * (p.c.D / 8);
-    const dim3 grid((unsigned)((n + 255) / 256), (unsigned)p.c.rows);
+    const int ch = bf16 && p.wide ? 8 : 4, per = 256 / (p.c.D / ch) * kReadPer;
+    const int blocks = (p.Tn + per - 1) / per;
+    const dim3 grid((unsigned)(blocks * p.c.heads), (unsigned)p.c.rows);
     return by_type(p.c.D, bf16, [&](auto d, auto e) {
-        hipLaunchKernelGGL((kv4_read_kernel<decltype(d)::value, decltype(e)>), grid, dim3(256), 0, s, p);
+        constexpr int D = decltype(d)::value;
+        using E = decltype(e);
+        if (ch == 8)
+            hipLaunchKernelGGL((kv4_read_kernel<D, E, sizeof(E) == 2 ? 8 : 4>), grid, dim3(256), 0, s, p, blocks);
+        else
+            hipLaunchKernelGGL((kv4_read_kernel<D, E, 4>), grid, dim3(256), 0, s, p, blocks);
     });
 }
 
@@ -205,6 +265,12 @@ namespace {
 
 constexpr int kKv4PerCu = 3;  // workgroups of a CU: what the registers allow
 
+// What a wave keeps in LDS where its scores pass through it.
+constexpr int kv4_wave_floats(int D, bool f32, int HB) {
+    const int keys = kv4_step(D) / 4;
+    return HB == 16 ? 0 : (f32 ? 3 : 1) * HB * keys + (f32 ? 3 : 2) * HB * keys / 2 + 16;
+}
+
 template <int D>
 __device__ __forceinline__ int kv4_steps(int len, int max_len) {
     constexpr int step = kv4_step(D);
@@ -213,7 +279,11 @@ __device__ __forceinline__ int kv4_steps(int len, int max_len) {
 
 }  // namespace
 
-template <int D, typename E>
+// HB: 16, or 1, 2, 4 or 8 (bf16), at least as many as there are query heads.  A product's result has heads along the
+// lanes, so that with few of them most lanes' softmax would be for nothing: below 16, the wave's scores pass through LDS to
+// all lanes, 64 / HB of them a head, and the probabilities back.  And the columns that are left take the other bf16
+// parts of queries and probabilities, part k of head i in column k HB + i: one product instead of two or three.
+template <int D, typename E, int HB>
 __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodeParams p) {
     constexpr bool F = sizeof(E) == 4;
     constexpr int PARTS = F ? 3 : 1;      // of q
@@ -222,7 +292,13 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
     constexpr int NK = D / 32;            // words of a key row per lane: products of a tile
     constexpr int VD = D / 16;            // columns of a value row per lane
     constexpr int LD = D + 4;
-    extern __shared__ __attribute__((aligned(16))) float lds[];  // o [4][heads][LD], then m, l [4][16]
+    constexpr int KEYS = 16 * T;          // of a wave's step
+    constexpr int LPH = 64 / HB, NV = KEYS / LPH;  // HB < 16: lanes of a head, keys of a lane
+    constexpr int PP = F ? 3 : 2;         // bf16 parts of a probability
+    static_assert(HB == 16 || PP * HB <= 16, "a column for every part");
+    // o [4][heads][LD], then m, l [4][16]; before that, HB < 16: every wave's scores [PARTS][HB][KEYS], parts of
+    // probabilities [PP][HB][KEYS] and factors [HB].  From q_at on, fp32: parts of q [3][heads, or HB][D].
+    extern __shared__ __attribute__((aligned(16))) float lds[];
 
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
     const int ht = p.head_tiles;
@@ -279,44 +355,48 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
     const uint8_t* V = p.c.v + h * p.c.sv.h;
     const uint8_t* KS = p.c.ks + h * p.c.sks.h;
     const uint8_t* VS = p.c.vs + h * p.c.svs.h;
-    const int k_at = col * (int)p.c.sk.t + g * (D / 8), ks_at = g * D / 128 * (int)p.c.sks.t + col;
-    const int v_at = 4 * g * (int)p.c.sv.t + col * (VD / 2), vs_at = col * D / 512 * (int)p.c.svs.t + 4 * g;
+    const uint32_t k_at = col * (uint32_t)p.c.sk.t + g * (D / 8), ks_at = g * D / 128 * (uint32_t)p.c.sks.t + col;
+    uint32_t v_at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * (uint32_t)p.c.sv.t + col * (VD / 2);
+    const uint32_t vs_at = col * D / 512 * (uint32_t)p.c.svs.t + 4 * g;
     uint32_t kr[T][NK], ksr[T], vr[T][4], vsr[T];
+    const int qn = HB == 16 ? gn : HB;
+    float* mine = lds + wave * kv4_wave_floats(D, F, HB);
 
     for (;;) {  // the rows of the share
         const int row = row0 + r, s0 = step - begin, s1 = min(stop, end) - begin;
         const int32_t* table = p.c.table + row * p.c.table_stride;
         const int base0 = s0 * STEP + 16 * T * wave;
         const int len = __builtin_amdgcn_readlane(mylen, r);
-        int next[T] = {};
-        auto read_pages = [&](int base) {
-#pragma unroll
-            for (int t = 0; t < T; ++t)
-                next[t] = table[min(__builtin_amdgcn_readfirstlane(base + 16 * t) >> p.c.page_shift, last_page)];
-        };
-        read_pages(base0);
+        // Lane t: the page of the step's tile t, read a step ahead (behind the end, where the table may hold anything, it
+        // is not used), and then the places of the tile's rows and scales, which go to scalar registers from there.
+        const int tile_key = 16 * (lane & (T - 1));
+        auto read_pages = [&](int base) { return table[min((base + tile_key) >> p.c.page_shift, last_page)]; };
+        int next = read_pages(base0);
         const int j1 = min(len, s1 * STEP);
 
-        // Q^T: column = head, the channels that a key's words have
-        bf16x8 qf[NK][PARTS];
-        {
+        // Q^T: column = head, the channels that a key's words have.  fp32: its parts lie in LDS, [3][heads][D] for all waves
+        // (in registers they would be 48 at D = 128: spills).
+        bf16x8 qf[F ? 1 : NK];
+        if constexpr (F) {
+            __bf16* dst = reinterpret_cast<__bf16*>(lds + p.q_at);
+            for (int i = tid; i < gn * (D / 8); i += 256) {
+                const int head = i / (D / 8), d = i % (D / 8) * 8;
+                const E* q = (const E*)p.q + row * p.sq.b + (int64_t)(h * p.G + g0 + head) * p.sq.h + d;
+                const Bf3x8 x = split3(ld4(q), ld4(q + 4));
+                *reinterpret_cast<bf16x8*>(dst + head * D + d) = x.h;
+                *reinterpret_cast<bf16x8*>(dst + (qn + head) * D + d) = x.m;
+                *reinterpret_cast<bf16x8*>(dst + (2 * qn + head) * D + d) = x.l;
+            }
+            __syncthreads();
+        } else {
             const E* q = (const E*)p.q + row * p.sq.b + (int64_t)(h * p.G + g0 + min(col, gn - 1)) * p.sq.h + g * (D / 4);
 #pragma unroll
             for (int s = 0; s < NK; ++s) {
-                const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-                const f32x4 a = col < gn ? ld4(q + 8 * s) : zero, b = col < gn ? ld4(q + 8 * s + 4) : zero;
-                if constexpr (F) {
-                    const Bf3x8 x = split3(a, b);
-                    qf[s][0] = x.h;
-                    qf[s][1] = x.m;
-                    qf[s][2] = x.l;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        qf[s][0][i] = (__bf16)a[i];
-                        qf[s][0][4 + i] = (__bf16)b[i];
-                    }
-                }
+                const u32x2* src = reinterpret_cast<const u32x2*>(q + 8 * s);
+                const u32x2 a = src[0], b = src[1];
+                qf[s] = __builtin_bit_cast(bf16x8, u32x4{a[0], a[1], b[0], b[1]});
             }
         }
 
@@ -326,92 +406,174 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
         float m = -INFINITY, l = 0.f;
         bool bad = false;
         for (int base = base0; base < j1; base += STEP) {
+            uint64_t places[4];
+            {
+                const bool in = (unsigned)next < (unsigned)p.c.n_pages;
+                bad |= !in && base + tile_key < j1;
+                const uint32_t page = in ? next : 0, at = (base + tile_key) & mask;
+                places[0] = (uint64_t)K + page * (uint64_t)p.c.sk.b + (uint64_t)at * (uint32_t)p.c.sk.t;
+                places[1] = (uint64_t)V + page * (uint64_t)p.c.sv.b + (uint64_t)at * (uint32_t)p.c.sv.t;
+                places[2] = (uint64_t)KS + page * (uint64_t)p.c.sks.b + at;
+                places[3] = (uint64_t)VS + page * (uint64_t)p.c.svs.b + at;
+            }
+            if (base + STEP < j1) next = read_pages(base + STEP);
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const bool in = (unsigned)next[t] < (unsigned)p.c.n_pages;
-                bad |= !in && base + 16 * t < j1;
-                const int64_t page = in ? next[t] : 0;
-                const int at = __builtin_amdgcn_readfirstlane(base + 16 * t) & mask;
-                const uint8_t* kp = K + page * p.c.sk.b + at * p.c.sk.t + k_at;
-                if constexpr (NK == 4) {
-                    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kp));
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) kr[t][s] = x[s];
-                } else if constexpr (NK == 2) {
-                    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(kp));
-                    kr[t][0] = x[0];
-                    kr[t][1] = x[1];
+                auto rows = [&](int i, uint32_t bytes) {
+                    const uint64_t a = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(places[i] >> 32), t) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)places[i], t);
+                    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(a), (short)0, (int)bytes, 0x00020000);
+                };
+                const auto kp = rows(0, 15 * (uint32_t)p.c.sk.t + D / 2);
+                const auto k = load_nt<4 * NK>(kp, k_at);
+                if constexpr (NK == 1) {
+                    kr[t][0] = k;
                 } else {
-                    kr[t][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(kp));
-                }
-                ksr[t] = KS[page * p.c.sks.b + at + ks_at];
-                const uint8_t* vp = V + page * p.c.sv.b + at * p.c.sv.t + v_at;
 #pragma unroll
-                for (int r = 0; r < 4; ++r, vp += p.c.sv.t) {
-                    if constexpr (VD == 8)
-                        vr[t][r] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vp));
-                    else if constexpr (VD == 4)
-                        vr[t][r] = __builtin_nontemporal_load(reinterpret_cast<const uint16_t*>(vp));
-                    else
-                        vr[t][r] = __builtin_nontemporal_load(vp);
+                    for (int s = 0; s < NK; ++s) kr[t][s] = k[s];
                 }
-                vsr[t] = *reinterpret_cast<const uint32_t*>(VS + page * p.c.svs.b + at + vs_at);
+                const auto vp = rows(1, 15 * (uint32_t)p.c.sv.t + D / 2);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vr[t][r] = load_nt<VD / 2>(vp, v_at[r]);
+                const auto ks = rows(2, (D / 32 - 1) * (uint32_t)p.c.sks.t + 16),
+                           vs = rows(3, (D / 32 - 1) * (uint32_t)p.c.svs.t + 16);
+                ksr[t] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(ks, (int)ks_at, 0, 0);
+                vsr[t] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(vs, (int)vs_at, 0, 0);
             }
-            if (base + STEP < j1) read_pages(base + STEP);
             __builtin_amdgcn_sched_barrier(0);  // all of the step's loads before its first product
-            float x[4 * T];
+            f32x4 st[T] = {};
+            const __bf16* qs = reinterpret_cast<const __bf16*>(lds + p.q_at) +
+                               (HB == 16 ? min(col, gn - 1) : min(col, 3 * HB - 1)) * D + g * (D / 4);
+            constexpr int QP = HB == 16 ? PARTS : 1;  // products a word
 #pragma unroll
-            for (int t = 0; t < T; ++t) {
-                f32x4 st = {0.f, 0.f, 0.f, 0.f};
-                const float ks = block_scale(ksr[t]);
+            for (int s = 0; s < NK; ++s) {
+                bf16x8 q[QP];
+                if constexpr (F) {
 #pragma unroll
-                for (int s = 0; s < NK; ++s) {
-                    const bf16x8 k = to_bf16(kr[t][s], ks);
-#pragma unroll
-                    for (int i = PARTS - 1; i >= 0; --i) st = mfma16x16x32bf16(k, qf[s][i], st);
+                    for (int i = 0; i < QP; ++i) q[i] = *reinterpret_cast<const bf16x8*>(qs + i * gn * D + 8 * s);
+                } else {
+                    q[0] = qf[s];
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[4 * t + r] = st[r] * p.cs;
+                for (int t = 0; t < T; ++t) {
+                    const bf16x8 k = to_bf16(kr[t][s], block_scale(ksr[t]));
+#pragma unroll
+                    for (int i = QP - 1; i >= 0; --i) st[t] = mfma16x16x32bf16(k, q[i], st[t]);
+                }
             }
-            if (base + 16 * T > j1) {  // keys behind the end: nothing of what their slots hold counts
+            const bool ends = base + KEYS > j1;  // keys behind the end: nothing of what their slots hold counts
+            if (ends) {
 #pragma unroll
                 for (int i = 0; i < 4 * T; ++i)
                     if (base + 16 * (i >> 2) + 4 * g + (i & 3) >= j1) {
-                        x[i] = -INFINITY;
+                        st[i >> 2][i & 3] = -INFINITY;
                         vr[i >> 2][i & 3] = 0;
                         vsr[i >> 2] = (vsr[i >> 2] & ~(255u << (8 * (i & 3)))) | 127u << (8 * (i & 3));
                     }
             }
+            // x: this lane's scores, then their probabilities: its head's, in the order of the products (HB = 16), or
+            // NV neighbouring keys of head lane / LPH
+            constexpr int NX = HB == 16 ? 4 * T : NV;
+            float x[NX];
+            if constexpr (HB == 16) {
+#pragma unroll
+                for (int i = 0; i < NX; ++i) x[i] = st[i >> 2][i & 3];
+            } else {
+                if (col < PARTS * HB) {
+#pragma unroll
+                    for (int t = 0; t < T; ++t) *reinterpret_cast<f32x4*>(mine + col * KEYS + 16 * t + 4 * g) = st[t];
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                const float* src = mine + min(lane / LPH, gn - 1) * KEYS + lane % LPH * NV;
+#pragma unroll
+                for (int i = 0; i < NX; ++i) {
+                    x[i] = src[i];
+                    if constexpr (F) x[i] += src[HB * KEYS + i] + src[2 * HB * KEYS + i];
+                }
+            }
             float mx = m;
 #pragma unroll
-            for (int i = 0; i < 4 * T; ++i) mx = fmaxf(mx, x[i]);
-            mx = max_xor32(max_xor16(mx));
+            for (int i = 0; i < NX; ++i) mx = fmaxf(mx, x[i]);
+            if constexpr (HB == 16) {
+                mx = max_xor32(max_xor16(mx));
+            } else {
+                if constexpr (LPH >= 2) mx = fmaxf(mx, dpp_mov<0xB1>(mx));
+                if constexpr (LPH >= 4) mx = fmaxf(mx, dpp_mov<0x4E>(mx));
+                if constexpr (LPH >= 8) mx = fmaxf(mx, dpp_mov<0x141>(mx));
+                if constexpr (LPH >= 16) mx = fmaxf(mx, dpp_mov<0x140>(mx));
+                if constexpr (LPH >= 32) mx = max_xor16(mx);
+                if constexpr (LPH >= 64) mx = max_xor32(mx);
+            }
             const float ref = mx == -INFINITY ? 0.f : mx;  // no key above -inf yet: keep everything at 0
-            const float alpha = fast_exp2(m - ref);
+            // differences before the scale: the largest one's is 0 at any magnitude, where a product less a rounded product may
+            // be anything
+            const float alpha = fast_exp2((m - ref) * p.cs);
+            const bool moved = __any(mx != m);
             m = mx;
             l *= alpha;
 #pragma unroll
-            for (int j = 0; j < VD; ++j) acc[j] *= alpha;
-#pragma unroll
-            for (int i = 0; i < 4 * T; ++i) {
-                x[i] = fast_exp2(x[i] - ref);
+            for (int i = 0; i < NX; ++i) {
+                x[i] = fast_exp2((x[i] - ref) * p.cs);
                 l += x[i];
+            }
+            float scale_acc = alpha;
+            __bf16* parts = reinterpret_cast<__bf16*>(mine + PARTS * HB * KEYS);
+            if constexpr (HB < 16) {
+                __bf16* dst = parts + lane / LPH * KEYS + lane % LPH * NV;
+                if constexpr (NV == 1) {
+                    float a = x[0];
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) {
+                        const __bf16 h = (__bf16)a;
+                        dst[k * HB * KEYS] = h;
+                        a -= (float)h;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NX - 1; i += 2) {  // words of two neighbouring keys
+                        float a = x[i], b = x[i + 1];
+#pragma unroll
+                        for (int k = 0; k < PP; ++k) {
+                            const bf16x2 h = {(__bf16)a, (__bf16)b};
+                            *reinterpret_cast<bf16x2*>(dst + k * HB * KEYS + i) = h;
+                            a -= (float)h[0];
+                            b -= (float)h[1];
+                        }
+                    }
+                }
+                float* factors = mine + PARTS * HB * KEYS + PP * HB * KEYS / 2;
+                if (moved && lane % LPH == 0) factors[lane / LPH] = alpha;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if (moved) scale_acc = factors[col % HB];
+            }
+            if (moved) {
+#pragma unroll
+                for (int j = 0; j < VD; ++j) acc[j] *= scale_acc;
             }
 #pragma unroll
             for (int t = 0; t < T; t += 2) {  // 32 keys a product
                 bf16x8 ph, pm, pl;
+                if constexpr (HB == 16) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    ph[i] = (__bf16)x[4 * t + i];
-                    const float rest = x[4 * t + i] - (float)ph[i];
-                    pm[i] = (__bf16)rest;
-                    if constexpr (F) pl[i] = (__bf16)(rest - (float)pm[i]);
+                    for (int i = 0; i < 8; ++i) {
+                        ph[i] = (__bf16)x[4 * t + i];
+                        const float rest = x[4 * t + i] - (float)ph[i];
+                        pm[i] = (__bf16)rest;
+                        if constexpr (F) pl[i] = (__bf16)(rest - (float)pm[i]);
+                    }
+                } else {
+                    // keys 4 g .. of the two tiles; a column past the parts is not used
+                    const __bf16* src = parts + min(col, PP * HB - 1) * KEYS + 16 * t + 4 * g;
+                    const bf16x4 lo = *reinterpret_cast<const bf16x4*>(src), hi = *reinterpret_cast<const bf16x4*>(src + 16);
+                    ph = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 }
                 uint32_t vb[8][VD / 2];  // eight keys' pairs of columns
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t w = vr[t + (i >> 2)][i & 3];
-                    const float vs = block_scale(vsr[t + (i >> 2)] >> (8 * (i & 3)) & 255);
+                    const uint32_t sw = vsr[t + (i >> 2)];
+                    const float vs = (i & 3) == 0 ? block_scale<0>(sw) : (i & 3) == 1 ? block_scale<1>(sw)
+                                   : (i & 3) == 2 ? block_scale<2>(sw) : block_scale<3>(sw);
                     vb[i][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vs, 0));
                     if constexpr (VD >= 4)
                         vb[i][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, vs, 1));
@@ -427,16 +589,33 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
 #pragma unroll
                     for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(vb[2 * i + 1][j >> 1], vb[2 * i][j >> 1], sel);
                     const bf16x8 v = __builtin_bit_cast(bf16x8, a);
-                    if constexpr (F) acc[j] = mfma16x16x32bf16(v, pl, acc[j]);
-                    acc[j] = mfma16x16x32bf16(v, pm, acc[j]);
+                    if constexpr (HB == 16) {
+                        if constexpr (F) acc[j] = mfma16x16x32bf16(v, pl, acc[j]);
+                        acc[j] = mfma16x16x32bf16(v, pm, acc[j]);
+                    }
                     acc[j] = mfma16x16x32bf16(v, ph, acc[j]);
                 }
             }
         }
 
         // Join the waves: lane (col, g) holds head col's o[VD (4 g + r) + j] in acc[j][r].
-        l += shfl_xor(l, 16);
-        l += shfl_xor(l, 32);
+        if constexpr (HB == 16) {
+            l += shfl_xor(l, 16);
+            l += shfl_xor(l, 32);
+        } else {
+            l = group_sum<(LPH < 32 ? LPH : 32)>(l);
+            if constexpr (LPH == 64) l += shfl_xor(l, 32);
+            // the parts' columns (row_shl: lane i <- i + n), the small ones first
+#pragma unroll
+            for (int j = 0; j < VD; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float low = dpp_mov<0x100 + HB>(acc[j][r]);
+                    if constexpr (F) low += dpp_mov<0x100 + 2 * HB>(acc[j][r]);
+                    acc[j][r] += low;
+                }
+            __syncthreads();  // the waves' scores are read
+        }
         if (__any(bad)) l = __builtin_nanf("");
         float* ms = lds + 4 * gn * LD;
         float* ls = ms + 64;
@@ -447,9 +626,9 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
 #pragma unroll
                 for (int j = 0; j < VD; ++j) dst[VD * r + j] = acc[j][r];
         }
-        if (g == 0) {
-            ms[wave * 16 + col] = m;
-            ls[wave * 16 + col] = l;
+        if (HB == 16 ? g == 0 : lane % LPH == 0) {
+            ms[wave * 16 + (HB == 16 ? col : lane / LPH)] = m * p.cs;
+            ls[wave * 16 + (HB == 16 ? col : lane / LPH)] = l;
         }
         __syncthreads();
         for (int i = tid; i < gn * D; i += 256) {
@@ -544,11 +723,24 @@ int kv4_groups(int rows, int heads, int G, int max_len, int D) {
 int launch_attn_decode_kv4(const Kv4DecodeParams& p, int bf16, hipStream_t s) {
     const dim3 grid((unsigned)paged_units(p.c.rows, p.c.heads, p.head_tiles, p.groups),
                     p.groups ? (unsigned)paged_blocks(p.c.rows) : 1u);
-    const size_t lds = (size_t)(4 * std::min(p.G, 16) * (p.c.D + 4) + 128) * sizeof(float);
+    const int heads = std::min(p.G, 16);
     return by_type(p.c.D, bf16, [&](auto d, auto e) {
         constexpr int D = decltype(d)::value;
         using E = decltype(e);
-        hipLaunchKernelGGL((kv4_split_kernel<D, E>), grid, dim3(256), lds, s, p);
+        auto go = [&](auto hb) {
+            constexpr int HB = decltype(hb)::value;
+            constexpr bool F = sizeof(E) == 4;
+            Kv4DecodeParams a = p;
+            a.q_at = std::max(4 * heads * (D + 4) + 128, 4 * kv4_wave_floats(D, F, HB));
+            const size_t lds = (size_t)(a.q_at + (F ? 3 * (HB == 16 ? heads : HB) * D / 2 : 0)) * sizeof(float);
+            hipLaunchKernelGGL((kv4_split_kernel<D, E, HB>), grid, dim3(256), lds, s, a);
+        };
+        using std::integral_constant;
+        if (heads == 1) go(integral_constant<int, 1>{});
+        else if (heads == 2) go(integral_constant<int, 2>{});
+        else if (heads <= 4) go(integral_constant<int, 4>{});
+        else if (heads <= 8 && sizeof(E) == 2) go(integral_constant<int, sizeof(E) == 2 ? 8 : 16>{});
+        else go(integral_constant<int, 16>{});
         if (p.groups)
             hipLaunchKernelGGL((kv4_join_kernel<D, E>), dim3((unsigned)((int64_t)p.c.rows * p.Hq)), dim3(256), 0, s, p);
     });

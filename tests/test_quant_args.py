@@ -128,6 +128,12 @@ def test_decode_grids():
     assert decode(c, hq=8192, max_len=65536, ws=FAKE, n=1 << 62) == 2
 
 
+def test_read_grids():
+    s = Strides(32 << 24, 32, 32, 1)
+    c = cache(rows=1, heads=1 << 24, D=32)
+    assert read(c, T=1, sk=s, sv=s) == 2
+
+
 def quantize(**kw):
     a = dict(x=FAKE, ldx=64, rows=8, cols=64, t=0, q=1 << 40, ldq=64, s=1 << 41, dt=0)
     a.update(kw)
