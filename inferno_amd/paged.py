@@ -18,6 +18,8 @@ from .ops import _check, _dt, strides_of
 # the current stream's handle on a device; the public spelling costs as much as a launch
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+# likewise the current device's number (asked of tensors on the GPU only: it is initialised)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 @contextlib.contextmanager
@@ -33,7 +35,7 @@ def _elsewhere(device, stream):
     """Whether a call on tensors of this device has to make another device or stream current first."""
     if device.type != "cuda":
         raise ValueError(f"tensors on the GPU expected, got {device}")
-    return stream is not None or device.index != torch.cuda.current_device()
+    return stream is not None or device.index != _current_device()
 
 
 def _of(t, name, dtype, device, shape=None):

@@ -7,12 +7,13 @@ raises InfernoError; launches go to torch's current stream on the tensors' devic
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import INF_BF16, INF_F32, PagedKV4Struct, Strides, default_scale, lib
-from .ops import _check, strides_of
-from .paged import PagedKV, _bytes, _elsewhere, _of, _on, _raw_stream, _size, _workspace
+from .ops import _check
+from .paged import PagedKV, _bytes, _elsewhere, _on, _raw_stream, _size, _workspace
 
 _DT = {torch.float32: INF_F32, torch.bfloat16: INF_BF16}
 
@@ -25,19 +26,45 @@ def _float(t, name):
     return dt
 
 
-def _matrix(t, name, device):
-    """(pointer, row stride) of a matrix with adjacent elements in a row."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+@functools.lru_cache(maxsize=4096)
+def _strides(s):
+    """inf_strides of a 4-D view's strides; the calls take it by value."""
+    return Strides(*s)
+
+
+# Checks of a call's tensors cost as much as its launch where they are made one by one: these take a
+# device's number and give back what the call needs.
+
+
+def _matrix(t, name, index):
+    """(pointer, row stride) of a matrix on this device with adjacent elements in a row."""
+    if t.dim() != 2:
+        raise ValueError(f"{name}: a matrix expected, got {t.dim()} dimensions")
+    ld, step = t.stride()
+    if step != 1 and t.shape[1] > 1:
         raise ValueError(f"{name}: a matrix with adjacent elements in a row expected")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, the others on {device}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on {t.device}, the others on device {index}")
+    return t.data_ptr(), ld if ld > t.shape[1] or t.shape[0] > 1 else t.shape[1]
 
 
-def _matrix_i8(t, name, device):
+def _matrix_i8(t, name, index):
     if t.dtype != torch.int8:
         raise TypeError(f"{name}: int8 expected, got {t.dtype}")
-    return _matrix(t, name, device)
+    return _matrix(t, name, index)
+
+
+def _vector(t, name, dtype, index, n):
+    """The pointer of n dense elements of this type on this device (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: {dtype} expected, got {t.dtype}")
+    if t.get_device() != index:
+        raise ValueError(f"{name}: on {t.device}, the others on device {index}")
+    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name}: {n} dense elements expected, got {tuple(t.shape)}")
+    return t.data_ptr()
 
 
 def _rows16(n, cols, device):
@@ -50,7 +77,7 @@ def quantize_i8(x, transpose=False, stream=None):
     [rows]; with ``transpose`` its columns, q [cols, rows] and scale [cols] (weights [in, out])."""
     dev = x.device
     dt = _float(x, "quantize_i8: x")
-    ptr, ld = _matrix(x, "quantize_i8: x", dev)
+    ptr, ld = _matrix(x, "quantize_i8: x", x.get_device())
     if _elsewhere(dev, stream):
         with _on(dev, stream):
             return quantize_i8(x, transpose)
@@ -84,42 +111,39 @@ def linear_i8_workspace(M, N, K, device="cuda"):
     return torch.empty(_product_bytes("inf_linear_i8_workspace", M, N, K), dtype=torch.uint8, device=device)
 
 
-def _product_args(what, x, w, w_scale, bias, dtype, out, dev):
-    """(w, ldw, w_scale, bias, out's shape) of a product, checked; pointers."""
-    if x.shape[1] != w.shape[1]:
-        raise ValueError(f"{what}: x [M, K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
-    pw, ldw = _matrix_i8(w, f"{what}: w", dev)
-    ps = _of(w_scale, f"{what}: w_scale", torch.float32, dev, w.shape[:1])
-    pb = _of(bias, f"{what}: bias", dtype, dev, w.shape[:1])
-    if out is not None and (out.shape != (x.shape[0], w.shape[0]) or out.dtype != dtype):
-        raise ValueError(f"{what}: out [{x.shape[0]}, {w.shape[0]}] of {dtype} expected")
-    return pw, ldw, ps, pb
+def _result(out, name, shape, dtype, device):
+    """(tensor, pointer, row stride) of a result, a new one where none is given."""
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=device)
+        return out, out.data_ptr(), shape[1]
+    if out.shape != shape or out.dtype != dtype:
+        raise ValueError(f"{name}: {list(shape)} of {dtype} expected, got {list(out.shape)} of {out.dtype}")
+    return out, *_matrix(out, name, device.index)
 
 
 def gemm_i8(x, x_scale, w, w_scale, bias=None, dtype=torch.float32, out=None, workspace=None, stream=None):
     """y [M, N] = x w^T times the scales of x's rows and w's rows, plus bias: x [M, K] and w [N, K] int8 with rows on
     16 bytes (quantize_i8's); y and bias of ``dtype``, float32 or bfloat16."""
-    dev = x.device
-    if x.dim() != 2 or w.dim() != 2:
-        raise ValueError("gemm_i8: x [M, K] and w [N, K] expected")
-    px, ldx = _matrix_i8(x, "gemm_i8: x", dev)
-    psx = _of(x_scale, "gemm_i8: x_scale", torch.float32, dev, x.shape[:1])
+    dev, index = x.device, x.get_device()
+    px, ldx = _matrix_i8(x, "gemm_i8: x", index)
+    pw, ldw = _matrix_i8(w, "gemm_i8: w", index)
+    (M, K), (N, Kw) = x.shape, w.shape
+    if K != Kw:
+        raise ValueError(f"gemm_i8: x [M, K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
     dtype = out.dtype if out is not None else dtype
     if dtype not in _DT:
         raise TypeError(f"gemm_i8: float32 or bfloat16 expected, got {dtype}")
-    pw, ldw, psw, pb = _product_args("gemm_i8", x, w, w_scale, bias, dtype, out, dev)
+    psx = _vector(x_scale, "gemm_i8: x_scale", torch.float32, index, M)
+    psw = _vector(w_scale, "gemm_i8: w_scale", torch.float32, index, N)
+    pb = _vector(bias, "gemm_i8: bias", dtype, index, N)
     if _elsewhere(dev, stream):
         with _on(dev, stream):
             return gemm_i8(x, x_scale, w, w_scale, bias, dtype, out, workspace)
-    M, K = x.shape
-    N = w.shape[0]
-    y = torch.empty((M, N), dtype=dtype, device=dev) if out is None else out
-    py, ldy = _matrix(y, "gemm_i8: out", dev)
+    y, py, ldy = _result(out, "gemm_i8: out", (M, N), dtype, dev)
     if M == 0:
         return y
     ws, ptr, n = _workspace(workspace, lambda: _product_bytes("inf_gemm_i8_workspace", M, N, K), dev)
-    st = lib().inf_gemm_i8(M, N, K, px, ldx, psx, pw, ldw, psw, pb, py, ldy, _DT[dtype], ptr, n,
-                           _raw_stream(dev.index))
+    st = lib().inf_gemm_i8(M, N, K, px, ldx, psx, pw, ldw, psw, pb, py, ldy, _DT[dtype], ptr, n, _raw_stream(index))
     _check(st, "inf_gemm_i8")
     return y
 
@@ -127,23 +151,23 @@ def gemm_i8(x, x_scale, w, w_scale, bias=None, dtype=torch.float32, out=None, wo
 def linear_i8(x, w, w_scale, bias=None, out=None, workspace=None, stream=None):
     """y [M, N] = x w^T + bias with the weights in 8 bits (w int8 [N, K], w_scale [N]: quantize_i8's, with
     ``transpose`` where they are held [in, out]); x [M, K] is taken in 8 bits row by row, y and bias have its type."""
-    dev = x.device
+    dev, index = x.device, x.get_device()
     dt = _float(x, "linear_i8: x")
-    if w.dim() != 2:
-        raise ValueError("linear_i8: w [N, K] expected")
-    px, ldx = _matrix(x, "linear_i8: x", dev)
-    pw, ldw, psw, pb = _product_args("linear_i8", x, w, w_scale, bias, x.dtype, out, dev)
+    px, ldx = _matrix(x, "linear_i8: x", index)
+    pw, ldw = _matrix_i8(w, "linear_i8: w", index)
+    (M, K), (N, Kw) = x.shape, w.shape
+    if K != Kw:
+        raise ValueError(f"linear_i8: x [M, K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
+    psw = _vector(w_scale, "linear_i8: w_scale", torch.float32, index, N)
+    pb = _vector(bias, "linear_i8: bias", x.dtype, index, N)
     if _elsewhere(dev, stream):
         with _on(dev, stream):
             return linear_i8(x, w, w_scale, bias, out, workspace)
-    M, K = x.shape
-    N = w.shape[0]
-    y = torch.empty((M, N), dtype=x.dtype, device=dev) if out is None else out
-    py, ldy = _matrix(y, "linear_i8: out", dev)
+    y, py, ldy = _result(out, "linear_i8: out", (M, N), x.dtype, dev)
     if M == 0:
         return y
     ws, ptr, n = _workspace(workspace, lambda: _product_bytes("inf_linear_i8_workspace", M, N, K), dev)
-    st = lib().inf_linear_i8(M, N, K, px, ldx, pw, ldw, psw, pb, py, ldy, dt, ptr, n, _raw_stream(dev.index))
+    st = lib().inf_linear_i8(M, N, K, px, ldx, pw, ldw, psw, pb, py, ldy, dt, ptr, n, _raw_stream(index))
     _check(st, "inf_linear_i8")
     return y
 
@@ -173,7 +197,7 @@ class PagedKV4:
         if any(t.device != k.device for t in (v, k_scale, v_scale, table, lens)):
             raise ValueError("PagedKV4: all tensors must be on one device")
         self.k, self.v, self.k_scale, self.v_scale, self._table, self._lens = k, v, k_scale, v_scale, table, lens
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.rows, self.heads, self.D, self.page_size = table.shape[0], heads, 2 * half, page_size
         self.capacity = table.shape[1] * page_size
         self.struct = PagedKV4Struct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
@@ -199,36 +223,35 @@ class PagedKV4:
     _row_stride = staticmethod(PagedKV._row_stride)
 
 
-def _dense4(t, name, cache, T):
-    if t.dim() != 4 or t.shape != (cache.rows, cache.heads, T, cache.D):
-        raise ValueError(f"{name}: [rows, heads, T, D] of the cache's rows, heads and D expected")
-    if t.device != cache.device:
+def _tokens(t, name, cache, T):
+    """(pointer, strides) of [rows, heads, T, D] of the cache's sizes and device."""
+    if t.shape != (cache.rows, cache.heads, T, cache.D):
+        raise ValueError(f"{name}: [{cache.rows}, {cache.heads}, {T}, {cache.D}] expected, got {list(t.shape)}")
+    if t.get_device() != cache.index:
         raise ValueError(f"{name}: on {t.device}, the cache on {cache.device}")
+    return t.data_ptr(), _strides(t.stride())
 
 
 def kv4_append(cache, k, v, counts=None, stream=None):
     """Writes k, v [rows, heads, T, D] (float32 or bfloat16) as the rows' last positions (``cache.lens`` counts them
     already); ``counts`` int32 [rows]: how many of the T tokens a row has."""
-    dev = cache.device
     dt = _float(k, "kv4_append: k")
     if k.dim() != 4 or v.dtype != k.dtype:
         raise ValueError("kv4_append: k and v [rows, heads, T, D] of one type expected")
     T = k.shape[2]
-    _dense4(k, "kv4_append: k", cache, T)
-    _dense4(v, "kv4_append: v", cache, T)
-    pc = _of(counts, "counts", torch.int32, dev, (cache.rows,))
-    if _elsewhere(dev, stream):
-        with _on(dev, stream):
+    pk, sk = _tokens(k, "kv4_append: k", cache, T)
+    pv, sv = _tokens(v, "kv4_append: v", cache, T)
+    pc = _vector(counts, "counts", torch.int32, cache.index, cache.rows)
+    if _elsewhere(cache.device, stream):
+        with _on(cache.device, stream):
             return kv4_append(cache, k, v, counts)
-    st = lib().inf_kv4_append(cache.ref, k.data_ptr(), strides_of(k), v.data_ptr(), strides_of(v), pc, T, dt,
-                              _raw_stream(dev.index))
+    st = lib().inf_kv4_append(cache.ref, pk, sk, pv, sv, pc, T, dt, _raw_stream(cache.index))
     _check(st, "inf_kv4_append")
 
 
 def kv4_read(cache, T, first=None, dtype=torch.float32, k_out=None, v_out=None, stream=None):
     """(k, v) [rows, heads, T, D]: positions first[row] + t of every row (``first`` int32 [rows], 0 by default),
     zeros outside a row's positions."""
-    dev = cache.device
     T = int(T)
     if (k_out is None) != (v_out is None):
         raise ValueError("kv4_read: k_out and v_out go together")
@@ -236,18 +259,22 @@ def kv4_read(cache, T, first=None, dtype=torch.float32, k_out=None, v_out=None, 
         dtype = k_out.dtype
         if v_out.dtype != dtype:
             raise TypeError("kv4_read: k_out and v_out of one type expected")
-        _dense4(k_out, "kv4_read: k_out", cache, T)
-        _dense4(v_out, "kv4_read: v_out", cache, T)
-    if dtype not in _DT:
+    dt = _DT.get(dtype)
+    if dt is None:
         raise TypeError(f"kv4_read: float32 or bfloat16 expected, got {dtype}")
-    pf = _of(first, "first", torch.int32, dev, (cache.rows,))
-    if _elsewhere(dev, stream):
-        with _on(dev, stream):
+    pf = _vector(first, "first", torch.int32, cache.index, cache.rows)
+    if _elsewhere(cache.device, stream):
+        with _on(cache.device, stream):
             return kv4_read(cache, T, first, dtype, k_out, v_out)
     if k_out is None:
-        k_out, v_out = torch.empty((2, cache.rows, cache.heads, max(T, 0), cache.D), dtype=dtype, device=dev)
-    st = lib().inf_kv4_read(cache.ref, pf, T, k_out.data_ptr(), strides_of(k_out), v_out.data_ptr(),
-                            strides_of(v_out), _DT[dtype], _raw_stream(dev.index))
+        k_out = torch.empty((cache.rows, cache.heads, max(T, 0), cache.D), dtype=dtype, device=cache.device)
+        v_out = torch.empty_like(k_out)
+        pk, pv = k_out.data_ptr(), v_out.data_ptr()
+        sk = sv = _strides(k_out.stride())
+    else:
+        pk, sk = _tokens(k_out, "kv4_read: k_out", cache, T)
+        pv, sv = _tokens(v_out, "kv4_read: v_out", cache, T)
+    st = lib().inf_kv4_read(cache.ref, pf, T, pk, sk, pv, sv, dt, _raw_stream(cache.index))
     _check(st, "inf_kv4_read")
     return k_out, v_out
 
@@ -265,26 +292,26 @@ def attn_decode_kv4_workspace(cache, q_heads, max_len=None):
 def attn_decode_kv4(q, cache, scale=None, max_len=None, out=None, workspace=None, stream=None):
     """Attention of one new token per row, q [rows, q_heads, 1, D] (float32 or bfloat16), over the row's
     ``cache.lens`` positions.  ``max_len`` bounds the lengths (the capacity by default)."""
-    dev = cache.device
     shape = q.shape
     if len(shape) != 4 or shape[0] != cache.rows or shape[2] != 1 or shape[3] != cache.D:
         raise ValueError("attn_decode_kv4: q [rows, q_heads, 1, D] of the cache's rows and D expected")
     dt = _float(q, "attn_decode_kv4: q")
-    if q.device != dev:
-        raise ValueError(f"attn_decode_kv4: q must be on {dev}")
+    if q.get_device() != cache.index:
+        raise ValueError(f"attn_decode_kv4: q must be on {cache.device}")
     heads = shape[1]
     max_len = cache.capacity if max_len is None else int(max_len)
-    if _elsewhere(dev, stream):
-        with _on(dev, stream):
+    if _elsewhere(cache.device, stream):
+        with _on(cache.device, stream):
             return attn_decode_kv4(q, cache, scale, max_len, out, workspace)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != shape or out.dtype != q.dtype or out.device != dev:
+    elif out.shape != shape or out.dtype != q.dtype or out.get_device() != cache.index:
         raise ValueError("attn_decode_kv4: out must be like q")
-    ws, ptr, n = _workspace(workspace, lambda: _decode_bytes(cache, heads, max_len), dev)
-    st = lib().inf_attn_decode_kv4(cache.ref, q.data_ptr(), strides_of(q), out.data_ptr(), strides_of(out), heads,
-                                   max_len, cache.scale if scale is None else float(scale), dt, ptr, n,
-                                   _raw_stream(dev.index))
+    ws, ptr, n = _workspace(workspace, lambda: _decode_bytes(cache, heads, max_len), cache.device)
+    st = lib().inf_attn_decode_kv4(cache.ref, q.data_ptr(), _strides(q.stride()), out.data_ptr(),
+                                   _strides(out.stride()), heads, max_len,
+                                   cache.scale if scale is None else float(scale), dt, ptr, n,
+                                   _raw_stream(cache.index))
     _check(st, "inf_attn_decode_kv4")
     return out
 
