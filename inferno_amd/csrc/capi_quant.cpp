@@ -86,6 +86,9 @@ int check_rest(const int8_t* w, int64_t ldw, const float* sw, const void* bias, 
 // Rows of elements that can be read four at a time.
 bool by_four(const void* x, int64_t ldx, inf_dtype dt) { return ldx % 4 == 0 && aligned(x, 4 * (size_t)esz(dt)); }
 
+// Rows that can be read 16 bytes at a time.
+bool on_16(const void* x, int64_t ldx, inf_dtype dt) { return ldx * esz(dt) % 16 == 0 && aligned(x, 16); }
+
 // What both forms of the product have in common.
 inf::GemmI8Params product(const int8_t* w, int64_t ldw, const float* sw, const void* bias, void* y, int64_t ldy,
                           int64_t M, int64_t N, int64_t K, inf_dtype dt) {
@@ -109,7 +112,7 @@ int quantize(const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpo
     p.scale = scale;
     p.rows = rows; p.cols = cols;
     p.ldx = ldx; p.ldq = ldq;
-    p.wide = by_four(x, ldx, dt);
+    p.wide = on_16(x, ldx, dt);
     return hip_status(inf::launch_quantize(p, transpose, dt == INF_BF16, stream));
 }
 
@@ -127,8 +130,9 @@ int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int 
                     float* scale, inf_dtype dt, void* stream) {
     if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
     if (rows < 0 || cols < 1 || rows > kMaxMN || cols > kMaxMN) return INF_ERR_BAD_SHAPE;
-    if (transpose ? rows < 1 : rows * 64 > kMaxThreads - 256) return INF_ERR_BAD_SHAPE;
+    if (transpose && rows < 1) return INF_ERR_BAD_SHAPE;
     if (rows == 0) return INF_OK;
+    if (inf::quantize_threads(rows, cols, transpose) > kMaxThreads) return INF_ERR_BAD_SHAPE;
     int st = check_x(x, ldx, cols, dt);
     if (st != INF_OK) return st;
     if (!scale) return INF_ERR_NULL_POINTER;
@@ -184,6 +188,7 @@ int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, c
     if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
     int st = check_product(M, N, K);
     if (st != INF_OK || (st = check_x(x, ldx, K, dt)) || (st = check_i8(w, ldw, K))) return st;
+    if (inf::quantize_threads(M, K, 0) > kMaxThreads) return INF_ERR_BAD_SHAPE;
     const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K, false);
     if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, linear_bytes(plan, M, N, K))))
         return st;
@@ -192,7 +197,7 @@ int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, c
     if (plan.fused) {
         p.xf = x;
         p.ldxf = ldx;
-        p.wide_x = by_four(x, ldx, dt);
+        p.wide_x = on_16(x, ldx, dt);
     } else {
         char* ws = static_cast<char*>(workspace);
         int8_t* q = reinterpret_cast<int8_t*>(ws);

@@ -351,14 +351,15 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Par
         const int T = one ? 64 * NW : 64, t = one ? tid : lane;
         for (int m = one ? 0 : wave; m < p.M; m += NW) {
             const typename E::T* x = (const typename E::T*)p.xf + (int64_t)m * p.ldxf;
+            constexpr int C = kChunk<E>;
             uint32_t top = 0;
             auto most = [&](auto vec) {
 #pragma unroll 2
-                for (int c = 8 * t; c < p.K; c += 8 * T) {
-                    float v[8];
-                    load8<E, decltype(vec)::value>(x, c, p.K, v);
+                for (int c = C * t; c < p.K; c += C * T) {
+                    float v[C];
+                    load_chunk<E, decltype(vec)::value, false>(x, c, p.K, v);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
+                    for (int i = 0; i < C; ++i) top = max(top, magnitude(v[i]));
                 }
             };
             if (p.wide_x) most(std::true_type{});
@@ -372,12 +373,12 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Par
             const RowScale s(top);
             auto write = [&](auto vec) {
 #pragma unroll 2
-                for (int c = 8 * t; c < x_stride - 16; c += 8 * T) {
-                    float v[8];
-                    int q[8];
-                    load8<E, decltype(vec)::value>(x, c, p.K, v);
+                for (int c = C * t; c < x_stride - 16; c += C * T) {
+                    float v[C];
+                    int q[C];
+                    load_chunk<E, decltype(vec)::value, false>(x, c, p.K, v);
                     round_all(v, s, q);
-                    *reinterpret_cast<uint2*>(xq + m * x_stride + c) = make_uint2(pack4(q, 0), pack4(q, 4));
+                    store_chunk(xq + m * x_stride + c, q);
                 }
             };
             if (p.wide_x) write(std::true_type{});

@@ -453,8 +453,13 @@ struct QuantizeParams {
     int8_t* q;             // rows (transposed: columns) of x, ldq bytes apart, 16-byte aligned
     float* scale;          // [rows] (transposed: [cols])
     int64_t rows, cols, ldx, ldq;
-    int wide;              // rows of x allow 16-byte loads
+    int wide;              // rows of x on 16 bytes
 };
+// Rows up to so many columns take a wave each, longer ones four; columns go 32 to a workgroup of 1024.
+constexpr int64_t kQuantizeWave = 1024;
+inline int64_t quantize_threads(int64_t rows, int64_t cols, int transpose) {
+    return transpose ? (cols + 31) / 32 * 1024 : cols <= kQuantizeWave ? (rows + 3) / 4 * 256 : rows * 256;
+}
 int launch_quantize(const QuantizeParams& p, int transpose, int bf16, hipStream_t s);
 
 struct GemmI8Params {
@@ -475,7 +480,7 @@ struct GemmI8Params {
     // a plan that is fused takes x as it is instead of x and sx
     const void* xf;        // [M, K] in y's type, row stride ldxf
     int64_t ldxf;
-    int wide_x;            // rows of xf allow loads of four elements
+    int wide_x;            // rows of xf on 16 bytes
 };
 struct GemmI8Plan {
     enum Kind { kRows, k64, k128, k256 } kind = kRows;  // few rows, or tiles of so many rows and columns

@@ -8,30 +8,30 @@
 
 namespace inf {
 
-// W waves a row, eight neighbouring columns a thread at a time, U of them held between the two passes over
-// the row; a longer row is read twice.  q's rows are written up to whole 16 bytes, with zeros.
+// W waves a row, 16 bytes of it a thread at a time, U times that held between the two passes over the row; a longer
+// row is read twice.  q's rows are written up to whole 16 bytes, with zeros.
 template <typename E, int W, int U, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeParams p) {
-    constexpr int T = 64 * W;
+    constexpr int T = 64 * W, C = kChunk<E>;
     __shared__ uint32_t tops[4];
     const int tid = threadIdx.x % T, wave = threadIdx.x >> 6;
     const int64_t row = (int64_t)blockIdx.x * (4 / W) + threadIdx.x / T;
     const bool there = row < p.rows;
     const typename E::T* x = (const typename E::T*)p.x + (there ? row : 0) * p.ldx;
     const int cols = (int)p.cols;
-    float v[U][8];
+    float v[U][C];
     uint32_t top = 0;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        load8<E, VEC>(x, 8 * (tid + T * u), cols, v[u]);
+    for (int u = 0; u < U; ++u) load_chunk<E, VEC, true>(x, C * (tid + T * u), cols, v[u]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[u][i]));
-    }
-    for (int c = 8 * (tid + T * U); c < cols; c += 8 * T) {
-        float y[8];
-        load8<E, VEC>(x, c, cols, y);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, magnitude(y[i]));
+        for (int i = 0; i < C; ++i) top = max(top, magnitude(v[u][i]));
+    for (int c = C * (tid + T * U); c < cols; c += C * T) {
+        float y[C];
+        load_chunk<E, VEC, false>(x, c, cols, y);
+#pragma unroll
+        for (int i = 0; i < C; ++i) top = max(top, magnitude(y[i]));
     }
     top = wave_all(top, [](uint32_t a, uint32_t b) { return max(a, b); });
     if constexpr (W > 1) {
@@ -43,16 +43,16 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantizeParams p) {
     const RowScale s(top);
     int8_t* q = p.q + row * p.ldq;
     const int end = (cols + 15) & ~15;
-    auto write = [&](int c, const float (&y)[8]) {
-        int r[8];
+    auto write = [&](int c, const float (&y)[C]) {
+        int r[C];
         round_all(y, s, r);
-        if (c < end) *reinterpret_cast<uint2*>(q + c) = make_uint2(pack4(r, 0), pack4(r, 4));
+        if (c < end) store_chunk(q + c, r);
     };
 #pragma unroll
-    for (int u = 0; u < U; ++u) write(8 * (tid + T * u), v[u]);
-    for (int c = 8 * (tid + T * U); c < end; c += 8 * T) {
-        float y[8];
-        load8<E, VEC>(x, c, cols, y);
+    for (int u = 0; u < U; ++u) write(C * (tid + T * u), v[u]);
+    for (int c = C * (tid + T * U); c < end; c += C * T) {
+        float y[C];
+        load_chunk<E, VEC, false>(x, c, cols, y);
         write(c, y);
     }
     if (tid == 0) p.scale[row] = s.scale;
@@ -98,12 +98,24 @@ static void launch_rows(const QuantizeParams& p, hipStream_t s) {
                            dim3(256), 0, s, p);
     };
     using std::integral_constant;
-    // one wave a row up to 1024 columns, else four
-    if (p.cols <= 512) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    else if (p.cols <= 1024) go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-    else if (p.cols <= 2048) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-    else if (p.cols <= 4096) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    else go(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    using C1 = integral_constant<int, 1>;
+    using C2 = integral_constant<int, 2>;
+    using C4 = integral_constant<int, 4>;
+    using C8 = integral_constant<int, 8>;
+    const int64_t chunks = (p.cols + kChunk<E> - 1) / kChunk<E>;
+    if (p.cols <= kQuantizeWave) {
+        if (chunks <= 64) go(C1{}, C1{});
+        else if (chunks <= 128) go(C1{}, C2{});
+        else go(C1{}, C4{});
+    } else if (chunks <= 256) {
+        go(C4{}, C1{});
+    } else if (chunks <= 512) {
+        go(C4{}, C2{});
+    } else if (chunks <= 1024) {
+        go(C4{}, C4{});
+    } else {
+        go(C4{}, C8{});
+    }
 }
 
 int launch_quantize(const QuantizeParams& p, int transpose, int bf16, hipStream_t s) {

@@ -58,20 +58,33 @@ __device__ __forceinline__ uint32_t pack4(const int (&q)[N], int at) {
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// Eight columns from c on, zeros behind the last.
-template <typename E, bool VEC>
-__device__ __forceinline__ void load8(const typename E::T* row, int c, int cols, float (&x)[8]) {
-    if (VEC && c + 8 <= cols) {
-        const f32x4 a = ld4(row + c), b = ld4(row + c + 4);
+// The columns that a thread takes at a time: 16 bytes.
+template <typename E>
+constexpr int kChunk = 16 / (int)sizeof(typename E::T);
+
+// Chunk of columns from c on, zeros behind the last.  VEC: rows on 16 bytes; NT: past the caches.
+template <typename E, bool VEC, bool NT>
+__device__ __forceinline__ void load_chunk(const typename E::T* row, int c, int cols, float (&x)[kChunk<E>]) {
+    constexpr int N = kChunk<E>;
+    if (VEC && c + N <= cols) {
+        const u32x4* src = reinterpret_cast<const u32x4*>(row + c);
+        const u32x4 v = NT ? __builtin_nontemporal_load(src) : *src;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[i] = a[i];
-            x[4 + i] = b[i];
-        }
+        for (int i = 0; i < N; ++i)
+            x[i] = __uint_as_float(N == 4 ? v[i & 3] : i & 1 ? v[(i >> 1) & 3] & 0xffff0000u : v[(i >> 1) & 3] << 16);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = c + i < cols ? E::ld(row + c + i) : 0.f;
+        for (int i = 0; i < N; ++i) x[i] = c + i < cols ? E::ld(row + c + i) : 0.f;
     }
+}
+
+// The chunk's whole numbers, a byte each.
+template <int N>
+__device__ __forceinline__ void store_chunk(void* q, const int (&r)[N]) {
+    if constexpr (N == 8)
+        *reinterpret_cast<uint2*>(q) = make_uint2(pack4(r, 0), pack4(r, 4));
+    else
+        *reinterpret_cast<uint32_t*>(q) = pack4(r, 0);
 }
 
 }  // namespace inf

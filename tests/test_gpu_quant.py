@@ -134,7 +134,9 @@ def check_product(y, acc, sx, sw, bias, dtype):
     assert (err <= bound).all(), (err / bound).max()  # NaN fails
 
 
-PRODUCTS = [(1, 1, 1), (1, 16, 16), (2, 17, 33), (15, 100, 63), (16, 64, 64), (17, 48, 65), (31, 200, 129),
+# few rows and few outputs: K ranges per wave; else tiles of 64, 128 or 256, those of 64 in K ranges where there are few
+PRODUCTS = [(40, 50, 8192), (8, 64, 8200), (64, 40, 5000), (50, 8300, 130), (20, 9000, 2100), (100, 100, 3000),
+            (700, 1100, 2050), (2100, 2200, 70), (1, 1, 1), (1, 16, 16), (2, 17, 33), (15, 100, 63), (16, 64, 64), (17, 48, 65), (31, 200, 129),
             (33, 130, 257), (48, 96, 1000), (64, 33, 500), (65, 127, 127), (100, 129, 1), (128, 128, 128),
             (129, 257, 300), (200, 130, 2000), (300, 515, 4090), (130, 100, 9000), (513, 70, 200), (70, 1030, 384)]
 
@@ -190,7 +192,9 @@ def test_strided_products(ia):
             assert (rest == 77.0).all()
 
 
-LINEARS = [(1, 2304, 768), (1, 100, 65), (7, 96, 1000), (16, 300, 4096), (33, 64, 128), (80, 200, 513), (260, 300, 96)]
+# one kernel takes x as it is where M K is at most 16384
+LINEARS = [(1, 2304, 768), (1, 100, 65), (1, 50, 16384), (1, 33, 16385), (31, 70, 528), (32, 100, 512), (3, 40, 2001),
+           (4, 4096, 4100), (7, 96, 1000), (16, 300, 4096), (33, 64, 128), (80, 200, 513), (260, 300, 96)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -144,6 +144,7 @@ def quantize(**kw):
 @pytest.mark.parametrize("kw,status", [
     (dict(x=None), 1), (dict(q=None), 1), (dict(s=None), 1), (dict(rows=-1), 2), (dict(cols=0), 2), (dict(rows=0), 0),
     (dict(rows=0, t=1), 2), (dict(rows=1 << 31), 2), (dict(cols=1 << 31, ldx=1 << 31), 2), (dict(rows=1 << 27), 2),
+    (dict(rows=1 << 24, cols=1025, ldx=1025), 2), (dict(cols=1 << 28, ldx=1 << 28, t=1), 2),
     (dict(dt=2), 4), (dict(dt=-1), 4), (dict(ldx=63), 3), (dict(ldq=48), 3), (dict(t=1, rows=65, ldq=64), 3),
     (dict(ldq=(1 << 22) + 16), 3), (dict(ldq=72), 7), (dict(q=FAKE + 8), 7), (dict(x=FAKE + 2), 7),
     (dict(x=FAKE + 1, dt=1), 7), (dict(s=FAKE + 2), 7)])
@@ -169,7 +170,7 @@ def linear(**kw):
 @pytest.mark.parametrize("call", [gemm, linear])
 @pytest.mark.parametrize("kw,status", [
     (dict(M=0), 2), (dict(N=0), 2), (dict(K=0), 2), (dict(M=1 << 31), 2), (dict(N=1 << 31), 2),
-    (dict(M=1 << 20, N=1 << 20), 2), (dict(K=1 << 17, ldx=1 << 17, ldw=1 << 17), 5), (dict(dt=2), 4),
+    (dict(M=1 << 20, N=1 << 20), 2), (dict(M=1 << 27, N=1, K=1), 2), (dict(K=1 << 17, ldx=1 << 17, ldw=1 << 17), 5), (dict(dt=2), 4),
     (dict(x=None), 1), (dict(w=None), 1), (dict(sw=None), 1), (dict(y=None), 1),
     (dict(ldx=63), 3), (dict(ldw=48), 3), (dict(ldw=(1 << 22) + 16), 3), (dict(ldy=31), 3),
     (dict(ldw=72), 7), (dict(w=FAKE + 4), 7), (dict(sw=FAKE + 1), 7), (dict(y=FAKE + 2), 7), (dict(b=FAKE + 2), 7)])
@@ -184,6 +185,10 @@ def test_results_over_what_is_read():
     assert gemm(y=far, x=far + 1008) == 3 and gemm(y=far, sx=far - 28) == 3
     assert linear(y=far, x=far + 992) == 3 and linear(M=100, y=far, ws=far + 512) == 3
     assert quantize(q=FAKE + 2032) == 3 and quantize(s=FAKE - 28) == 3 and quantize(s=FAKE + 2044, t=1) == 3
+
+
+def test_rows_that_no_grid_holds():
+    assert linear(M=1 << 24, N=1, K=1040, ldx=1040, ldw=1040) == 2
 
 
 def test_product_arguments_of_one_form():
