@@ -35,29 +35,47 @@ __device__ __forceinline__ i32x4 first_bytes(i32x4 v, int n) {
     return v;
 }
 
-// Four neighbouring results of row m from column n on.  NT: past the caches, where whole lines are written.
-template <typename E, bool NT = false>
-__device__ __forceinline__ void finish4(const GemmI8Params& p, int m, int n, i32x4 sum, float sx) {
-    typename E::T* y = (typename E::T*)p.y + (int64_t)m * p.ldy + n;
-    const typename E::T* bias = (const typename E::T*)p.bias;
-    // the same roundings however the columns are aligned
-    auto one = [&](int i, float sw, float b) { return fmaf((float)sum[i] * sx, sw, b); };
-    if (p.wide && n + 4 <= p.N) {
-        const f32x4 sw = ld4(p.sw + n), b = bias ? ld4(bias + n) : f32x4{0.f, 0.f, 0.f, 0.f};
-        const f32x4 v = {one(0, sw[0], b[0]), one(1, sw[1], b[1]), one(2, sw[2], b[2]), one(3, sw[3], b[3])};
-        if constexpr (!NT)
+// Four neighbouring columns from n on: their scales and bias.
+template <typename E>
+struct Columns {
+    f32x4 sw, bias;
+    bool whole;  // all four there, on 16 bytes
+    __device__ __forceinline__ Columns(const GemmI8Params& p, int n) : whole(p.wide && n + 4 <= p.N) {
+        const typename E::T* b = (const typename E::T*)p.bias;
+        sw = bias = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (whole) {
+            sw = ld4(p.sw + n);
+            if (b) bias = ld4(b + n);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < p.N) {
+                    sw[i] = p.sw[n + i];
+                    if (b) bias[i] = E::ld(b + n + i);
+                }
+        }
+    }
+    // Their results in row m.  NT: past the caches, where whole lines are written.
+    template <bool NT>
+    __device__ __forceinline__ void store(const GemmI8Params& p, int m, int n, i32x4 sum, float sx) const {
+        typename E::T* y = (typename E::T*)p.y + (int64_t)m * p.ldy + n;
+        f32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = fmaf((float)sum[i] * sx, sw[i], bias[i]);
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n + i < p.N) E::st(y + i, v[i]);
+        } else if constexpr (!NT) {
             st4(y, v);
-        else if constexpr (sizeof(typename E::T) == 4)
+        } else if constexpr (sizeof(typename E::T) == 4) {
             __builtin_nontemporal_store(v, reinterpret_cast<f32x4*>(y));
-        else
+        } else {
             __builtin_nontemporal_store(u16x4{f32_to_bf16(v[0]), f32_to_bf16(v[1]), f32_to_bf16(v[2]), f32_to_bf16(v[3])},
                                         reinterpret_cast<u16x4*>(y));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < p.N) E::st(y + i, one(i, p.sw[n + i], bias ? E::ld(bias + n + i) : 0.f));
+        }
     }
-}
+};
 
 }  // namespace
 
@@ -240,6 +258,17 @@ __global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * BK * S > 81920
     static_assert(HOLD * 4 >= NW, "a block in LDS for every wave");
     const int which = wave / HOLD;
     i32x4* turn = reinterpret_cast<i32x4*>(which == 0 ? w0 : which == 1 ? x0 : which == 2 ? w1 : x1) + wave % HOLD * 32 * U;
+    // a lane's columns stay the same: what scales them is loaded once, and its rows' scales ahead of the stores
+    static_assert(64 % U == 0, "one piece of the columns to a lane");
+    const int m_wave = m0 + wm * (BM / WM) + lane / U, n = n0 + wn * (BN / WN) + 4 * (lane % U);
+    float sx[FM][U / 2];
+    if constexpr (!SPLIT) {
+#pragma unroll
+        for (int h = 0; h < FM; ++h)
+#pragma unroll
+            for (int i = 0; i < U / 2; ++i) sx[h][i] = p.sx[min(m_wave + 32 * h + 64 / U * i, p.M - 1)];
+    }
+    const Columns<E> columns(p, SPLIT ? p.N : n);
 #pragma unroll
     for (int h = 0; h < FM; ++h) {
 #pragma unroll
@@ -251,14 +280,13 @@ __global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * BK * S > 81920
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int i = 0; i < U / 2; ++i) {
-            const int r = (64 * i + lane) / U, c = (64 * i + lane) % U;
-            const int m = m0 + wm * (BM / WM) + 32 * h + r, n = n0 + wn * (BN / WN) + 4 * c;
-            const i32x4 v = turn[r * U + (c ^ (r & 7))];
+            const int r = lane / U + 64 / U * i, m = m_wave + 32 * h + 64 / U * i;
+            const i32x4 v = turn[r * U + (lane % U ^ (r & 7))];
             if (m >= p.M || n >= p.N) continue;
             if constexpr (SPLIT)
                 *reinterpret_cast<i32x4*>(p.part + ((int64_t)split * p.M + m) * p.ldp + n) = v;
             else
-                finish4<E, true>(p, m, n, v, p.sx[m]);
+                columns.template store<true>(p, m, n, v, sx[h][i]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
@@ -275,7 +303,7 @@ __global__ __launch_bounds__(256) void gemm_i8_join_kernel(GemmI8Params p) {
     i32x4 sum = *reinterpret_cast<const i32x4*>(src);
     for (int s = 1; s < p.ksplit; ++s)
         sum += *reinterpret_cast<const i32x4*>(src + (int64_t)s * p.M * p.ldp);
-    finish4<E>(p, m, n, sum, p.sx[m]);
+    Columns<E>(p, n).template store<false>(p, m, n, sum, p.sx[m]);
 }
 
 // ============================================================================
@@ -457,7 +485,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Par
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] += sums[((w * FM + h) * 16 + 4 * j + r) * 64 + lane];
         const int m = 32 * h + l32, n = n0 + 8 * j + 4 * g;
-        if (m < p.M && n < p.N) finish4<E>(p, m, n, v, FUSED ? scales[m] : p.sx[m]);
+        if (m < p.M && n < p.N) Columns<E>(p, n).template store<false>(p, m, n, v, FUSED ? scales[m] : p.sx[m]);
     }
 }
 
