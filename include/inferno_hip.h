@@ -575,7 +575,8 @@ int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int 
                     float* scale, inf_dtype dt, void* stream);
 
 /* y[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n] + bias[n]: x [M, K] and w [N, K] in 8 bits, the sum exact
- * (K < 2^17), y and bias (may be NULL) fp32 or bf16 by dt, rounded once.  Rows of x and w lie on 16 bytes and are read
+ * (K < 2^17); then in fp32, in this order (the sum times x_scale has to be finite); y and bias (may be NULL) fp32 or bf16
+ * by dt, rounded once.  Rows of x and w lie on 16 bytes and are read
  * in pieces of 16 (up to K in whole 16 bytes; what lies behind K does not matter).  y must not overlap what is read.
  * workspace: inf_gemm_i8_workspace bytes (may be 0: then NULL), 256-byte aligned.  Calls that share one must not
  * overlap.  The same bits on every run. */

@@ -268,6 +268,54 @@ def test_decode_many_rows(ia, dtype):
         check(ia.attn_decode_kv4(q.cuda(), cache), q, ks, vs, heads)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_decode_many_heads(ia, dtype):
+    """More heads than workgroups at once: a block of rows in one share."""
+    gen = torch.Generator().manual_seed(10)
+    few, ks, vs, _ = make_cache(ia, gen, [1030, 0, 513], 8, 32, 16)
+    pools = (t.repeat(1, 100, 1, 1) for t in (few.k, few.v, few.k_scale, few.v_scale))
+    cache = ia.PagedKV4(*pools, few.table, few.lens)
+    q = torch.randn((3, 800, 1, 32), generator=gen).to(dtype)
+    o = ia.attn_decode_kv4(q.cuda(), cache)
+    check(o, q, [k.repeat(100, 1, 1) for k in ks], [v.repeat(100, 1, 1) for v in vs], 800)
+
+
+def test_rows_of_the_same_pages(ia):
+    """A common beginning held once, and one row twice."""
+    gen = torch.Generator().manual_seed(11)
+    cache, ks, vs, _ = make_cache(ia, gen, [900, 700, 0, 0], 2, 64, 16)
+    cache.table[2] = cache.table[0]
+    cache.table[3] = cache.table[0]
+    cache.lens[2], cache.lens[3] = 900, 333
+    q = torch.randn((4, 6, 1, 64), generator=gen)
+    q[2] = q[0]
+    ks, vs = ([x[0], x[1], x[0], x[0][:, :333]] for x in (ks, vs))
+    o = ia.attn_decode_kv4(q.cuda(), cache)
+    check(o, q, ks, vs, 2)
+    k, v = ia.kv4_read(cache, 900)
+    assert torch.equal(k[2], k[0]) and torch.equal(v[3, :, :333], v[0, :, :333]) and not v[3, :, 333:].any()
+
+
+def test_captured_twice(ia):
+    """Two captured calls of one cache, workspace and result, replayed in turn with eager calls between."""
+    gen = torch.Generator().manual_seed(12)
+    cache, ks, vs, _ = make_cache(ia, gen, [2000, 31, 0, 700], 2, 64, 16)
+    ws = ia.attn_decode_kv4_workspace(cache, 4)
+    qs = [torch.randn((4, 4, 1, 64), generator=gen) for _ in range(2)]
+    dev = [q.cuda() for q in qs]
+    out = torch.empty_like(dev[0])
+    want = [ia.attn_decode_kv4(q, cache) for q in dev]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, q in zip(graphs, dev):
+        with torch.cuda.graph(graph):
+            ia.attn_decode_kv4(q, cache, out=out, workspace=ws)
+    for i in range(6):
+        graphs[i % 2].replay()
+        assert torch.equal(out, want[i % 2])
+        assert torch.equal(ia.attn_decode_kv4(dev[1 - i % 2], cache, workspace=ws), want[1 - i % 2])
+    check(want[0], qs[0], ks, vs, 2)
+
+
 def test_decode_strided_and_in_place(ia):
     gen = torch.Generator().manual_seed(4)
     cache, ks, vs, _ = make_cache(ia, gen, [40, 700], 2, 64, 16)

@@ -222,6 +222,21 @@ def test_linear(ia, M, N, K, dtype):
     assert torch.equal(ia.linear_i8(x.cuda(), w, sw, bias=bias.cuda(), workspace=ws), y)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(1, 70, 301), (5, 70, 301), (40, 70, 301), (200, 70, 301), (1, 70, 512), (6, 70, 512)])
+def test_linear_strided_rows(ia, M, N, K, dtype):
+    """Rows of x further apart and at odd places: the bits that dense rows give."""
+    gen = torch.Generator().manual_seed(M + K)
+    x = torch.randn((M, K), generator=gen).to(dtype).cuda()
+    w, sw = ia.quantize_i8(torch.randn((K, N), generator=gen).cuda(), transpose=True)
+    want = ia.linear_i8(x, w, sw)
+    for ld, off in ((K + 1, 0), (K + 1, 1), (K + 8, 4), (K + 19, 3)):
+        store = torch.full((M * ld + off,), float("nan"), dtype=dtype, device="cuda")
+        view = torch.as_strided(store, (M, K), (ld, 1), off)
+        view.copy_(x)
+        assert torch.equal(ia.linear_i8(view, w, sw), want)
+
+
 @pytest.mark.parametrize("M", [1, 5, 40, 200])
 def test_linear_special_rows(ia, M):
     """A non-finite row is NaN and leaves the others alone; a row of zeros is the bias."""
