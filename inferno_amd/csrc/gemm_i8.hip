@@ -505,14 +505,23 @@ GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
         plan.fused = !quantised && M * K <= 16384 && M <= 32;
         return plan;
     }
+    // Tiles of 256, one workgroup a CU (us, theirs and tiles of 128, bf16 results): 4096 x 4096 x 4096 67 and 88, x 512 18.1 and
+    // 20.3; with 69 % of a round's CUs busy, 2816 x 4096 x 4096, 56 and 65, but 53 %, 4352 x 4096 x 4096, 108 and 94.  A short
+    // K leaves the results' writing in the open, which two workgroups a CU hide: 75 %, 16384 x 2304 x 768 in
+    // fp32, 70 and 55.
     const int64_t t256 = tiles(256), rounds = (t256 + 255) / 256;
-    if (steps >= 16 && t256 * 10 >= rounds * 256 * 7) {
+    if (steps >= 4 && t256 * 10 >= rounds * 256 * (steps >= 16 ? 7 : 9)) {
         plan.kind = GemmI8Plan::k256;
-    } else if (tiles(128) >= 256) {
+    } else if (tiles(128) >= 208) {  // 208 of them, 1664 x 2048 x 4096: 25.5, of 64 29.5; 192, 768 x 4096 x 4096: 25.3 and 22.8
         plan.kind = GemmI8Plan::k128;
     } else {
         plan.kind = GemmI8Plan::k64;
+        // Where there is one tile a CU, or two, nothing but their own loads hides the memory: three steps ahead and one
+        // (weights from memory) 128 x 8192 x 8192 24 and 47, 333 x 4096 x 4096 18.7 and 24.9; but with three tiles a CU, 768 x
+        // 4096 x 4096, 28.8 and 22.8.
         plan.deep = tiles(64) <= 512 && steps >= 16;
+        // K ranges, for a join of about 5 us, where they take 24 steps off the longest: 128 x 1024 x 8192 9.9 in eight,
+        // 15.7 in one; 200 x 2048 x 4096 (three) 11.9 and 9.9.
         const int64_t ks = std::min<int64_t>(384 / tiles(64), steps / 8);
         if (ks > 1 && steps * (ks - 1) > 24 * ks) {
             plan.kchunk = (int)((steps + ks - 1) / ks * kI8Step);
