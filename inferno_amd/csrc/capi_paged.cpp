@@ -195,7 +195,7 @@ int check_decode4(const inf_paged_kv4* c, int q_heads, int max_len) {
         return INF_ERR_BAD_SHAPE;
     if ((int64_t)c->rows * q_heads > (1 << 24)) return INF_ERR_BAD_SHAPE;
     // the steps of a block of rows are counted in 32 bits
-    if ((int64_t)std::min(c->rows, inf::kPagedBlock) * (max_len / inf::kv4_step(c->D) + 1) > (1 << 30))
+    if ((int64_t)std::min(c->rows, inf::kPagedBlock) * (max_len / inf::kKv4Step + 1) > (1 << 30))
         return INF_ERR_BAD_SHAPE;
     return INF_OK;
 }

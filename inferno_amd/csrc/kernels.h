@@ -541,7 +541,7 @@ struct Kv4DecodeParams {
     int q_at;              // place of q's parts in LDS (set by the launcher)
 };
 // Keys that a workgroup takes per step.
-constexpr int kv4_step(int D) { return D == 128 ? 256 : 512; }
+constexpr int kKv4Step = 256;
 int kv4_groups(int rows, int heads, int G, int max_len, int D);
 
 int launch_kv4_append(const Kv4AppendParams& p, int bf16, hipStream_t s);

@@ -263,18 +263,16 @@ int launch_kv4_read(const Kv4ReadParams& p, int bf16, hipStream_t s) {
 // ============================================================================
 namespace {
 
-constexpr int kKv4PerCu = 3;  // workgroups of a CU: what the registers allow
+constexpr int kv4_per_cu(int D) { return D == 128 ? 3 : 4; }  // workgroups of a CU: what the registers allow
 
 // What a wave keeps in LDS where its scores pass through it.
-constexpr int kv4_wave_floats(int D, bool f32, int HB) {
-    const int keys = kv4_step(D) / 4;
+constexpr int kv4_wave_floats(bool f32, int HB) {
+    const int keys = kKv4Step / 4;
     return HB == 16 ? 0 : (f32 ? 3 : 1) * HB * keys + (f32 ? 3 : 2) * HB * keys / 2 + 16;
 }
 
-template <int D>
 __device__ __forceinline__ int kv4_steps(int len, int max_len) {
-    constexpr int step = kv4_step(D);
-    return len > max_len ? 0 : (max(len, 0) + step - 1) / step;
+    return len > max_len ? 0 : (max(len, 0) + kKv4Step - 1) / kKv4Step;
 }
 
 }  // namespace
@@ -284,10 +282,10 @@ __device__ __forceinline__ int kv4_steps(int len, int max_len) {
 // all lanes, 64 / HB of them a head, and the probabilities back.  And the columns that are left take the other bf16
 // parts of queries and probabilities, part k of head i in column k HB + i: one product instead of two or three.
 template <int D, typename E, int HB>
-__global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodeParams p) {
+__global__ __launch_bounds__(256, kv4_per_cu(D)) void kv4_split_kernel(Kv4DecodeParams p) {
     constexpr bool F = sizeof(E) == 4;
     constexpr int PARTS = F ? 3 : 1;      // of q
-    constexpr int STEP = kv4_step(D);
+    constexpr int STEP = kKv4Step;
     constexpr int T = STEP / 64;          // tiles of 16 keys per wave
     constexpr int NK = D / 32;            // words of a key row per lane: products of a tile
     constexpr int VD = D / 16;            // columns of a value row per lane
@@ -300,7 +298,8 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
     // probabilities [PP][HB][KEYS] and factors [HB].  From q_at on, fp32: parts of q [3][heads, or HB][D].
     extern __shared__ __attribute__((aligned(16))) float lds[];
 
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ht = p.head_tiles;
     int unit = blockIdx.x, tile = 0;
     if (ht > 1) {
@@ -317,7 +316,7 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
     // Lane i: the first step of the block's row i.  This share's are [step, stop) of them; row r, the first
     // one, has [begin, end).
     const int mylen = lane < nrows ? p.c.lens[row0 + lane] : 0;
-    int step = 0, r = 0, begin = 0, steps = kv4_steps<D>(mylen, p.max_len), starts = steps;
+    int step = 0, r = 0, begin = 0, steps = kv4_steps(mylen, p.max_len), starts = steps;
     if (nrows > 1) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -353,16 +352,22 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
     // this lane's places in a tile: key col, channels D / 4 * g on; values of keys 4 g + r, channels VD * col on
     const uint8_t* K = p.c.k + h * p.c.sk.h;
     const uint8_t* V = p.c.v + h * p.c.sv.h;
-    const uint8_t* KS = p.c.ks + h * p.c.sks.h;
-    const uint8_t* VS = p.c.vs + h * p.c.svs.h;
-    const uint32_t k_at = col * (uint32_t)p.c.sk.t + g * (D / 8), ks_at = g * D / 128 * (uint32_t)p.c.sks.t + col;
+    const uint32_t k_at = col * (uint32_t)p.c.sk.t + g * (D / 8);
     uint32_t v_at[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * (uint32_t)p.c.sv.t + col * (VD / 2);
-    const uint32_t vs_at = col * D / 512 * (uint32_t)p.c.svs.t + 4 * g;
+    // A step's scales come in one load: tile t's of keys 4 q .. and block b to lane t + T q + 4 T b, and from there to
+    // the lanes that need them.  (A load costs the same at any width: with two of each tile's scales, 4 rows of 131071 keys took
+    // 32.4 us, 31.3 so.)
+    static_assert(4 * T * NK <= 64, "a lane for every four scales");
+    const int scale_block = min(lane / (4 * T), NK - 1), scale_key = lane / T % 4 * 4;
+    const uint8_t* KS = p.c.ks + h * p.c.sks.h + scale_block * p.c.sks.t + scale_key;
+    const uint8_t* VS = p.c.vs + h * p.c.svs.h + scale_block * p.c.svs.t + scale_key;
+    const int ks_lane = 4 * (T * (col / 4) + 4 * T * (g * D / 128)), ks_bit = 8 * (col % 4);
+    const int vs_lane = 4 * (T * g + 4 * T * (col * D / 512));
     uint32_t kr[T][NK], ksr[T], vr[T][4], vsr[T];
     const int qn = HB == 16 ? gn : HB;
-    float* mine = lds + wave * kv4_wave_floats(D, F, HB);
+    float* mine = lds + wave * kv4_wave_floats(F, HB);
 
     for (;;) {  // the rows of the share
         const int row = row0 + r, s0 = step - begin, s1 = min(stop, end) - begin;
@@ -406,15 +411,16 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
         float m = -INFINITY, l = 0.f;
         bool bad = false;
         for (int base = base0; base < j1; base += STEP) {
-            uint64_t places[4];
+            uint64_t places[2];
+            uint32_t ks_words, vs_words;
             {
                 const bool in = (unsigned)next < (unsigned)p.c.n_pages;
                 bad |= !in && base + tile_key < j1;
                 const uint32_t page = in ? next : 0, at = (base + tile_key) & mask;
                 places[0] = (uint64_t)K + page * (uint64_t)p.c.sk.b + (uint64_t)at * (uint32_t)p.c.sk.t;
                 places[1] = (uint64_t)V + page * (uint64_t)p.c.sv.b + (uint64_t)at * (uint32_t)p.c.sv.t;
-                places[2] = (uint64_t)KS + page * (uint64_t)p.c.sks.b + at;
-                places[3] = (uint64_t)VS + page * (uint64_t)p.c.svs.b + at;
+                ks_words = *reinterpret_cast<const uint32_t*>(KS + page * (uint64_t)p.c.sks.b + at);
+                vs_words = *reinterpret_cast<const uint32_t*>(VS + page * (uint64_t)p.c.svs.b + at);
             }
             if (base + STEP < j1) next = read_pages(base + STEP);
 #pragma unroll
@@ -435,12 +441,13 @@ __global__ __launch_bounds__(256, kKv4PerCu) void kv4_split_kernel(Kv4DecodePara
                 const auto vp = rows(1, 15 * (uint32_t)p.c.sv.t + D / 2);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) vr[t][r] = load_nt<VD / 2>(vp, v_at[r]);
-                const auto ks = rows(2, (D / 32 - 1) * (uint32_t)p.c.sks.t + 16),
-                           vs = rows(3, (D / 32 - 1) * (uint32_t)p.c.svs.t + 16);
-                ksr[t] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(ks, (int)ks_at, 0, 0);
-                vsr[t] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(vs, (int)vs_at, 0, 0);
             }
             __builtin_amdgcn_sched_barrier(0);  // all of the step's loads before its first product
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                ksr[t] = (uint32_t)__builtin_amdgcn_ds_bpermute(ks_lane + 4 * t, (int)ks_words) >> ks_bit;
+                vsr[t] = (uint32_t)__builtin_amdgcn_ds_bpermute(vs_lane + 4 * t, (int)vs_words);
+            }
             f32x4 st[T] = {};
             const __bf16* qs = reinterpret_cast<const __bf16*>(lds + p.q_at) +
                                (HB == 16 ? min(col, gn - 1) : min(col, 3 * HB - 1)) * D + g * (D / 4);
@@ -670,7 +677,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4DecodeParams p) {
     __shared__ f32x4 osh[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq;
-    const int len = p.c.lens[row], steps = kv4_steps<D>(len, p.max_len);
+    const int len = p.c.lens[row], steps = kv4_steps(len, p.max_len);
     E* out = (E*)p.o + row * p.so.b + hq * p.so.h;
     if (!steps) {
         if (tid < D) store1(out + tid, len > p.max_len ? __builtin_nanf("") : 0.f);
@@ -712,12 +719,13 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4DecodeParams p) {
 // Whole rows to the workgroups, with no parts to join, where there are as many (row, head) pairs for each slot of
 // the device as the longest row has steps.
 int kv4_groups(int rows, int heads, int G, int max_len, int D) {
-    const int step = kv4_step(D);
-    const int64_t slots = 256 * kKv4PerCu, pairs = (int64_t)heads * ((G + 15) / 16);
-    const int64_t steps = ((int64_t)max_len + step - 1) / step;
+    const int64_t slots = 256 * kv4_per_cu(D), pairs = (int64_t)heads * ((G + 15) / 16);
+    const int64_t steps = ((int64_t)max_len + kKv4Step - 1) / kKv4Step;
     if (steps == 1 || rows * pairs >= slots * steps) return 0;
     const int64_t most = std::min(rows, kPagedBlock) * steps;
-    return (int)std::max<int64_t>(1, std::min({slots / pairs, most, (int64_t)kPagedMaxGroups}));
+    const int64_t groups = std::max<int64_t>(1, std::min({slots / pairs, most, (int64_t)kPagedMaxGroups}));
+    const int64_t share = (most + groups - 1) / groups;  // of the longest rows; no more shares than come out even
+    return (int)((most + share - 1) / share);
 }
 
 int launch_attn_decode_kv4(const Kv4DecodeParams& p, int bf16, hipStream_t s) {
@@ -731,7 +739,7 @@ int launch_attn_decode_kv4(const Kv4DecodeParams& p, int bf16, hipStream_t s) {
             constexpr int HB = decltype(hb)::value;
             constexpr bool F = sizeof(E) == 4;
             Kv4DecodeParams a = p;
-            a.q_at = std::max(4 * heads * (D + 4) + 128, 4 * kv4_wave_floats(D, F, HB));
+            a.q_at = std::max(4 * heads * (D + 4) + 128, 4 * kv4_wave_floats(F, HB));
             const size_t lds = (size_t)(a.q_at + (F ? 3 * (HB == 16 ? heads : HB) * D / 2 : 0)) * sizeof(float);
             hipLaunchKernelGGL((kv4_split_kernel<D, E, HB>), grid, dim3(256), lds, s, a);
         };
