@@ -261,7 +261,7 @@ def test_decode_one_row(ia, n, D, dtype):
 def test_decode_many_rows(ia, dtype):
     """More rows than are shared out together, whole rows to the workgroups and in shares."""
     gen = torch.Generator().manual_seed(3)
-    for rows, heads, longest in ((300, 8, 500), (150, 1, 900)):
+    for rows, heads, longest in ((300, 8, 500), (150, 1, 900), (150, 1, 1400), (600, 4, 1300)):
         lens = torch.randint(0, longest + 1, (rows,), generator=gen).tolist()
         cache, ks, vs, _ = make_cache(ia, gen, lens, heads, 32, 32)
         q = torch.randn((rows, heads, 1, 32), generator=gen).to(dtype)
