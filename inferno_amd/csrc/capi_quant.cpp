@@ -132,7 +132,7 @@ int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int 
     if (rows < 0 || cols < 1 || rows > kMaxMN || cols > kMaxMN) return INF_ERR_BAD_SHAPE;
     if (transpose && rows < 1) return INF_ERR_BAD_SHAPE;
     if (rows == 0) return INF_OK;
-    if (inf::quantize_threads(rows, cols, transpose) > kMaxThreads) return INF_ERR_BAD_SHAPE;
+    if (inf::quantize_threads(rows, cols, transpose, esz(dt)) > kMaxThreads) return INF_ERR_BAD_SHAPE;
     int st = check_x(x, ldx, cols, dt);
     if (st != INF_OK) return st;
     if (!scale) return INF_ERR_NULL_POINTER;
@@ -188,7 +188,7 @@ int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, c
     if (!dtype_ok(dt)) return INF_ERR_BAD_DTYPE;
     int st = check_product(M, N, K);
     if (st != INF_OK || (st = check_x(x, ldx, K, dt)) || (st = check_i8(w, ldw, K))) return st;
-    if (inf::quantize_threads(M, K, 0) > kMaxThreads) return INF_ERR_BAD_SHAPE;
+    if (inf::quantize_threads(M, K, 0, esz(dt)) > kMaxThreads) return INF_ERR_BAD_SHAPE;
     const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K, false);
     if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, linear_bytes(plan, M, N, K))))
         return st;

@@ -313,7 +313,7 @@ __global__ __launch_bounds__(256) void gemm_i8_join_kernel(GemmI8Params p) {
 // every 16 outputs, 32 x 16384 x 4096 took 16 us, 13 so).  The waves' sums meet in LDS.
 //
 // FUSED: x comes as it is, and the workgroup quantises all of it while its first weights are on their way.
-// Every workgroup does, so that pays where x is small.
+// Every workgroup does, so that pays where x is small: 1 x 2304 x 768 fp32 4.9 us, of which 2 are a launch.
 // ============================================================================
 constexpr int kRowsWaves = 4;
 
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Par
     __shared__ __attribute__((aligned(16))) char r0[NW * STEP], r1[NW * STEP], r2[NW * STEP],
         r3[S > 3 ? NW * STEP : 16];
     extern __shared__ __attribute__((aligned(16))) char xq[];  // FUSED: [M][x_stride]
-    __shared__ float scales[32];
+    __shared__ float scales[8];
     __shared__ uint32_t tops[NW];
 
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
@@ -502,7 +502,10 @@ GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
     // 32 x 4096 x 16384 21 and 15.2.
     if (M <= 64 && (N + 31) / 32 <= 256 && steps <= 64) {
         plan.kind = GemmI8Plan::kRows;
-        plan.fused = !quantised && M * K <= 16384 && M <= 32;
+        // x quantised by every workgroup, where that takes no longer than a launch of its own (us, so and with one): 1 x 2304
+        // x 768 4.1 and 6.0, 1 x 4096 x 4096 6.9 and 7.8, 4 x 2304 x 768 4.8 and 6.2, 8 x 768 x 768 6.1 and 6.2; but 4 x 4096
+        // x 4096 13.1 and 8.2, 32 x 2304 x 64 9.1 and 5.9.
+        plan.fused = !quantised && (M == 1 || (M <= 8 && (M + 3) / 4 * K <= 1024));
         return plan;
     }
     // Tiles of 256, one workgroup a CU (us, theirs and tiles of 128, bf16 results): 4096 x 4096 x 4096 67 and 88, x 512 18.1 and

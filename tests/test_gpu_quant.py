@@ -49,7 +49,8 @@ def check_quantized(q, scale, x):
 
 
 SHAPES = [(1, 1), (3, 15), (5, 16), (7, 17), (2, 511), (9, 512), (3, 513), (4, 1024), (5, 1025), (2, 2048), (3, 2049),
-          (2, 4104), (1, 8192), (3, 9001), (2, 20000)]
+          (2, 4104), (1, 8192), (3, 9001), (2, 20000), (1025, 5), (1026, 500), (1027, 1024), (1024, 1025), (1100, 2048),
+          (1023, 700)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -205,9 +206,10 @@ def test_strided_products(ia):
             assert (rest == 77.0).all()
 
 
-# one kernel takes x as it is where M K is at most 16384
+# one kernel takes x as it is for one row, and for few short ones
 LINEARS = [(1, 2304, 768), (1, 100, 65), (1, 50, 16384), (1, 33, 16385), (31, 70, 528), (32, 100, 512), (3, 40, 2001),
-           (4, 4096, 4100), (7, 96, 1000), (16, 300, 4096), (33, 64, 128), (80, 200, 513), (260, 300, 96)]
+           (4, 4096, 4100), (7, 96, 1000), (16, 300, 4096), (33, 64, 128), (80, 200, 513), (260, 300, 96),
+           (1, 100, 8192), (2, 70, 1024), (4, 70, 1025), (5, 70, 130), (8, 70, 512), (8, 70, 513), (9, 70, 300)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
