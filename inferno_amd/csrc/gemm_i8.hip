@@ -89,6 +89,14 @@ struct Columns {
 // One barrier a step, before its last 32 k: by then every wave has read all of the step's operands (the last 32 k's are
 // in registers), so its buffer takes the loads of S steps on, while the products of these 32 k hide the first reads of
 // the next step's.
+//
+// What bounds it, and what it measured (bf16 results):
+//   tiles of 256 (two waves a SIMD, 128 KB of LDS): 16384 x 8192 x 8192 in 884-916 us, 2.4-2.5 POP/s, matrix cores busy
+//     67 % at 1.76 GHz: the power limit sets that clock.  Four waves of 128 x 128 took 1050, BK = 64 with S = 4 more too;
+//   tiles of 128 (two workgroups a CU, one's results leave while the other's products run): 8192 x 2304 x 768 in fp32
+//     30-35 us, of which 75 MB of results are 15 and every step of k 1.7: both in part in the open.  Tiles of 128 x
+//     192, 128 x 256 and 64 x 128 took 35-37, BK = 64 37;
+//   tiles of 64: weights, 32 x 16384 x 4096 in 12.7 us, 5.3 TB/s; or L2's latency and rate, 333 x 4096 x 4096 in 15.
 // ============================================================================
 template <typename E, int BN, int BM, int WN, int WM, int BK, int S, bool SPLIT>
 __global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * BK * S > 81920 ? 1 : 2) / 4) void gemm_i8_kernel(
@@ -251,7 +259,8 @@ __global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * BK * S > 81920
     }
 
     // Results leave in whole lines: each wave turns 32 rows of its block at a time in LDS (a lane holds runs of four
-    // columns of one row), pieces of 16 bytes at places that vary with the row, as above.
+    // columns of one row), pieces of 16 bytes at places that vary with the row, as above.  (From the registers, 16 bytes of
+    // 64 rows a store: 8192 x 2304 x 768 in fp32 48 us instead of 31.)
     __syncthreads();
     constexpr int U = BN / WN / 4;                       // pieces of four results in a wave's row
     constexpr int HOLD = (BN < BM ? BN : BM) * BK / (32 * U * 16);  // waves' blocks in an array of the ring

@@ -83,6 +83,7 @@ __device__ __forceinline__ void store1(E* dst, float v) {
 // ============================================================================
 // Append: a thread takes eight channels of a token's key and of its value, four neighbouring threads a block; channels
 // fastest, then heads, then tokens, as a projection's output lies.  The values are loaded while the token's page is looked up.
+// 8 prompts of 1024 tokens, 12 heads of 64, fp32: 57 MB in 8.3 us; 64 single tokens 3.1, a launch and three dependent reads.
 // ============================================================================
 namespace {
 
@@ -145,7 +146,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendParams p) {
 // ============================================================================
 // Read: positions first[row] + t as dense rows; zeros outside the row, NaN where its table names no page of the pool's.  A
 // thread takes CH channels of a key and of its value, one store of 16 bytes each (8 where bf16 rows are aligned to that
-// only), past the caches and in the results' order.
+// only), past the caches and in the results' order.  Bound by what it writes: 16 rows of 4512 positions, 8 heads of 128, bf16, in
+// 82 us, 4.6 TB/s read and written.  Stores that fill no whole line cost twice that past the caches (40 -> 97 us at 100 MB).
 // ============================================================================
 namespace {
 
@@ -259,7 +261,13 @@ int launch_kv4_read(const Kv4ReadParams& p, int bf16, hipStream_t s) {
 // (keys x heads), online softmax down the lane's column, O^T += V^T P^T; parts joined by a second launch.
 //
 // Keys and values become bf16 in registers, exactly.  fp32 queries and their probabilities are taken in three bf16
-// parts (24 bits), bf16 ones' probabilities in two.
+// parts (24 bits), bf16 ones' probabilities in two (2^-17, below the result's own rounding).
+//
+// Bound by memory, and near it by what the CUs do with it: 64 rows of up to 8191 keys, 8 heads of 128 with four query heads
+// each, bf16: 286 MB in 54-59 us, 4.9-5.3 TB/s (from the caches 39-45: the load path is busy for 68 % of the time, the vector
+// units for 40); 4 rows of 131071, two heads, eight query heads each: 143 MB in 31.3; 32 rows of 2048, 12 heads of 64, fp32:
+// 54 MB in 17, half of it waits.  The join's launch is another 4-5.  A step's loads ahead of the last one's products (two
+// register sets) gave nothing, nor did two or four workgroups a CU at D = 128.
 // ============================================================================
 namespace {
 
@@ -277,10 +285,13 @@ __device__ __forceinline__ int kv4_steps(int len, int max_len) {
 
 }  // namespace
 
-// HB: 16, or 1, 2, 4 or 8 (bf16), at least as many as there are query heads.  A product's result has heads along the
+// HB: 16, or 1, 2 or 4, at least as many as there are query heads.  A product's result has heads along the
 // lanes, so that with few of them most lanes' softmax would be for nothing: below 16, the wave's scores pass through LDS to
 // all lanes, 64 / HB of them a head, and the probabilities back.  And the columns that are left take the other bf16
 // parts of queries and probabilities, part k of head i in column k HB + i: one product instead of two or three.
+// (With the join, us, so and with 16: 32 rows of 2048 keys, 12 heads of 64, fp32, one query head each 19.1 and 24.2, two 20.7
+// and 24.0, four 23.1 and 24.8; 32 of 4096, 8 heads of 128, bf16, four 35.4 and 37.0; but eight in bf16, with a fourth kind,
+// 38.9 and 39.0.)
 template <int D, typename E, int HB>
 __global__ __launch_bounds__(256, kv4_per_cu(D)) void kv4_split_kernel(Kv4DecodeParams p) {
     constexpr bool F = sizeof(E) == 4;
@@ -749,7 +760,6 @@ int launch_attn_decode_kv4(const Kv4DecodeParams& p, int bf16, hipStream_t s) {
         if (heads == 1) go(integral_constant<int, 1>{});
         else if (heads == 2) go(integral_constant<int, 2>{});
         else if (heads <= 4) go(integral_constant<int, 4>{});
-        else if (heads <= 8 && sizeof(E) == 2) go(integral_constant<int, sizeof(E) == 2 ? 8 : 16>{});
         else go(integral_constant<int, 16>{});
         if (p.groups)
             hipLaunchKernelGGL((kv4_join_kernel<D, E>), dim3((unsigned)((int64_t)p.c.rows * p.Hq)), dim3(256), 0, s, p);
