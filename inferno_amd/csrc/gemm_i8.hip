@@ -524,8 +524,13 @@ GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
     const int64_t t256 = tiles(256), rounds = (t256 + 255) / 256;
     if (steps >= 4 && t256 * 10 >= rounds * 256 * (steps >= 16 ? 7 : 9)) {
         plan.kind = GemmI8Plan::k256;
-    } else if (tiles(128) >= 208) {  // 208 of them, 1664 x 2048 x 4096: 25.5, of 64 29.5; 192, 768 x 4096 x 4096: 25.3 and 22.8
+    } else if (tiles(128) >= (steps >= 24 ? 192 : 208)) {
+        // Of 128, three steps ahead where one a CU has nothing else to hide the memory (that fills its LDS): 2048 x 2048 x 4096
+        // 24.9, one step ahead 31.5, of 64 28.7; 768 x 4096 x 4096, 192 of them, 21.1, 25.3 and 22.8; but 1408 x 2048 x 4096, 176
+        // of them, 22.9 and of 64 21.1.  A shorter K, one step ahead and of 64: 2048 x 2048 x 2048 15.6 (three ahead 16.4) and
+        // 16.1, 1792 x 2048 x 1024 10.2 and 10.2; 208 of them, 1664 x 2048 x 4096 25.5 and 29.5.
         plan.kind = GemmI8Plan::k128;
+        plan.deep = tiles(128) <= 256 && steps >= 24;
     } else {
         plan.kind = GemmI8Plan::k64;
         // Where there is one tile a CU, or two, nothing but their own loads hides the memory: three steps ahead and one
@@ -569,7 +574,8 @@ static int launch_t(GemmI8Params p, const GemmI8Plan& plan, hipStream_t s) {
     } else if (plan.kind == GemmI8Plan::k256) {
         launch_tiles<E, 256, 256, 2, 4, 128, 2, false>(p, s);
     } else if (plan.kind == GemmI8Plan::k128) {
-        launch_tiles<E, 128, 128, 2, 2, 128, 2, false>(p, s);
+        if (plan.deep) launch_tiles<E, 128, 128, 2, 2, 128, 4, false>(p, s);
+        else launch_tiles<E, 128, 128, 2, 2, 128, 2, false>(p, s);
     } else if (p.ksplit > 1) {
         launch_tiles<E, 64, 64, 2, 2, 128, 4, true>(p, s);
         hipLaunchKernelGGL((gemm_i8_join_kernel<E>), dim3((unsigned)(((int64_t)p.M * (p.ldp / 4) + 255) / 256)),

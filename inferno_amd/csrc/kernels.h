@@ -488,7 +488,7 @@ struct GemmI8Plan {
     enum Kind { kRows, k64, k128, k256 } kind = kRows;  // few rows, or tiles of so many rows and columns
     int ksplit = 1, kchunk = 0;  // K ranges; more than one need ksplit * M * ldp sums of workspace
     bool fused = false;          // x is quantised by the product's kernel
-    bool deep = false;           // tiles of 64: loads three steps ahead
+    bool deep = false;           // tiles of 64 or 128: loads three steps ahead
 };
 // quantised: x is in 8 bits already.
 GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised);
