@@ -13,7 +13,7 @@ import torch
 
 from . import INF_BF16, INF_F32, PagedKV4Struct, Strides, default_scale, lib
 from .ops import _check
-from .paged import PagedKV, _bytes, _elsewhere, _on, _raw_stream, _size, _workspace
+from .paged import PagedKV, _bytes, _current_device, _elsewhere, _on, _raw_stream, _size
 
 _DT = {torch.float32: INF_F32, torch.bfloat16: INF_BF16}
 
@@ -36,20 +36,39 @@ def _strides(s):
 # device's number and give back what the call needs.
 
 
+def _away(index, device, stream):
+    """Whether a call on tensors of this device has to make another device or stream current first."""
+    return (stream is not None or index < 0 or index != _current_device()) and _elsewhere(device, stream)
+
+
+def _space(ws, nbytes, index, device):
+    """(tensor, pointer, bytes) of the workspace: the caller's, else a new one of nbytes() bytes."""
+    if ws is None:
+        n = nbytes()
+        if not n:
+            return None, None, 0
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+    elif ws.get_device() != index or not ws.is_contiguous():
+        raise ValueError(f"workspace: a dense tensor on {device} expected")
+    return ws, ws.data_ptr() or None, ws.nbytes
+
+
 def _matrix(t, name, index):
-    """(pointer, row stride) of a matrix on this device with adjacent elements in a row."""
-    if t.dim() != 2:
-        raise ValueError(f"{name}: a matrix expected, got {t.dim()} dimensions")
+    """(pointer, row stride, rows, columns) of a matrix on this device with adjacent elements in a row."""
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"{name}: a matrix expected, got {len(shape)} dimensions")
+    rows, cols = shape
     ld, step = t.stride()
-    if step != 1 and t.shape[1] > 1:
+    if step != 1 and cols > 1:
         raise ValueError(f"{name}: a matrix with adjacent elements in a row expected")
     if t.get_device() != index:
         raise ValueError(f"{name}: on {t.device}, the others on device {index}")
-    return t.data_ptr(), ld if ld > t.shape[1] or t.shape[0] > 1 else t.shape[1]
+    return t.data_ptr(), ld if rows > 1 or ld > cols else cols, rows, cols
 
 
 def _matrix_i8(t, name, index):
-    if t.dtype != torch.int8:
+    if t.dtype is not torch.int8:
         raise TypeError(f"{name}: int8 expected, got {t.dtype}")
     return _matrix(t, name, index)
 
@@ -58,11 +77,11 @@ def _vector(t, name, dtype, index, n):
     """The pointer of n dense elements of this type on this device (None stays None)."""
     if t is None:
         return None
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: {dtype} expected, got {t.dtype}")
     if t.get_device() != index:
         raise ValueError(f"{name}: on {t.device}, the others on device {index}")
-    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
+    if t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name}: {n} dense elements expected, got {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -75,18 +94,17 @@ def _rows16(n, cols, device):
 def quantize_i8(x, transpose=False, stream=None):
     """(q, scale): the rows of x [rows, cols] in 8 bits, q int8 [rows, cols] (rows on 16 bytes) and scale float32
     [rows]; with ``transpose`` its columns, q [cols, rows] and scale [cols] (weights [in, out])."""
-    dev = x.device
+    dev, index = x.device, x.get_device()
     dt = _float(x, "quantize_i8: x")
-    ptr, ld = _matrix(x, "quantize_i8: x", x.get_device())
-    if _elsewhere(dev, stream):
+    ptr, ld, rows, cols = _matrix(x, "quantize_i8: x", index)
+    if _away(index, dev, stream):
         with _on(dev, stream):
             return quantize_i8(x, transpose)
-    rows, cols = x.shape
     n, k = (cols, rows) if transpose else (rows, cols)
     q = _rows16(n, k, dev)
     scale = torch.empty(n, dtype=torch.float32, device=dev)
     st = lib().inf_quantize_i8(ptr, ld, rows, cols, int(bool(transpose)), q.data_ptr(), -(-k // 16) * 16,
-                               scale.data_ptr(), dt, _raw_stream(dev.index))
+                               scale.data_ptr(), dt, _raw_stream(index))
     _check(st, "inf_quantize_i8")
     return q, scale
 
@@ -111,23 +129,22 @@ def linear_i8_workspace(M, N, K, device="cuda"):
     return torch.empty(_product_bytes("inf_linear_i8_workspace", M, N, K), dtype=torch.uint8, device=device)
 
 
-def _result(out, name, shape, dtype, device):
-    """(tensor, pointer, row stride) of a result, a new one where none is given."""
+def _result(out, name, shape, dtype, like, index):
+    """(tensor, pointer, row stride) of a result, a new one beside `like` where none is given."""
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = like.new_empty(shape, dtype=dtype)
         return out, out.data_ptr(), shape[1]
-    if out.shape != shape or out.dtype != dtype:
+    if out.shape != shape or out.dtype is not dtype:
         raise ValueError(f"{name}: {list(shape)} of {dtype} expected, got {list(out.shape)} of {out.dtype}")
-    return out, *_matrix(out, name, device.index)
+    return out, *_matrix(out, name, index)[:2]
 
 
 def gemm_i8(x, x_scale, w, w_scale, bias=None, dtype=torch.float32, out=None, workspace=None, stream=None):
     """y [M, N] = x w^T times the scales of x's rows and w's rows, plus bias: x [M, K] and w [N, K] int8 with rows on
     16 bytes (quantize_i8's); y and bias of ``dtype``, float32 or bfloat16."""
     dev, index = x.device, x.get_device()
-    px, ldx = _matrix_i8(x, "gemm_i8: x", index)
-    pw, ldw = _matrix_i8(w, "gemm_i8: w", index)
-    (M, K), (N, Kw) = x.shape, w.shape
+    px, ldx, M, K = _matrix_i8(x, "gemm_i8: x", index)
+    pw, ldw, N, Kw = _matrix_i8(w, "gemm_i8: w", index)
     if K != Kw:
         raise ValueError(f"gemm_i8: x [M, K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
     dtype = out.dtype if out is not None else dtype
@@ -136,13 +153,13 @@ def gemm_i8(x, x_scale, w, w_scale, bias=None, dtype=torch.float32, out=None, wo
     psx = _vector(x_scale, "gemm_i8: x_scale", torch.float32, index, M)
     psw = _vector(w_scale, "gemm_i8: w_scale", torch.float32, index, N)
     pb = _vector(bias, "gemm_i8: bias", dtype, index, N)
-    if _elsewhere(dev, stream):
+    if _away(index, dev, stream):
         with _on(dev, stream):
             return gemm_i8(x, x_scale, w, w_scale, bias, dtype, out, workspace)
-    y, py, ldy = _result(out, "gemm_i8: out", (M, N), dtype, dev)
+    y, py, ldy = _result(out, "gemm_i8: out", (M, N), dtype, x, index)
     if M == 0:
         return y
-    ws, ptr, n = _workspace(workspace, lambda: _product_bytes("inf_gemm_i8_workspace", M, N, K), dev)
+    ws, ptr, n = _space(workspace, lambda: _product_bytes("inf_gemm_i8_workspace", M, N, K), index, dev)
     st = lib().inf_gemm_i8(M, N, K, px, ldx, psx, pw, ldw, psw, pb, py, ldy, _DT[dtype], ptr, n, _raw_stream(index))
     _check(st, "inf_gemm_i8")
     return y
@@ -153,20 +170,19 @@ def linear_i8(x, w, w_scale, bias=None, out=None, workspace=None, stream=None):
     ``transpose`` where they are held [in, out]); x [M, K] is taken in 8 bits row by row, y and bias have its type."""
     dev, index = x.device, x.get_device()
     dt = _float(x, "linear_i8: x")
-    px, ldx = _matrix(x, "linear_i8: x", index)
-    pw, ldw = _matrix_i8(w, "linear_i8: w", index)
-    (M, K), (N, Kw) = x.shape, w.shape
+    px, ldx, M, K = _matrix(x, "linear_i8: x", index)
+    pw, ldw, N, Kw = _matrix_i8(w, "linear_i8: w", index)
     if K != Kw:
         raise ValueError(f"linear_i8: x [M, K] and w [N, K] expected, got {tuple(x.shape)} and {tuple(w.shape)}")
     psw = _vector(w_scale, "linear_i8: w_scale", torch.float32, index, N)
     pb = _vector(bias, "linear_i8: bias", x.dtype, index, N)
-    if _elsewhere(dev, stream):
+    if _away(index, dev, stream):
         with _on(dev, stream):
             return linear_i8(x, w, w_scale, bias, out, workspace)
-    y, py, ldy = _result(out, "linear_i8: out", (M, N), x.dtype, dev)
+    y, py, ldy = _result(out, "linear_i8: out", (M, N), x.dtype, x, index)
     if M == 0:
         return y
-    ws, ptr, n = _workspace(workspace, lambda: _product_bytes("inf_linear_i8_workspace", M, N, K), dev)
+    ws, ptr, n = _space(workspace, lambda: _product_bytes("inf_linear_i8_workspace", M, N, K), index, dev)
     st = lib().inf_linear_i8(M, N, K, px, ldx, pw, ldw, psw, pb, py, ldy, dt, ptr, n, _raw_stream(index))
     _check(st, "inf_linear_i8")
     return y
@@ -242,7 +258,7 @@ def kv4_append(cache, k, v, counts=None, stream=None):
     pk, sk = _tokens(k, "kv4_append: k", cache, T)
     pv, sv = _tokens(v, "kv4_append: v", cache, T)
     pc = _vector(counts, "counts", torch.int32, cache.index, cache.rows)
-    if _elsewhere(cache.device, stream):
+    if _away(cache.index, cache.device, stream):
         with _on(cache.device, stream):
             return kv4_append(cache, k, v, counts)
     st = lib().inf_kv4_append(cache.ref, pk, sk, pv, sv, pc, T, dt, _raw_stream(cache.index))
@@ -263,7 +279,7 @@ def kv4_read(cache, T, first=None, dtype=torch.float32, k_out=None, v_out=None, 
     if dt is None:
         raise TypeError(f"kv4_read: float32 or bfloat16 expected, got {dtype}")
     pf = _vector(first, "first", torch.int32, cache.index, cache.rows)
-    if _elsewhere(cache.device, stream):
+    if _away(cache.index, cache.device, stream):
         with _on(cache.device, stream):
             return kv4_read(cache, T, first, dtype, k_out, v_out)
     if k_out is None:
@@ -300,14 +316,14 @@ def attn_decode_kv4(q, cache, scale=None, max_len=None, out=None, workspace=None
         raise ValueError(f"attn_decode_kv4: q must be on {cache.device}")
     heads = shape[1]
     max_len = cache.capacity if max_len is None else int(max_len)
-    if _elsewhere(cache.device, stream):
+    if _away(cache.index, cache.device, stream):
         with _on(cache.device, stream):
             return attn_decode_kv4(q, cache, scale, max_len, out, workspace)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype != q.dtype or out.get_device() != cache.index:
         raise ValueError("attn_decode_kv4: out must be like q")
-    ws, ptr, n = _workspace(workspace, lambda: _decode_bytes(cache, heads, max_len), cache.device)
+    ws, ptr, n = _space(workspace, lambda: _decode_bytes(cache, heads, max_len), cache.index, cache.device)
     st = lib().inf_attn_decode_kv4(cache.ref, q.data_ptr(), _strides(q.stride()), out.data_ptr(),
                                    _strides(out.stride()), heads, max_len,
                                    cache.scale if scale is None else float(scale), dt, ptr, n,
