@@ -283,7 +283,7 @@ def kv4_read(cache, T, first=None, dtype=torch.float32, k_out=None, v_out=None, 
         with _on(cache.device, stream):
             return kv4_read(cache, T, first, dtype, k_out, v_out)
     if k_out is None:
-        k_out = torch.empty((cache.rows, cache.heads, max(T, 0), cache.D), dtype=dtype, device=cache.device)
+        k_out = cache.k.new_empty((cache.rows, cache.heads, max(T, 0), cache.D), dtype=dtype)
         v_out = torch.empty_like(k_out)
         pk, pv = k_out.data_ptr(), v_out.data_ptr()
         sk = sv = _strides(k_out.stride())
