@@ -267,7 +267,8 @@ int launch_kv4_read(const Kv4ReadParams& p, int bf16, hipStream_t s) {
 // each, bf16: 286 MB in 54-59 us, 4.9-5.3 TB/s (from the caches 39-45: the load path is busy for 68 % of the time, the vector
 // units for 40); 4 rows of 131071, two heads, eight query heads each: 143 MB in 31.3; 32 rows of 2048, 12 heads of 64, fp32:
 // 54 MB in 17, half of it waits.  The join's launch is another 4-5.  A step's loads ahead of the last one's products (two
-// register sets) gave nothing, nor did two or four workgroups a CU at D = 128.
+// register sets) gave nothing, nor did two or four workgroups a CU at D = 128; two tiles' values in one load of twice the width,
+// exchanged between neighbouring lanes, took 61, 34.5 and 18.3.
 // ============================================================================
 namespace {
 
@@ -368,8 +369,8 @@ __global__ __launch_bounds__(256, kv4_per_cu(D)) void kv4_split_kernel(Kv4Decode
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_at[i] = (4 * g + i) * (uint32_t)p.c.sv.t + col * (VD / 2);
     // A step's scales come in one load: tile t's of keys 4 q .. and block b to lane t + T q + 4 T b, and from there to
-    // the lanes that need them.  (A load costs the same at any width: with two of each tile's scales, 4 rows of 131071 keys took
-    // 32.4 us, 31.3 so.)
+    // the lanes that need them.  (With two loads for each tile's scales, 4 rows of 131071 keys took 32.4 us,
+    // 31.3 so.)
     static_assert(4 * T * NK <= 64, "a lane for every four scales");
     const int scale_block = min(lane / (4 * T), NK - 1), scale_key = lane / T % 4 * 4;
     const uint8_t* KS = p.c.ks + h * p.c.sks.h + scale_block * p.c.sks.t + scale_key;
