@@ -170,16 +170,17 @@ int check_cache4(const inf_paged_kv4* c, bool written, inf::Paged4View* out) {
     return INF_OK;
 }
 
-// The decode's workspace: as DecodeSizes, without scores.
+// The decode's workspace: as DecodeSizes, without scores.  `most`: enough for every shorter max_len too (shares that
+// come out even may be more of them at a shorter one).
 struct Decode4Sizes {
     int groups;
     size_t part, stats, first;
     size_t total() const { return part + stats + first; }
 };
-Decode4Sizes decode4_sizes(const inf_paged_kv4* c, int q_heads, int max_len) {
+Decode4Sizes decode4_sizes(const inf_paged_kv4* c, int q_heads, int max_len, bool most = false) {
     Decode4Sizes s{};
     const int blocks = inf::paged_blocks(c->rows);
-    s.groups = inf::kv4_groups(c->rows, c->heads, q_heads / c->heads, max_len, c->D);
+    s.groups = inf::kv4_groups(c->rows, c->heads, q_heads / c->heads, max_len, c->D, most);
     if (s.groups == 0) return s;
     const size_t parts = ((size_t)c->rows + (size_t)blocks * s.groups) * q_heads;
     s.part = round_up(parts * c->D * sizeof(float));
@@ -470,7 +471,7 @@ int inf_attn_decode_kv4_workspace(const inf_paged_kv4* cache, int q_heads, int m
     *out_bytes = 0;
     const int st = check_decode4(cache, q_heads, max_len);
     if (st != INF_OK) return st;
-    *out_bytes = decode4_sizes(cache, q_heads, max_len).total();
+    *out_bytes = decode4_sizes(cache, q_heads, max_len, true).total();
     return INF_OK;
 }
 

@@ -544,7 +544,8 @@ struct Kv4DecodeParams {
 };
 // Keys that a workgroup takes per step.
 constexpr int kKv4Step = 256;
-int kv4_groups(int rows, int heads, int G, int max_len, int D);
+// Shares of a block of rows; `most`: an upper bound of it, which no shorter max_len exceeds.
+int kv4_groups(int rows, int heads, int G, int max_len, int D, bool most = false);
 
 int launch_kv4_append(const Kv4AppendParams& p, int bf16, hipStream_t s);
 int launch_kv4_read(const Kv4ReadParams& p, int bf16, hipStream_t s);

@@ -732,14 +732,15 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4DecodeParams p) {
 // graph replays, whole and shared out, us: one row, 12 heads fp32, 500 keys 5.4 and 7.8, 1000 7.4 and 7.7; 32 rows
 // 7.5 and 10.6, 11.3 and 13.6), and where there are as many (row, head) pairs for each slot of the device as the
 // longest row has steps.
-int kv4_groups(int rows, int heads, int G, int max_len, int D) {
+int kv4_groups(int rows, int heads, int G, int max_len, int D, bool most) {
     const int64_t slots = 256 * kv4_per_cu(D), pairs = (int64_t)heads * ((G + 15) / 16);
     const int64_t steps = ((int64_t)max_len + kKv4Step - 1) / kKv4Step;
     if (steps <= 4 || rows * pairs >= slots * steps) return 0;
-    const int64_t most = std::min(rows, kPagedBlock) * steps;
-    const int64_t groups = std::max<int64_t>(1, std::min({slots / pairs, most, (int64_t)kPagedMaxGroups}));
-    const int64_t share = (most + groups - 1) / groups;  // of the longest rows; no more shares than come out even
-    return (int)((most + share - 1) / share);
+    const int64_t all = std::min(rows, kPagedBlock) * steps;
+    const int64_t groups = std::max<int64_t>(1, std::min({slots / pairs, all, (int64_t)kPagedMaxGroups}));
+    if (most) return (int)groups;
+    const int64_t share = (all + groups - 1) / groups;  // of the longest rows; no more shares than come out even
+    return (int)((all + share - 1) / share);
 }
 
 int launch_attn_decode_kv4(const Kv4DecodeParams& p, int bf16, hipStream_t s) {
