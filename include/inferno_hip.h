@@ -578,15 +578,16 @@ int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int 
  * (K < 2^17); then in fp32, in this order (the sum times x_scale has to be finite); y and bias (may be NULL) fp32 or bf16
  * by dt, rounded once.  Rows of x and w lie on 16 bytes and are read
  * in pieces of 16 (up to K in whole 16 bytes; what lies behind K does not matter).  y must not overlap what is read.
- * workspace: inf_gemm_i8_workspace bytes (may be 0: then NULL), 256-byte aligned.  Calls that share one must not
- * overlap.  The same bits on every run. */
+ * workspace: inf_gemm_i8_workspace bytes (may be 0: then NULL), 256-byte aligned; M rows' is enough for fewer.  Calls
+ * that share one must not overlap.  The same bits on every run. */
 int inf_gemm_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes);
 int inf_gemm_i8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, const float* x_scale, const int8_t* w,
                 int64_t ldw, const float* w_scale, const void* bias, void* y, int64_t ldy, inf_dtype dt,
                 void* workspace, size_t ws_bytes, void* stream);
 
 /* A linear layer with weights in 8 bits: inf_quantize_i8 of the rows of x [M, K] (fp32 or bf16 by dt, as y), then
- * inf_gemm_i8, to the same bits.  workspace: inf_linear_i8_workspace bytes (may be 0: then NULL), 256-byte aligned. */
+ * inf_gemm_i8, to the same bits.  workspace: inf_linear_i8_workspace bytes (may be 0: then NULL), 256-byte aligned; M
+ * rows' is enough for fewer. */
 int inf_linear_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes);
 int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const int8_t* w, int64_t ldw,
                   const float* w_scale, const void* bias, void* y, int64_t ldy, inf_dtype dt, void* workspace,

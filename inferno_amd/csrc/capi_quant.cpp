@@ -2,6 +2,7 @@
 // validation on the host, workspace sizing, launches.  Nothing here allocates.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
 
@@ -50,6 +51,16 @@ size_t q_bytes(int64_t M, int64_t K) { return round_up((size_t)M * whole16(K)); 
 size_t scale_bytes(int64_t M) { return round_up((size_t)M * 4); }
 size_t linear_bytes(const inf::GemmI8Plan& plan, int64_t M, int64_t N, int64_t K) {
     return plan.fused ? 0 : q_bytes(M, K) + scale_bytes(M) + part_bytes(plan, M, N);
+}
+
+// Bytes of up to M rows: fewer rows may have more K ranges, and so need more.
+template <typename F>
+size_t most_bytes(int64_t M, int64_t N, int64_t K, bool quantised, F bytes) {
+    size_t n = bytes(inf::gemm_i8_plan(M, N, K, quantised), M);
+    const int64_t split = inf::gemm_i8_split_rows(N);
+    for (int64_t m = 64; m < M && m <= split; m += 64)
+        n = std::max(n, bytes(inf::gemm_i8_plan(m, N, K, quantised), m));
+    return n;
 }
 
 // Whether y [M, N] lies over the n bytes from a on (which may be null: then not).
@@ -149,7 +160,8 @@ int inf_gemm_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes) {
     if (!out_bytes) return INF_ERR_NULL_POINTER;
     *out_bytes = 0;
     const int st = check_product(M, N, K);
-    if (st == INF_OK) *out_bytes = part_bytes(inf::gemm_i8_plan(M, N, K, true), M, N);
+    if (st == INF_OK)
+        *out_bytes = most_bytes(M, N, K, true, [&](const auto& plan, int64_t m) { return part_bytes(plan, m, N); });
     return st;
 }
 
@@ -178,7 +190,8 @@ int inf_linear_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes) 
     if (!out_bytes) return INF_ERR_NULL_POINTER;
     *out_bytes = 0;
     const int st = check_product(M, N, K);
-    if (st == INF_OK) *out_bytes = linear_bytes(inf::gemm_i8_plan(M, N, K, false), M, N, K);
+    if (st == INF_OK)
+        *out_bytes = most_bytes(M, N, K, false, [&](const auto& plan, int64_t m) { return linear_bytes(plan, m, N, K); });
     return st;
 }
 

@@ -500,6 +500,10 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Par
 
 // K ranges are whole steps of any kernel.
 constexpr int kI8Step = 128;
+// Tiles of 64 by ranges, at most.
+constexpr int kI8Ranges = 384;
+
+int64_t gemm_i8_split_rows(int64_t N) { return 64 * (kI8Ranges / 2 / ((N + 63) / 64)); }
 
 GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
     GemmI8Plan plan;
@@ -539,7 +543,7 @@ GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
         plan.deep = tiles(64) <= 512 && steps >= 16;
         // K ranges, for a join of about 5 us, where they take 24 steps off the longest: 128 x 1024 x 8192 9.9 in eight,
         // 15.7 in one; 200 x 2048 x 4096 (three) 11.9 and 9.9.
-        const int64_t ks = std::min<int64_t>(384 / tiles(64), steps / 8);
+        const int64_t ks = std::min<int64_t>(kI8Ranges / tiles(64), steps / 8);
         if (ks > 1 && steps * (ks - 1) > 24 * ks) {
             plan.kchunk = (int)((steps + ks - 1) / ks * kI8Step);
             plan.ksplit = (int)((K + plan.kchunk - 1) / plan.kchunk);

@@ -492,6 +492,8 @@ struct GemmI8Plan {
 };
 // quantised: x is in 8 bits already.
 GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised);
+// Rows past which no product has K ranges.  Up to there a plan is that of all numbers of rows in the same 64.
+int64_t gemm_i8_split_rows(int64_t N);
 int launch_gemm_i8(const GemmI8Params& p, const GemmI8Plan& plan, int bf16, hipStream_t s);
 
 // ---- a paged key-value cache in 4 bits (paged4.hip) -----------------------------

@@ -120,12 +120,12 @@ def _product_bytes(call, M, N, K):
 
 
 def gemm_i8_workspace(M, N, K, device="cuda"):
-    """A workspace for gemm_i8 of these sizes."""
+    """A workspace for gemm_i8 of these sizes, or of fewer rows."""
     return torch.empty(_product_bytes("inf_gemm_i8_workspace", M, N, K), dtype=torch.uint8, device=device)
 
 
 def linear_i8_workspace(M, N, K, device="cuda"):
-    """A workspace for linear_i8 of these sizes."""
+    """A workspace for linear_i8 of these sizes, or of fewer rows."""
     return torch.empty(_product_bytes("inf_linear_i8_workspace", M, N, K), dtype=torch.uint8, device=device)
 
 
@@ -300,7 +300,7 @@ def _decode_bytes(cache, q_heads, max_len):
 
 
 def attn_decode_kv4_workspace(cache, q_heads, max_len=None):
-    """A workspace for attn_decode_kv4 with these arguments."""
+    """A workspace for attn_decode_kv4 with these arguments, or a shorter max_len."""
     n = _decode_bytes(cache, q_heads, cache.capacity if max_len is None else max_len)
     return torch.empty(n, dtype=torch.uint8, device=cache.device)
 

@@ -7,7 +7,7 @@ import pytest
 
 import inferno_amd as ia
 from inferno_amd import Strides
-from test_quant_args import FAKE, cache, decode
+from test_quant_args import FAKE, cache, decode, linear
 
 ODD = FAKE + 16
 
@@ -36,3 +36,27 @@ def test_decode_workspace_of_the_longest(rows, heads, hq, D, longest):
             assert decode(c, sq=q, so=q, hq=hq, max_len=max_len, ws=ODD, n=whole) == 7
             assert decode(c, sq=q, so=q, hq=hq, max_len=max_len, ws=ODD, n=n) == 7
             assert decode(c, sq=q, so=q, hq=hq, max_len=max_len, ws=ODD, n=255) == 6
+
+
+def product_bytes(call, M, N, K):
+    n = ctypes.c_size_t()
+    assert getattr(ia.lib(), f"inf_{call}_i8_workspace")(M, N, K, ctypes.byref(n)) == 0
+    return n.value
+
+
+# one short K range, several, none; few outputs and many; the few-row kernel's border and past it
+@pytest.mark.parametrize("N,K", [(4096, 16384), (1024, 8192), (130, 9000), (2048, 4096), (33, 100000), (64, 131071),
+                                 (768, 768), (16384, 4096), (50257, 768), (1, 1), (300, 8192), (8193, 8193)])
+def test_product_workspace_of_the_most_rows(N, K):
+    ld = -(-K // 16) * 16
+    rows = (*range(1, 300), *range(300, 1400, 37), 2047, 2048, 2049, 4096, 8192)
+    for call in ("gemm", "linear"):
+        before = 0
+        for M in rows:
+            n = product_bytes(call, M, N, K)
+            assert n >= before  # one's is enough for all before it
+            before = n
+    for M in rows[8:]:  # from nine rows on the linear layer needs some
+        args = dict(M=M, N=N, K=K, ldx=ld, ldw=ld, ldy=N, y=1 << 50, ws=ODD)
+        assert linear(**args, n=product_bytes("linear", M, N, K)) == 7
+        assert linear(**args, n=M * K - 1) == 6
