@@ -554,7 +554,8 @@ int inf_kv4_append(const inf_paged_kv4* cache, const void* k, inf_strides sk, co
 
 /* Reads positions first[n] .. first[n] + T - 1 of every row (first: device, [rows]; NULL: from 0) into k, v
  * [rows, heads, T, D] (fp32 or bf16 by dt, both exact), as the dense attention takes them: what follows a long prompt
- * attends to.  Positions outside the row (negative, or at or past lens[n]) are zeros, in a page outside the pool NaN. */
+ * attends to.  Positions outside the row (negative, or at or past lens[n]) are zeros, in a page outside the pool NaN.
+ * k and v must overlap neither each other nor the cache or first. */
 int inf_kv4_read(const inf_paged_kv4* cache, const int32_t* first, int T, void* k, inf_strides sk, void* v,
                  inf_strides sv, inf_dtype dt, void* stream);
 

@@ -12,6 +12,7 @@
 
 #include "inferno_hip.h"
 #include "kernels.h"
+#include "overlap.h"
 
 namespace {
 
@@ -169,6 +170,26 @@ int check_cache4(const inf_paged_kv4* c, bool written, inf::Paged4View* out) {
                            page_shift(c->page_size), c->D};
     return INF_OK;
 }
+
+inf::Memory memory(const void* p, const inf_strides& s, int64_t B, int64_t H, int64_t T, int64_t D, int es) {
+    return {p, B, s.b * es, H, s.h * es, T, s.t * es, D * es};
+}
+inf::Memory ints(const int32_t* p, int64_t n) { return {p, 4 * n}; }
+
+// What a call reads of the cache.
+struct CacheMemory {
+    inf::Memory k, v, ks, vs, table, lens;
+    explicit CacheMemory(const inf_paged_kv4& c)
+        : k(memory(c.k, c.sk, c.n_pages, c.heads, c.page_size, c.D / 2, 1)),
+          v(memory(c.v, c.sv, c.n_pages, c.heads, c.page_size, c.D / 2, 1)),
+          ks(memory(c.k_scale, c.sks, c.n_pages, c.heads, c.D / 32, c.page_size, 1)),
+          vs(memory(c.v_scale, c.svs, c.n_pages, c.heads, c.D / 32, c.page_size, 1)),
+          table(c.table, c.rows, 4 * c.table_stride, 4 * (int64_t)c.max_pages),
+          lens(ints(c.lens, c.rows)) {}
+    bool over(const inf::Memory& m) const {
+        return m.over(k) || m.over(v) || m.over(ks) || m.over(vs) || m.over(table) || m.over(lens);
+    }
+};
 
 // The decode's workspace: as DecodeSizes, without scores.  `most`: enough for every shorter max_len too (shares that
 // come out even may be more of them at a shorter one).
@@ -458,6 +479,11 @@ int inf_kv4_read(const inf_paged_kv4* cache, const int32_t* first, int T, void* 
     // a workgroup takes at least 32 positions of a head
     if ((int64_t)T * cache->heads * cache->D > kMaxBlocks || (T / 32 + 1) * (int64_t)cache->heads * 256 > kMaxThreads)
         return INF_ERR_BAD_SHAPE;
+    // other workgroups still read the cache, and write the other result
+    const inf::Memory mk = memory(k, sk, cache->rows, cache->heads, T, cache->D, es),
+                      mv = memory(v, sv, cache->rows, cache->heads, T, cache->D, es), mf = ints(first, cache->rows);
+    const CacheMemory held(*cache);
+    if (mk.over(mv) || held.over(mk) || held.over(mv) || mk.over(mf) || mv.over(mf)) return INF_ERR_BAD_STRIDE;
     p.k = k; p.v = v;
     p.sk = view(sk); p.sv = view(sv);
     p.first = first;

@@ -42,3 +42,52 @@ def test_linear_with_one_workspace(ia, N, K):
         assert torch.equal(ia.linear_i8(x[:M], w, sw, workspace=ws), want)
         q, s = ia.quantize_i8(x[:M])
         assert torch.equal(ia.gemm_i8(q, s, w, sw, dtype=BF16, workspace=product_ws), want)
+
+
+class Arena:
+    """Tensors one behind the other in one piece of memory."""
+
+    def __init__(self, nbytes):
+        self.data, self.at = torch.zeros(nbytes, dtype=torch.uint8, device="cuda"), 0
+
+    def take(self, shape, dtype):
+        n = torch.empty(shape, dtype=dtype, device="meta").nbytes
+        t = self.data[self.at:self.at + n].view(dtype).view(shape)
+        self.at += -(-n // 16) * 16
+        return t
+
+
+def in_one_arena(ia, cache, arena):
+    """The same cache with a page's keys, their scales, values and theirs side by side, then its table and lengths."""
+    pages, heads, P, half = cache.k.shape
+    parts = [cache.k, cache.k_scale, cache.v, cache.v_scale]
+    page = arena.take((pages, sum(t[0].numel() for t in parts)), torch.uint8)
+    mine, at = [], 0
+    for t in parts:
+        n = t[0].numel()
+        mine.append(page[:, at:at + n].unflatten(1, t.shape[1:]))
+        mine[-1].copy_(t)
+        at += n
+    table, lens = arena.take(cache.table.shape, torch.int32), arena.take(cache.lens.shape, torch.int32)
+    table.copy_(cache.table)
+    lens.copy_(cache.lens)
+    return ia.PagedKV4(mine[0], mine[2], mine[1], mine[3], table, lens)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_read_beside_the_cache(ia, D):
+    """Cache and results in one piece of memory, keys and values beside each other."""
+    gen = torch.Generator().manual_seed(D)
+    cache, ks, vs, _ = make_cache(ia, gen, [9, 30], 2, D, 16)
+    for dtype in (F32, BF16):
+        arena = Arena(1 << 20)
+        both = arena.take((2, 30, 2, 2, D), dtype)
+        here = in_one_arena(ia, cache, arena)
+        other = arena.take((2, 2, 30, 2, D), dtype)
+        first = arena.take((2,), torch.int32)
+        for k, v in ((both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)), (other[:, :, :, 0], other[:, :, :, 1])):
+            ia.kv4_read(here, 30, first=first, k_out=k, v_out=v)
+            assert torch.equal(k[1].cpu().double(), ks[1]) and torch.equal(v[1].cpu().double(), vs[1])
+            assert torch.equal(v[0, :, :9].cpu().double(), vs[0]) and not k[0, :, 9:].any()
+        with pytest.raises(ia.InfernoError):
+            ia.kv4_read(here, 30, k_out=k, v_out=k)

@@ -1,0 +1,55 @@
+"""Results of weights in 8 bits and a cache in 4 that lie over what other workgroups still read or write: refused on the
+host, without a GPU (every call here is refused, so it returns before any HIP call)."""
+import ctypes
+
+import pytest
+
+import inferno_amd as ia
+from inferno_amd import Strides
+from test_quant_args import cache
+
+OVERLAP = 3
+BIG = 1 << 34
+# a cache of 4 rows, 2 heads of 64, 32 pages of 16 slots: what lies where, and its bytes
+POOL = dict(k=32 * 1024, v=32 * 1024, k_scale=32 * 64, v_scale=32 * 64, table=4 * 4 * 4, lens=16)
+AT = {name: (i + 1) * BIG for i, name in enumerate(POOL)}
+
+
+def far_cache(**kw):
+    return cache(**{**AT, **kw})
+
+
+def places(of, n, m, align):
+    """Addresses of n bytes that meet the m bytes from `of` on, at either end and inside."""
+    return sorted({of, of + (m - 1) // align * align, of - (n - 1) // align * align, of + m // 2 // align * align})
+
+
+NEW = Strides(8 * 2 * 64, 64, 2 * 64, 1)  # [rows, heads, T, D] out of [rows, T, heads, D]
+NEW_BYTES = 4 * 8 * 2 * 64 * 4
+
+
+def read(c, k, v, first=None, s=NEW, sv=None, T=8, dt=0):
+    return ia.lib().inf_kv4_read(ctypes.byref(c), first, T, k, s, v, sv or s, dt, None)
+
+
+@pytest.mark.parametrize("what", POOL)
+def test_read_over_the_cache(what):
+    for at in places(AT[what], NEW_BYTES, POOL[what], 16):
+        assert read(far_cache(), at, 20 * BIG) == OVERLAP
+        assert read(far_cache(), 20 * BIG, at) == OVERLAP
+
+
+def test_read_over_its_arguments():
+    for at in places(20 * BIG, NEW_BYTES, NEW_BYTES, 16):
+        assert read(far_cache(), 20 * BIG, at) == OVERLAP  # keys over values
+        assert read(far_cache(), 20 * BIG, at, sv=Strides(8 * 2 * 64, 8 * 64, 64, 1)) == OVERLAP
+    for at in places(21 * BIG, NEW_BYTES, 16, 16):
+        assert read(far_cache(), at, 20 * BIG, first=21 * BIG) == OVERLAP
+        assert read(far_cache(), 20 * BIG, at, first=21 * BIG) == OVERLAP
+
+
+def test_read_side_by_side_but_one():
+    """Keys and values out of [rows, T, 3, heads, D], where the values begin a head early."""
+    s = Strides(8 * 3 * 128, 64, 3 * 128, 1)
+    assert read(far_cache(), 20 * BIG, 20 * BIG + 4 * 64, s=s) == OVERLAP
+    assert read(far_cache(), 20 * BIG, 20 * BIG + 4 * 5 * 64, s=s) == OVERLAP  # the next token's
