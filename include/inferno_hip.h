@@ -560,7 +560,8 @@ int inf_kv4_read(const inf_paged_kv4* cache, const int32_t* first, int T, void* 
                  inf_strides sv, inf_dtype dt, void* stream);
 
 /* Attention of one new token per row over its whole cache, as inf_attn_decode_paged (without weights); q and o are fp32 or
- * bf16 by dt.  A workspace of max_len's size is enough for every shorter one. */
+ * bf16 by dt.  o may be q itself, but not overlap it in part, nor the cache; the workspace must overlap none of them.
+ * One of max_len's size is enough for every shorter one. */
 int inf_attn_decode_kv4_workspace(const inf_paged_kv4* cache, int q_heads, int max_len, size_t* out_bytes);
 int inf_attn_decode_kv4(const inf_paged_kv4* cache, const void* q, inf_strides sq, void* o, inf_strides so,
                         int q_heads, int max_len, float scale, inf_dtype dt, void* workspace, size_t ws_bytes,

@@ -520,6 +520,16 @@ int inf_attn_decode_kv4(const inf_paged_kv4* cache, const void* q, inf_strides s
         return INF_ERR_BAD_SHAPE;
     if (s.total() && (!workspace || ws_bytes < s.total())) return INF_ERR_WORKSPACE;
     if (s.total() && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
+    // other workgroups still read these while one writes; a workgroup's own queries are read before
+    const inf::Memory mq = memory(q, sq, cache->rows, q_heads, 1, cache->D, es),
+                      mo = memory(o, so, cache->rows, q_heads, 1, cache->D, es);
+    const bool same = q == o && (cache->rows == 1 || sq.b == so.b) && (q_heads == 1 || sq.h == so.h);
+    const CacheMemory held(*cache);
+    if ((!same && mo.over(mq)) || held.over(mo)) return INF_ERR_BAD_STRIDE;
+    if (s.total()) {
+        const inf::Memory mw(workspace, (int64_t)s.total());
+        if (mw.over(mq) || mw.over(mo) || held.over(mw)) return INF_ERR_BAD_STRIDE;
+    }
     p.q = q; p.o = o;
     p.sq = view(sq); p.so = view(so);
     p.Hq = q_heads;

@@ -91,3 +91,27 @@ def test_read_beside_the_cache(ia, D):
             assert torch.equal(v[0, :, :9].cpu().double(), vs[0]) and not k[0, :, 9:].any()
         with pytest.raises(ia.InfernoError):
             ia.kv4_read(here, 30, k_out=k, v_out=k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens", [[40, 700], [0, 3001]])
+def test_attention_beside_the_cache(ia, lens, dtype):
+    """Queries, cache, workspace and results in one piece of memory; results in the queries' place, whole rows to the
+    workgroups and in shares."""
+    gen = torch.Generator().manual_seed(lens[1])
+    cache, ks, vs, _ = make_cache(ia, gen, lens, 2, 64, 16)
+    n = ia.attn_decode_kv4_workspace(cache, 6).nbytes
+    assert bool(n) == (lens[1] > 1024)
+    arena = Arena(n + (2 << 20))
+    ws = arena.take((n,), torch.uint8)  # at the start: on 256 bytes
+    both = arena.take((2, 12, 1, 64), dtype)
+    here = in_one_arena(ia, cache, arena)
+    q = torch.randn((2, 6, 1, 64), generator=gen).to(dtype)
+    both[:, :6].copy_(q)
+    ia.attn_decode_kv4(both[:, :6], here, out=both[:, 6:], workspace=ws)
+    check(both[:, 6:], q, ks, vs, 2)
+    want = both[:, 6:].clone()
+    ia.attn_decode_kv4(both[:, :6], here, out=both[:, :6], workspace=ws)
+    assert torch.equal(both[:, :6], want) and torch.equal(both[:, 6:], want)
+    with pytest.raises(ia.InfernoError):
+        ia.attn_decode_kv4(both[:, :6], here, out=both[:, 5:11], workspace=ws)

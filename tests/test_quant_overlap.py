@@ -53,3 +53,40 @@ def test_read_side_by_side_but_one():
     s = Strides(8 * 3 * 128, 64, 3 * 128, 1)
     assert read(far_cache(), 20 * BIG, 20 * BIG + 4 * 64, s=s) == OVERLAP
     assert read(far_cache(), 20 * BIG, 20 * BIG + 4 * 5 * 64, s=s) == OVERLAP  # the next token's
+
+
+ROW = Strides(4 * 64, 64, 64, 1)  # q and o [rows, q_heads, 1, D], dense
+ROW_BYTES = 4 * 4 * 64 * 4
+
+
+def decode(c, q, o, sq=ROW, so=ROW, ws=None, n=0, max_len=64, dt=0):
+    return ia.lib().inf_attn_decode_kv4(ctypes.byref(c), q, sq, o, so, 4, max_len, 0.125, dt, ws, n, None)
+
+
+@pytest.mark.parametrize("what", POOL)
+def test_attention_over_the_cache(what):
+    for at in places(AT[what], ROW_BYTES, POOL[what], 16):
+        assert decode(far_cache(), 20 * BIG, at) == OVERLAP
+
+
+def test_attention_over_its_queries():
+    """The result may be the queries themselves, but not other heads' or rows' of them."""
+    for at in places(20 * BIG, ROW_BYTES, ROW_BYTES, 16):
+        if at != 20 * BIG:
+            assert decode(far_cache(), 20 * BIG, at) == OVERLAP
+    assert decode(far_cache(), 20 * BIG, 20 * BIG, so=Strides(64, 4 * 64, 64, 1)) == OVERLAP  # [heads, rows]
+    wide = Strides(8 * 64, 64, 64, 1)  # out of [rows, 8 heads]
+    assert decode(far_cache(), 20 * BIG, 20 * BIG + 4 * 3 * 64, sq=wide, so=wide) == OVERLAP
+    assert decode(far_cache(), 20 * BIG, 20 * BIG + 4 * 5 * 64, sq=wide, so=wide) == OVERLAP  # the next row's
+
+
+def test_attention_over_its_workspace():
+    rows, longest = 3, 16000
+    c = far_cache(rows=rows, max_pages=1000, table_stride=1000, n_pages=3000)
+    n = ctypes.c_size_t()
+    assert ia.lib().inf_attn_decode_kv4_workspace(ctypes.byref(c), 4, longest, ctypes.byref(n)) == 0 and n.value
+    size = dict(k=3000 * 1024, v=3000 * 1024, k_scale=3000 * 64, v_scale=3000 * 64, table=3000 * 4, lens=12)
+    q, o, mine = 20 * BIG, 21 * BIG, rows * 4 * 64 * 4
+    for of, m in [(AT[name], size[name]) for name in POOL] + [(q, mine), (o, mine)]:
+        for at in (of, of + (m - 1) // 256 * 256, of - (n.value - 1) // 256 * 256):
+            assert decode(c, q, o, ws=at, n=n.value, max_len=longest) == OVERLAP
