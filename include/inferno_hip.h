@@ -548,7 +548,7 @@ typedef struct {
 /* Writes the keys and values k, v [rows, heads, T, D] (fp32 or bf16 by dt) of row n's last counts[n] positions as
  * inf_kv_append does.  A block's power of two is that of its largest magnitude, two lower and at least 2^-125: this one comes to
  * lie in [4, 8) times it.  Every channel goes to the nearest value of the grid, ties to the even code, past 6 to 6.
- * A block with an infinity or a NaN reads as NaN. */
+ * A block with an infinity or a NaN reads as NaN.  The pools must overlap neither each other nor what is read. */
 int inf_kv4_append(const inf_paged_kv4* cache, const void* k, inf_strides sk, const void* v, inf_strides sv,
                    const int32_t* counts, int T, inf_dtype dt, void* stream);
 

@@ -456,6 +456,18 @@ int inf_kv4_append(const inf_paged_kv4* cache, const void* k, inf_strides sk, co
     const int es = esz(dt);
     if ((st = check_view(k, sk, es, 4 * es)) || (st = check_view(v, sv, es, 4 * es))) return st;
     if ((int64_t)T * cache->heads * cache->D > kMaxBlocks) return INF_ERR_BAD_SHAPE;
+    // other workgroups still read the new keys and values, the table and the lengths, and write the other pools
+    const CacheMemory held(*cache);
+    const inf::Memory read[] = {memory(k, sk, cache->rows, cache->heads, T, cache->D, es),
+                                memory(v, sv, cache->rows, cache->heads, T, cache->D, es),
+                                ints(counts, cache->rows), held.table, held.lens};
+    const inf::Memory* pools[] = {&held.k, &held.v, &held.ks, &held.vs};
+    for (int i = 0; i < 4; ++i) {
+        for (const inf::Memory& m : read)
+            if (pools[i]->over(m)) return INF_ERR_BAD_STRIDE;
+        for (int j = 0; j < i; ++j)
+            if (pools[i]->over(*pools[j])) return INF_ERR_BAD_STRIDE;
+    }
     p.k = k; p.v = v;
     p.sk = view(sk); p.sv = view(sv);
     p.counts = counts;

@@ -115,3 +115,23 @@ def test_attention_beside_the_cache(ia, lens, dtype):
     assert torch.equal(both[:, :6], want) and torch.equal(both[:, 6:], want)
     with pytest.raises(ia.InfernoError):
         ia.attn_decode_kv4(both[:, :6], here, out=both[:, 5:11], workspace=ws)
+
+
+@pytest.mark.parametrize("D,layout", [(32, "heads"), (64, "slots"), (128, "joint")])
+def test_append_beside_the_cache(ia, D, layout):
+    """New keys and values, counts and cache in one piece of memory: what a cache of separate tensors holds."""
+    gen = torch.Generator().manual_seed(D + 1)
+    cache, _, _, _ = make_cache(ia, gen, [9, 30, 16], 2, D, 16, layout=layout)
+    arena = Arena(1 << 20)
+    qkv = arena.take((3, 7, 3, 2, D), F32)
+    here = in_one_arena(ia, cache, arena)
+    counts = arena.take((3,), torch.int32)
+    qkv.copy_(torch.randn(qkv.shape, generator=gen))
+    counts.copy_(torch.tensor([7, 0, 5], dtype=torch.int32))
+    for c in (cache, here):
+        ia.kv4_append(c, qkv[:, :, 1].transpose(1, 2), qkv[:, :, 2].transpose(1, 2), counts=counts)
+    for a, b in ((cache.k, here.k), (cache.v, here.v), (cache.k_scale, here.k_scale), (cache.v_scale, here.v_scale)):
+        assert torch.equal(a, b)
+    with pytest.raises(ia.InfernoError):  # keys and values in one pool
+        ia.kv4_append(ia.PagedKV4(here.k, here.k, here.k_scale, here.v_scale, here.table, here.lens),
+                      qkv[:, :, 1].transpose(1, 2), qkv[:, :, 2].transpose(1, 2))

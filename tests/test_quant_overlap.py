@@ -90,3 +90,26 @@ def test_attention_over_its_workspace():
     for of, m in [(AT[name], size[name]) for name in POOL] + [(q, mine), (o, mine)]:
         for at in (of, of + (m - 1) // 256 * 256, of - (n.value - 1) // 256 * 256):
             assert decode(c, q, o, ws=at, n=n.value, max_len=longest) == OVERLAP
+
+
+def append(c, k, v, counts=None, s=NEW, T=8, dt=0):
+    return ia.lib().inf_kv4_append(ctypes.byref(c), k, s, v, s, counts, T, dt, None)
+
+
+@pytest.mark.parametrize("what", ["k", "v", "k_scale", "v_scale"])
+def test_append_over_what_it_reads(what):
+    for at in places(AT[what], NEW_BYTES, POOL[what], 16):
+        assert append(far_cache(), at, 20 * BIG) == OVERLAP
+        assert append(far_cache(), 20 * BIG, at) == OVERLAP
+    for at in places(AT[what], 16, POOL[what], 4):
+        assert append(far_cache(), 20 * BIG, 21 * BIG, counts=at) == OVERLAP
+        assert append(far_cache(lens=at), 20 * BIG, 21 * BIG) == OVERLAP
+        assert append(far_cache(table=at), 20 * BIG, 21 * BIG) == OVERLAP
+
+
+@pytest.mark.parametrize("a", ["k", "v", "k_scale", "v_scale"])
+@pytest.mark.parametrize("b", ["k", "v", "k_scale", "v_scale"])
+def test_append_to_pools_over_each_other(a, b):
+    if a != b:
+        for at in places(AT[a], POOL[b], POOL[a], 16):
+            assert append(far_cache(**{b: at}), 20 * BIG, 21 * BIG) == OVERLAP
