@@ -572,14 +572,14 @@ int inf_attn_decode_kv4(const inf_paged_kv4* cache, const void* q, inf_strides s
  * or a NaN has scale NaN and zeros; one whose scale would be below 2^-126 scale 0 and zeros.
  * transpose: the columns of x instead, q [cols, rows] and scale [cols] -- weights [in, out] with one scale per output.
  * q's rows lie ldq bytes apart, on 16 bytes, and are written up to whole 16 bytes, with zeros; neither they nor the
- * scales may overlap x. */
+ * scales may overlap x, nor each other. */
 int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int transpose, int8_t* q, int64_t ldq,
                     float* scale, inf_dtype dt, void* stream);
 
 /* y[m, n] = (sum_k x[m, k] w[n, k]) x_scale[m] w_scale[n] + bias[n]: x [M, K] and w [N, K] in 8 bits, the sum exact
  * (K < 2^17); then in fp32, in this order (the sum times x_scale has to be finite); y and bias (may be NULL) fp32 or bf16
- * by dt, rounded once.  Rows of x and w lie on 16 bytes and are read
- * in pieces of 16 (up to K in whole 16 bytes; what lies behind K does not matter).  y must not overlap what is read.
+ * by dt, rounded once.  Rows of x and w lie on 16 bytes and are read in pieces of 16 (up to K in whole 16 bytes; what
+ * lies behind K does not matter).  Neither y nor the workspace may overlap what is read, nor each other.
  * workspace: inf_gemm_i8_workspace bytes (may be 0: then NULL), 256-byte aligned; M rows' is enough for fewer.  Calls
  * that share one must not overlap.  The same bits on every run. */
 int inf_gemm_i8_workspace(int64_t M, int64_t N, int64_t K, size_t* out_bytes);

@@ -8,6 +8,7 @@
 
 #include "inferno_hip.h"
 #include "kernels.h"
+#include "overlap.h"
 
 namespace {
 
@@ -91,6 +92,9 @@ int check_rest(const int8_t* w, int64_t ldw, const float* sw, const void* bias, 
         return INF_ERR_BAD_STRIDE;
     if (need && (!workspace || ws_bytes < need)) return INF_ERR_WORKSPACE;
     if (need && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
+    // it is written while these are read
+    const inf::Memory mw(workspace, (int64_t)need);
+    if (mw.over({w, N, ldw, K}) || mw.over({sw, 4 * N}) || mw.over({bias, (int64_t)es * N})) return INF_ERR_BAD_STRIDE;
     return INF_OK;
 }
 
@@ -153,6 +157,7 @@ int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int 
     const int64_t n = transpose ? cols : rows, k = whole16(transpose ? rows : cols);
     const Result rx = result(x, ldx, rows, cols, dt);
     if (rx.over(q, (n - 1) * ldq + k) || rx.over(scale, 4 * n)) return INF_ERR_BAD_STRIDE;
+    if (inf::Memory(q, n, ldq, k).over({scale, 4 * n})) return INF_ERR_BAD_STRIDE;
     return quantize(x, ldx, rows, cols, transpose, q, ldq, scale, dt, (hipStream_t)stream);
 }
 
@@ -178,6 +183,8 @@ int inf_gemm_i8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, c
         return st;
     const Result r = result(y, ldy, M, N, dt);
     if (r.over(x, (M - 1) * ldx + K) || r.over(x_scale, 4 * M)) return INF_ERR_BAD_STRIDE;
+    const inf::Memory mw(workspace, (int64_t)part_bytes(plan, M, N));
+    if (mw.over({x, M, ldx, K}) || mw.over({x_scale, 4 * M})) return INF_ERR_BAD_STRIDE;
     inf::GemmI8Params p = product(w, ldw, w_scale, bias, y, ldy, M, N, K, dt);
     p.x = x;
     p.ldx = ldx;
@@ -206,6 +213,8 @@ int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, c
     if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, linear_bytes(plan, M, N, K))))
         return st;
     if (result(y, ldy, M, N, dt).over(x, ((M - 1) * ldx + K) * esz(dt))) return INF_ERR_BAD_STRIDE;
+    const inf::Memory mw(workspace, (int64_t)linear_bytes(plan, M, N, K));
+    if (mw.over({x, M, ldx * esz(dt), K * esz(dt)})) return INF_ERR_BAD_STRIDE;
     inf::GemmI8Params p = product(w, ldw, w_scale, bias, y, ldy, M, N, K, dt);
     if (plan.fused) {
         p.xf = x;

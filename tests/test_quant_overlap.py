@@ -113,3 +113,34 @@ def test_append_to_pools_over_each_other(a, b):
     if a != b:
         for at in places(AT[a], POOL[b], POOL[a], 16):
             assert append(far_cache(**{b: at}), 20 * BIG, 21 * BIG) == OVERLAP
+
+
+# ---- matrices in 8 bits
+
+
+def product_bytes(call, M, N, K):
+    n = ctypes.c_size_t()
+    assert getattr(ia.lib(), f"inf_{call}_i8_workspace")(M, N, K, ctypes.byref(n)) == 0 and n.value
+    return n.value
+
+
+def test_workspace_over_what_is_read():
+    M, N, K = 64, 130, 9000  # in K ranges
+    x, w, sw, b, y, sx = (i * BIG for i in range(20, 26))
+    ld = 9008
+    for dt, es in ((0, 4), (1, 2)):
+        n = product_bytes("linear", M, N, K)
+        for of, m in ((x, M * K * es), (w, (N - 1) * ld + K), (sw, 4 * N), (b, es * N), (y, M * N * es)):
+            for at in (of, of + (m - 1) // 256 * 256, of - (n - 1) // 256 * 256):
+                assert ia.lib().inf_linear_i8(M, N, K, x, K, w, ld, sw, b, y, N, dt, at, n, None) == OVERLAP
+        n = product_bytes("gemm", M, N, K)
+        for of, m in ((x, (M - 1) * ld + K), (w, (N - 1) * ld + K), (sx, 4 * M), (sw, 4 * N), (b, es * N),
+                      (y, M * N * es)):
+            for at in (of, of + (m - 1) // 256 * 256, of - (n - 1) // 256 * 256):
+                assert ia.lib().inf_gemm_i8(M, N, K, x, ld, sx, w, ld, sw, b, y, N, dt, at, n, None) == OVERLAP
+
+
+def test_quantized_rows_over_their_scales():
+    q = 20 * BIG
+    for s in (q, q + 7 * 64 + 60, q - 28):
+        assert ia.lib().inf_quantize_i8(21 * BIG, 64, 8, 64, 0, q, 64, s, 0, None) == OVERLAP
