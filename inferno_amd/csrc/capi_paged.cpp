@@ -172,7 +172,8 @@ int check_cache4(const inf_paged_kv4* c, bool written, inf::Paged4View* out) {
 }
 
 inf::Memory memory(const void* p, const inf_strides& s, int64_t B, int64_t H, int64_t T, int64_t D, int es) {
-    return {p, B, s.b * es, H, s.h * es, T, s.t * es, D * es};
+    auto bytes = [&](int64_t n) { return inf::Memory::bytes(n, es); };
+    return {p, B, bytes(s.b), H, bytes(s.h), T, bytes(s.t), D * es};
 }
 inf::Memory ints(const int32_t* p, int64_t n) { return {p, 4 * n}; }
 
@@ -184,7 +185,7 @@ struct CacheMemory {
           v(memory(c.v, c.sv, c.n_pages, c.heads, c.page_size, c.D / 2, 1)),
           ks(memory(c.k_scale, c.sks, c.n_pages, c.heads, c.D / 32, c.page_size, 1)),
           vs(memory(c.v_scale, c.svs, c.n_pages, c.heads, c.D / 32, c.page_size, 1)),
-          table(c.table, c.rows, 4 * c.table_stride, 4 * (int64_t)c.max_pages),
+          table(c.table, c.rows, inf::Memory::bytes(c.table_stride, 4), 4 * (int64_t)c.max_pages),
           lens(ints(c.lens, c.rows)) {}
     bool over(const inf::Memory& m) const {
         return m.over(k) || m.over(v) || m.over(ks) || m.over(vs) || m.over(table) || m.over(lens);

@@ -64,18 +64,9 @@ size_t most_bytes(int64_t M, int64_t N, int64_t K, bool quantised, F bytes) {
     return n;
 }
 
-// Whether y [M, N] lies over the n bytes from a on (which may be null: then not).
-struct Result {
-    uintptr_t first, end;
-    bool over(const void* a, int64_t n) const {
-        const uintptr_t x = reinterpret_cast<uintptr_t>(a);
-        return a && x < end && first < x + (uintptr_t)n;
-    }
-};
-
-Result result(const void* y, int64_t ldy, int64_t M, int64_t N, inf_dtype dt) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(y);
-    return {x, x + (uintptr_t)(((M - 1) * ldy + N) * esz(dt))};
+// A matrix of elements of this type.
+inf::Memory elements(const void* x, int64_t ld, int64_t rows, int64_t cols, inf_dtype dt) {
+    return {x, rows, inf::Memory::bytes(ld, esz(dt)), cols * esz(dt)};
 }
 
 // The arguments that both forms of the product share.
@@ -86,16 +77,14 @@ int check_rest(const int8_t* w, int64_t ldw, const float* sw, const void* bias, 
     const size_t es = (size_t)esz(dt);
     if (!aligned(sw, 4) || !aligned(y, es) || !aligned(bias, es)) return INF_ERR_ALIGNMENT;
     // other workgroups read these while one writes its results
-    const Result r = result(y, ldy, M, N, dt);
-    if (r.over(w, (N - 1) * ldw + K) || r.over(sw, 4 * N) || r.over(bias, (int64_t)es * N) ||
-        r.over(workspace, (int64_t)need))
-        return INF_ERR_BAD_STRIDE;
+    const inf::Memory my = elements(y, ldy, M, N, dt), mw(workspace, (int64_t)need);
+    auto read = [&](const inf::Memory& m) {
+        return m.over({w, N, ldw, K}) || m.over({sw, 4 * N}) || m.over({bias, (int64_t)es * N});
+    };
+    if (read(my) || my.over(mw)) return INF_ERR_BAD_STRIDE;
     if (need && (!workspace || ws_bytes < need)) return INF_ERR_WORKSPACE;
     if (need && !aligned(workspace, kAlign)) return INF_ERR_ALIGNMENT;
-    // it is written while these are read
-    const inf::Memory mw(workspace, (int64_t)need);
-    if (mw.over({w, N, ldw, K}) || mw.over({sw, 4 * N}) || mw.over({bias, (int64_t)es * N})) return INF_ERR_BAD_STRIDE;
-    return INF_OK;
+    return read(mw) ? INF_ERR_BAD_STRIDE : INF_OK;
 }
 
 // Rows of elements that can be read four at a time.
@@ -155,9 +144,8 @@ int inf_quantize_i8(const void* x, int64_t ldx, int64_t rows, int64_t cols, int 
     if ((st = check_i8(q, ldq, transpose ? rows : cols))) return st;
     // other workgroups still read x
     const int64_t n = transpose ? cols : rows, k = whole16(transpose ? rows : cols);
-    const Result rx = result(x, ldx, rows, cols, dt);
-    if (rx.over(q, (n - 1) * ldq + k) || rx.over(scale, 4 * n)) return INF_ERR_BAD_STRIDE;
-    if (inf::Memory(q, n, ldq, k).over({scale, 4 * n})) return INF_ERR_BAD_STRIDE;
+    const inf::Memory mx = elements(x, ldx, rows, cols, dt), mq(q, n, ldq, k), ms(scale, 4 * n);
+    if (mx.over(mq) || mx.over(ms) || mq.over(ms)) return INF_ERR_BAD_STRIDE;
     return quantize(x, ldx, rows, cols, transpose, q, ldq, scale, dt, (hipStream_t)stream);
 }
 
@@ -181,10 +169,9 @@ int inf_gemm_i8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, c
     const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K, true);
     if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, part_bytes(plan, M, N))))
         return st;
-    const Result r = result(y, ldy, M, N, dt);
-    if (r.over(x, (M - 1) * ldx + K) || r.over(x_scale, 4 * M)) return INF_ERR_BAD_STRIDE;
-    const inf::Memory mw(workspace, (int64_t)part_bytes(plan, M, N));
-    if (mw.over({x, M, ldx, K}) || mw.over({x_scale, 4 * M})) return INF_ERR_BAD_STRIDE;
+    const inf::Memory mx(x, M, ldx, K), ms(x_scale, 4 * M);
+    for (const inf::Memory& m : {elements(y, ldy, M, N, dt), inf::Memory(workspace, (int64_t)part_bytes(plan, M, N))})
+        if (m.over(mx) || m.over(ms)) return INF_ERR_BAD_STRIDE;
     inf::GemmI8Params p = product(w, ldw, w_scale, bias, y, ldy, M, N, K, dt);
     p.x = x;
     p.ldx = ldx;
@@ -212,9 +199,9 @@ int inf_linear_i8(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, c
     const inf::GemmI8Plan plan = inf::gemm_i8_plan(M, N, K, false);
     if ((st = check_rest(w, ldw, w_scale, bias, y, ldy, M, N, K, dt, workspace, ws_bytes, linear_bytes(plan, M, N, K))))
         return st;
-    if (result(y, ldy, M, N, dt).over(x, ((M - 1) * ldx + K) * esz(dt))) return INF_ERR_BAD_STRIDE;
-    const inf::Memory mw(workspace, (int64_t)linear_bytes(plan, M, N, K));
-    if (mw.over({x, M, ldx * esz(dt), K * esz(dt)})) return INF_ERR_BAD_STRIDE;
+    const inf::Memory mx = elements(x, ldx, M, K, dt);
+    if (mx.over(elements(y, ldy, M, N, dt)) || mx.over({workspace, (int64_t)linear_bytes(plan, M, N, K)}))
+        return INF_ERR_BAD_STRIDE;
     inf::GemmI8Params p = product(w, ldw, w_scale, bias, y, ldy, M, N, K, dt);
     if (plan.fused) {
         p.xf = x;

@@ -33,6 +33,9 @@ public:
         }
     }
 
+    // The bytes of so many elements, in 64 bits.
+    static int64_t bytes(int64_t n, int es) { return std::min(n, kFar / es) * es; }
+
     // A null pointer has no memory.
     bool over(const Memory& o) const {
         if (!at_ || !o.at_ || run_ <= 0 || o.run_ <= 0) return false;

@@ -44,6 +44,34 @@ def test_linear_with_one_workspace(ia, N, K):
         assert torch.equal(ia.gemm_i8(q, s, w, sw, dtype=BF16, workspace=product_ws), want)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M", [1, 4, 40, 200])
+def test_linear_within_one_matrix(ia, M, dtype):
+    """Input and result are columns of one matrix, bias and scales lie behind a row's end."""
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    K, N = 96, 100
+    buf = torch.full((M, K + N + 60), 7.0, dtype=dtype, device="cuda")
+    x = torch.randn((M, K), generator=gen, device="cuda").to(dtype)
+    w, sw = ia.quantize_i8(torch.randn((K, N), generator=gen, device="cuda"), transpose=True)
+    bias = torch.randn(N, generator=gen, device="cuda").to(dtype)
+    want = ia.linear_i8(x, w, sw, bias=bias)
+    for first in (True, False):  # the input before the result, and behind it
+        buf.fill_(7.0)
+        a, b = (buf[:, :K], buf[:, K:K + N]) if first else (buf[:, N:N + K], buf[:, :N])
+        a.copy_(x)
+        ia.linear_i8(a, w, sw, bias=bias, out=b)
+        assert torch.equal(b, want) and torch.equal(a, x) and (buf[:, K + N:] == 7).all()
+        if M > 1:
+            with pytest.raises(ia.InfernoError):
+                ia.linear_i8(a, w, sw, bias=bias, out=buf[:, 1:N + 1])
+    q, s = ia.quantize_i8(x)
+    rows = torch.full((M, 96 + 4 * N + 16), 9, dtype=torch.uint8, device="cuda")  # rows in 8 bits, the result's behind
+    q2, y = rows[:, :K].view(torch.int8), rows[:, 96:96 + 4 * N].view(F32)
+    q2.copy_(q)
+    ia.gemm_i8(q2, s, w, sw, out=y)
+    assert torch.equal(y, ia.gemm_i8(q, s, w, sw)) and torch.equal(q2, q) and (rows[:, 96 + 4 * N:] == 9).all()
+
+
 class Arena:
     """Tensors one behind the other in one piece of memory."""
 

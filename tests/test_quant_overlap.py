@@ -144,3 +144,21 @@ def test_quantized_rows_over_their_scales():
     q = 20 * BIG
     for s in (q, q + 7 * 64 + 60, q - 28):
         assert ia.lib().inf_quantize_i8(21 * BIG, 64, 8, 64, 0, q, 64, s, 0, None) == OVERLAP
+
+
+def test_results_beside_what_is_read():
+    """Between y's rows there is room: not refused (6: the next check's, the workspace's)."""
+    M, N, K, y = 100, 32, 64, 20 * BIG
+    for dt, es in ((0, 4), (1, 2)):
+        for place in ("w", "sw", "b"):
+            for off in (es * N, es * N + 16):
+                a = dict(w=21 * BIG, sw=22 * BIG, b=23 * BIG)
+                a[place] = y + off
+                kw = dict(w=K) if place == "w" else {}
+                pitch = 4096
+                n = 1 if place == "w" else N
+                assert ia.lib().inf_linear_i8(M, n, K, 24 * BIG, K, a["w"], K, a["sw"], a["b"], y, pitch // es, dt, None,
+                                              0, None) == 6
+                a[place] = y + pitch - 64 if place == "w" else y + 3 * pitch - 4
+                assert ia.lib().inf_linear_i8(M, N, K, 24 * BIG, K, a["w"], K, a["sw"], a["b"], y, pitch // es, dt,
+                                              None, 0, None) == OVERLAP
