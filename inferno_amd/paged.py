@@ -146,9 +146,12 @@ def _one_layer(cache, what):
 
 
 def _bytes(cache, call, *args):
-    """The workspace bytes that the C-ABI's `call` gives, asked once per cache and arguments."""
+    """The workspace bytes that the C-ABI's `call` gives, asked once per cache and arguments (a bounded number of them:
+    ``max_len`` may be another one at every token)."""
     n = cache.sizes.get((call, args))
     if n is None:
+        if len(cache.sizes) >= 4096:
+            cache.sizes.clear()
         n = cache.sizes[call, args] = _size(getattr(lib(), call), cache.ref, *args)
     return n
 

@@ -109,14 +109,9 @@ def quantize_i8(x, transpose=False, stream=None):
     return q, scale
 
 
-_sizes = {}
-
-
+@functools.lru_cache(maxsize=4096)
 def _product_bytes(call, M, N, K):
-    n = _sizes.get((call, M, N, K))
-    if n is None:
-        n = _sizes[call, M, N, K] = _size(getattr(lib(), call), M, N, K)
-    return n
+    return _size(getattr(lib(), call), M, N, K)
 
 
 def gemm_i8_workspace(M, N, K, device="cuda"):

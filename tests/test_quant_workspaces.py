@@ -60,3 +60,20 @@ def test_product_workspace_of_the_most_rows(N, K):
         args = dict(M=M, N=N, K=K, ldx=ld, ldw=ld, ldy=N, y=1 << 50, ws=ODD)
         assert linear(**args, n=product_bytes("linear", M, N, K)) == 7
         assert linear(**args, n=M * K - 1) == 6
+
+
+def test_sizes_kept_are_bounded():
+    """A server that asks for every length and number of rows keeps some sizes, not all that it ever asked for."""
+    torch = pytest.importorskip("torch")
+    quant, paged = ia.quant, ia.paged
+    for M in range(1, 6000):
+        assert quant._product_bytes("inf_linear_i8_workspace", M, 64, 64) == product_bytes("linear", M, 64, 64)
+    assert quant._product_bytes.cache_info().currsize <= 4096
+    table, lens = torch.zeros((2, 512), dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    pool = torch.zeros((4, 1, 16, 64))
+    for c, call, more in ((ia.PagedKV4.empty(4, 1, 16, 64, table, lens), "inf_attn_decode_kv4_workspace", ()),
+                          (ia.PagedKV(pool, pool, table, lens), "inf_attn_decode_paged_workspace", (0,))):
+        for n in range(1, 6000):
+            size = paged._bytes(c, call, 1, n, *more)
+            assert size == paged._bytes(c, call, 1, n, *more)
+        assert len(c.sizes) <= 4096
