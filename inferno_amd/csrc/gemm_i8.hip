@@ -21,6 +21,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 namespace {
 
 constexpr uint32_t kNowhere = 0x80000000u;  // past the end of every buffer resource
+constexpr int kI8Step = 128;  // a step's k in any kernel; K ranges are whole ones
 
 __device__ __forceinline__ i32x16 mfma32x32x32i8(i32x4 a, i32x4 b, i32x16 c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
@@ -81,10 +82,10 @@ struct Columns {
 
 // ============================================================================
 // Tiles.  A workgroup of WN x WM waves forms BN x BM results, each wave 32 x 32 blocks of them in its registers, with
-// k in steps of BK bytes through a ring of S buffers in LDS, filled by direct-to-LDS loads S - 1 steps ahead.
+// k in steps of 128 bytes through a ring of S buffers in LDS, filled by direct-to-LDS loads S - 1 steps ahead.
 // A step's 16-byte pieces of a row lie in an order that varies with the row, so that any eight rows' pieces of
 // one k lie in different banks.  A direct-to-LDS load fills 16 bytes a lane in the lanes' order, so the
-// lanes fetch the pieces in that order: four (BK = 64) or eight lanes still take one run of a row.
+// lanes fetch the pieces in that order: eight lanes still take one run of a row.
 //
 // One barrier a step, before its last 32 k: by then every wave has read all of the step's operands (the last 32 k's are
 // in registers), so its buffer takes the loads of S steps on, while the products of these 32 k hide the first reads of
@@ -92,16 +93,16 @@ struct Columns {
 //
 // What bounds it, and what it measured (bf16 results):
 //   tiles of 256 (two waves a SIMD, 128 KB of LDS): 16384 x 8192 x 8192 in 884-916 us, 2.4-2.5 POP/s, matrix cores busy
-//     67 % at 1.76 GHz: the power limit sets that clock.  Four waves of 128 x 128 took 1050, BK = 64 with S = 4 more too;
+//     67 % at 1.76 GHz: the power limit sets that clock.  Four waves of 128 x 128 took 1050, steps of 64 with S = 4 more too;
 //   tiles of 128 (two workgroups a CU, one's results leave while the other's products run): 8192 x 2304 x 768 in fp32
 //     30-35 us, of which 75 MB of results are 15 and every step of k 1.7: both in part in the open.  Tiles of 128 x
-//     192, 128 x 256 and 64 x 128 took 35-37, BK = 64 37;
+//     192, 128 x 256 and 64 x 128 took 35-37, steps of 64 37;
 //   tiles of 64: weights, 32 x 16384 x 4096 in 12.7 us, 5.3 TB/s; or L2's latency and rate, 333 x 4096 x 4096 in 15.
 // ============================================================================
-template <typename E, int BN, int BM, int WN, int WM, int BK, int S, bool SPLIT>
-__global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * BK * S > 81920 ? 1 : 2) / 4) void gemm_i8_kernel(
+template <typename E, int BN, int BM, int WN, int WM, int S, bool SPLIT>
+__global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * kI8Step * S > 81920 ? 1 : 2) / 4) void gemm_i8_kernel(
     GemmI8Params p) {
-    constexpr int NW = WN * WM;
+    constexpr int NW = WN * WM, BK = kI8Step;
     constexpr int FN = BN / WN / 32, FM = BM / WM / 32;
     constexpr int P = BK / 16, RI = 64 / P;                     // pieces a row; rows a load instruction
     constexpr int IN = BN / RI / NW, IM = BM / RI / NW;         // instructions a wave and step
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(64 * WN * WM, WN * WM * ((BN + BM) * BK * S > 81920
     const int8_t* W = p.w + (int64_t)n0 * p.ldw;
     const int8_t* X = p.x + (int64_t)m0 * p.ldx;
     const int rows_n = min(p.N - n0, BN), rows_m = min(p.M - m0, BM);
-    auto order = [](int row) { return P == 8 ? row & 7 : (row >> 1) & 3; };
+    auto order = [](int row) { return row & 7; };
     const int piece = 16 * ((lane % P) ^ order(lane / P));  // this lane's of a step's row
     uint32_t vw[IN], vx[IM];
 #pragma unroll
@@ -328,7 +329,7 @@ constexpr int kRowsWaves = 4;
 
 template <typename E, int FM, int S, bool FUSED>
 __global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Params p) {
-    constexpr int BK = 128, BN = 32, NW = kRowsWaves;
+    constexpr int BK = kI8Step, BN = 32, NW = kRowsWaves;
     constexpr int XB = FUSED ? 0 : 32 * FM;                  // rows of x in the ring
     constexpr int L = (BN + XB) / 8;                         // load instructions a step
     constexpr int STEP = (BN + XB) * BK;
@@ -498,8 +499,6 @@ __global__ __launch_bounds__(64 * kRowsWaves) void gemm_i8_rows_kernel(GemmI8Par
     }
 }
 
-// K ranges are whole steps of any kernel.
-constexpr int kI8Step = 128;
 // Tiles of 64 by ranges, at most.
 constexpr int kI8Ranges = 384;
 
@@ -552,12 +551,12 @@ GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
     return plan;
 }
 
-template <typename E, int BN, int BM, int WN, int WM, int BK, int S, bool SPLIT>
+template <typename E, int BN, int BM, int WN, int WM, int S, bool SPLIT>
 static void launch_tiles(GemmI8Params& p, hipStream_t s) {
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
     p.items = p.tiles_m * p.tiles_n * p.ksplit;
-    hipLaunchKernelGGL((gemm_i8_kernel<E, BN, BM, WN, WM, BK, S, SPLIT>), dim3((unsigned)((p.items + 7) / 8 * 8)),
+    hipLaunchKernelGGL((gemm_i8_kernel<E, BN, BM, WN, WM, S, SPLIT>), dim3((unsigned)((p.items + 7) / 8 * 8)),
                        dim3(64 * WN * WM), 0, s, p);
 }
 
@@ -576,18 +575,18 @@ static int launch_t(GemmI8Params p, const GemmI8Plan& plan, hipStream_t s) {
             hipLaunchKernelGGL((gemm_i8_rows_kernel<E, 2, 3, false>), grid, block, 0, s, p);
         }
     } else if (plan.kind == GemmI8Plan::k256) {
-        launch_tiles<E, 256, 256, 2, 4, 128, 2, false>(p, s);
+        launch_tiles<E, 256, 256, 2, 4, 2, false>(p, s);
     } else if (plan.kind == GemmI8Plan::k128) {
-        if (plan.deep) launch_tiles<E, 128, 128, 2, 2, 128, 4, false>(p, s);
-        else launch_tiles<E, 128, 128, 2, 2, 128, 2, false>(p, s);
+        if (plan.deep) launch_tiles<E, 128, 128, 2, 2, 4, false>(p, s);
+        else launch_tiles<E, 128, 128, 2, 2, 2, false>(p, s);
     } else if (p.ksplit > 1) {
-        launch_tiles<E, 64, 64, 2, 2, 128, 4, true>(p, s);
+        launch_tiles<E, 64, 64, 2, 2, 4, true>(p, s);
         hipLaunchKernelGGL((gemm_i8_join_kernel<E>), dim3((unsigned)(((int64_t)p.M * (p.ldp / 4) + 255) / 256)),
                            dim3(256), 0, s, p);
     } else if (plan.deep) {
-        launch_tiles<E, 64, 64, 2, 2, 128, 4, false>(p, s);
+        launch_tiles<E, 64, 64, 2, 2, 4, false>(p, s);
     } else {
-        launch_tiles<E, 64, 64, 2, 2, 128, 2, false>(p, s);
+        launch_tiles<E, 64, 64, 2, 2, 2, false>(p, s);
     }
     return (int)hipGetLastError();
 }
