@@ -1,9 +1,11 @@
-"""Calls of weights in 8 bits and a cache in 4 as programs make them: one workspace for rows that grow."""
+"""Calls of weights in 8 bits and a cache in 4 as programs make them: one workspace for rows that grow, results beside
+what is read, two query heads a kv head, few rows of a vocabulary's width."""
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from test_gpu_kv4 import check, ia, make_cache  # noqa: E402,F401
+from test_gpu_quant import check_product, rand_i8, ref_quantize  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -163,3 +165,48 @@ def test_append_beside_the_cache(ia, D, layout):
     with pytest.raises(ia.InfernoError):  # keys and values in one pool
         ia.kv4_append(ia.PagedKV4(here.k, here.k, here.k_scale, here.v_scale, here.table, here.lens),
                       qkv[:, :, 1].transpose(1, 2), qkv[:, :, 2].transpose(1, 2))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_two_query_heads(ia, D, dtype):
+    """Two query heads a kv head, whole rows to the workgroups and in shares."""
+    gen = torch.Generator().manual_seed(D + 2)
+    for lens in ([0, 1, 15, 16, 17, 255, 256, 257, 513, 1000], [3000, 0, 700, 1]):
+        cache, ks, vs, _ = make_cache(ia, gen, lens, 3, D, 16)
+        q = torch.randn((len(lens), 6, 1, D), generator=gen).to(dtype)
+        check(ia.attn_decode_kv4(q.cuda(), cache), q, ks, vs, 3)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_read_on_8_bytes(ia, D):
+    """bf16 results whose rows lie on 8 bytes only; what lies beside them stays."""
+    gen = torch.Generator().manual_seed(D + 3)
+    cache, ks, vs, _ = make_cache(ia, gen, [9, 0, 77], 2, D, 16)
+    first = torch.tensor([2, 0, 1], dtype=torch.int32).cuda()
+    store = torch.full((2, 3, 2, 80, D + 4), 5.0, dtype=BF16, device="cuda")
+    k, v = store[0, ..., 4:], store[1, ..., :D]
+    ia.kv4_read(cache, 80, first=first, k_out=k, v_out=v)
+    for got, want in ((k, ks), (v, vs)):
+        for r, n in enumerate([9, 0, 77]):
+            f = int(first[r])
+            m = max(n - f, 0)
+            assert torch.equal(got[r, :, :m].cpu().double(), want[r][:, f:]) and not got[r, :, m:].any()
+    assert (store[0, ..., :4] == 5).all() and (store[1, ..., D:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,N,K", [(1, 50257, 768), (2, 50257, 130), (17, 50257, 768), (33, 50257, 768), (64, 32000, 300),
+                                   (1, 8200, 9000), (1, 700, 14336), (5, 300, 11008), (1, 28672, 1000)])
+def test_few_rows_of_wide_layers(ia, M, N, K, dtype):
+    """A vocabulary's projection and long inner layers at few tokens, past the few-row kernel's sizes."""
+    gen = torch.Generator().manual_seed(M + N + K)
+    x = torch.randn((M, K), generator=gen).to(dtype)
+    w, dw = rand_i8(gen, N, K)
+    sw = torch.rand(N, generator=gen) + 0.1
+    bias = (torch.randn(N, generator=gen) * 1000).to(dtype)
+    qx, sx = ref_quantize(x)
+    y = ia.linear_i8(x.cuda(), dw, sw.cuda(), bias=bias.cuda())
+    check_product(y, qx @ w.double().t(), sx, sw, bias, dtype)
+    q, s = ia.quantize_i8(x.cuda())
+    assert torch.equal(ia.gemm_i8(q, s, dw, sw.cuda(), bias=bias.cuda(), dtype=dtype), y)
