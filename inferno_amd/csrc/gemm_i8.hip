@@ -511,7 +511,8 @@ GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
     const int64_t steps = (K + kI8Step - 1) / kI8Step;
     // Few rows: where their kernel is at most one workgroup a CU and no row too long for one (us, its and tiles of 64):
     // 32 x 4096 x 4096 6.9 and 9.6, 8 x 8192 x 8192 13.5 and 14.0; but 32 x 16384 x 4096 19 and 12.9,
-    // 32 x 4096 x 16384 21 and 15.2.
+    // 32 x 4096 x 16384 21 and 15.2.  One row goes the same way past this border, where its x is quantised by a launch of its
+    // own (whole calls, weights from memory): 1 x 8192 x 8192, inside, 17.5; 1 x 16384 x 4096 20.8, 1 x 4096 x 14336 26.5.
     if (M <= 64 && (N + 31) / 32 <= 256 && steps <= 64) {
         plan.kind = GemmI8Plan::kRows;
         // x quantised by every workgroup, where that takes no longer than a launch of its own (us, so and with one): 1 x 2304
@@ -523,7 +524,8 @@ GemmI8Plan gemm_i8_plan(int64_t M, int64_t N, int64_t K, bool quantised) {
     // Tiles of 256, one workgroup a CU (us, theirs and tiles of 128, bf16 results): 4096 x 4096 x 4096 67 and 88, x 512 18.1 and
     // 20.3; with 69 % of a round's CUs busy, 2816 x 4096 x 4096, 56 and 65, but 53 %, 4352 x 4096 x 4096, 108 and 94.  A short
     // K leaves the results' writing in the open, which two workgroups a CU hide: 75 %, 16384 x 2304 x 768 in
-    // fp32, 70 and 55.
+    // fp32, 70 and 55.  The rule counts tiles, full or not: few rows of a vocabulary's width take them for their weights
+    // (whole calls): 1 x 50257 x 4096 62 us, 32 62, 64 68; of 128, 1 x 50257 x 768 15.4, 1 x 28672 x 8192 52.
     const int64_t t256 = tiles(256), rounds = (t256 + 255) / 256;
     if (steps >= 4 && t256 * 10 >= rounds * 256 * (steps >= 16 ? 7 : 9)) {
         plan.kind = GemmI8Plan::k256;

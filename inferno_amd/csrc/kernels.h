@@ -497,8 +497,8 @@ int64_t gemm_i8_split_rows(int64_t N);
 int launch_gemm_i8(const GemmI8Params& p, const GemmI8Plan& plan, int bf16, hipStream_t s);
 
 // ---- a paged key-value cache in 4 bits (paged4.hip) -----------------------------
-// Pools of bytes, two channels each, [n_pages, heads, slots, D / 2] and of scales [n_pages, heads, slots, D / 32],
-// through strides in bytes; table, lens and page numbers as in PagedView.
+// Pools of bytes, two channels each, [n_pages, heads, slots, D / 2] and of scales [n_pages, heads, D / 32, slots] (t from
+// block to block, slots adjacent), through strides in bytes; table, lens and page numbers as in PagedView.
 struct Paged4View {
     uint8_t* k;
     uint8_t* v;
